@@ -168,11 +168,9 @@ def _mass_inputs(case: dict[str, Any], g: torch.Generator) -> dict[str, Any]:
         seen = (seen - T + 1 + torch.arange(T, device="cuda", dtype=torch.int32)).clamp(min=1)
     scale = 1.0 / math.sqrt(D)
     # the rows' log-sum-exp, as the pass's attention leaves it
-    lse = torch.empty(T, Hq, dtype=torch.float32, device="cuda")
     hidden = torch.arange(n, device="cuda")[None, None, :] >= seen[:, None, None]
-    for h in range(Hk):
-        s = _scores(q, K[h, :n], h, case, scale).masked_fill(hidden, -math.inf)
-        lse[:, h * (Hq // Hk):(h + 1) * (Hq // Hk)] = torch.logsumexp(s, dim=-1)
+    scores = _scores(q, K[:, :n], case, scale).masked_fill_(hidden, -math.inf)
+    lse = torch.logsumexp(scores, dim=-1).transpose(0, 1).reshape(T, Hq)
     mass = torch.rand(Hk, n + 9, generator=g, device="cuda") ** 4 * 8.0
     return {"q": q, "K": K, "lse": lse, "seen": seen, "mass": mass, "scale": scale}
 
@@ -287,45 +285,39 @@ def _plain_rope(s: dict[str, Any]) -> Any:
     return turned(heads[:, :Hq], s["wq"]).reshape(T, Hq * D), s["K"], s["V"]
 
 
-def _scores(q: torch.Tensor, K: torch.Tensor, h: int, c: dict[str, Any], scale: float) -> torch.Tensor:
-    """one kv head's scores [T, G, keys] in 32 bits"""
-    G = c["Hq"] // c["Hk"]
-    rows = q.view(c["T"], c["Hq"], c["D"])[:, h * G:(h + 1) * G].float().reshape(c["T"] * G, c["D"])
-    return ((rows * scale) @ K.float().t()).view(c["T"], G, -1)
+def _scores(q: torch.Tensor, K: torch.Tensor, c: dict[str, Any], scale: float) -> torch.Tensor:
+    """the scores [Hk, T, G, keys] in 32 bits"""
+    T, Hk, D = c["T"], c["Hk"], c["D"]
+    rows = q.view(T, Hk, -1, D).transpose(0, 1).float().reshape(Hk, -1, D) * scale
+    return torch.matmul(rows, K.float().transpose(1, 2)).view(Hk, T, -1, K.shape[1])
 
 
 def _plain_shared(s: dict[str, Any]) -> Any:
     c = s["case"]
     T, Hq, Hk, D, P = (c[k] for k in ("T", "Hq", "Hk", "D", "P"))
-    G, off = Hq // Hk, s["off"]
+    off = s["off"]
     first, lens = s["lay"]
     step = torch.arange(c["own"], device="cuda")
     at = first[:, None] + torch.minimum(step[None, :], lens[:, None] - 1)  # [T, own], a row's last key again past its end
     past = (step[None, :] >= lens[:, None])[:, None, :]
-    out = torch.empty(T, Hk, G, D, dtype=torch.float32, device="cuda")
-    lse = torch.empty(T, Hk, G, dtype=torch.float32, device="cuda")
-    q = s["q"].view(T, Hk, G, D)
-    for h in range(Hk):
-        K, V = s["K"][h], s["V"][h]
-        far = _scores(s["q"], K[off:off + P], h, c, s["scale"])
-        near = torch.matmul(q[:, h].float() * s["scale"], K[at].float().transpose(1, 2)).masked_fill(past, -math.inf)
-        top = torch.maximum(far.amax(dim=-1), near.amax(dim=-1))
-        far, near = torch.exp(far - top[..., None]), torch.exp(near - top[..., None])
-        total = far.sum(dim=-1) + near.sum(dim=-1)
-        acc = (far.view(T * G, P) @ V[off:off + P].float()).view(T, G, D) + torch.matmul(near, V[at].float())
-        out[:, h], lse[:, h] = acc / total[..., None], top + torch.log(total)
-    return out.to(torch.bfloat16).view(T, Hq * D), lse.view(T, Hq)
+    far = _scores(s["q"], s["K"][:, off:off + P], c, s["scale"])
+    rows = s["q"].view(T, Hk, -1, D).transpose(0, 1).float() * s["scale"]
+    near = torch.matmul(rows, s["K"][:, at].float().transpose(2, 3)).masked_fill_(past, -math.inf)
+    top = torch.maximum(far.amax(dim=-1), near.amax(dim=-1))
+    far, near = far.sub_(top[..., None]).exp_(), near.sub_(top[..., None]).exp_()
+    total = far.sum(dim=-1) + near.sum(dim=-1)
+    out = torch.matmul(far.view(Hk, -1, P), s["V"][:, off:off + P].float()).view(rows.shape)
+    out = (out + torch.matmul(near, s["V"][:, at].float())) / total[..., None]
+    return (out.to(torch.bfloat16).transpose(0, 1).reshape(T, Hq * D), (top + torch.log(total)).transpose(0, 1).reshape(T, Hq))
 
 
 def _plain_mass(s: dict[str, Any]) -> Any:
     c = s["case"]
-    n, G = c["n"], c["Hq"] // c["Hk"]
+    n = c["n"]
     hidden = torch.arange(n, device="cuda")[None, None, :] >= s["seen"][:, None, None]
-    out = torch.empty(c["Hk"], n, dtype=torch.float32, device="cuda")
-    for h in range(c["Hk"]):
-        p = torch.exp(_scores(s["q"], s["K"][h, :n], h, c, s["scale"]) - s["lse"][:, h * G:(h + 1) * G, None])
-        out[h] = s["mass"][h, :n] + p.masked_fill(hidden, 0.0).sum(dim=(0, 1))
-    return out
+    lse = s["lse"].view(c["T"], c["Hk"], -1).transpose(0, 1)[..., None]
+    p = _scores(s["q"], s["K"][:, :n], c, s["scale"]).sub_(lse).exp_()
+    return s["mass"][:, :n] + p.masked_fill_(hidden, 0.0).sum(dim=(1, 2))
 
 
 def _plain_evict(s: dict[str, Any]) -> Any:
