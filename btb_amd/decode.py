@@ -82,6 +82,17 @@ def rope_tables(cfg: StackConfig, positions: int, device: Any) -> tuple[torch.Te
     return emb.cos().to(torch.bfloat16).contiguous(), emb.sin().to(torch.bfloat16).contiguous()
 
 
+def rope_axes(sections: list[int], device: Any, interleaved: bool = False) -> torch.Tensor:
+    """which position axis turns each frequency, uint8 [sum(sections)], as `HipCard.norm_rope_axes` reads it: `sections[a]`
+    frequencies of axis a, in runs, or dealt in turn while an axis has any left"""
+    if not sections or min(sections) < 0 or len(sections) > 255:
+        raise ValueError(f"[decode] up to 255 axes, each of some frequencies, got {sections}")
+    axes = [a for a, n in enumerate(sections) for _ in range(n)]
+    if interleaved:
+        axes = [a for i in range(max(sections)) for a, n in enumerate(sections) if i < n]
+    return torch.tensor(axes, dtype=torch.uint8, device=device)
+
+
 def pass_spans(cus: int, T: int, Hq: int, Hk: int, cap: int) -> int:
     """how many spans the attention of a pass of T rows cuts a cache of `cap` slots into. Its workgroup walks a span in
     batches of 128 keys for up to 32 (row, head) pairs of a kv head, so: a workgroup a CU, spans whole batches. Where a kv

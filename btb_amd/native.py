@@ -108,6 +108,15 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "btb_hip_attn_decode_qkv_span": (_i32, [_vp, _vp, _vp, ctypes.c_float, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                             _sz, _sz, _sz, _sz, ctypes.c_int64, ctypes.c_int64, ctypes.c_float, _sz,
                                             _sz, _vp, _vp]),
+    "btb_hip_norm_rope_axes": (_i32, [_vp, _vp, _vp, ctypes.c_float, _vp, _vp, _i32, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp,
+                                      _vp, _sz, _sz, _sz, _sz, _sz, ctypes.c_int64, ctypes.c_int64, _i32, _vp]),
+    "btb_hip_attn_shared_floats": (_sz, [_sz, _sz, _sz, _sz, _sz, _sz]),
+    "btb_hip_attn_shared": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, ctypes.c_int64, ctypes.c_int64,
+                                   ctypes.c_float, _sz, _sz, _vp, _vp]),
+    "btb_hip_attn_mass": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz] + [ctypes.c_int64] * 4 +
+                          [ctypes.c_float, _vp]),
+    "btb_hip_kv_evict": (_i32, [_vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp] + [ctypes.c_int64] * 3 + [_sz] * 5 +
+                         [_i32, _i32, _vp, _vp] + [ctypes.c_int64] * 3 + [_vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp]),
     "btb_hip_silu_mul": (_i32, [_vp, _vp, _sz, _sz, _vp]),
     "btb_hip_argmax": (_i32, [_vp, _vp, _sz, _sz, _vp]),
     "btb_hip_publish": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
@@ -1036,6 +1045,160 @@ class HipCard(CardLaunch):
                    _p(cos_t), _p(sin_t), _p(n0), p(depth), p(par), _p(K), _p(V),
                    _p(att), T, Hq, Hk, D, int(K.stride(0)), int(K.stride(1)), float(scale), int(K.shape[1]), S,
                    _p(scratch), _stream())
+
+    # -- a batch over one shared, bounded cache -----------------------------------------------------------------------
+
+    @staticmethod
+    def _cache_views(K: torch.Tensor, V: torch.Tensor, Hk: int, D: int, what: str) -> None:
+        """one layer's keys and values as the operators below take them"""
+        for t in (K, V):
+            if not isinstance(t, _Tensor) or t.dtype is not torch.bfloat16 or not t.is_cuda or t.dim() != 3:
+                raise ValueError(f"[hip] {what}: K and V are bf16 [Hk, cap, D] views on the GPU")
+        if K.shape != V.shape or K.stride() != V.stride() or K.shape[0] != Hk or K.shape[2] != D or K.stride(2) != 1:
+            raise ValueError(f"[hip] {what}: K and V are [{Hk}, cap, {D}] views with the same strides, D contiguous")
+
+    def norm_rope_axes(self, qkv: torch.Tensor, wq: torch.Tensor | None, wk: torch.Tensor | None, eps: float,
+                       cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, axes: torch.Tensor, slots: torch.Tensor,
+                       K: torch.Tensor, V: torch.Tensor, q: torch.Tensor, Hq: int, Hk: int, D: int,
+                       centered: bool = False) -> None:
+        """q / k norm, a rotation by several position axes and the cache write, where a row's slot is not its position: row t
+        stands at pos[a, t] (int32 [A, T]) on axis a, frequency i turns by axis axes[i] (uint8 [D / 2], `rope_axes`), and
+        the new k and v go to cache row slots[t] (int32 [T], distinct; outside the cache: not written). cos / sin:
+        [positions, D] or [positions, D / 2], bf16 or float32. f32 throughout, rounded once."""
+        self._need(qkv, torch.bfloat16, "qkv")
+        self._need(q, torch.bfloat16, "q")
+        for t, what in ((wq, "wq"), (wk, "wk")):
+            if t is not None:
+                self._need(t, torch.bfloat16, what)
+                if t.numel() != D:
+                    raise ValueError(f"[hip] norm_rope_axes: {what} holds {t.numel()} values, head_dim is {D}")
+        if cos.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError("[hip] norm_rope_axes: the tables are bf16 or float32")
+        self._need(cos, cos.dtype, "cos")
+        self._need(sin, cos.dtype, "sin")
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] not in (D, D // 2):
+            raise ValueError(f"[hip] norm_rope_axes: the tables are [positions, {D}] or [positions, {D // 2}]")
+        self._need(pos, torch.int32, "pos")
+        self._need(axes, torch.uint8, "axes")
+        self._need(slots, torch.int32, "slots")
+        self._cache_views(K, V, Hk, D, "norm_rope_axes")
+        T = int(slots.numel())
+        if T < 1 or qkv.numel() != T * (Hq + 2 * Hk) * D or q.numel() != T * Hq * D:
+            raise ValueError("[hip] norm_rope_axes: qkv is [T, (Hq + 2 Hk) D], q [T, Hq D], slots [T]")
+        if pos.dim() != 2 or pos.shape[1] != T or axes.numel() != D // 2:
+            raise ValueError(f"[hip] norm_rope_axes: pos is [axes, {T}], axes names the axis of {D // 2} frequencies")
+        p = lambda t: None if t is None else _p(t)
+        self._call("btb_hip_norm_rope_axes", _p(qkv), p(wq), p(wk), float(eps), _p(cos), _p(sin),
+                   int(cos.dtype is torch.float32), cos.shape[0], cos.shape[1], _p(pos), pos.shape[0], _p(axes), _p(slots),
+                   _p(K), _p(V), _p(q), T, Hq, Hk, D, K.shape[1], K.stride(0), K.stride(1), int(bool(centered)), _stream())
+
+    @staticmethod
+    def shared_layout(off: int, n: int, rows: Sequence[tuple[int, int]], pad_to: int = 0, device: Any = "cuda") -> torch.Tensor:
+        """The layout `attn_shared` reads: int32 [off, n, then (off, n) a row] - the shared prefix's slots, then each row's own.
+        Rows past `rows` up to `pad_to` are padding (length -1), which the kernels skip."""
+        lay = [int(off), int(n)]
+        for o, k in rows:
+            lay += [int(o), int(k)]
+        lay += [0, -1] * max(0, int(pad_to) - len(rows))
+        return torch.tensor(lay, dtype=torch.int32, device=device)
+
+    def attn_shared_scratch(self, T: int, Hq: int, Hk: int, D: int, prefix_cap: int, own_cap: int,
+                            device: Any = "cuda") -> torch.Tensor:
+        """the f32 scratch `attn_shared` leaves its states in, at these sizes"""
+        n = int(self.lib.btb_hip_attn_shared_floats(T, Hq, Hk, D, prefix_cap, own_cap))
+        if n == 0:
+            raise ValueError("[hip] attn_shared takes head_dim 64 or 128 and 1 .. 32 query heads a kv head")
+        return torch.empty(n, dtype=torch.float32, device=device)
+
+    def attn_shared(self, q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, att: torch.Tensor, lay: torch.Tensor, Hq: int,
+                    Hk: int, D: int, scale: float, prefix_cap: int, own_cap: int, scratch: torch.Tensor,
+                    lse: torch.Tensor | None = None) -> None:
+        """att [T, Hq D] = attention of T rows over a prefix they share, read once for all of them, and keys of their own,
+        both as `shared_layout` lays them out in one layer's cache; lse (float32 [T, Hq]): the rows' log-sum-exp. The
+        lengths are read on the device; prefix_cap and own_cap are the most they may be."""
+        self._need(q, torch.bfloat16, "q")
+        self._need(att, torch.bfloat16, "att")
+        self._need(lay, torch.int32, "lay")
+        self._need(scratch, torch.float32, "scratch")
+        self._cache_views(K, V, Hk, D, "attn_shared")
+        T = int(lay.numel()) // 2 - 1
+        if T < 1 or lay.numel() != 2 + 2 * T or q.numel() != T * Hq * D or att.numel() != T * Hq * D:
+            raise ValueError("[hip] attn_shared: the layout holds 2 + 2 T words, q and att are [T, Hq D]")
+        if lse is not None:
+            self._need(lse, torch.float32, "lse")
+            if lse.numel() != T * Hq:
+                raise ValueError(f"[hip] attn_shared: lse holds {lse.numel()} values, the rows have {T * Hq} heads")
+        cap = K.shape[1]
+        if not (0 <= prefix_cap <= cap and 0 <= own_cap <= cap):
+            raise ValueError(f"[hip] attn_shared: the lengths' bounds {prefix_cap} and {own_cap} lie within the cache's {cap} rows")
+        need = self.lib.btb_hip_attn_shared_floats(T, Hq, Hk, D, prefix_cap, own_cap)
+        if scratch.numel() < need:
+            raise ValueError(f"[hip] attn_shared: scratch holds {scratch.numel()} floats, {need} are needed")
+        self._call("btb_hip_attn_shared", _p(q), _p(K), _p(V), _p(att), None if lse is None else _p(lse), _p(lay), T, Hq, Hk, D,
+                   cap, K.stride(0), K.stride(1), float(scale), prefix_cap, own_cap, _p(scratch), _stream())
+
+    def attn_mass(self, q: torch.Tensor, K: torch.Tensor, lse: torch.Tensor, seen: torch.Tensor, mass: torch.Tensor | None,
+                  Hq: int, Hk: int, D: int, scale: float, n: int, out: torch.Tensor | None = None) -> torch.Tensor:
+        """out [Hk, >= n] = mass + the attention weight that each of the first n keys received from the pass's rows q
+        [T, Hq D], row t seeing keys 0 .. seen[t] - 1 (int32 [T]) with log-sum-exp lse (float32 [T, Hq], `attn_shared`'s).
+        mass None: zeros; out None: mass itself."""
+        self._need(q, torch.bfloat16, "q")
+        self._need(lse, torch.float32, "lse")
+        self._need(seen, torch.int32, "seen")
+        self._cache_views(K, K, Hk, D, "attn_mass")
+        if out is None:
+            out = mass if mass is not None else torch.empty(Hk, n, dtype=torch.float32, device=q.device)
+        T = int(seen.numel())
+        if T < 1 or q.numel() != T * Hq * D or lse.numel() != T * Hq:
+            raise ValueError("[hip] attn_mass: q is [T, Hq D], lse [T, Hq], seen [T]")
+        if not 0 < n <= K.shape[1]:
+            raise ValueError(f"[hip] attn_mass: n is 1 .. the cache's {K.shape[1]} rows, got {n}")
+        for t, what in ((mass, "mass"), (out, "out")):
+            if t is not None and (not isinstance(t, _Tensor) or t.dtype is not torch.float32 or not t.is_cuda or t.dim() != 2
+                                  or t.shape[0] != Hk or t.shape[1] < n or t.stride(1) != 1):
+                raise ValueError(f"[hip] attn_mass: {what} is float32 [{Hk}, >= {n}] on the GPU, a head's values together")
+        self._call("btb_hip_attn_mass", _p(q), _p(K), _p(lse), _p(seen), None if mass is None else _p(mass), _p(out), T, Hq, Hk,
+                   D, n, K.stride(0), K.stride(1), 0 if mass is None else mass.stride(0), out.stride(0), float(scale), _stream())
+        return out
+
+    def kv_evict(self, mass: torch.Tensor, pos: torch.Tensor, K: torch.Tensor, V: torch.Tensor, n: int, budget: int,
+                 K_out: torch.Tensor, V_out: torch.Tensor, mass_out: torch.Tensor, pos_out: torch.Tensor, idx: torch.Tensor,
+                 sinks: int = 0, recent_from: int = 0x7FFFFFFF) -> int:
+        """the cache K, V [L, Hk, cap, D] (or one layer's [Hk, cap, D]), n keys a head, cut to its min(n, budget) heaviest by
+        mass (float32 [L, Hk, cap]); keys of position (pos, int32 [L, Hk, cap]) below `sinks` or from `recent_from` on come
+        first. What stays below the new length stays in its slot, the rest fills the slots in between; idx (int32 [L, Hk,
+        kept]): the slot each came from. The outputs may be the inputs. Returns how many keys a head holds now."""
+        four = lambda t: t if t.dim() == 4 else t.unsqueeze(0)
+        three = lambda t: t if t.dim() == 3 else t.unsqueeze(0)
+        for t in (K, V, K_out, V_out):
+            if not isinstance(t, _Tensor) or t.dtype is not torch.bfloat16 or not t.is_cuda or t.dim() not in (3, 4):
+                raise ValueError("[hip] kv_evict: K and V are bf16 [L, Hk, cap, D] views on the GPU")
+        k4, ko = four(K), four(K_out)
+        L, Hk, cap, D = k4.shape
+        kept = min(n, budget)
+        if not 0 < n <= cap or budget < 1:
+            raise ValueError(f"[hip] kv_evict: n is 1 .. the cache's {cap} rows and the budget 1 or more, got {n} and {budget}")
+        if K.shape != V.shape or K.stride() != V.stride() or K_out.shape != V_out.shape or K_out.stride() != V_out.stride() \
+                or k4.stride(3) != 1 or ko.stride(3) != 1:
+            raise ValueError("[hip] kv_evict: K and V have the same strides, and their outputs, with D contiguous")
+        if (ko.shape[0], ko.shape[1], ko.shape[3]) != (L, Hk, D) or ko.shape[2] < kept:
+            raise ValueError(f"[hip] kv_evict: the outputs are [{L}, {Hk}, >= {kept}, {D}]")
+        strides = []
+        for t, dtype, rows, what in ((mass, torch.float32, n, "mass"), (pos, torch.int32, n, "pos"),
+                                     (mass_out, torch.float32, kept, "mass_out"), (pos_out, torch.int32, kept, "pos_out")):
+            if not isinstance(t, _Tensor) or t.dtype is not dtype or not t.is_cuda or t.dim() not in (2, 3):
+                raise ValueError(f"[hip] kv_evict: {what} is a {dtype} tensor [L, Hk, >= {rows}] on the GPU")
+            t = three(t)
+            if t.shape[:2] != (L, Hk) or t.shape[2] < rows or t.stride(2) != 1 or (L > 1 and t.stride(0) != Hk * t.stride(1)):
+                raise ValueError(f"[hip] kv_evict: {what} is [{L}, {Hk}, >= {rows}], its heads evenly apart")
+            strides.append(t.stride(1))
+        self._need(idx, torch.int32, "idx")
+        if idx.numel() != L * Hk * kept:
+            raise ValueError(f"[hip] kv_evict: idx names {idx.numel()} slots, {L * Hk * kept} stay")
+        self._call("btb_hip_kv_evict", _p(mass), strides[0], _p(pos), strides[1], _p(K), _p(V), k4.stride(0), k4.stride(1),
+                   k4.stride(2), L, Hk, D, n, budget, int(sinks), int(recent_from), _p(K_out), _p(V_out), ko.stride(0),
+                   ko.stride(1), ko.stride(2), _p(mass_out), strides[2], _p(pos_out), strides[3], _p(idx), _stream())
+        return kept
 
     def silu_mul(self, gu: torch.Tensor, m: torch.Tensor) -> torch.Tensor:
         self._need(gu, torch.bfloat16, "gu")

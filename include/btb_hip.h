@@ -458,6 +458,59 @@ int32_t btb_hip_attn_decode_qkv_span(const void* qkv, const void* wq, const void
                                      size_t D, int64_t hs, int64_t rs, float scale, size_t cap, size_t S,
                                      float* workspace, void* stream);
 
+/* ---- a batch over one shared, bounded cache -------------------------------------------------------------
+ * Rows whose place in the cache is not their position: no counterpart in the reference. */
+
+/* The q / k norm, a rotation by several position axes and the cache write, in one pass over qkv [T, (Hq + 2 Hk) D] bf16
+ * (q, k, v heads). y = x rstd w (w: 1 + w where `centered`; wq / wk NULL: y = x), then for i < D / 2 with c and s the
+ * values at column i of the tables' row pos[axes[i]][t]:
+ *     out[i] = y[i] c - y[i + D/2] s,  out[i + D/2] = y[i + D/2] c + y[i] s
+ * in f32, rounded to bf16 once (btb_hip_norm_rope_kv rounds the normed value and the first product too). pos: i32 [A, T],
+ * a row's place on each of A axes (a place outside the tables is taken as their first or last row); axes: u8 [D / 2], the
+ * axis that turns each frequency (an axis past A - 1 is A - 1); slots: i32 [T], distinct, the cache rows that the new k and
+ * v go to - a slot outside 0 .. cap - 1 is not written. cos_t / sin_t: [positions] rows `table_stride` values apart,
+ * of which the first D / 2 are read; bf16, or f32 where table_f32 is 1. q [T, Hq D]. K, V: one layer's, `cap` rows a head, strides hs
+ * and rs in values. D 64, 128 or 256; qkv, q, K and V 16-byte aligned, hs and rs multiples of 8. */
+int32_t btb_hip_norm_rope_axes(const void* qkv, const void* wq, const void* wk, float eps, const void* cos_t,
+                               const void* sin_t, int32_t table_f32, size_t positions, size_t table_stride,
+                               const int32_t* pos, size_t A, const uint8_t* axes, const int32_t* slots, void* K, void* V,
+                               void* q, size_t T, size_t Hq, size_t Hk, size_t D, size_t cap, int64_t hs, int64_t rs,
+                               int32_t centered, void* stream);
+
+/* Attention of T rows over a prefix they share and keys of their own: att [T, Hq D] bf16 and, where lse is not NULL, the
+ * rows' log-sum-exp [T, Hq] f32 (natural units, of scale q . k). layout: i32 [2 + 2 T] on the device - the prefix's first
+ * slot and length, then each row's; every row sees the prefix's slots and its own, in any order, without a mask (rows of one
+ * chain name growing stretches of the same slots). A row of own length < 0 is padding, left as it was; a row with no
+ * key at all gets zeros and -inf. prefix_cap and own_cap bound the lengths (a longer stretch is cut there, and at the
+ * cache's `cap` rows): they size the launch and the workspace (btb_hip_attn_shared_floats, this call's own), the lengths
+ * are read on the device. The prefix's keys are read once for all the rows. D 64 or 128, Hq / Hk up to 32, scale > 0; q,
+ * K, V, att and workspace 16-byte aligned, hs and rs multiples of 8. */
+size_t btb_hip_attn_shared_floats(size_t T, size_t Hq, size_t Hk, size_t D, size_t prefix_cap, size_t own_cap);
+int32_t btb_hip_attn_shared(const void* q, const void* K, const void* V, void* att, float* lse, const int32_t* layout,
+                            size_t T, size_t Hq, size_t Hk, size_t D, size_t cap, int64_t hs, int64_t rs, float scale,
+                            size_t prefix_cap, size_t own_cap, float* workspace, void* stream);
+
+/* The attention weight every key received from a pass, added to what it had: for kv head g and key j < n
+ *     out[g][j] = mass[g][j] + sum over rows t with j < seen[t] and g's query heads h of exp(scale q[t][h] . K[g][j] - lse[t][h])
+ * with lse [T, Hq] as btb_hip_attn_shared leaves it (a row whose lse is -inf adds nothing). seen: i32 [T]. mass and out:
+ * f32 rows mass_stride / out_stride apart; mass NULL: zeros; out may be mass. The additions' order is fixed. D 64 or 128,
+ * Hq / Hk up to 32, scale > 0; q and K 16-byte aligned, hs and rs multiples of 8. */
+int32_t btb_hip_attn_mass(const void* q, const void* K, const float* lse, const int32_t* seen, const float* mass, float* out,
+                          size_t T, size_t Hq, size_t Hk, size_t D, size_t n, int64_t hs, int64_t rs, int64_t mass_stride,
+                          int64_t out_stride, float scale, void* stream);
+
+/* A cache of L layers x Hk heads cut to its heaviest keys. Of a head's n keys the first kept = min(n, budget) in the order
+ * (mass descending, slot ascending) stay, where a key with pos < sinks or pos >= recent_from counts as +inf and a NaN as
+ * -inf. Kept keys in slots 0 .. kept - 1 stay there; the others, ascending, fill the slots in between, ascending. K, V, mass
+ * and pos of slot idx[j] go to slot j of the outputs; idx: i32 [L Hk][kept], dense. Strides: ls / hs / rs (lo / ho / ro) of
+ * a layer, head and row of K and V, ms / ps (mo / po) of a head of mass and pos. The outputs may be the inputs, all four
+ * with the same strides (only what moves is then written), or must not overlap them. D a multiple of 8 up to 1024; K and V
+ * 16-byte aligned, their strides multiples of 8. */
+int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t* pos, int64_t ps, const void* K, const void* V,
+                         int64_t ls, int64_t hs, int64_t rs, size_t L, size_t Hk, size_t D, size_t n, size_t budget,
+                         int32_t sinks, int32_t recent_from, void* K_out, void* V_out, int64_t lo, int64_t ho, int64_t ro,
+                         float* mass_out, int64_t mo, int32_t* pos_out, int64_t po, int32_t* idx, void* stream);
+
 /* m [T, I] = bf16(bf16(silu(g)) * u) over gu [T, 2I] (gate then up). Replaces btb_silu_mul
  * (native/cuda/btb_kernels.cu:467-484); the matvec btb_hip_gemv_silu_bf16 folds the same values into its x load. */
 int32_t btb_hip_silu_mul(const void* gu, void* m, size_t T, size_t I, void* stream);
