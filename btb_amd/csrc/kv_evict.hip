@@ -4,8 +4,12 @@
 // idx[j] is the slot that slot j's key comes from. Sources of moved keys lie past every destination, so the same cache may
 // be given as input and output. Attention does not depend on the keys' order; `pos` tells what stood where.
 //
-// Two launches: the choice, a workgroup a head - the mass of the last key that stays by its bits, eight at a time, then
-// the ranks by running counts - and the rows' move, 16 bytes a lane.
+// The choice, then the rows' move, 16 bytes a lane. The choice finds the rank of the last key that stays, eleven, eleven and
+// ten bits at a time from the top (histograms in LDS), counts what stays and then writes the order. A wave takes a stretch of
+// the slots below `kept` and one of those above, so its own running count is all that its keys' order needs, and the waves
+// meet in one scan. A workgroup takes a head of up to 8192 keys alone, ranks in LDS, one launch; a longer one is cut over
+// workgroups of 8192 keys and the rounds are launches (six), since what a key costs is arithmetic: 131072 keys x 32 heads
+// took one workgroup a head 358 us.
 // Bound: memory: mass and pos read, the moved rows read and written.
 
 #include "btb_common.hpp"
@@ -15,15 +19,43 @@
 
 namespace btb {
 
-constexpr int EV_THREADS = 1024;
+constexpr int EV_THREADS = 1024, EV_WAVES = EV_THREADS / 64, EV_BINS = 2048;
+constexpr int EV_KEYS = 8192, EV_PER = EV_KEYS / EV_THREADS;  // keys a workgroup, and a thread
+constexpr int EV_BLOCKS = 1024;                               // workgroups a head: their counts meet in one scan
+
+// what a long head keeps between the launches, in the call's workspace
+struct EvictWork {
+    uint32_t* rank;   // [n]
+    uint32_t* first;  // [blocks][EV_BINS / 2] two counts a word: the first round's histograms
+    int* later;       // [2][EV_BINS]: the later rounds'
+    int* state;       // [4][2]: after a round, the bits found so far and how many keys of them stay
+    int* counts;      // [blocks][4]: above and with the last rank, below slot `kept` and past it
+    int* list;        // [n / 2]: the slots of the kept keys at or past `kept`
+};
+__host__ __device__ inline size_t evict_words(size_t n) {
+    const size_t blocks = (n + EV_KEYS - 1) / EV_KEYS;
+    return n + blocks * (EV_BINS / 2) + 2 * EV_BINS + 8 + 4 * blocks + n / 2;
+}
 
 struct EvictArgs {
     const float* mass;
     const int32_t* pos;
-    int32_t* idx;        // [heads, kept]
-    long long ms, ps;    // values between two heads of mass and of pos
+    int32_t* idx;      // [heads, kept]
+    uint32_t* work;    // [heads][evict_words(n)]
+    long long ms, ps;  // values between two heads of mass and of pos
     int n, kept, sinks, recent_from;
 };
+__device__ __forceinline__ EvictWork work_of(const EvictArgs& p, int head) {
+    const size_t blocks = (p.n + EV_KEYS - 1) / EV_KEYS;
+    EvictWork w;
+    w.rank = p.work + (size_t)head * evict_words(p.n);
+    w.first = w.rank + p.n;
+    w.later = reinterpret_cast<int*>(w.first + blocks * (EV_BINS / 2));
+    w.state = w.later + 2 * EV_BINS;
+    w.counts = w.state + 8;
+    w.list = w.counts + 4 * blocks;
+    return w;
+}
 
 // a key's rank as an unsigned number, larger stays first
 __device__ __forceinline__ uint32_t rank_bits(float m, int pos, int sinks, int recent_from) {
@@ -33,107 +65,319 @@ __device__ __forceinline__ uint32_t rank_bits(float m, int pos, int sinks, int r
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// the sum of v over the threads before this one, and over all, in thread order
-__device__ __forceinline__ int before(int v, int* waves, int& total) {
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    int run = v;
+// One more in the bin of every lane that counts. Many keys share one rank - those that received nothing, those that stay
+// whatever they weigh - and additions to one word wait for one another, so the lanes of two bins a wave are added at once.
+__device__ __forceinline__ void count(int* hist, int bin, bool counts, int lane) {
+    unsigned long long todo = __ballot(counts);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(run, d, WAVE);
-        if (lane >= d) run += o;
+    for (int i = 0; i < 2; ++i) {
+        if (todo == 0) return;
+        const int leader = __builtin_ctzll(todo);
+        const int theirs = __builtin_amdgcn_readlane(bin, leader);
+        const unsigned long long same = __ballot(counts && bin == theirs) & todo;
+        if (lane == leader) atomicAdd(&hist[theirs], __popcll(same));
+        todo &= ~same;
     }
-    if (lane == 63) waves[wv] = run;
-    __syncthreads();
-    int ahead = 0;
-    total = 0;
-    for (int i = 0; i < EV_THREADS / 64; ++i) {
-        if (i < wv) ahead += waves[i];
-        total += waves[i];
-    }
-    __syncthreads();
-    return ahead + run - v;
+    if ((todo >> lane) & 1) atomicAdd(&hist[bin], 1);
+}
+__device__ __forceinline__ int digit(uint32_t r, int round) {
+    return (int)(round == 0 ? r >> 21 : round == 1 ? (r >> 10) & 2047u : r & 1023u);
+}
+// whether a rank has the bits that the rounds before this one found
+__device__ __forceinline__ bool with(uint32_t r, uint32_t last, int round) {
+    return round == 0 || (round == 1 ? (r ^ last) >> 21 == 0 : (r ^ last) >> 10 == 0);
 }
 
+// the sum over the lanes up to this one
+__device__ __forceinline__ int wave_running(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // lane 15 of a row into the next, lane 31 into the upper half
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+// the sum over the threads before this one; `waves` is free again after the caller's next barrier
+__device__ __forceinline__ int before(int v, int* waves, int lane, int wv) {
+    const int run = wave_running(v);
+    if (lane == 63) waves[wv] = run;
+    __syncthreads();
+    const int all = wave_running(lane < EV_WAVES ? waves[lane] : 0);
+    return run - v + (wv > 0 ? __builtin_amdgcn_readlane(all, wv - 1) : 0);
+}
+
+// The bin, from the largest down, in which the count of keys reaches `left`, and how many of that bin that takes: a thread has
+// the counts of bins EV_BINS - 1 - 2 tid and the one below.
+__device__ __forceinline__ void find(int h0, int h1, int& left, uint32_t& bin, int* waves, int* pick, int tid, int lane, int wv) {
+    const int more = before(h0 + h1, waves, lane, wv);
+    if (more < left && more + h0 + h1 >= left) {
+        const bool upper = more + h0 >= left;
+        pick[0] = EV_BINS - 1 - 2 * tid - (upper ? 0 : 1);
+        pick[1] = left - more - (upper ? 0 : h0);
+    }
+    __syncthreads();
+    bin = (uint32_t)pick[0];
+    left = pick[1];
+    __syncthreads();
+}
+
+// keys above the last rank and with it, of a wave's stretch
+__device__ __forceinline__ void tally(uint32_t r, bool in, uint32_t last, int& above, int& same) {
+    above += __popcll(__ballot(in && r > last));
+    same += __popcll(__ballot(in && r == last));
+}
+// whether the lane's key stays: above the last rank, or among the first `left` with it; `ties` counts those so far
+__device__ __forceinline__ bool stays(uint32_t r, bool in, uint32_t last, int left, int& ties, int lane) {
+    const unsigned long long same = __ballot(in && r == last), mine = 1ull << lane;
+    const bool s = in && (r > last || ((same & mine) && ties + __popcll(same & (mine - 1)) < left));
+    ties += __popcll(same);
+    return s;
+}
+__device__ __forceinline__ int lanes_before(unsigned long long set, int lane) { return __popcll(set & ((1ull << lane) - 1)); }
+
+// a wave's share of slots [begin, end), whole groups of 64
+__device__ __forceinline__ void share(int begin, int end, int wv, int& from, int& to) {
+    const int per = ((end - begin + EV_WAVES - 1) / EV_WAVES + 63) / 64 * 64;
+    from = min(begin + wv * per, end);
+    to = min(from + per, end);
+}
+
+// a head of up to EV_KEYS keys
 __global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(EvictArgs p) {
-    __shared__ int hist[256], waves[EV_THREADS / 64], pick[2];
-    const int tid = threadIdx.x;
+    extern __shared__ __align__(16) uint32_t rank[];  // [n], then the list [n / 2]
+    __shared__ int hist[EV_BINS], waves[EV_WAVES], pick[2], counts[2][2][EV_WAVES];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float* mass = p.mass + (size_t)blockIdx.x * p.ms;
     const int32_t* pos = p.pos + (size_t)blockIdx.x * p.ps;
     int32_t* idx = p.idx + (size_t)blockIdx.x * p.kept;
-    auto rank = [&](int j) { return rank_bits(mass[j], pos[j], p.sinks, p.recent_from); };
-    // the rank of the last key that stays, and how many of that rank do
-    uint32_t prefix = 0;
+    uint32_t* list = rank + p.n;
+    uint32_t r[EV_PER];
+#pragma unroll
+    for (int i = 0; i < EV_PER; ++i) {
+        const int j = EV_THREADS * i + tid;
+        r[i] = j < p.n ? rank_bits(mass[j], pos[j], p.sinks, p.recent_from) : 0u;
+        if (j < p.n) rank[j] = r[i];
+    }
+    uint32_t last = 0;
     int left = p.kept;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
+    for (int round = 0; round < 3; ++round) {
+        hist[tid] = hist[tid + EV_THREADS] = 0;
         __syncthreads();
-        for (int j = tid; j < p.n; j += EV_THREADS) {
-            const uint32_t r = rank(j);
-            if (shift == 24 || (r >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(r >> shift) & 255u], 1);
+#pragma unroll
+        for (int i = 0; i < EV_PER; ++i) {
+            if (EV_THREADS * i >= p.n) break;  // uniform
+            count(hist, digit(r[i], round), EV_THREADS * i + tid < p.n && with(r[i], last, round), lane);
         }
         __syncthreads();
-        if (tid == 0) {
-            int b = 255, more = 0;
-            while (b > 0 && more + hist[b] < left) more += hist[b--];
-            pick[0] = b;
-            pick[1] = left - more;
+        uint32_t bin;
+        find(hist[EV_BINS - 1 - 2 * tid], hist[EV_BINS - 2 - 2 * tid], left, bin, waves, pick, tid, lane, wv);
+        last |= bin << (round == 0 ? 21 : round == 1 ? 10 : 0);
+    }
+    int from[2], to[2];
+    share(0, p.kept, wv, from[0], to[0]);
+    share(p.kept, p.n, wv, from[1], to[1]);
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+        int above = 0, same = 0;
+        for (int j0 = from[side]; j0 < to[side]; j0 += 64) {
+            const bool in = j0 + lane < to[side];
+            tally(in ? rank[j0 + lane] : 0u, in, last, above, same);
         }
-        __syncthreads();
-        prefix |= (uint32_t)pick[0] << shift;
-        left = pick[1];
-        __syncthreads();
-    }
-    const uint32_t last = prefix;
-    // of the keys of that rank the first `left` stay
-    auto stays = [&](int j, int end, int& equal) {
-        const uint32_t r = j < end ? rank(j) : 0u;
-        const bool same = j < end && r == last;
-        int all;
-        const int mine = equal + before(same ? 1 : 0, waves, all);
-        equal += all;
-        return j < end && (r > last || (same && mine < left));
-    };
-    int equal = 0;
-    for (int j0 = 0; j0 < p.kept; j0 += EV_THREADS) {
-        int all;
-        const int j = j0 + tid;
-        before(j < p.kept && rank(j) == last ? 1 : 0, waves, all);
-        equal += all;
-    }
-    // the kept keys past the end, in order, into the first places of idx
-    int over = 0;
-    for (int j0 = p.kept; j0 < p.n; j0 += EV_THREADS) {
-        const int j = j0 + tid;
-        const bool s = stays(j, p.n, equal);
-        int all;
-        const int at = over + before(s ? 1 : 0, waves, all);
-        if (s) idx[at] = j;
-        over += all;
+        if (lane == 0) {
+            counts[side][0][wv] = above;
+            counts[side][1][wv] = same;
+        }
     }
     __syncthreads();
-    // from the end on, so that a hole's key is read before its place is written: the i-th hole lies at slot i or later
-    int end = over, tie = 0;
-    for (int j0 = 0; j0 < p.kept; j0 += EV_THREADS) {
-        int all;
-        const int j = j0 + tid;
-        before(j < p.kept && rank(j) == last ? 1 : 0, waves, all);
-        tie += all;
+    // ties ahead of the wave's stretches, holes (below) and movers (past) ahead: a lane a stretch
+    int tie[2], at[2];
+    {
+        const int side = (lane / EV_WAVES) & 1, w = lane % EV_WAVES;
+        int f, t;
+        share(side ? p.kept : 0, side ? p.n : p.kept, w, f, t);
+        const bool live = lane < 2 * EV_WAVES;
+        const int same = live ? counts[side][1][w] : 0;
+        const int ties = wave_running(same) - same;
+        const int stay = live ? counts[side][0][w] + min(max(left - ties, 0), same) : 0;
+        const int holes = live && !side ? t - f - stay : 0, movers = live && side ? stay : 0;
+        const int hole_run = wave_running(holes) - holes, mover_run = wave_running(movers) - movers;
+        tie[0] = __builtin_amdgcn_readlane(ties, wv);
+        tie[1] = __builtin_amdgcn_readlane(ties, EV_WAVES + wv);
+        at[0] = __builtin_amdgcn_readlane(hole_run, wv);
+        at[1] = __builtin_amdgcn_readlane(mover_run, EV_WAVES + wv);
     }
-    for (int j0 = (p.kept - 1) / EV_THREADS * EV_THREADS; j0 >= 0; j0 -= EV_THREADS) {
-        const int j = j0 + tid;
-        const uint32_t r = j < p.kept ? rank(j) : 0u;
-        const bool same = j < p.kept && r == last;
-        int all;
-        const int ahead = before(same ? 1 : 0, waves, all);
-        tie -= all;
-        const bool s = j < p.kept && (r > last || (same && tie + ahead < left));
-        const int holes_ahead = before(j < p.kept && !s ? 1 : 0, waves, all);
-        end -= all;
-        int from = j;
-        if (j < p.kept && !s) from = idx[end + holes_ahead];
+    for (int j0 = from[1]; j0 < to[1]; j0 += 64) {
+        const bool in = j0 + lane < to[1], s = stays(in ? rank[j0 + lane] : 0u, in, last, left, tie[1], lane);
+        const unsigned long long all = __ballot(s);
+        if (s) list[at[1] + lanes_before(all, lane)] = j0 + lane;
+        at[1] += __popcll(all);
+    }
+    __syncthreads();
+    for (int j0 = from[0]; j0 < to[0]; j0 += 64) {
+        const int j = j0 + lane;
+        const bool in = j < to[0], hole = !stays(in ? rank[j] : 0u, in, last, left, tie[0], lane) && in;
+        const unsigned long long all = __ballot(hole);
+        if (in) idx[j] = hole ? (int)list[at[0] + lanes_before(all, lane)] : j;
+        at[0] += __popcll(all);
+    }
+}
+
+// A longer head, a workgroup EV_KEYS of its keys; wave w takes 512 of them in a row. Rounds 0, 1 and 2: this round's histogram,
+// and before it what the last one's says. Round 3: how many keys stay.
+template <int ROUND>
+__global__ void __launch_bounds__(EV_THREADS) evict_round_kernel(EvictArgs p) {
+    __shared__ int hist[EV_BINS], waves[EV_WAVES], pick[2];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), block = blockIdx.x;
+    const EvictWork w = work_of(p, blockIdx.y);
+    const int j0 = block * EV_KEYS + wv * (EV_KEYS / EV_WAVES) + lane;
+    uint32_t r[EV_PER];
+#pragma unroll
+    for (int i = 0; i < EV_PER; ++i) {
+        const int j = j0 + 64 * i;
+        if (ROUND == 0)
+            r[i] = j < p.n ? rank_bits(p.mass[(size_t)blockIdx.y * p.ms + j], p.pos[(size_t)blockIdx.y * p.ps + j], p.sinks,
+                                       p.recent_from)
+                           : 0u;
+        else
+            r[i] = j < p.n ? w.rank[j] : 0u;
+    }
+    hist[tid] = hist[tid + EV_THREADS] = 0;
+    uint32_t last = 0;
+    if constexpr (ROUND > 0) {
+        int left = ROUND == 1 ? p.kept : w.state[2 * (ROUND - 1) + 1];
+        int h0 = 0, h1 = 0;
+        if constexpr (ROUND == 1) {
+            for (int b = 0; b < (int)gridDim.x; ++b) {
+                const uint32_t two = w.first[(size_t)b * (EV_BINS / 2) + EV_BINS / 2 - 1 - tid];
+                h0 += two >> 16;
+                h1 += two & 0xFFFFu;
+            }
+        } else {
+            const int* from = w.later + (ROUND - 2) * EV_BINS;
+            h0 = from[EV_BINS - 1 - 2 * tid];
+            h1 = from[EV_BINS - 2 - 2 * tid];
+        }
+        uint32_t bin;
+        find(h0, h1, left, bin, waves, pick, tid, lane, wv);
+        last = (ROUND == 1 ? 0u : (uint32_t)w.state[2 * (ROUND - 1)]) | bin << (ROUND == 1 ? 21 : ROUND == 2 ? 10 : 0);
+        if (block == 0 && tid == 0) {
+            w.state[2 * ROUND] = (int)last;
+            w.state[2 * ROUND + 1] = left;
+        }
+    }
+    if constexpr (ROUND < 3) {
         __syncthreads();
-        if (j < p.kept) idx[j] = from;
+#pragma unroll
+        for (int i = 0; i < EV_PER; ++i) {
+            const bool in = j0 + 64 * i < p.n;
+            if (ROUND == 0 && in) w.rank[j0 + 64 * i] = r[i];
+            count(hist, digit(r[i], ROUND), in && with(r[i], last, ROUND), lane);
+        }
         __syncthreads();
+        if constexpr (ROUND == 0) {
+            w.first[(size_t)block * (EV_BINS / 2) + tid] = (uint32_t)hist[2 * tid] | (uint32_t)hist[2 * tid + 1] << 16;
+            if (block == 0)
+                for (int i = tid; i < 2 * EV_BINS; i += EV_THREADS) w.later[i] = 0;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int b = tid + EV_THREADS * i;
+                if (hist[b] != 0) atomicAdd(&w.later[(ROUND - 1) * EV_BINS + b], hist[b]);
+            }
+        }
+    } else {
+        int c[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < EV_PER; ++i) {
+            const int j = j0 + 64 * i;
+            tally(r[i], j < min(p.kept, p.n), last, c[0], c[1]);
+            tally(r[i], j >= p.kept && j < p.n, last, c[2], c[3]);
+        }
+        if (lane < 4) hist[4 * wv + lane] = lane == 0 ? c[0] : lane == 1 ? c[1] : lane == 2 ? c[2] : c[3];
+        __syncthreads();
+        if (tid < 4) {
+            int sum = 0;
+            for (int i = 0; i < EV_WAVES; ++i) sum += hist[4 * i + tid];
+            w.counts[4 * block + tid] = sum;
+        }
+    }
+}
+
+// MOVERS: the kept keys past slot `kept` into the list; else the slots below, whose holes take them
+template <bool MOVERS>
+__global__ void __launch_bounds__(EV_THREADS) evict_order_kernel(EvictArgs p, int blocks, int first_block) {
+    __shared__ int waves[EV_WAVES], got[2], tallies[2][EV_WAVES];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int block = blockIdx.x + first_block;
+    const EvictWork w = work_of(p, blockIdx.y);
+    const int begin = max(block * EV_KEYS, MOVERS ? p.kept : 0), end = min(min(block * EV_KEYS + EV_KEYS, p.n), MOVERS ? p.n : p.kept);
+    const int j0 = block * EV_KEYS + wv * (EV_KEYS / EV_WAVES) + lane;
+    uint32_t r[EV_PER];
+#pragma unroll
+    for (int i = 0; i < EV_PER; ++i) r[i] = j0 + 64 * i < p.n ? w.rank[j0 + 64 * i] : 0u;
+    const uint32_t last = (uint32_t)w.state[6];
+    const int left = w.state[7];
+    // ties ahead of this workgroup's stretch - the slots below `kept` come first - and holes or movers ahead
+    int low[2] = {0, 0}, high[2] = {0, 0};
+    if (tid < blocks) {
+        low[0] = w.counts[4 * tid];
+        low[1] = w.counts[4 * tid + 1];
+        high[0] = w.counts[4 * tid + 2];
+        high[1] = w.counts[4 * tid + 3];
+    }
+    const int low_ties = before(low[1], waves, lane, wv);
+    if (tid == EV_THREADS - 1) got[0] = low_ties + low[1];
+    __syncthreads();
+    const int all_low = got[0];
+    int ties = low_ties, stay = low[0] + min(max(left - ties, 0), low[1]);
+    int units = tid < blocks ? max(min(tid * EV_KEYS + EV_KEYS, p.kept) - tid * EV_KEYS, 0) - stay : 0;  // holes
+    if (MOVERS) {
+        ties = all_low + before(high[1], waves, lane, wv);
+        units = high[0] + min(max(left - ties, 0), high[1]);
+        __syncthreads();
+    }
+    const int ahead = before(units, waves, lane, wv);
+    if (tid == block) {
+        got[0] = ties;
+        got[1] = ahead;
+    }
+    // and ahead of the wave's own within the workgroup
+    int above = 0, same = 0;
+#pragma unroll
+    for (int i = 0; i < EV_PER; ++i) {
+        const int j = j0 + 64 * i;
+        tally(r[i], j >= begin && j < end, last, above, same);
+    }
+    if (lane == 0) {
+        tallies[0][wv] = above;
+        tallies[1][wv] = same;
+    }
+    __syncthreads();
+    const int base_ties = got[0], base_units = got[1];
+    int tie, at;
+    {
+        const bool live = lane < EV_WAVES;
+        const int mine = live ? tallies[1][lane] : 0, f = block * EV_KEYS + lane * (EV_KEYS / EV_WAVES);
+        const int t = base_ties + wave_running(mine) - mine;
+        const int st = live ? tallies[0][lane] + min(max(left - t, 0), mine) : 0;
+        const int length = live ? max(min(f + EV_KEYS / EV_WAVES, end) - max(f, begin), 0) : 0;
+        const int u = MOVERS ? st : length - st;
+        tie = __builtin_amdgcn_readlane(t, wv);
+        at = base_units + __builtin_amdgcn_readlane(wave_running(u) - u, wv);
+    }
+#pragma unroll
+    for (int i = 0; i < EV_PER; ++i) {
+        const int j = j0 + 64 * i;
+        const bool in = j >= begin && j < end, s = stays(r[i], in, last, left, tie, lane);
+        const unsigned long long all = __ballot(MOVERS ? s : in && !s);
+        const int place = at + lanes_before(all, lane);
+        if (MOVERS) {
+            if (s) w.list[place] = j;
+        } else if (in) {
+            p.idx[(size_t)blockIdx.y * p.kept + j] = s ? j : w.list[place];
+        }
+        at += __popcll(all);
     }
 }
 
@@ -149,46 +393,70 @@ struct MoveArgs {
     const int32_t* idx;
     long long ls, hs, rs, lo, ho, ro;  // strides of the layers, heads and rows, in and out
     long long ms, ps, mo, po;
-    int Hk, kept, chunks;  // 16-byte chunks a row
-    int in_place;
+    int Hk, kept, in_place;
 };
 
+// a workgroup takes EV_MOVE rows, a thread 16 bytes of some of them: all of its loads before its first store
+constexpr int EV_MOVE = 64;
+
+template <int CHUNKS>
 __global__ void __launch_bounds__(256) evict_move_kernel(MoveArgs p) {
-    const int head = blockIdx.y, layer = head / p.Hk, g = head % p.Hk;
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int j = (int)(at / p.chunks), c = (int)(at % p.chunks);
-    if (j >= p.kept) return;
-    const int from = p.idx[(size_t)head * p.kept + j];
-    if (p.in_place && from == j) return;
-    const size_t src = (size_t)layer * p.ls + (size_t)g * p.hs + (size_t)from * p.rs + 8 * c;
-    const size_t dst = (size_t)layer * p.lo + (size_t)g * p.ho + (size_t)j * p.ro + 8 * c;
-    *reinterpret_cast<uint4*>(p.K_out + dst) = *reinterpret_cast<const uint4*>(p.K + src);
-    *reinterpret_cast<uint4*>(p.V_out + dst) = *reinterpret_cast<const uint4*>(p.V + src);
-    if (c == 0) {
-        p.mass_out[(size_t)head * p.mo + j] = p.mass[(size_t)head * p.ms + from];
-        p.pos_out[(size_t)head * p.po + j] = p.pos[(size_t)head * p.ps + from];
+    constexpr int STEP = 256 / CHUNKS, ROWS = EV_MOVE / STEP;  // rows at a time, and a thread's
+    const int head = blockIdx.y, layer = head / p.Hk, g = head % p.Hk, c = threadIdx.x % CHUNKS;
+    const int j0 = blockIdx.x * EV_MOVE + threadIdx.x / CHUNKS;
+    const size_t src = (size_t)layer * p.ls + (size_t)g * p.hs + 8 * c, dst = (size_t)layer * p.lo + (size_t)g * p.ho + 8 * c;
+    const int32_t* idx = p.idx + (size_t)head * p.kept;
+    int from[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int j = j0 + STEP * i;
+        from[i] = j < p.kept ? idx[j] : -1;
+        if (p.in_place && from[i] == j) from[i] = -1;
     }
+    uint4 k[ROWS], v[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+        if (from[i] >= 0) {
+            k[i] = load_stream16(reinterpret_cast<const uint4*>(p.K + src + (size_t)from[i] * p.rs));
+            v[i] = load_stream16(reinterpret_cast<const uint4*>(p.V + src + (size_t)from[i] * p.rs));
+        }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+        if (from[i] >= 0) {
+            const int j = j0 + STEP * i;
+            *reinterpret_cast<uint4*>(p.K_out + dst + (size_t)j * p.ro) = k[i];
+            *reinterpret_cast<uint4*>(p.V_out + dst + (size_t)j * p.ro) = v[i];
+            if (c == 0) {
+                p.mass_out[(size_t)head * p.mo + j] = p.mass[(size_t)head * p.ms + from[i]];
+                p.pos_out[(size_t)head * p.po + j] = p.pos[(size_t)head * p.ps + from[i]];
+            }
+        }
 }
 
 }  // namespace btb
 
 using namespace btb;
 
+extern "C" size_t btb_hip_kv_evict_words(size_t L, size_t Hk, size_t n) {
+    return n <= (size_t)EV_KEYS ? 0 : L * Hk * evict_words(n);
+}
+
 extern "C" int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t* pos, int64_t ps, const void* K, const void* V,
                                     int64_t ls, int64_t hs, int64_t rs, size_t L, size_t Hk, size_t D, size_t n, size_t budget,
                                     int32_t sinks, int32_t recent_from, void* K_out, void* V_out, int64_t lo, int64_t ho,
                                     int64_t ro, float* mass_out, int64_t mo, int32_t* pos_out, int64_t po, int32_t* idx,
-                                    void* stream) {
+                                    uint32_t* workspace, void* stream) {
     if (!mass || !pos || !K || !V || !K_out || !V_out || !mass_out || !pos_out || !idx) return ERR_NULL;
+    if (workspace == nullptr && btb_hip_kv_evict_words(1, 1, n) != 0) return ERR_NULL;
     auto loose = [](const void* a) { return ((uintptr_t)a & 15u) != 0; };
     auto odd = [](int64_t s) { return s < 0 || s % 8 != 0; };
     const bool in_place = K == K_out;
-    if (L == 0 || Hk == 0 || L > 65535 || Hk > 65535 || L * Hk > 65535 || D == 0 || D % 8 || D > 1024 || n == 0 ||
-        n > 0x7FFFF000u || budget == 0 || ms < 0 || ps < 0 || mo < 0 || po < 0 || odd(ls) || odd(hs) || odd(rs) || odd(lo) ||
+    if (L == 0 || Hk == 0 || L > 65535 || Hk > 65535 || L * Hk > 65535 || (D != 64 && D != 128 && D != 256) || n == 0 ||
+        n > (size_t)EV_KEYS * EV_BLOCKS || budget == 0 || ms < 0 || ps < 0 || mo < 0 || po < 0 || odd(ls) || odd(hs) || odd(rs) || odd(lo) ||
         odd(ho) || odd(ro) || loose(K) || loose(V) || loose(K_out) || loose(V_out) || in_place != (V == V_out) ||
         in_place != (mass == mass_out) || in_place != (pos == pos_out) ||
         (in_place && (ls != lo || hs != ho || rs != ro || ms != mo || ps != po))) {
-        set_error("kv_evict: at most 65535 heads in all, head_dim a multiple of 8, K and V 16-byte aligned with strides in "
+        set_error("kv_evict: at most 65535 heads in all of at most 2^23 keys, head_dim 64, 128 or 256, K and V 16-byte aligned with strides in "
                   "multiples of 8; in place: all four outputs the inputs with their strides, or none");
         return ERR_DOMAIN;
     }
@@ -203,7 +471,22 @@ extern "C" int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t
     e.sinks = sinks;
     e.recent_from = recent_from;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(evict_choose_kernel, dim3((unsigned)(L * Hk)), dim3(EV_THREADS), 0, st, e);
+    e.work = workspace;
+    const unsigned heads = (unsigned)(L * Hk);
+    if (n <= (size_t)EV_KEYS) {
+        hipLaunchKernelGGL(evict_choose_kernel, dim3(heads), dim3(EV_THREADS), 4 * (n + n / 2), st, e);
+    } else {
+        const int blocks = (int)((n + EV_KEYS - 1) / EV_KEYS), below = (e.kept + EV_KEYS - 1) / EV_KEYS;
+        const dim3 grid((unsigned)blocks, heads), threads(EV_THREADS);
+        hipLaunchKernelGGL(evict_round_kernel<0>, grid, threads, 0, st, e);
+        hipLaunchKernelGGL(evict_round_kernel<1>, grid, threads, 0, st, e);
+        hipLaunchKernelGGL(evict_round_kernel<2>, grid, threads, 0, st, e);
+        hipLaunchKernelGGL(evict_round_kernel<3>, grid, threads, 0, st, e);
+        if (e.kept < e.n)
+            hipLaunchKernelGGL(evict_order_kernel<true>, dim3((unsigned)(blocks - e.kept / EV_KEYS), heads), threads, 0, st, e,
+                               blocks, e.kept / EV_KEYS);
+        hipLaunchKernelGGL(evict_order_kernel<false>, dim3((unsigned)below, heads), threads, 0, st, e, blocks, 0);
+    }
     MoveArgs m;
     m.K = static_cast<const uint16_t*>(K);
     m.V = static_cast<const uint16_t*>(V);
@@ -226,9 +509,13 @@ extern "C" int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t
     m.po = po;
     m.Hk = (int)Hk;
     m.kept = e.kept;
-    m.chunks = (int)(D / 8);
     m.in_place = in_place ? 1 : 0;
-    const unsigned blocks = (unsigned)(((size_t)e.kept * m.chunks + 255) / 256);
-    hipLaunchKernelGGL(evict_move_kernel, dim3(blocks, (unsigned)(L * Hk)), dim3(256), 0, st, m);
+    const dim3 grid((unsigned)((e.kept + EV_MOVE - 1) / EV_MOVE), (unsigned)(L * Hk));
+    if (D == 64)
+        hipLaunchKernelGGL(evict_move_kernel<8>, grid, dim3(256), 0, st, m);
+    else if (D == 128)
+        hipLaunchKernelGGL(evict_move_kernel<16>, grid, dim3(256), 0, st, m);
+    else
+        hipLaunchKernelGGL(evict_move_kernel<32>, grid, dim3(256), 0, st, m);
     return hip_status(hipGetLastError(), "kv_evict launch");
 }

@@ -116,7 +116,8 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "btb_hip_attn_mass": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz] + [ctypes.c_int64] * 4 +
                           [ctypes.c_float, _vp]),
     "btb_hip_kv_evict": (_i32, [_vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp] + [ctypes.c_int64] * 3 + [_sz] * 5 +
-                         [_i32, _i32, _vp, _vp] + [ctypes.c_int64] * 3 + [_vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp]),
+                         [_i32, _i32, _vp, _vp] + [ctypes.c_int64] * 3 + [_vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp, _vp]),
+    "btb_hip_kv_evict_words": (_sz, [_sz, _sz, _sz]),
     "btb_hip_silu_mul": (_i32, [_vp, _vp, _sz, _sz, _vp]),
     "btb_hip_argmax": (_i32, [_vp, _vp, _sz, _sz, _vp]),
     "btb_hip_publish": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
@@ -1195,9 +1196,12 @@ class HipCard(CardLaunch):
         self._need(idx, torch.int32, "idx")
         if idx.numel() != L * Hk * kept:
             raise ValueError(f"[hip] kv_evict: idx names {idx.numel()} slots, {L * Hk * kept} stay")
+        words = self.lib.btb_hip_kv_evict_words(L, Hk, n)
+        ws = torch.empty(words, dtype=torch.int32, device=K.device) if words else None
         self._call("btb_hip_kv_evict", _p(mass), strides[0], _p(pos), strides[1], _p(K), _p(V), k4.stride(0), k4.stride(1),
                    k4.stride(2), L, Hk, D, n, budget, int(sinks), int(recent_from), _p(K_out), _p(V_out), ko.stride(0),
-                   ko.stride(1), ko.stride(2), _p(mass_out), strides[2], _p(pos_out), strides[3], _p(idx), _stream())
+                   ko.stride(1), ko.stride(2), _p(mass_out), strides[2], _p(pos_out), strides[3], _p(idx),
+                   None if ws is None else _p(ws), _stream())
         return kept
 
     def silu_mul(self, gu: torch.Tensor, m: torch.Tensor) -> torch.Tensor:
