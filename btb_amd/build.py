@@ -40,6 +40,14 @@ HIPCC_FLAGS = [
     "-Wno-unused-function",
 ]
 
+# Files whose matrix-core results are worked on between products (a softmax's weights, outputs that move to a new maximum):
+# the products write ordinary registers. Left to itself the compiler keeps them in the accumulation registers and copies all
+# of them out and back where a branch may touch them, 256 moves a tile of keys.
+FILE_FLAGS = {
+    "attn_shared.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "attn_mass.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+}
+
 
 def hipcc() -> str:
     for cand in (shutil.which("hipcc"), "/opt/rocm/bin/hipcc"):
@@ -65,7 +73,7 @@ def _compile(src: str, incremental: bool = False) -> str:
     obj = os.path.join(OBJ, os.path.basename(src)[:-4] + ".o")
     if incremental and _fresh(src, obj):
         return obj
-    cmd = [hipcc(), *HIPCC_FLAGS, "-c", src, "-o", obj]
+    cmd = [hipcc(), *HIPCC_FLAGS, *FILE_FLAGS.get(os.path.basename(src), []), "-c", src, "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
     noise = "is not a recognized feature for this target"
     err = "\n".join(ln for ln in r.stderr.splitlines() if noise not in ln)

@@ -35,7 +35,7 @@ struct SharedArgs {
     float scale_log2;
     int T, Hq, Hk, G, cap, prefix_cap, own_cap;
     int pair_tiles, prefix_spans, own_spans;  // workgroups: Hk x pair_tiles x prefix_spans, then Hk x T x own_spans
-    int prefix_states, states;                // states a (row, head): of the prefix, in all
+    int states;                               // states a (row, head)
 };
 
 struct Keys {
@@ -46,6 +46,8 @@ __device__ __forceinline__ Keys stretch(int off, int len, int most, int cap) {
     Keys k;
     k.first = min(max(off, 0), cap);
     k.count = off < 0 ? 0 : min(max(len, 0), min(most, cap - k.first));
+    k.first = __builtin_amdgcn_readfirstlane(k.first);
+    k.count = __builtin_amdgcn_readfirstlane(k.count);
     return k;
 }
 // part `i` of `parts` of a stretch, in whole stages
@@ -58,127 +60,246 @@ __device__ __forceinline__ Keys part_of(const Keys& k, int i, int parts) {
     return r;
 }
 
-// one wave's 32 pairs against its keys of a stretch. ALL: every key of the stretch, else the wave's tile of each stage.
-// `row(c)`: the q row of pair c; `state(c)`: where pair c's state goes, negative: nowhere.
-template <int D, bool ALL, class Row, class State>
+// A workgroup's pairs against a stretch of keys. QW waves take 32 pairs each, KW = 4 / QW of them share the same pairs and
+// divide a stage's four tiles. Every wave brings one tile of K and one of V into LDS a stage. K's is asked for again as soon as
+// the scores are made and V's as soon as the outputs are, so each travels while the other product and the softmax run, and one
+// buffer of each does: 64 KB, two workgroups a CU, whose products and exponentials run beside one another's. Where waves read
+// one another's tiles (QW > 1) a stage costs four barriers, else none. `row(r)`: the q row of the workgroup's pair r;
+// `state(r)`: where its state goes, negative: nowhere.
+template <int D, int QW, class Row, class State>
 __device__ __forceinline__ void walk(const SharedArgs& p, const uint16_t* Kg, const uint16_t* Vg, const Keys& keys, uint8_t* lds,
-                                     Row row, State state) {
-    constexpr int STEPS = D / 16, DT = D / 32, TILE = TK * 2 * D, REGS = TILE / 1024;
+                                     float* meet, Row row, State state) {
+    constexpr int STEPS = D / 16, DT = D / 32, TILE = TK * 2 * D, KW = 4 / QW, TPW = QW, PAIRS = 32 * QW;
+    constexpr int N = TileLoads<D>::N;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = lane & 31, h = lane >> 5;
+    const int c = lane & 31, h = lane >> 5, qw = wv / KW, kw = wv % KW;
     const float ninf = bits_f32(0xff800000u);
+    TileLoads<D> loads;
+    loads.make(p.rs, lane);
+    const uint16_t* Kb = Kg + (size_t)keys.first * p.rs;
+    const uint16_t* Vb = Vg + (size_t)keys.first * p.rs;
+    // the wave's tile of the stage that starts at key kb (a tile wholly past the end: the last key)
+    auto issue_k = [&](int kb) {
+        const int k0 = min(kb + TK * wv, keys.count - 1);
+        loads.template issue<true>(Kb + (size_t)k0 * p.rs, p.rs, keys.count - k0, lds + wv * TILE, lane);
+    };
+    auto issue_v = [&](int kb) {
+        const int k0 = min(kb + TK * wv, keys.count - 1);
+        loads.template issue<false>(Vb + (size_t)k0 * p.rs, p.rs, keys.count - k0, lds + (4 + wv) * TILE, lane);
+    };
+    auto barrier = [&] {
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (QW > 1) asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    f32x16 o[DT];
+    float m = ninf, l = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = zero16();
     bf16x8 qf[STEPS];
     {
-        const uint16_t* qr = row(c) + 8 * h;
+        const uint16_t* qr = row(32 * qw + c) + 8 * h;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) qf[s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(qr + 16 * s));
     }
-    f32x16 o[DT];
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): q is here, and no register of the loop waits for a load
+    __builtin_amdgcn_sched_barrier(0);
+    if (keys.count > 0) {
+        issue_k(0);
+        issue_v(0);
+    }
+    // the wave's tiles of a stage in groups of at most two: a group's scores are made while the one before is weighed
+    constexpr int GT = TPW < 2 ? TPW : 2, GROUPS = TPW / GT;
+    f32x16 st[GT];
+    bf16x8 pf[GT][2];
+    auto scores = [&](const uint8_t* k_lds, int group, f32x16(&to)[GT]) {
 #pragma unroll
-    for (int d = 0; d < DT; ++d) o[d] = zero16();
-    float m = ninf, l = 0.f;
-    uint8_t* k_lds = lds;
-    uint8_t* v_lds = lds + 4 * TILE;
-    for (int kb = 0; kb < keys.count; kb += SH_KEYS) {
-        // the wave's tile of the stage, keys past the end as zeros
-        __syncthreads();
+        for (int j = 0; j < GT; ++j) {
+            const uint8_t* tile = k_lds + (kw + KW * (GT * group + j)) * TILE;
+            to[j] = zero16();
 #pragma unroll
-        for (int i = 0; i < REGS; ++i) {
-            const int at = i * 64 + lane, key = at / (D / 8), chunk = at % (D / 8), j = kb + TK * wv + key;
-            uint4 kw = make_uint4(0u, 0u, 0u, 0u), vw = kw;
-            if (j < keys.count) {
-                const size_t from = (size_t)(keys.first + j) * p.rs + 8 * chunk;
-                kw = *reinterpret_cast<const uint4*>(Kg + from);
-                vw = *reinterpret_cast<const uint4*>(Vg + from);
-            }
-            *reinterpret_cast<uint4*>(k_lds + wv * TILE + key * 2 * D + 16 * k_chunk<D>(key, chunk)) = kw;
-            *reinterpret_cast<uint4*>(v_lds + wv * TILE + key * 2 * D + 16 * v_chunk(key, chunk)) = vw;
+            for (int i = 0; i < STEPS; ++i) to[j] = mfma32(k_fragment<D>(tile, i, lane), qf[i], to[j]);
         }
-        __syncthreads();
-#pragma unroll 1
-        for (int s = ALL ? 0 : wv; s < (ALL ? 4 : wv + 1); ++s) {
-            const int left = keys.count - kb - TK * s;  // keys of this tile
-            if (left <= 0) break;
-            f32x16 st = zero16();
+    };
+    // keys past the end; the group's maximum; the state moved to it where it has to be
+    auto settle = [&](int kb, bool more, int group) {
+        if (!more) {
 #pragma unroll
-            for (int i = 0; i < STEPS; ++i) st = mfma32(k_fragment<D>(k_lds + s * TILE, i, lane), qf[i], st);
-            float w[16];
-            float top = ninf;
+            for (int j = 0; j < GT; ++j) {
+                const int left = keys.count - kb - TK * (kw + KW * (GT * group + j));
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                w[i] = 8 * (i / 4) + 4 * h + i % 4 < left ? st[i] * p.scale_log2 : ninf;
-                top = fmaxf(top, w[i]);
+                for (int i = 0; i < 16; ++i)
+                    if (8 * (i / 4) + 4 * h + i % 4 >= left) st[j][i] = ninf;
             }
-            top = fmaxf(top, xor32(top));
-            const float mn = fmaxf(m, top);
+        }
+        float top = st[0][0];
+#pragma unroll
+        for (int j = 0; j < GT; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, st[j][i]);
+        top = fmaxf(top, xor32(top)) * p.scale_log2;
+        // The state moves to a new maximum only where that is 2^8 past its own: weights of up to 2^8 are as exact, and most
+        // groups then leave the outputs alone. A pair's decision is its own, whatever its neighbours'.
+        const bool moves = top > m + 8.f || m == ninf;
+        if (__any(moves)) {
+            const float mn = moves ? top : m;
             const float corr = m == ninf ? 0.f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                w[i] = w[i] == ninf ? 0.f : __builtin_amdgcn_exp2f(w[i] - mn);
-                sum += w[i];
-            }
-            l = fmaf(l, corr, sum);
+            l *= corr;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= corr;
+        }
+    };
+    auto weigh = [&] {
+        const float ref = m == ninf ? 0.f : m;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const bf16x8 pf = weight_fragment(w + 8 * u);
+        for (int j = 0; j < GT; ++j) {
+            float w[16], sum = 0.f;
 #pragma unroll
-                for (int d = 0; d < DT; ++d) o[d] = mfma32(v_fragment<D>(v_lds + s * TILE, d, u, lane), pf, o[d]);
+            for (int i = 0; i < 16; ++i) {
+                w[i] = __builtin_amdgcn_exp2f(fmaf(st[j][i], p.scale_log2, -ref));
+                sum += w[i];
             }
+            l += sum;
+            pf[j][0] = weight_fragment(w);
+            pf[j][1] = weight_fragment(w + 8);
+        }
+    };
+    auto outputs = [&](const uint8_t* v_lds, int group) {
+#pragma unroll
+        for (int j = 0; j < GT; ++j) {
+            const uint8_t* tile = v_lds + (kw + KW * (GT * group + j)) * TILE;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[d] = mfma32(v_fragment<D>(tile, d, u, lane), pf[j][u], o[d]);
+        }
+    };
+    for (int kb = 0; kb < keys.count; kb += SH_KEYS) {
+        const bool more = kb + SH_KEYS < keys.count;
+        uint32_t ak = 0, av = 4 * TILE;
+        wait_loads<N>(ak);
+        barrier();
+        scores(lds + ak, 0, st);
+        settle(kb, more, 0);
+        f32x16 next[GT];
+        if constexpr (GROUPS > 1) scores(lds + ak, 1, next);
+        weigh();
+        barrier();
+        if (more) {
+            issue_k(kb + SH_KEYS);
+            wait_loads<N>(av);
+        } else {
+            wait_loads<0>(av);
+            const int mine = keys.count - kb - TK * wv;
+            if (mine < TK) TileLoads<D>::clear_past(lds + av + wv * TILE, mine, lane);
+            if constexpr (QW > 1) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+        barrier();
+        outputs(lds + av, 0);
+        if constexpr (GROUPS > 1) {
+#pragma unroll
+            for (int j = 0; j < GT; ++j) st[j] = next[j];
+            settle(kb, more, 1);
+            weigh();
+            outputs(lds + av, 1);
+        }
+        barrier();
+        if (more) issue_v(kb + SH_KEYS);
+    }
+    // the waves of the same pairs meet: their maxima and sums, then their outputs, through the stage's LDS
+    float* mm = meet;  // [4][32] maxima, then sums
+    float* ml = meet + 4 * 32;
+    l += xor32(l);
+    if (h == 0) {
+        mm[wv * 32 + c] = m;
+        ml[wv * 32 + c] = l;
+    }
+    __syncthreads();
+    float* all = reinterpret_cast<float*>(lds);  // [4 waves][32 pairs][D], a pair's 16-byte chunks permuted
+    {
+        float top = ninf;
+#pragma unroll
+        for (int i = 0; i < KW; ++i) top = fmaxf(top, mm[(qw * KW + i) * 32 + c]);
+        const float f = m == ninf ? 0.f : __builtin_amdgcn_exp2f(m - top);
+        float* dst = all + (size_t)(wv * 32 + c) * D;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                float4 v = make_float4(o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]);
+                if (KW > 1 && m == ninf) v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (KW > 1) v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+                *reinterpret_cast<float4*>(dst + 4 * ((8 * d + 2 * b + h) ^ (c & (D / 4 - 1)))) = v;
+            }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < PAIRS * (D / 4); e += 256) {
+        const int r = e / (D / 4), chunk = e % (D / 4), group = r / 32, in = r % 32;
+        const long long to = state(r);
+        if (to < 0) continue;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < KW; ++i) {
+            const float4 x =
+                *reinterpret_cast<const float4*>(all + (size_t)((group * KW + i) * 32 + in) * D + 4 * (chunk ^ (in & (D / 4 - 1))));
+            v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+        }
+        *reinterpret_cast<float4*>(p.part_acc + (size_t)to * D + 4 * chunk) = v;
+        if (chunk == 0) {
+            float top = ninf, sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < KW; ++i) top = fmaxf(top, mm[(group * KW + i) * 32 + in]);
+#pragma unroll
+            for (int i = 0; i < KW; ++i) {
+                const float mw = mm[(group * KW + i) * 32 + in];
+                sum = fmaf(mw == ninf ? 0.f : __builtin_amdgcn_exp2f(mw - top), ml[(group * KW + i) * 32 + in], sum);
+            }
+            p.part_m[to] = top;
+            p.part_l[to] = sum;
         }
     }
-    l += xor32(l);
-    const long long at = state(c);
-    if (at < 0) return;
-    if (h == 0) {
-        p.part_m[at] = m;
-        p.part_l[at] = l;
-    }
-    if (m == ninf) return;  // nothing seen (or nothing that is a number, which the sum says): the fold does not read the output
-    float* dst = p.part_acc + (size_t)at * D + 4 * h;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-            *reinterpret_cast<float4*>(dst + 32 * d + 8 * b) = make_float4(o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]);
 }
 
-// MANY: a prefix workgroup takes 128 pairs, 32 a wave; else 32, every wave the same and a quarter of the keys
-template <int D, bool MANY>
+// The prefix's workgroups and the rows' own are dealt in turn, so that what the matrix cores bound and what memory bounds run
+// side by side; eight neighbours at a time, one a die, so that the workgroups that read the same keys for other pairs are
+// on one die together.
+template <int D, int QW>
 __global__ void __launch_bounds__(256, 2) attn_shared_kernel(SharedArgs p) {
-    __shared__ __align__(16) uint8_t lds[8 * TK * 2 * D];
-    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int pairs = p.T * p.G, prefix_wgs = p.Hk * p.pair_tiles * p.prefix_spans;
-    int id = blockIdx.x;
-    if (id < prefix_wgs) {
-        const int g = id % p.Hk, sp = id / p.Hk % p.prefix_spans, tile = id / (p.Hk * p.prefix_spans);
+    extern __shared__ __align__(16) uint8_t lds[];  // a stage
+    __shared__ float meet[2 * 4 * 32];
+    const int pairs = p.T * p.G;
+    const int prefix = p.Hk * p.pair_tiles * p.prefix_spans, own = p.Hk * p.T * p.own_spans;
+    const long long pe = (prefix + 7) / 8, all = pe + (own + 7) / 8, oct = blockIdx.x / 8;
+    const int ahead = (int)(oct * pe / all);  // the prefix's octets before this one
+    if ((int)((oct + 1) * pe / all) > ahead) {
+        const int id = 8 * ahead + blockIdx.x % 8;
+        if (id >= prefix) return;
+        const int g = id % p.Hk, tile = id / p.Hk % p.pair_tiles, sp = id / (p.Hk * p.pair_tiles);
         const Keys keys = part_of(stretch(p.lay[0], p.lay[1], p.prefix_cap, p.cap), sp, p.prefix_spans);
-        const int r0 = MANY ? 128 * tile + 32 * wv : 0;
-        auto row = [&](int c) {
-            const int r = min(r0 + c, pairs - 1), t = r / p.G;
+        const int r0 = 32 * QW * tile;
+        auto row = [&](int i) {
+            const int r = min(r0 + i, pairs - 1), t = r / p.G;
             return p.q + ((size_t)t * p.Hq + g * p.G + (r - t * p.G)) * D;
         };
-        auto state = [&](int c) -> long long {
-            const int r = r0 + c, t = r / p.G;
-            if (r >= pairs) return -1;
-            return ((long long)t * p.Hq + g * p.G + (r - t * p.G)) * p.states + (MANY ? sp : 4 * sp + wv);
+        auto state = [&](int i) -> long long {
+            const int r = r0 + i, t = r / p.G;
+            return r < pairs ? ((long long)t * p.Hq + g * p.G + (r - t * p.G)) * p.states + sp : -1;
         };
-        walk<D, MANY>(p, p.K + (size_t)g * p.hs, p.V + (size_t)g * p.hs, keys, lds, row, state);
+        walk<D, QW>(p, p.K + (size_t)g * p.hs, p.V + (size_t)g * p.hs, keys, lds, meet, row, state);
         return;
     }
-    id -= prefix_wgs;
+    const int id = 8 * (int)(oct - ahead) + blockIdx.x % 8;
+    if (id >= own) return;
     const int g = id % p.Hk, t = id / p.Hk % p.T, sp = id / (p.Hk * p.T);
     const Keys keys = part_of(stretch(p.lay[2 + 2 * t], p.lay[3 + 2 * t], p.own_cap, p.cap), sp, p.own_spans);
-    auto row = [&](int c) { return p.q + ((size_t)t * p.Hq + g * p.G + min(c, p.G - 1)) * D; };
-    auto state = [&](int c) -> long long {
-        return c < p.G ? ((long long)t * p.Hq + g * p.G + c) * p.states + p.prefix_states + 4 * sp + wv : -1;
+    auto row = [&](int i) { return p.q + ((size_t)t * p.Hq + g * p.G + min(i, p.G - 1)) * D; };
+    auto state = [&](int i) -> long long {
+        return i < p.G ? ((long long)t * p.Hq + g * p.G + i) * p.states + p.prefix_spans + sp : -1;
     };
-    walk<D, false>(p, p.K + (size_t)g * p.hs, p.V + (size_t)g * p.hs, keys, lds, row, state);
+    walk<D, 1>(p, p.K + (size_t)g * p.hs, p.V + (size_t)g * p.hs, keys, lds, meet, row, state);
 }
 
 // a workgroup a (row, head): the states' common maximum, their factors, their outputs in a fixed order
@@ -229,24 +350,41 @@ __global__ void __launch_bounds__(256) attn_shared_fold_kernel(SharedArgs p, uin
 }
 
 struct SharedPlan {
-    bool many;
-    int pair_tiles, prefix_spans, own_spans, prefix_states, states;
+    int qw;  // waves with 32 pairs of their own
+    int pair_tiles, prefix_spans, own_spans, states;
 };
 static SharedPlan shared_plan(size_t T, size_t Hq, size_t Hk, size_t prefix_cap, size_t own_cap) {
-    const size_t pairs = T * (Hq / Hk), target = 2 * (size_t)device_info().cus;
+    const size_t pairs = T * (Hq / Hk), wgs = 2 * (size_t)device_info().cus;
     auto spans = [&](size_t groups, size_t cap) {
-        const size_t most = (cap + SH_KEYS - 1) / SH_KEYS, want = (target + groups - 1) / groups;
+        const size_t most = (cap + SH_KEYS - 1) / SH_KEYS, want = (wgs + groups - 1) / groups;
         const size_t s = want < most ? want : most;
         return (int)(s > 0 ? s : 1);
     };
     SharedPlan r;
-    r.many = pairs > 32;
-    r.pair_tiles = r.many ? (int)((pairs + 127) / 128) : 1;
+    r.qw = pairs <= 32 ? 1 : pairs <= 64 ? 2 : 4;
+    const size_t wide = 32 * (size_t)r.qw;
+    r.pair_tiles = (int)((pairs + wide - 1) / wide);
     r.prefix_spans = spans(Hk * r.pair_tiles, prefix_cap);
     r.own_spans = spans(Hk * T, own_cap);
-    r.prefix_states = r.many ? r.prefix_spans : 4 * r.prefix_spans;
-    r.states = r.prefix_states + 4 * r.own_spans;
+    r.states = r.prefix_spans + r.own_spans;
     return r;
+}
+template <int D, int QW>
+static int32_t launch_one(const dim3& grid, const SharedArgs& p, hipStream_t st) {
+    constexpr int lds = 8 * TK * 2 * D, most = 64 * 1024 - 1024;
+    if (lds > most) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_shared_kernel<D, QW>),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return hip_status(e, "hipFuncSetAttribute");
+    }
+    hipLaunchKernelGGL((attn_shared_kernel<D, QW>), grid, dim3(256), lds, st, p);
+    return hip_status(hipGetLastError(), "attn_shared launch");
+}
+template <int D>
+static int32_t launch_walk(const SharedPlan& s, const dim3& grid, const SharedArgs& p, hipStream_t st) {
+    if (s.qw == 1) return launch_one<D, 1>(grid, p, st);
+    if (s.qw == 2) return launch_one<D, 2>(grid, p, st);
+    return launch_one<D, 4>(grid, p, st);
 }
 static bool shared_sizes_fit(size_t T, size_t Hq, size_t Hk, size_t D, size_t prefix_cap, size_t own_cap) {
     return T > 0 && T <= 65536 && Hk > 0 && Hk <= 1024 && Hq > 0 && Hq % Hk == 0 && Hq / Hk <= 32 && T * Hq <= (1u << 24) && (D == 64 || D == 128) &&
@@ -272,10 +410,10 @@ int32_t btb_hip_attn_shared(const void* q, const void* K, const void* V, void* a
     if (!q || !K || !V || !att || !layout || !workspace) return ERR_NULL;
     auto loose = [](const void* a) { return ((uintptr_t)a & 15u) != 0; };
     if (!shared_sizes_fit(T, Hq, Hk, D, prefix_cap, own_cap) || cap == 0 || cap > 0x7FFFFFFFu || prefix_cap > cap ||
-        own_cap > cap || hs < 0 || rs < 0 || hs % 8 || rs % 8 || !(scale > 0.f) || !(scale < __builtin_inff()) || loose(q) ||
+        own_cap > cap || hs < 0 || rs < 0 || rs > (1 << 25) || hs % 8 || rs % 8 || !(scale > 0.f) || !(scale < __builtin_inff()) || loose(q) ||
         loose(K) || loose(V) || loose(att) || loose(workspace)) {
         set_error("attn_shared: head_dim 64 or 128, up to 32 query heads a kv head, capacities within the cache's, a positive "
-                  "scale, q, K, V, att and the workspace 16-byte aligned with strides in multiples of 8");
+                  "scale, q, K, V, att and the workspace 16-byte aligned with strides in multiples of 8, a row's up to 2^25");
         return ERR_DOMAIN;
     }
     const SharedPlan s = shared_plan(T, Hq, Hk, prefix_cap, own_cap);
@@ -301,24 +439,16 @@ int32_t btb_hip_attn_shared(const void* q, const void* K, const void* V, void* a
     p.pair_tiles = s.pair_tiles;
     p.prefix_spans = s.prefix_spans;
     p.own_spans = s.own_spans;
-    p.prefix_states = s.prefix_states;
     p.states = s.states;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const dim3 grid((unsigned)(Hk * ((size_t)s.pair_tiles * s.prefix_spans + T * s.own_spans)));
-#define AS(DD)                                                                                   \
-    do {                                                                                         \
-        if (s.many)                                                                              \
-            hipLaunchKernelGGL((attn_shared_kernel<DD, true>), grid, dim3(256), 0, st, p);       \
-        else                                                                                     \
-            hipLaunchKernelGGL((attn_shared_kernel<DD, false>), grid, dim3(256), 0, st, p);      \
-        hipLaunchKernelGGL((attn_shared_fold_kernel<DD>), dim3((unsigned)(T * Hq)), dim3(256), 0, st, p, \
-                           static_cast<uint16_t*>(att), lse);                                    \
-    } while (0)
+    const size_t prefix = Hk * (size_t)s.pair_tiles * s.prefix_spans, own = Hk * T * (size_t)s.own_spans;
+    const dim3 grid((unsigned)(8 * ((prefix + 7) / 8 + (own + 7) / 8)));
+    const int32_t rc = D == 64 ? launch_walk<64>(s, grid, p, st) : launch_walk<128>(s, grid, p, st);
+    if (rc != OK) return rc;
     if (D == 64)
-        AS(64);
+        hipLaunchKernelGGL(attn_shared_fold_kernel<64>, dim3((unsigned)(T * Hq)), dim3(256), 0, st, p, static_cast<uint16_t*>(att), lse);
     else
-        AS(128);
-#undef AS
+        hipLaunchKernelGGL(attn_shared_fold_kernel<128>, dim3((unsigned)(T * Hq)), dim3(256), 0, st, p, static_cast<uint16_t*>(att), lse);
     return hip_status(hipGetLastError(), "attn_shared launch");
 }
 

@@ -50,6 +50,90 @@ __device__ __forceinline__ bf16x8 v_fragment(const uint8_t* tile, int dt, int u,
     return __builtin_bit_cast(bf16x8, both);
 }
 
+// ---- a wave's own tiles straight from memory into LDS -----------------------------------------------------------------
+// global_load_lds_dwordx4 writes lane l's 16 bytes at a wave's LDS base plus 16 l: the place in the tile is fixed, so the
+// permutation of a key's chunks is made on the way out of memory, within the key's own row.
+
+// Four such loads, 16 bytes a lane each: from base, base + step, + 2 step and + 3 step (uniform) + the lane's offsets to LDS bytes `to` (uniform) + 16 lane and 1, 2 and 3 KB on. Written out, because behind the builtin the
+// compiler makes every transposing read of LDS wait for all such loads there are, the next stage's among them. They write no
+// register; what they write is waited for by count (wait_loads), and a wait of the compiler's own for another load can only come out
+// longer. M0 is left as it was.
+__device__ __forceinline__ void load4_to_lds(const char* base, size_t step, uint32_t o0, uint32_t o1, uint32_t o2, uint32_t o3,
+                                             uint32_t to) {
+    uint32_t kept;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %6\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %7\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %8\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %9\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(kept)
+        : "s"(to), "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "s"(base + step), "s"(base + 2 * step), "s"(base + 3 * step)
+        : "memory", "scc");
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+template <class T>
+__device__ __forceinline__ T* uniform(T* p) {
+    const uint64_t v = (uint64_t)p;
+    // (the builtin returns a signed number: its top bit must not spread over the other half)
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
+    return (T*)((uint64_t)lo | (uint64_t)hi << 32);
+}
+
+template <int D>
+struct TileLoads {
+    static constexpr int N = TK * 2 * D / 1024;      // instructions a tile of K, and of V
+    static constexpr int CH = D / 8, KPI = 64 / CH;  // chunks a row, keys an instruction
+    static constexpr int KP = D / 8 / KPI;           // instructions after which K's permutation is the same again (V's: each)
+    uint32_t k[KP], v;                               // the lane's bytes from the first key of an instruction
+
+    __device__ __forceinline__ void make(long long rs, int lane) {
+        const uint32_t row = (uint32_t)(lane / CH * rs * 2);
+#pragma unroll
+        for (int i = 0; i < KP; ++i) k[i] = row + 16 * k_chunk<D>(KPI * i + lane / CH, lane % CH);
+        v = row + 16 * v_chunk(lane / CH, lane % CH);
+    }
+    // the tile of `left` >= 1 keys at `from` (uniform) into LDS: K's, or V's; keys past the last are the last again
+    template <bool IS_K>
+    __device__ __forceinline__ void issue(const uint16_t* from, long long rs, int left, uint8_t* tile, int lane) const {
+        const char* base = reinterpret_cast<const char*>(uniform(from));
+        const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_address(tile));
+        if (left >= TK) {
+            const size_t step = (size_t)KPI * rs * 2;
+#pragma unroll
+            for (int i = 0; i < N; i += 4) {
+                auto at = [&](int j) { return IS_K ? k[(i + j) % KP] : v; };
+                load4_to_lds(base + i * step, step, at(0), at(1), at(2), at(3), to + 1024 * i);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i += 4) {
+                auto at = [&](int j) {
+                    const int key = KPI * (i + j) + lane / CH;
+                    return (uint32_t)(min(key, left - 1) * rs * 2) + 16 * (IS_K ? k_chunk<D>(key, lane % CH) : v_chunk(key, lane % CH));
+                };
+                load4_to_lds(base, 0, at(0), at(1), at(2), at(3), to + 1024 * i);
+            }
+        }
+    }
+    // V's rows past the last key as zeros, once the tile has landed: weight 0 times what lies there must not make a NaN
+    __device__ __forceinline__ static void clear_past(uint8_t* v_lds, int left, int lane) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (KPI * i + lane / CH >= left) *reinterpret_cast<uint4*>(v_lds + 1024 * i + 16 * lane) = make_uint4(0u, 0u, 0u, 0u);
+    }
+};
+
+// All but the youngest N loads have landed. A direct-to-LDS load is, to the compiler, a store made where it was issued; the
+// reads behind the wait take their place from `at`, which this statement "writes", so they stay behind it.
+template <int N>
+__device__ __forceinline__ void wait_loads(uint32_t& at) {
+    asm volatile("s_waitcnt vmcnt(%1)" : "+v"(at) : "n"(N) : "memory");
+}
+
 // eight weights as an operand
 __device__ __forceinline__ bf16x8 weight_fragment(const float* p) {
     return __builtin_bit_cast(bf16x8, make_uint4(f32x2_bf16(p[0], p[1]), f32x2_bf16(p[2], p[3]), f32x2_bf16(p[4], p[5]),
