@@ -22,6 +22,7 @@
 namespace btb {
 
 constexpr int SH_KEYS = 128;  // keys a stage: a tile a wave loads
+constexpr int SH_DEAL = 32;   // workgroups of a kind in a row: 8 dies x 4
 
 struct SharedArgs {
     const uint16_t* q;
@@ -108,38 +109,49 @@ __device__ __forceinline__ void walk(const SharedArgs& p, const uint16_t* Kg, co
         issue_k(0);
         issue_v(0);
     }
-    // the wave's tiles of a stage in groups of at most two: a group's scores are made while the one before is weighed
-    constexpr int GT = TPW < 2 ? TPW : 2, GROUPS = TPW / GT;
-    f32x16 st[GT];
+    // The wave's tiles of a stage in groups of at most two. The order within a stage is written down: left alone the compiler
+    // reads a fragment, waits for it and multiplies, an LDS round trip a product. Fragments are asked for AHEAD products early,
+    // and what vector arithmetic there is to do meanwhile - a group's weights under the next one's scores, that one's maximum
+    // under the first one's outputs - is dealt out between the products.
+    constexpr int GT = TPW < 2 ? TPW : 2, GROUPS = TPW / GT, AHEAD = 4;
+    f32x16 st[GROUPS][GT];
     bf16x8 pf[GT][2];
-    auto scores = [&](const uint8_t* k_lds, int group, f32x16(&to)[GT]) {
+    auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
+    // products GT STEPS; work(i) after each of the STEPS
+    auto scores = [&](uint32_t at, int group, f32x16(&to)[GT], auto work) {
+        bf16x8 kf[STEPS * GT];
+        auto read = [&](int e) { return k_fragment(lds + kw * TILE, at, KW * (GT * group + e % GT) * TILE, e / GT); };
 #pragma unroll
-        for (int j = 0; j < GT; ++j) {
-            const uint8_t* tile = k_lds + (kw + KW * (GT * group + j)) * TILE;
-            to[j] = zero16();
+        for (int j = 0; j < GT; ++j) to[j] = zero16();
 #pragma unroll
-            for (int i = 0; i < STEPS; ++i) to[j] = mfma32(k_fragment<D>(tile, i, lane), qf[i], to[j]);
-        }
-    };
-    // keys past the end; the group's maximum; the state moved to it where it has to be
-    auto settle = [&](int kb, bool more, int group) {
-        if (!more) {
+        for (int e = 0; e < AHEAD; ++e) kf[e] = read(e);
+        fence();
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
 #pragma unroll
             for (int j = 0; j < GT; ++j) {
-                const int left = keys.count - kb - TK * (kw + KW * (GT * group + j));
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (8 * (i / 4) + 4 * h + i % 4 >= left) st[j][i] = ninf;
+                const int e = i * GT + j;
+                if (e + AHEAD < STEPS * GT) kf[e + AHEAD] = read(e + AHEAD);
+                to[j] = mfma32(kf[e], qf[i], to[j]);
             }
+            work(i);
+            fence();
         }
-        float top = st[0][0];
+    };
+    // keys past the end
+    auto mask = [&](int kb, int group) {
 #pragma unroll
-        for (int j = 0; j < GT; ++j)
+        for (int j = 0; j < GT; ++j) {
+            const int left = keys.count - kb - TK * (kw + KW * (GT * group + j));
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, st[j][i]);
+            for (int i = 0; i < 16; ++i)
+                if (8 * (i / 4) + 4 * h + i % 4 >= left) st[group][j][i] = ninf;
+        }
+    };
+    // The state moves to a new maximum only where that is 2^8 past its own: weights of up to 2^8 are as exact, and most groups
+    // then leave the outputs alone. A pair's decision is its own, whatever its neighbours'.
+    auto settle = [&](float top) {
         top = fmaxf(top, xor32(top)) * p.scale_log2;
-        // The state moves to a new maximum only where that is 2^8 past its own: weights of up to 2^8 are as exact, and most
-        // groups then leave the outputs alone. A pair's decision is its own, whatever its neighbours'.
         const bool moves = top > m + 8.f || m == ninf;
         if (__any(moves)) {
             const float mn = moves ? top : m;
@@ -152,41 +164,68 @@ __device__ __forceinline__ void walk(const SharedArgs& p, const uint16_t* Kg, co
                 for (int i = 0; i < 16; ++i) o[d][i] *= corr;
         }
     };
-    auto weigh = [&] {
-        const float ref = m == ninf ? 0.f : m;
+    // scores [from, to) of a group as weights
+    float w[GT][16];
+    auto weigh = [&](int group, float ref, int from, int to) {
+        float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < GT; ++j) {
-            float w[16], sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                w[i] = __builtin_amdgcn_exp2f(fmaf(st[j][i], p.scale_log2, -ref));
-                sum += w[i];
+        for (int e = 0; e < GT * 16; ++e)
+            if (e >= from && e < to) {
+                w[e / 16][e % 16] = __builtin_amdgcn_exp2f(fmaf(st[group][e / 16][e % 16], p.scale_log2, -ref));
+                sum += w[e / 16][e % 16];
+                if (e % 8 == 7) {
+                    pf[e / 16][e % 16 / 8] = weight_fragment(&w[e / 16][e % 16 - 7]);
+                    made(pf[e / 16][e % 16 / 8]);
+                }
             }
-            l += sum;
-            pf[j][0] = weight_fragment(w);
-            pf[j][1] = weight_fragment(w + 8);
+        l += sum;
+    };
+    // products GT 2 DT; work(r) after every second
+    auto outputs = [&](uint32_t at, int group, auto work) {
+        constexpr int ALL = GT * 2 * DT;
+        bf16x8 vf[ALL];
+        auto read = [&](int e) {
+            return v_fragment<D>(lds + (4 + kw) * TILE, at, KW * (GT * group + e / (2 * DT)) * TILE, e % DT, e / DT % 2);
+        };
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) vf[e] = read(e);
+        fence();
+#pragma unroll
+        for (int e = 0; e < ALL; ++e) {
+            if (e + AHEAD < ALL) vf[e + AHEAD] = read(e + AHEAD);
+            o[e % DT] = mfma32(vf[e], pf[e / (2 * DT)][e / DT % 2], o[e % DT]);
+            if (e % 2 == 1) {
+                work(e / 2);
+                fence();
+            }
         }
     };
-    auto outputs = [&](const uint8_t* v_lds, int group) {
-#pragma unroll
-        for (int j = 0; j < GT; ++j) {
-            const uint8_t* tile = v_lds + (kw + KW * (GT * group + j)) * TILE;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int d = 0; d < DT; ++d) o[d] = mfma32(v_fragment<D>(tile, d, u, lane), pf[j][u], o[d]);
-        }
-    };
+    auto nothing = [](int) {};
+    const uint32_t k_at = k_place<D>(lane), v_at = v_place<D>(lane);
     for (int kb = 0; kb < keys.count; kb += SH_KEYS) {
         const bool more = kb + SH_KEYS < keys.count;
-        uint32_t ak = 0, av = 4 * TILE;
+        uint32_t ak = k_at, av = v_at;
         wait_loads<N>(ak);
         barrier();
-        scores(lds + ak, 0, st);
-        settle(kb, more, 0);
-        f32x16 next[GT];
-        if constexpr (GROUPS > 1) scores(lds + ak, 1, next);
-        weigh();
+        scores(ak, 0, st[0], nothing);
+        if (!more) mask(kb, 0);
+        float top = st[0][0][0];
+#pragma unroll
+        for (int j = 0; j < GT; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, st[0][j][i]);
+        settle(top);
+        fence();
+        {
+            const float ref = m == ninf ? 0.f : m;
+            constexpr int EACH = GT * 16 / STEPS;
+            if constexpr (GROUPS > 1) {
+                scores(ak, 1, st[GROUPS - 1], [&](int i) { weigh(0, ref, i * EACH, i * EACH + EACH); });
+                if (!more) mask(kb, GROUPS - 1);
+            } else {
+                weigh(0, ref, 0, GT * 16);
+            }
+        }
         barrier();
         if (more) {
             issue_k(kb + SH_KEYS);
@@ -194,18 +233,23 @@ __device__ __forceinline__ void walk(const SharedArgs& p, const uint16_t* Kg, co
         } else {
             wait_loads<0>(av);
             const int mine = keys.count - kb - TK * wv;
-            if (mine < TK) TileLoads<D>::clear_past(lds + av + wv * TILE, mine, lane);
+            if (mine < TK) TileLoads<D>::clear_past(lds + (4 + wv) * TILE, mine, lane);
             if constexpr (QW > 1) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
         barrier();
-        outputs(lds + av, 0);
         if constexpr (GROUPS > 1) {
+            constexpr int EACH = GT * 16 / (GT * DT);
+            top = st[1][0][0];
+            outputs(av, 0, [&](int r) {
 #pragma unroll
-            for (int j = 0; j < GT; ++j) st[j] = next[j];
-            settle(kb, more, 1);
-            weigh();
-            outputs(lds + av, 1);
+                for (int e = 0; e < GT * 16; ++e)
+                    if (e >= r * EACH && e < r * EACH + EACH) top = fmaxf(top, st[1][e / 16][e % 16]);
+            });
+            settle(top);
+            weigh(1, m == ninf ? 0.f : m, 0, GT * 16);
+            fence();
         }
+        outputs(av, GROUPS - 1, nothing);
         barrier();
         if (more) issue_v(kb + SH_KEYS);
     }
@@ -264,18 +308,18 @@ __device__ __forceinline__ void walk(const SharedArgs& p, const uint16_t* Kg, co
 }
 
 // The prefix's workgroups and the rows' own are dealt in turn, so that what the matrix cores bound and what memory bounds run
-// side by side; eight neighbours at a time, one a die, so that the workgroups that read the same keys for other pairs are
-// on one die together.
+// side by side; SH_DEAL neighbours at a time, one for each of a die's four arrays of CUs, which take workgroups by turns
+// (dealt by eight, one a die, 512 of each kind put all of the prefix's on half of the chip: 64 rows x 131072 keys 251 us).
 template <int D, int QW>
 __global__ void __launch_bounds__(256, 2) attn_shared_kernel(SharedArgs p) {
     extern __shared__ __align__(16) uint8_t lds[];  // a stage
     __shared__ float meet[2 * 4 * 32];
     const int pairs = p.T * p.G;
     const int prefix = p.Hk * p.pair_tiles * p.prefix_spans, own = p.Hk * p.T * p.own_spans;
-    const long long pe = (prefix + 7) / 8, all = pe + (own + 7) / 8, oct = blockIdx.x / 8;
-    const int ahead = (int)(oct * pe / all);  // the prefix's octets before this one
-    if ((int)((oct + 1) * pe / all) > ahead) {
-        const int id = 8 * ahead + blockIdx.x % 8;
+    const long long pe = (prefix + SH_DEAL - 1) / SH_DEAL, all = pe + (own + SH_DEAL - 1) / SH_DEAL, hand = blockIdx.x / SH_DEAL;
+    const int ahead = (int)(hand * pe / all);  // the prefix's hands before this one
+    if ((int)((hand + 1) * pe / all) > ahead) {
+        const int id = SH_DEAL * ahead + blockIdx.x % SH_DEAL;
         if (id >= prefix) return;
         const int g = id % p.Hk, tile = id / p.Hk % p.pair_tiles, sp = id / (p.Hk * p.pair_tiles);
         const Keys keys = part_of(stretch(p.lay[0], p.lay[1], p.prefix_cap, p.cap), sp, p.prefix_spans);
@@ -291,7 +335,7 @@ __global__ void __launch_bounds__(256, 2) attn_shared_kernel(SharedArgs p) {
         walk<D, QW>(p, p.K + (size_t)g * p.hs, p.V + (size_t)g * p.hs, keys, lds, meet, row, state);
         return;
     }
-    const int id = 8 * (int)(oct - ahead) + blockIdx.x % 8;
+    const int id = SH_DEAL * (int)(hand - ahead) + blockIdx.x % SH_DEAL;
     if (id >= own) return;
     const int g = id % p.Hk, t = id / p.Hk % p.T, sp = id / (p.Hk * p.T);
     const Keys keys = part_of(stretch(p.lay[2 + 2 * t], p.lay[3 + 2 * t], p.own_cap, p.cap), sp, p.own_spans);
@@ -358,7 +402,7 @@ static SharedPlan shared_plan(size_t T, size_t Hq, size_t Hk, size_t prefix_cap,
     auto spans = [&](size_t groups, size_t cap) {
         const size_t most = (cap + SH_KEYS - 1) / SH_KEYS, want = (wgs + groups - 1) / groups;
         const size_t s = want < most ? want : most;
-        return (int)(s > 0 ? s : 1);
+        return (int)s;
     };
     SharedPlan r;
     r.qw = pairs <= 32 ? 1 : pairs <= 64 ? 2 : 4;
@@ -366,6 +410,7 @@ static SharedPlan shared_plan(size_t T, size_t Hq, size_t Hk, size_t prefix_cap,
     r.pair_tiles = (int)((pairs + wide - 1) / wide);
     r.prefix_spans = spans(Hk * r.pair_tiles, prefix_cap);
     r.own_spans = spans(Hk * T, own_cap);
+    if (r.prefix_spans + r.own_spans == 0) r.own_spans = 1;  // no key anywhere: states that say so
     r.states = r.prefix_spans + r.own_spans;
     return r;
 }
@@ -442,7 +487,7 @@ int32_t btb_hip_attn_shared(const void* q, const void* K, const void* V, void* a
     p.states = s.states;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const size_t prefix = Hk * (size_t)s.pair_tiles * s.prefix_spans, own = Hk * T * (size_t)s.own_spans;
-    const dim3 grid((unsigned)(8 * ((prefix + 7) / 8 + (own + 7) / 8)));
+    const dim3 grid((unsigned)(SH_DEAL * ((prefix + SH_DEAL - 1) / SH_DEAL + (own + SH_DEAL - 1) / SH_DEAL)));
     const int32_t rc = D == 64 ? launch_walk<64>(s, grid, p, st) : launch_walk<128>(s, grid, p, st);
     if (rc != OK) return rc;
     if (D == 64)

@@ -27,22 +27,26 @@ __device__ __forceinline__ int k_chunk(int key, int chunk) {
 }
 __device__ __forceinline__ int v_chunk(int key, int chunk) { return chunk ^ ((key & 3) << 1); }
 
-// K's fragment of 16 dims: lane (c, h) key c, dims 16 step + 8 h .. + 7
+// K's fragment of 16 dims: lane (c, h) key c, dims 16 step + 8 h .. + 7. A lane's place in a tile is one number for all steps:
+// the step's chunk is an exclusive or with it.
 template <int D>
-__device__ __forceinline__ bf16x8 k_fragment(const uint8_t* tile, int step, int lane) {
-    const int key = lane & 31;
-    return __builtin_bit_cast(
-        bf16x8, *reinterpret_cast<const uint4*>(tile + key * 2 * D + 16 * k_chunk<D>(key, 2 * step + (lane >> 5))));
+__device__ __forceinline__ uint32_t k_place(int lane) {
+    return (uint32_t)((lane & 31) * 2 * D + 16 * k_chunk<D>(lane & 31, lane >> 5));
+}
+__device__ __forceinline__ bf16x8 k_fragment(const uint8_t* tiles, uint32_t place, int tile_at, int step) {
+    return __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(tiles + (place ^ (uint32_t)(32 * step)) + tile_at));
 }
 
 // V^T's fragment of 32 dims (dt) against 16 keys (u): lane (c, h) dim 32 dt + c, keys 16 u + 8 (e / 4) + 4 h + e % 4.
 // Two transposing reads: in each group of 16 lanes, lane l asks for 4 dims of key l / 4 and gets dim l of the four keys.
 template <int D>
-__device__ __forceinline__ bf16x8 v_fragment(const uint8_t* tile, int dt, int u, int lane) {
-    const int l = lane & 15, group = lane >> 4;
-    const int key = 16 * u + 4 * (group >> 1) + (l >> 2);
-    const int chunk = 4 * dt + 2 * (group & 1) + ((l & 3) >> 1);
-    const uint8_t* at = tile + key * 2 * D + 16 * v_chunk(key, chunk) + 8 * (l & 1);
+__device__ __forceinline__ uint32_t v_place(int lane) {
+    const int l = lane & 15, group = lane >> 4, key = 4 * (group >> 1) + (l >> 2);
+    return (uint32_t)(key * 2 * D + 16 * v_chunk(key, 2 * (group & 1) + ((l & 3) >> 1)) + 8 * (l & 1));
+}
+template <int D>
+__device__ __forceinline__ bf16x8 v_fragment(const uint8_t* tiles, uint32_t place, int tile_at, int dt, int u) {
+    const uint8_t* at = tiles + (place ^ (uint32_t)(64 * dt)) + tile_at + u * 16 * 2 * D;
     const i16x4 first = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(at));
     const i16x4 second = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(at + 8 * 2 * D));
     typedef __attribute__((ext_vector_type(8))) short i16x8;
@@ -149,6 +153,13 @@ __device__ __forceinline__ f32x16 zero16() {
 #pragma unroll
     for (int i = 0; i < 16; ++i) z[i] = 0.f;
     return z;
+}
+
+// the value is made here, not where it is first used
+__device__ __forceinline__ void made(bf16x8& v) {
+    u32x4 w = __builtin_bit_cast(u32x4, v);
+    asm volatile("" : "+v"(w));
+    v = __builtin_bit_cast(bf16x8, w);
 }
 
 }  // namespace btb
