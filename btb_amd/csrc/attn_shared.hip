@@ -22,7 +22,6 @@
 namespace btb {
 
 constexpr int SH_KEYS = 128;  // keys a stage: a tile a wave loads
-constexpr int SH_DEAL = 32;   // workgroups of a kind in a row: 8 dies x 4
 
 struct SharedArgs {
     const uint16_t* q;
@@ -307,20 +306,15 @@ __device__ __forceinline__ void walk(const SharedArgs& p, const uint16_t* Kg, co
     }
 }
 
-// The prefix's workgroups and the rows' own are dealt in turn, so that what the matrix cores bound and what memory bounds run
-// side by side; SH_DEAL neighbours at a time, one for each of a die's four arrays of CUs, which take workgroups by turns
-// (dealt by eight, one a die, 512 of each kind put all of the prefix's on half of the chip: 64 rows x 131072 keys 251 us).
+// The prefix's workgroups come first, the long ones; the rows' own take what room is left beside them and after them.
 template <int D, int QW>
 __global__ void __launch_bounds__(256, 2) attn_shared_kernel(SharedArgs p) {
     extern __shared__ __align__(16) uint8_t lds[];  // a stage
     __shared__ float meet[2 * 4 * 32];
     const int pairs = p.T * p.G;
-    const int prefix = p.Hk * p.pair_tiles * p.prefix_spans, own = p.Hk * p.T * p.own_spans;
-    const long long pe = (prefix + SH_DEAL - 1) / SH_DEAL, all = pe + (own + SH_DEAL - 1) / SH_DEAL, hand = blockIdx.x / SH_DEAL;
-    const int ahead = (int)(hand * pe / all);  // the prefix's hands before this one
-    if ((int)((hand + 1) * pe / all) > ahead) {
-        const int id = SH_DEAL * ahead + blockIdx.x % SH_DEAL;
-        if (id >= prefix) return;
+    const int prefix = p.Hk * p.pair_tiles * p.prefix_spans;
+    int id = blockIdx.x;
+    if (id < prefix) {
         const int g = id % p.Hk, tile = id / p.Hk % p.pair_tiles, sp = id / (p.Hk * p.pair_tiles);
         const Keys keys = part_of(stretch(p.lay[0], p.lay[1], p.prefix_cap, p.cap), sp, p.prefix_spans);
         const int r0 = 32 * QW * tile;
@@ -335,8 +329,7 @@ __global__ void __launch_bounds__(256, 2) attn_shared_kernel(SharedArgs p) {
         walk<D, QW>(p, p.K + (size_t)g * p.hs, p.V + (size_t)g * p.hs, keys, lds, meet, row, state);
         return;
     }
-    const int id = SH_DEAL * (int)(hand - ahead) + blockIdx.x % SH_DEAL;
-    if (id >= own) return;
+    id -= prefix;
     const int g = id % p.Hk, t = id / p.Hk % p.T, sp = id / (p.Hk * p.T);
     const Keys keys = part_of(stretch(p.lay[2 + 2 * t], p.lay[3 + 2 * t], p.own_cap, p.cap), sp, p.own_spans);
     auto row = [&](int i) { return p.q + ((size_t)t * p.Hq + g * p.G + min(i, p.G - 1)) * D; };
@@ -346,70 +339,75 @@ __global__ void __launch_bounds__(256, 2) attn_shared_kernel(SharedArgs p) {
     walk<D, 1>(p, p.K + (size_t)g * p.hs, p.V + (size_t)g * p.hs, keys, lds, meet, row, state);
 }
 
-// a workgroup a (row, head): the states' common maximum, their factors, their outputs in a fixed order
-template <int D>
+// WAVES waves a (row, head): the states' common maximum, their factors, their outputs in a fixed order - a lane two dims, at
+// head_dim 64 the halves of a wave in turn. One wave where there are heads enough to fill the chip, else four.
+template <int D, int WAVES>
 __global__ void __launch_bounds__(256) attn_shared_fold_kernel(SharedArgs p, uint16_t* att, float* lse) {
-    constexpr int LANES = D / 2, GROUPS = 256 / LANES;
-    __shared__ float red[4], sums[4], acc[GROUPS][D];
-    const int t = blockIdx.x / p.Hq, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    if (p.lay[3 + 2 * t] < 0) return;  // padding
-    const size_t base = (size_t)blockIdx.x * p.states;
+    constexpr int HEADS = 4 / WAVES, PART = 128 / D * WAVES;  // heads a workgroup, parts that the states are taken in
+    __shared__ float2 acc[WAVES > 1 ? 4 : 1][64];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int head = blockIdx.x * HEADS + wv / WAVES, w = wv % WAVES;
+    const bool live = head < p.T * p.Hq && p.lay[3 + 2 * (min(head, p.T * p.Hq - 1) / p.Hq)] >= 0;  // uniform in the wave
+    if (WAVES == 1 && !live) return;
+    const size_t base = (size_t)(live ? head : 0) * p.states;
     const float ninf = bits_f32(0xff800000u);
-    float m = ninf;
-    for (int s = tid; s < p.states; s += 256) m = fmaxf(m, p.part_m[base + s]);
+    float m = ninf, l = 0.f;
+    for (int s = lane; s < p.states; s += 64) m = fmaxf(m, p.part_m[base + s]);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, WAVE));
-    if (lane == 0) red[wv] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     auto factor = [&](float ms) { return ms == ninf ? 0.f : __builtin_amdgcn_exp2f(ms - m); };
-    float l = 0.f;
-    for (int s = tid; s < p.states; s += 256) l = fmaf(factor(p.part_m[base + s]), p.part_l[base + s], l);
+    for (int s = lane; s < p.states; s += 64) l = fmaf(factor(p.part_m[base + s]), p.part_l[base + s], l);
     l = wave_sum(l);
-    if (lane == 0) sums[wv] = l;
-    const int group = tid / LANES, dl = 2 * (tid % LANES);
-    float a0 = 0.f, a1 = 0.f;
-    for (int s = group; s < p.states; s += GROUPS) {
+    const int dl = 2 * lane % D;
+    float2 a = make_float2(0.f, 0.f);
+#pragma unroll 8
+    for (int s = w + WAVES * (2 * lane / D); s < p.states; s += PART) {
         const float ms = p.part_m[base + s];
-        if (ms == ninf) continue;
-        const float f = factor(ms);
         const float2 v = *reinterpret_cast<const float2*>(p.part_acc + (base + s) * D + dl);
-        a0 = fmaf(f, v.x, a0);
-        a1 = fmaf(f, v.y, a1);
+        const float f = factor(ms);
+        a.x = fmaf(f, ms == ninf ? 0.f : v.x, a.x);
+        a.y = fmaf(f, ms == ninf ? 0.f : v.y, a.y);
     }
-    acc[group][dl] = a0;
-    acc[group][dl + 1] = a1;
-    __syncthreads();
-    l = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-    if (tid < LANES) {
-        float x = 0.f, y = 0.f;
+    if (WAVES > 1) {
+        acc[wv][lane] = a;
+        __syncthreads();
+        if (w != 0 || !live) return;
 #pragma unroll
-        for (int i = 0; i < GROUPS; ++i) {
-            x += acc[i][2 * tid];
-            y += acc[i][2 * tid + 1];
+        for (int i = 1; i < WAVES; ++i) {
+            a.x += acc[wv + i][lane].x;
+            a.y += acc[wv + i][lane].y;
         }
-        reinterpret_cast<uint32_t*>(att + (size_t)blockIdx.x * D)[tid] = l == 0.f ? 0u : f32x2_bf16(x / l, y / l);
     }
-    if (tid == 0 && lse != nullptr) lse[blockIdx.x] = l == 0.f ? ninf : fmaf(m, 0.693147180559945309f, logf(l));
+    if (D == 64) {
+        a.x += xor32(a.x);
+        a.y += xor32(a.y);
+    }
+    if (lane < D / 2) reinterpret_cast<uint32_t*>(att + (size_t)head * D)[lane] = l == 0.f ? 0u : f32x2_bf16(a.x / l, a.y / l);
+    if (lane == 0 && lse != nullptr) lse[head] = l == 0.f ? ninf : fmaf(m, 0.693147180559945309f, logf(l));
 }
 
 struct SharedPlan {
     int qw;  // waves with 32 pairs of their own
     int pair_tiles, prefix_spans, own_spans, states;
 };
+// A prefix workgroup a CU, the rows' own beside them; two a CU where the products are what the prefix costs - 128 pairs of a head and
+// more, spans of eight stages and more - and the rows' own keys, read at 5.1 TB/s, cost less than half of that (at 900 TFLOP/s).
+// us, one a CU / two: 16 rows x 131072 keys, 100 own 107 / 119; 4 rows 102 / 107; 256 x 32768, 640 own 235 / 273, 64 own 192 /
+// 172, 64 x 131072, 640 own 212 / 196; 41 rows of 40 heads x 64 over 6001, 485 own 22.7 / 27.0, none 17.6 / 19.3.
 static SharedPlan shared_plan(size_t T, size_t Hq, size_t Hk, size_t prefix_cap, size_t own_cap) {
-    const size_t pairs = T * (Hq / Hk), wgs = 2 * (size_t)device_info().cus;
-    auto spans = [&](size_t groups, size_t cap) {
+    const size_t G = Hq / Hk, pairs = T * G, cus = (size_t)device_info().cus;
+    auto spans = [&](size_t groups, size_t cap, size_t wgs) {
         const size_t most = (cap + SH_KEYS - 1) / SH_KEYS, want = (wgs + groups - 1) / groups;
-        const size_t s = want < most ? want : most;
-        return (int)s;
+        return (int)(want < most ? want : most);
     };
     SharedPlan r;
     r.qw = pairs <= 32 ? 1 : pairs <= 64 ? 2 : 4;
     const size_t wide = 32 * (size_t)r.qw;
     r.pair_tiles = (int)((pairs + wide - 1) / wide);
-    r.prefix_spans = spans(Hk * r.pair_tiles, prefix_cap);
-    r.own_spans = spans(Hk * T, own_cap);
+    const size_t groups = Hk * r.pair_tiles;
+    const bool twice = pairs >= 128 && prefix_cap * groups >= 2 * cus * 8 * SH_KEYS && own_cap * 352 < G * prefix_cap;
+    r.prefix_spans = spans(groups, prefix_cap, (twice ? 2 : 1) * cus);
+    r.own_spans = spans(Hk * T, own_cap, cus);
     if (r.prefix_spans + r.own_spans == 0) r.own_spans = 1;  // no key anywhere: states that say so
     r.states = r.prefix_spans + r.own_spans;
     return r;
@@ -487,13 +485,24 @@ int32_t btb_hip_attn_shared(const void* q, const void* K, const void* V, void* a
     p.states = s.states;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const size_t prefix = Hk * (size_t)s.pair_tiles * s.prefix_spans, own = Hk * T * (size_t)s.own_spans;
-    const dim3 grid((unsigned)(SH_DEAL * ((prefix + SH_DEAL - 1) / SH_DEAL + (own + SH_DEAL - 1) / SH_DEAL)));
+    const dim3 grid((unsigned)(prefix + own));
     const int32_t rc = D == 64 ? launch_walk<64>(s, grid, p, st) : launch_walk<128>(s, grid, p, st);
     if (rc != OK) return rc;
-    if (D == 64)
-        hipLaunchKernelGGL(attn_shared_fold_kernel<64>, dim3((unsigned)(T * Hq)), dim3(256), 0, st, p, static_cast<uint16_t*>(att), lse);
-    else
-        hipLaunchKernelGGL(attn_shared_fold_kernel<128>, dim3((unsigned)(T * Hq)), dim3(256), 0, st, p, static_cast<uint16_t*>(att), lse);
+    const size_t heads = T * Hq;
+    uint16_t* out = static_cast<uint16_t*>(att);
+    if (heads >= 2048) {
+        const dim3 wgs((unsigned)((heads + 3) / 4));
+        if (D == 64)
+            hipLaunchKernelGGL((attn_shared_fold_kernel<64, 1>), wgs, dim3(256), 0, st, p, out, lse);
+        else
+            hipLaunchKernelGGL((attn_shared_fold_kernel<128, 1>), wgs, dim3(256), 0, st, p, out, lse);
+    } else {
+        const dim3 wgs((unsigned)heads);
+        if (D == 64)
+            hipLaunchKernelGGL((attn_shared_fold_kernel<64, 4>), wgs, dim3(256), 0, st, p, out, lse);
+        else
+            hipLaunchKernelGGL((attn_shared_fold_kernel<128, 4>), wgs, dim3(256), 0, st, p, out, lse);
+    }
     return hip_status(hipGetLastError(), "attn_shared launch");
 }
 
