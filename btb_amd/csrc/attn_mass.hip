@@ -2,9 +2,16 @@
 //
 //   out[g, j] = mass[g, j] + sum over rows t with j < seen[t], query heads h of g, of exp(scale q_{t,h} . k_j - lse[t, h])
 //
-// lse is what the pass's attention left (btb_hip_attn_shared). A wave holds 32 keys as a stationary operand and takes the
-// pass's (row, head) pairs 32 at a time; a lane's sixteen sums (btb_tile32.hpp) stay in its registers until the end, so the
-// order of the additions is fixed. Everything after the product is f32.
+// lse is what the pass's attention left (btb_hip_attn_shared). Scores are made as S = Q K^T, 32 pairs against 32 keys: lane (c, h)
+// ends with key c's against pairs 8 (i / 4) + 4 h + i % 4, so a key's sum over the pairs is a lane's own and one exchange between
+// the halves at the end. The order of the additions is fixed. Everything after the product is f32. Two kernels:
+//
+//   many pairs: a wave holds 64 keys as stationary operands and takes the pass's (row, head) pairs 32 at a time out of LDS, where the
+//     workgroup's four waves bring them a stage ahead. A tile's weights are made between the next tile's products. Where keys are
+//     few, the pairs are cut over workgroups too, whose sums a second launch adds in order. Bound: the exponentials, sixteen of
+//     a quarter's rate a lane beside sixteen multiply-adds and additions a tile, against eight products of head_dim 128.
+//   few pairs (64 and less): they lie in LDS and the keys go by, a tile of 32 a wave ahead of the one at work. Bound: K's
+//     trip from memory.
 
 #include "btb_common.hpp"
 #include "btb_tile32.hpp"
@@ -14,6 +21,10 @@
 
 namespace btb {
 
+constexpr int MA_KEYS = 256;   // many pairs: keys a workgroup, four waves of two tiles
+constexpr int MA_META = 2048;  // pairs whose log-sums and limits lie in LDS at a time
+constexpr int MA_FEW = 64;     // few pairs, at most
+
 struct MassArgs {
     const uint16_t* q;
     const uint16_t* K;
@@ -21,50 +32,313 @@ struct MassArgs {
     const int32_t* seen;   // [T]
     const float* mass;     // rows of `ms` floats, or none
     float* out;            // rows of `os` floats
+    float* work;           // [parts][Hk][n] where parts > 1
     long long hs, rs, ms, os;
     float scale_log2;
-    int T, Hq, G, n;
+    int T, Hq, Hk, G, n, parts;
 };
 
+// A pair's log-sum in units of log 2 and how many keys it sees. A pair past the last, or one that saw nothing, sees none.
+__device__ __forceinline__ void pair_facts(const MassArgs& p, int g, int r, int pairs, int row, float& z, int& seen) {
+    z = 0.f;
+    seen = 0;
+    if (r < pairs) {
+        const float raw = p.lse[(size_t)row * p.Hq + g * p.G + (r - row * p.G)];
+        if (raw != -__builtin_inff()) {
+            z = raw * 1.44269504088896341f;
+            seen = p.seen[row];
+        }
+    }
+}
+// the smallest of 32 lanes' numbers, in each
+__device__ __forceinline__ int half_min(int v) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) v = min(v, __shfl_xor(v, d, WAVE));
+    return v;
+}
+// sixteen of a tile's 32 values, those of the lane's pairs, from LDS
+__device__ __forceinline__ void of_pairs(const float* from, int h, float (&v)[16]) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const float4 x = *reinterpret_cast<const float4*>(from + 8 * b + 4 * h);
+        v[4 * b] = x.x;
+        v[4 * b + 1] = x.y;
+        v[4 * b + 2] = x.z;
+        v[4 * b + 3] = x.w;
+    }
+}
+
 template <int D>
-__global__ void __launch_bounds__(256) attn_mass_kernel(MassArgs p) {
-    constexpr int STEPS = D / 16;
-    const int g = blockIdx.y, lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
-    const int k0 = (blockIdx.x * 4 + wv) * TK;
-    if (k0 >= p.n) return;
-    const uint16_t* kr = p.K + (size_t)g * p.hs + (size_t)min(k0 + c, p.n - 1) * p.rs + 8 * h;
-    bf16x8 kf[STEPS];
+__global__ void __launch_bounds__(256, 2) attn_mass_kernel(MassArgs p) {
+    constexpr int STEPS = D / 16, CH = D / 8, KPI = 64 / CH;
+    constexpr int STAGE = 16 * KPI, TILES = STAGE / 32, TILE = TK * 2 * D, AHEAD = 4;  // pairs a stage (four loads a wave), its tiles
+    __shared__ __align__(16) uint8_t q_lds[2][TILES * TILE];
+    __shared__ __align__(16) float logs[MA_META];
+    __shared__ __align__(16) int limits[MA_META];
+    __shared__ int least[MA_META / 32];  // the smallest limit of a tile
+    const int g = blockIdx.y, lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
+    const int k0 = blockIdx.x * MA_KEYS + 64 * wv;
+    const int pairs = p.T * p.G, stages = (pairs + STAGE - 1) / STAGE;
+    const int per = (stages + p.parts - 1) / p.parts, first = blockIdx.z * per, end = min(first + per, stages);
+    // the lane's pairs of a stage: STAGE s + mine + KPI i. r / G by multiplication (G <= 32, r < 2^24: exact)
+    const int mine = 4 * KPI * wv + lane / CH;
+    const uint32_t by_g = 0xFFFFFFFFu / (uint32_t)p.G + 1;
+    auto row_of = [&](int r) { return p.G == 1 ? r : (int)__umulhi((uint32_t)r, by_g); };
+    const char* qb = reinterpret_cast<const char*>(uniform(p.q));
+    auto issue = [&](int s, int b) {
+        uint32_t off[4];
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) kf[s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(kr + 16 * s));
-    const int pairs = p.T * p.G;
-    float sum[16];
+        for (int i = 0; i < 4; ++i) {
+            const int r = min(s * STAGE + mine + KPI * i, pairs - 1), t = row_of(r);
+            off[i] = (uint32_t)(t * p.Hq + g * p.G + (r - t * p.G)) * (2 * D) + 16 * k_chunk<D>((mine + KPI * i) & 31, lane % CH);
+        }
+        load4_to_lds(qb, 0, off[0], off[1], off[2], off[3],
+                     (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_address(&q_lds[b][4 * KPI * wv * 2 * D])));
+    };
+    bf16x8 kf[2][STEPS];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sum[i] = 0.f;
-    for (int r0 = 0; r0 < pairs; r0 += 32) {
-        const int r = min(r0 + c, pairs - 1), t = r / p.G;
-        const size_t at = (size_t)t * p.Hq + g * p.G + (r - t * p.G);
-        const float z = p.lse[at];
-        // a pair past the last, or one that saw nothing, adds nothing
-        const int lim = r0 + c < pairs && z != -__builtin_inff() ? p.seen[t] : 0;
-        const float zl = z * 1.44269504088896341f;
-        f32x16 st = zero16();
+    for (int k = 0; k < 2; ++k) {
+        const uint16_t* kr = p.K + (size_t)g * p.hs + (size_t)min(k0 + 32 * k + c, p.n - 1) * p.rs + 8 * h;
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-            st = mfma32(kf[s], __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(p.q + at * D + 16 * s + 8 * h)), st);
+        for (int s = 0; s < STEPS; ++s) kf[k][s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(kr + 16 * s));
+    }
+    float sum[2] = {0.f, 0.f}, z[16];
+    f32x16 st[2], next[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) st[k] = zero16();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = __builtin_inff();  // the tile before the first: weights of zero
+    auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
+    // the next tile's scores; work(i) after each of the STEPS
+    auto scores = [&](const uint8_t* tile, uint32_t at, auto work) {
+        bf16x8 qf[STEPS];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) next[k] = zero16();
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) qf[i] = k_fragment(tile, at, 0, i);
+        fence();
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            if (i + AHEAD < STEPS) qf[i + AHEAD] = k_fragment(tile, at, 0, i + AHEAD);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) next[k] = mfma32(qf[i], kf[k][i], next[k]);
+            work(i);
+            fence();
+        }
+    };
+    constexpr int EACH = 16 / STEPS;
+    bool plain = true;
+    auto weigh = [&](int step) {  // keys that every pair of the tile sees
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            sum[i] += k0 + 8 * (i / 4) + 4 * h + i % 4 < lim ? __builtin_amdgcn_exp2f(fmaf(st[i], p.scale_log2, -zl)) : 0.f;
-    }
-    // over the 32 pairs of a tile: the same key in the 32 lanes of a half
+            if (i / EACH == step)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        float v = sum[i];
+                for (int k = 0; k < 2; ++k) sum[k] += __builtin_amdgcn_exp2f(fmaf(st[k][i], p.scale_log2, -z[i]));
+    };
+    auto weigh_seen = [&](const int* limit) {
+        float lim[16];
+        of_pairs(reinterpret_cast<const float*>(limit), h, lim);
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) v += __shfl_xor(v, d, WAVE);
-        const int key = k0 + 8 * (i / 4) + 4 * h + i % 4;
-        if (c == i && key < p.n)
-            p.out[(size_t)g * p.os + key] = v + (p.mass != nullptr ? p.mass[(size_t)g * p.ms + key] : 0.f);
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                sum[k] += k0 + 32 * k + c < __builtin_bit_cast(int, lim[i])
+                              ? __builtin_amdgcn_exp2f(fmaf(st[k][i], p.scale_log2, -z[i]))
+                              : 0.f;
+    };
+    if (first < end) issue(first, 0);
+    const uint32_t place = k_place<D>(lane);
+    int before = 0;  // the pair of the stages' LDS that the tile in st starts with
+    for (int s = first; s < end; ++s) {
+        const int b = (s - first) & 1, at_meta = (s - first) * STAGE % MA_META;
+        if (at_meta == 0) {  // uniform
+            if (s > first) {
+                if (plain) {
+                    for (int i = 0; i < STEPS; ++i) weigh(i);
+                } else {
+                    weigh_seen(limits + before);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) z[i] = __builtin_inff();
+                plain = true;
+            }
+            __syncthreads();
+            for (int e = threadIdx.x; e < MA_META; e += 256) {
+                const int r = s * STAGE + e;
+                int seen;
+                pair_facts(p, g, r, pairs, row_of(min(r, pairs - 1)), logs[e], seen);
+                limits[e] = seen;
+                const int low = half_min(seen);
+                if (c == 0) least[e / 32] = low;
+            }
+        }
+        uint32_t at = place;
+        wait_loads<0>(at);
+        __syncthreads();  // the stage is here, and the other buffer free
+        if (s + 1 < end) issue(s + 1, b ^ 1);
+#pragma unroll 1
+        for (int q = 0; q < TILES; ++q) {
+            asm volatile("" : "+v"(at));  // eight places a lane are made each time and not kept
+            if (plain) {
+                scores(q_lds[b] + q * TILE, at, weigh);
+            } else {
+                scores(q_lds[b] + q * TILE, at, [](int) {});
+                weigh_seen(limits + before);
+            }
+            st[0] = next[0];
+            st[1] = next[1];
+            before = at_meta + 32 * q;
+            of_pairs(logs + before, h, z);
+            plain = least[before / 32] >= k0 + 64;
+        }
     }
+    if (plain) {
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) weigh(i);
+    } else {
+        weigh_seen(limits + before);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const float v = sum[k] + xor32(sum[k]);
+        const int key = k0 + 32 * k + c;
+        if (h == 0 && key < p.n) {
+            if (p.parts > 1)
+                p.work[((size_t)blockIdx.z * p.Hk + g) * p.n + key] = v;
+            else
+                p.out[(size_t)g * p.os + key] = v + (p.mass != nullptr ? p.mass[(size_t)g * p.ms + key] : 0.f);
+        }
+    }
+}
+
+// Few pairs: QT tiles of 32. A wave of eight takes every (8 gridDim.x)-th tile of a head's keys, two LDS buffers of its own. Sums
+// meet the mass they are added to eight tiles at a time: the wait for a loaded register waits for the keys on their way too.
+template <int D, int QT>
+__global__ void __launch_bounds__(512, 2) attn_mass_few_kernel(MassArgs p) {
+    constexpr int STEPS = D / 16, TILE = TK * 2 * D, N = TileLoads<D>::N;
+    extern __shared__ __align__(16) uint8_t lds[];  // [8 waves][2] tiles of keys
+    __shared__ __align__(16) float logs[32 * QT];
+    __shared__ __align__(16) int limits[32 * QT];
+    __shared__ float kept[8][8][32];
+    const int g = blockIdx.y, lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
+    const int pairs = p.T * p.G, tiles = (p.n + TK - 1) / TK, step = 8 * gridDim.x;
+    const uint16_t* Kg = p.K + (size_t)g * p.hs;
+    uint8_t* mine = lds + wv * 2 * TILE;
+    TileLoads<D> loads;
+    loads.make(p.rs, lane);
+    auto issue = [&](int tile, int b) {
+        loads.template issue<true>(Kg + (size_t)tile * TK * p.rs, p.rs, p.n - tile * TK, mine + b * TILE, lane);
+    };
+    const int first = blockIdx.x + gridDim.x * wv;
+    if (first < tiles) issue(first, 0);
+    if (threadIdx.x < 32 * QT) {
+        const int r = threadIdx.x;
+        int seen;
+        pair_facts(p, g, r, pairs, min(r, pairs - 1) / p.G, logs[r], seen);
+        limits[r] = seen;
+    }
+    bf16x8 qf[QT][STEPS];
+#pragma unroll
+    for (int q = 0; q < QT; ++q) {
+        const int r = min(32 * q + c, pairs - 1), t = r / p.G;
+        const uint16_t* qr = p.q + ((size_t)t * p.Hq + g * p.G + (r - t * p.G)) * D + 8 * h;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) qf[q][s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(qr + 16 * s));
+    }
+    __syncthreads();  // (and every load so far: the counted waits below find only the keys')
+    float z[QT][16], lim[QT][16];
+    int least = 0x7FFFFFFF;
+#pragma unroll
+    for (int q = 0; q < QT; ++q) {
+        of_pairs(logs + 32 * q, h, z[q]);
+        of_pairs(reinterpret_cast<const float*>(limits) + 32 * q, h, lim[q]);
+        least = min(least, half_min(limits[32 * q + c]));
+    }
+    least = __builtin_amdgcn_readfirstlane(least);
+    const uint32_t place = k_place<D>(lane);
+    int held = 0;
+    for (int tile = first, b = 0; tile < tiles; tile += step, b ^= 1) {
+        uint32_t at = place;
+        if (tile + step < tiles) {
+            issue(tile + step, b ^ 1);
+            wait_loads<N>(at);
+        } else {
+            wait_loads<0>(at);
+        }
+        const int key = tile * TK + c;
+        f32x16 st[QT];
+#pragma unroll
+        for (int q = 0; q < QT; ++q) st[q] = zero16();
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            const bf16x8 kf = k_fragment(mine + b * TILE, at, 0, i);
+#pragma unroll
+            for (int q = 0; q < QT; ++q) st[q] = mfma32(qf[q][i], kf, st[q]);
+        }
+        float sum = 0.f;
+        if (least >= tile * TK + TK) {
+#pragma unroll
+            for (int q = 0; q < QT; ++q)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f(fmaf(st[q][i], p.scale_log2, -z[q][i]));
+        } else {
+#pragma unroll
+            for (int q = 0; q < QT; ++q)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    sum += key < __builtin_bit_cast(int, lim[q][i]) ? __builtin_amdgcn_exp2f(fmaf(st[q][i], p.scale_log2, -z[q][i])) : 0.f;
+        }
+        sum += xor32(sum);
+        if (h == 0) kept[wv][held][c] = sum;
+        ++held;
+        if (held == 8 || tile + step >= tiles) {  // uniform
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const int key = (tile - (held - 1 - i - h) * step) * TK + c;
+                if (i + h < held && key < p.n)
+                    p.out[(size_t)g * p.os + key] = kept[wv][i + h][c] + (p.mass != nullptr ? p.mass[(size_t)g * p.ms + key] : 0.f);
+            }
+            held = 0;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+__global__ void __launch_bounds__(256) attn_mass_add_kernel(MassArgs p) {
+    const int key = blockIdx.x * 256 + threadIdx.x, g = blockIdx.y;
+    if (key >= p.n) return;
+    float v = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < p.parts; ++i) v += p.work[((size_t)i * p.Hk + g) * p.n + key];
+    p.out[(size_t)g * p.os + key] = v + (p.mass != nullptr ? p.mass[(size_t)g * p.ms + key] : 0.f);
+}
+
+// workgroups the pairs are cut over: until there are two a CU, each with two stages and more
+static int mass_parts(size_t T, size_t Hq, size_t Hk, size_t D, size_t n) {
+    if (T * (Hq / Hk) <= (size_t)MA_FEW) return 1;
+    const size_t wgs = Hk * ((n + MA_KEYS - 1) / MA_KEYS), stages = (T * (Hq / Hk) * D / 64 + 127) / 128;
+    const size_t want = 2 * (size_t)device_info().cus / wgs, most = stages / 2;
+    const size_t parts = want < most ? want : most;
+    return (int)(parts > 1 ? parts : 1);
+}
+static bool mass_sizes_fit(size_t T, size_t Hq, size_t Hk, size_t D, size_t n) {
+    return T > 0 && Hk > 0 && Hk <= 1024 && Hq > 0 && Hq % Hk == 0 && Hq / Hk <= 32 && T <= (1u << 23) / Hq && (D == 64 || D == 128) &&
+           n > 0 && n <= 0x7FFFFF00u;
+}
+
+template <int D, int QT>
+static int32_t launch_few(const MassArgs& p, hipStream_t st) {
+    constexpr int lds = 16 * TK * 2 * D;
+    const void* kern = reinterpret_cast<const void*>(attn_mass_few_kernel<D, QT>);
+    if (lds > 60 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return hip_status(e, "hipFuncSetAttribute");
+    }
+    // a workgroup a CU, a tile a wave at least
+    const int tiles = (p.n + TK - 1) / TK, cus = device_info().cus, most = (tiles + 7) / 8, want = (cus + p.Hk - 1) / p.Hk;
+    const dim3 grid((unsigned)(want < most ? want : most), (unsigned)p.Hk);
+    hipLaunchKernelGGL((attn_mass_few_kernel<D, QT>), grid, dim3(512), lds, st, p);
+    return hip_status(hipGetLastError(), "attn_mass launch");
 }
 
 }  // namespace btb
@@ -73,18 +347,25 @@ using namespace btb;
 
 extern "C" {
 
+size_t btb_hip_attn_mass_floats(size_t T, size_t Hq, size_t Hk, size_t D, size_t n) {
+    if (!mass_sizes_fit(T, Hq, Hk, D, n)) return 0;
+    const size_t parts = (size_t)mass_parts(T, Hq, Hk, D, n);
+    return parts > 1 ? parts * Hk * n : 0;
+}
+
 int32_t btb_hip_attn_mass(const void* q, const void* K, const float* lse, const int32_t* seen, const float* mass, float* out,
                           size_t T, size_t Hq, size_t Hk, size_t D, size_t n, int64_t hs, int64_t rs, int64_t mass_stride,
-                          int64_t out_stride, float scale, void* stream) {
+                          int64_t out_stride, float scale, float* workspace, void* stream) {
     if (!q || !K || !lse || !seen || !out) return ERR_NULL;
     auto loose = [](const void* a) { return ((uintptr_t)a & 15u) != 0; };
-    if (T == 0 || T > 65536 || Hk == 0 || Hk > 1024 || Hq == 0 || Hq % Hk != 0 || Hq / Hk > 32 || (D != 64 && D != 128) ||
-        n == 0 || n > 0x7FFFFF00u || hs < 0 || rs < 0 || hs % 8 || rs % 8 || mass_stride < 0 || out_stride < 0 ||
+    if (!mass_sizes_fit(T, Hq, Hk, D, n) || hs < 0 || rs < 0 || rs > (1 << 25) || hs % 8 || rs % 8 || mass_stride < 0 || out_stride < 0 ||
         !(scale > 0.f) || !(scale < __builtin_inff()) || loose(q) || loose(K)) {
         set_error("attn_mass: head_dim 64 or 128, up to 32 query heads a kv head, a positive scale, q and K 16-byte aligned "
-                  "with strides in multiples of 8");
+                  "with strides in multiples of 8, a row's up to 2^25");
         return ERR_DOMAIN;
     }
+    const int parts = mass_parts(T, Hq, Hk, D, n);
+    if (parts > 1 && workspace == nullptr) return ERR_NULL;
     MassArgs p;
     p.q = static_cast<const uint16_t*>(q);
     p.K = static_cast<const uint16_t*>(K);
@@ -92,6 +373,9 @@ int32_t btb_hip_attn_mass(const void* q, const void* K, const float* lse, const 
     p.seen = seen;
     p.mass = mass;
     p.out = out;
+    p.work = workspace;
+    p.parts = parts;
+    p.Hk = (int)Hk;
     p.hs = hs;
     p.rs = rs;
     p.ms = mass_stride;
@@ -102,11 +386,17 @@ int32_t btb_hip_attn_mass(const void* q, const void* K, const float* lse, const 
     p.G = (int)(Hq / Hk);
     p.n = (int)n;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const dim3 grid((unsigned)((n + 4 * TK - 1) / (4 * TK)), (unsigned)Hk);
+    const size_t pairs = T * (Hq / Hk);
+    if (pairs <= (size_t)MA_FEW) {
+        if (D == 64) return pairs <= 32 ? launch_few<64, 1>(p, st) : launch_few<64, 2>(p, st);
+        return pairs <= 32 ? launch_few<128, 1>(p, st) : launch_few<128, 2>(p, st);
+    }
+    const dim3 grid((unsigned)((n + MA_KEYS - 1) / MA_KEYS), (unsigned)Hk, (unsigned)parts);
     if (D == 64)
         hipLaunchKernelGGL(attn_mass_kernel<64>, grid, dim3(256), 0, st, p);
     else
         hipLaunchKernelGGL(attn_mass_kernel<128>, grid, dim3(256), 0, st, p);
+    if (parts > 1) hipLaunchKernelGGL(attn_mass_add_kernel, dim3((unsigned)((n + 255) / 256), (unsigned)Hk), dim3(256), 0, st, p);
     return hip_status(hipGetLastError(), "attn_mass launch");
 }
 

@@ -114,7 +114,8 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "btb_hip_attn_shared": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, ctypes.c_int64, ctypes.c_int64,
                                    ctypes.c_float, _sz, _sz, _vp, _vp]),
     "btb_hip_attn_mass": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz] + [ctypes.c_int64] * 4 +
-                          [ctypes.c_float, _vp]),
+                          [ctypes.c_float, _vp, _vp]),
+    "btb_hip_attn_mass_floats": (_sz, [_sz] * 5),
     "btb_hip_kv_evict": (_i32, [_vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp] + [ctypes.c_int64] * 3 + [_sz] * 5 +
                          [_i32, _i32, _vp, _vp] + [ctypes.c_int64] * 3 + [_vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp, _vp]),
     "btb_hip_kv_evict_words": (_sz, [_sz, _sz, _sz]),
@@ -1158,8 +1159,11 @@ class HipCard(CardLaunch):
             if t is not None and (not isinstance(t, _Tensor) or t.dtype is not torch.float32 or not t.is_cuda or t.dim() != 2
                                   or t.shape[0] != Hk or t.shape[1] < n or t.stride(1) != 1):
                 raise ValueError(f"[hip] attn_mass: {what} is float32 [{Hk}, >= {n}] on the GPU, a head's values together")
+        floats = self.lib.btb_hip_attn_mass_floats(T, Hq, Hk, D, n)
+        ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
         self._call("btb_hip_attn_mass", _p(q), _p(K), _p(lse), _p(seen), None if mass is None else _p(mass), _p(out), T, Hq, Hk,
-                   D, n, K.stride(0), K.stride(1), 0 if mass is None else mass.stride(0), out.stride(0), float(scale), _stream())
+                   D, n, K.stride(0), K.stride(1), 0 if mass is None else mass.stride(0), out.stride(0), float(scale),
+                   None if ws is None else _p(ws), _stream())
         return out
 
     def kv_evict(self, mass: torch.Tensor, pos: torch.Tensor, K: torch.Tensor, V: torch.Tensor, n: int, budget: int,

@@ -478,7 +478,7 @@ def test_refusals(card):
     lib, p = card.lib, lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())
     assert lib.btb_hip_attn_shared(None, p(K), p(V), p(att), None, p(lay), T, Hq, Hk, D, cap, 1, 1, 0.1, 20, 4, p(scratch), None) == -1
     assert lib.btb_hip_attn_shared(p(q), p(K), p(V), p(att), None, p(lay), T, 7, 2, D, cap, 8, 8, 0.1, 20, 4, p(scratch), None) == -6
-    assert lib.btb_hip_attn_mass(p(q), p(K), p(lse), None, None, p(lse), T, Hq, Hk, D, 10, 8, 8, 0, 0, 0.1, None) == -1
+    assert lib.btb_hip_attn_mass(p(q), p(K), p(lse), None, None, p(lse), T, Hq, Hk, D, 10, 8, 8, 0, 0, 0.1, None, None) == -1
     assert lib.btb_hip_kv_evict(p(mass), 1, None, 1, p(K), p(V), 0, 8, 8, 1, Hk, D, 16, 8, 0, 0, p(K), p(V), 0, 8, 8, p(mass), 1, p(p32), 1,
                                 p(idx), None, None) == -1
     assert lib.btb_hip_norm_rope_axes(p(qkv), None, None, 1e-6, p(cos), p(cos), 0, 16, D, p(pos), 3, p(axes), None, p(K), p(V), p(q), T, Hq,
