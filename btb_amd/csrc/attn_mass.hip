@@ -147,6 +147,8 @@ __global__ void __launch_bounds__(256, 2) attn_mass_kernel(MassArgs p) {
                               : 0.f;
     };
     if (first < end) issue(first, 0);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the keys are here, and no register of the loop waits for a load
+    __builtin_amdgcn_sched_barrier(0);
     const uint32_t place = k_place<D>(lane);
     int before = 0;  // the pair of the stages' LDS that the tile in st starts with
     for (int s = first; s < end; ++s) {
