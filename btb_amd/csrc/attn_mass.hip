@@ -22,7 +22,7 @@
 namespace btb {
 
 constexpr int MA_KEYS = 256;   // many pairs: keys a workgroup, four waves of two tiles
-constexpr int MA_META = 2048;  // pairs whose log-sums and limits lie in LDS at a time
+constexpr int MA_META = 1024;  // pairs whose log-sums and limits lie in LDS at a time
 constexpr int MA_FEW = 64;     // few pairs, at most
 
 struct MassArgs {
@@ -71,7 +71,7 @@ __device__ __forceinline__ void of_pairs(const float* from, int h, float (&v)[16
 template <int D>
 __global__ void __launch_bounds__(256, 2) attn_mass_kernel(MassArgs p) {
     constexpr int STEPS = D / 16, CH = D / 8, KPI = 64 / CH;
-    constexpr int STAGE = 16 * KPI, TILES = STAGE / 32, TILE = TK * 2 * D, AHEAD = 4;  // pairs a stage (four loads a wave), its tiles
+    constexpr int STAGE = 32 * KPI, TILES = STAGE / 32, TILE = TK * 2 * D, AHEAD = 4;  // pairs a stage (eight loads a wave), its tiles
     __shared__ __align__(16) uint8_t q_lds[2][TILES * TILE];
     __shared__ __align__(16) float logs[MA_META];
     __shared__ __align__(16) int limits[MA_META];
@@ -81,19 +81,22 @@ __global__ void __launch_bounds__(256, 2) attn_mass_kernel(MassArgs p) {
     const int pairs = p.T * p.G, stages = (pairs + STAGE - 1) / STAGE;
     const int per = (stages + p.parts - 1) / p.parts, first = blockIdx.z * per, end = min(first + per, stages);
     // the lane's pairs of a stage: STAGE s + mine + KPI i. r / G by multiplication (G <= 32, r < 2^24: exact)
-    const int mine = 4 * KPI * wv + lane / CH;
+    const int mine = 8 * KPI * wv + lane / CH;
     const uint32_t by_g = 0xFFFFFFFFu / (uint32_t)p.G + 1;
     auto row_of = [&](int r) { return p.G == 1 ? r : (int)__umulhi((uint32_t)r, by_g); };
     const char* qb = reinterpret_cast<const char*>(uniform(p.q));
     auto issue = [&](int s, int b) {
-        uint32_t off[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = min(s * STAGE + mine + KPI * i, pairs - 1), t = row_of(r);
-            off[i] = (uint32_t)(t * p.Hq + g * p.G + (r - t * p.G)) * (2 * D) + 16 * k_chunk<D>((mine + KPI * i) & 31, lane % CH);
+        for (int half = 0; half < 2; ++half) {
+            uint32_t off[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = mine + KPI * (4 * half + i), r = min(s * STAGE + at, pairs - 1), t = row_of(r);
+                off[i] = (uint32_t)(t * p.Hq + g * p.G + (r - t * p.G)) * (2 * D) + 16 * k_chunk<D>(at & 31, lane % CH);
+            }
+            const uint32_t to = lds_address(&q_lds[b][(8 * KPI * wv + 4 * KPI * half) * 2 * D]);
+            load4_to_lds(qb, 0, off[0], off[1], off[2], off[3], (uint32_t)__builtin_amdgcn_readfirstlane((int)to));
         }
-        load4_to_lds(qb, 0, off[0], off[1], off[2], off[3],
-                     (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_address(&q_lds[b][4 * KPI * wv * 2 * D])));
     };
     bf16x8 kf[2][STEPS];
 #pragma unroll
@@ -102,68 +105,94 @@ __global__ void __launch_bounds__(256, 2) attn_mass_kernel(MassArgs p) {
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) kf[k][s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(kr + 16 * s));
     }
-    float sum[2] = {0.f, 0.f}, z[16];
-    f32x16 st[2], next[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) st[k] = zero16();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) z[i] = __builtin_inff();  // the tile before the first: weights of zero
-    auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
-    // the next tile's scores; work(i) after each of the STEPS
-    auto scores = [&](const uint8_t* tile, uint32_t at, auto work) {
-        bf16x8 qf[STEPS];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) next[k] = zero16();
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) qf[i] = k_fragment(tile, at, 0, i);
-        fence();
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            if (i + AHEAD < STEPS) qf[i + AHEAD] = k_fragment(tile, at, 0, i + AHEAD);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) next[k] = mfma32(qf[i], kf[k][i], next[k]);
-            work(i);
-            fence();
-        }
+    // a tile's scores against the wave's two tiles of keys, its pairs' log-sums, its first pair among those in `logs`, and whether
+    // its pairs see all of the wave's keys
+    struct Tile {
+        f32x16 s[2];
+        float z[16];
+        int pair, least;
     };
+    Tile one, two;
+    float sum[2] = {0.f, 0.f};
+    auto empty = [&](Tile& t) {  // no tile: weights of zero
+#pragma unroll
+        for (int k = 0; k < 2; ++k) t.s[k] = zero16();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t.z[i] = __builtin_inff();
+        t.pair = 0;
+        t.least = 0x7FFFFFFF;
+    };
+    auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
     constexpr int EACH = 16 / STEPS;
-    bool plain = true;
-    auto weigh = [&](int step) {  // keys that every pair of the tile sees
+    auto weigh = [&](const Tile& t, int step) {  // keys that every pair of the tile sees
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             if (i / EACH == step)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) sum[k] += __builtin_amdgcn_exp2f(fmaf(st[k][i], p.scale_log2, -z[i]));
+                for (int k = 0; k < 2; ++k) sum[k] += __builtin_amdgcn_exp2f(fmaf(t.s[k][i], p.scale_log2, -t.z[i]));
     };
-    auto weigh_seen = [&](const int* limit) {
+    auto weigh_seen = [&](const Tile& t) {
         float lim[16];
-        of_pairs(reinterpret_cast<const float*>(limit), h, lim);
+        of_pairs(reinterpret_cast<const float*>(limits) + t.pair, h, lim);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
 #pragma unroll
             for (int k = 0; k < 2; ++k)
                 sum[k] += k0 + 32 * k + c < __builtin_bit_cast(int, lim[i])
-                              ? __builtin_amdgcn_exp2f(fmaf(st[k][i], p.scale_log2, -z[i]))
+                              ? __builtin_amdgcn_exp2f(fmaf(t.s[k][i], p.scale_log2, -t.z[i]))
                               : 0.f;
     };
+    auto settle = [&](const Tile& t) {
+        if (t.least >= k0 + 64) {
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) weigh(t, i);
+        } else {
+            weigh_seen(t);
+        }
+    };
+    // Tile q of the stage: its scores into `to` while `from` is weighed. Its first fragments are in `head`; the next tile's come
+    // into it on the way.
+    bf16x8 head[AHEAD];
+    auto step = [&](const Tile& from, Tile& to, const uint8_t* tiles, uint32_t at, int q, int pair) {
+        to.pair = pair;
+        to.least = least[pair / 32];
+        of_pairs(logs + pair, h, to.z);
+        auto scores = [&](auto work) {
+            bf16x8 qf[STEPS + AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) qf[i] = head[i];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) to.s[k] = zero16();
+            fence();
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) {
+                if (i + AHEAD < STEPS || q + 1 < TILES)
+                    qf[i + AHEAD] = k_fragment(tiles, at, (q + (i + AHEAD) / STEPS) * TILE, (i + AHEAD) % STEPS);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) to.s[k] = mfma32(qf[i], kf[k][i], to.s[k]);
+                work(i);
+                fence();
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) head[i] = qf[q + 1 < TILES ? STEPS + i : i];
+        };
+        if (from.least >= k0 + 64) {
+            scores([&](int i) { weigh(from, i); });
+        } else {
+            scores([](int) {});
+            weigh_seen(from);
+        }
+    };
+    empty(one);
     if (first < end) issue(first, 0);
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the keys are here, and no register of the loop waits for a load
-    __builtin_amdgcn_sched_barrier(0);
+    fence();
     const uint32_t place = k_place<D>(lane);
-    int before = 0;  // the pair of the stages' LDS that the tile in st starts with
     for (int s = first; s < end; ++s) {
         const int b = (s - first) & 1, at_meta = (s - first) * STAGE % MA_META;
         if (at_meta == 0) {  // uniform
-            if (s > first) {
-                if (plain) {
-                    for (int i = 0; i < STEPS; ++i) weigh(i);
-                } else {
-                    weigh_seen(limits + before);
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) z[i] = __builtin_inff();
-                plain = true;
-            }
+            settle(one);
+            empty(one);
             __syncthreads();
             for (int e = threadIdx.x; e < MA_META; e += 256) {
                 const int r = s * STAGE + e;
@@ -178,28 +207,16 @@ __global__ void __launch_bounds__(256, 2) attn_mass_kernel(MassArgs p) {
         wait_loads<0>(at);
         __syncthreads();  // the stage is here, and the other buffer free
         if (s + 1 < end) issue(s + 1, b ^ 1);
-#pragma unroll 1
-        for (int q = 0; q < TILES; ++q) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) head[i] = k_fragment(q_lds[b], at, 0, i);
+#pragma unroll
+        for (int q = 0; q < TILES; q += 2) {
             asm volatile("" : "+v"(at));  // eight places a lane are made each time and not kept
-            if (plain) {
-                scores(q_lds[b] + q * TILE, at, weigh);
-            } else {
-                scores(q_lds[b] + q * TILE, at, [](int) {});
-                weigh_seen(limits + before);
-            }
-            st[0] = next[0];
-            st[1] = next[1];
-            before = at_meta + 32 * q;
-            of_pairs(logs + before, h, z);
-            plain = least[before / 32] >= k0 + 64;
+            step(one, two, q_lds[b], at, q, at_meta + 32 * q);
+            step(two, one, q_lds[b], at, q + 1, at_meta + 32 * q + 32);
         }
     }
-    if (plain) {
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) weigh(i);
-    } else {
-        weigh_seen(limits + before);
-    }
+    settle(one);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const float v = sum[k] + xor32(sum[k]);
