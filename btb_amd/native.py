@@ -1051,13 +1051,20 @@ class HipCard(CardLaunch):
     # -- a batch over one shared, bounded cache -----------------------------------------------------------------------
 
     @staticmethod
-    def _cache_views(K: torch.Tensor, V: torch.Tensor, Hk: int, D: int, what: str) -> None:
-        """one layer's keys and values as the operators below take them"""
-        for t in (K, V):
-            if not isinstance(t, _Tensor) or t.dtype is not torch.bfloat16 or not t.is_cuda or t.dim() != 3:
-                raise ValueError(f"[hip] {what}: K and V are bf16 [Hk, cap, D] views on the GPU")
-        if K.shape != V.shape or K.stride() != V.stride() or K.shape[0] != Hk or K.shape[2] != D or K.stride(2) != 1:
+    def _plain(t: torch.Tensor, dtype: torch.dtype) -> bool:
+        """whether t is a contiguous tensor of this type on the GPU"""
+        return isinstance(t, _Tensor) and t.dtype is dtype and t.is_cuda and t.is_contiguous()
+
+    @staticmethod
+    def _cache_strides(K: torch.Tensor, V: torch.Tensor, Hk: int, D: int, what: str) -> tuple[int, int, int]:
+        """one layer's keys and values as the operators below take them: strides of a head and of a row, rows"""
+        if not (isinstance(K, _Tensor) and isinstance(V, _Tensor) and K.dtype is torch.bfloat16 and V.dtype is torch.bfloat16
+                and K.is_cuda and V.is_cuda and K.dim() == 3):
+            raise ValueError(f"[hip] {what}: K and V are bf16 [Hk, cap, D] views on the GPU")
+        strides, shape = K.stride(), K.shape
+        if V.shape != shape or V.stride() != strides or shape[0] != Hk or shape[2] != D or strides[2] != 1:
             raise ValueError(f"[hip] {what}: K and V are [{Hk}, cap, {D}] views with the same strides, D contiguous")
+        return strides[0], strides[1], shape[1]
 
     def norm_rope_axes(self, qkv: torch.Tensor, wq: torch.Tensor | None, wk: torch.Tensor | None, eps: float,
                        cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, axes: torch.Tensor, slots: torch.Tensor,
@@ -1067,32 +1074,28 @@ class HipCard(CardLaunch):
         stands at pos[a, t] (int32 [A, T]) on axis a, frequency i turns by axis axes[i] (uint8 [D / 2], `rope_axes`), and
         the new k and v go to cache row slots[t] (int32 [T], distinct; outside the cache: not written). cos / sin:
         [positions, D] or [positions, D / 2], bf16 or float32. f32 throughout, rounded once."""
-        self._need(qkv, torch.bfloat16, "qkv")
-        self._need(q, torch.bfloat16, "q")
-        for t, what in ((wq, "wq"), (wk, "wk")):
-            if t is not None:
-                self._need(t, torch.bfloat16, what)
-                if t.numel() != D:
-                    raise ValueError(f"[hip] norm_rope_axes: {what} holds {t.numel()} values, head_dim is {D}")
-        if cos.dtype not in (torch.bfloat16, torch.float32):
-            raise ValueError("[hip] norm_rope_axes: the tables are bf16 or float32")
-        self._need(cos, cos.dtype, "cos")
-        self._need(sin, cos.dtype, "sin")
-        if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] not in (D, D // 2):
-            raise ValueError(f"[hip] norm_rope_axes: the tables are [positions, {D}] or [positions, {D // 2}]")
-        self._need(pos, torch.int32, "pos")
-        self._need(axes, torch.uint8, "axes")
-        self._need(slots, torch.int32, "slots")
-        self._cache_views(K, V, Hk, D, "norm_rope_axes")
-        T = int(slots.numel())
+        bf, f32 = torch.bfloat16, torch.float32
+        tables = cos.dtype
+        if not (self._plain(qkv, bf) and self._plain(q, bf) and self._plain(cos, tables) and self._plain(sin, tables)
+                and (tables is bf or tables is f32) and self._plain(pos, torch.int32) and self._plain(axes, torch.uint8)
+                and self._plain(slots, torch.int32) and (wq is None or self._plain(wq, bf)) and (wk is None or self._plain(wk, bf))):
+            raise ValueError("[hip] norm_rope_axes: qkv, q, wq and wk are bfloat16, cos and sin bfloat16 or float32, pos and slots int32, "
+                             "axes uint8, all contiguous on the GPU")
+        hs, rs, cap = self._cache_strides(K, V, Hk, D, "norm_rope_axes")
+        T = slots.numel()
+        positions, width = cos.shape
+        A, cols = pos.shape
         if T < 1 or qkv.numel() != T * (Hq + 2 * Hk) * D or q.numel() != T * Hq * D:
             raise ValueError("[hip] norm_rope_axes: qkv is [T, (Hq + 2 Hk) D], q [T, Hq D], slots [T]")
-        if pos.dim() != 2 or pos.shape[1] != T or axes.numel() != D // 2:
-            raise ValueError(f"[hip] norm_rope_axes: pos is [axes, {T}], axes names the axis of {D // 2} frequencies")
-        p = lambda t: None if t is None else _p(t)
-        self._call("btb_hip_norm_rope_axes", _p(qkv), p(wq), p(wk), float(eps), _p(cos), _p(sin),
-                   int(cos.dtype is torch.float32), cos.shape[0], cos.shape[1], _p(pos), pos.shape[0], _p(axes), _p(slots),
-                   _p(K), _p(V), _p(q), T, Hq, Hk, D, K.shape[1], K.stride(0), K.stride(1), int(bool(centered)), _stream())
+        if cols != T or axes.numel() != D // 2 or (width != D and width != D // 2) or sin.shape != cos.shape:
+            raise ValueError(f"[hip] norm_rope_axes: pos is [axes, {T}], axes names the axis of {D // 2} frequencies, the tables are "
+                             f"[positions, {D}] or [positions, {D // 2}]")
+        if (wq is not None and wq.numel() != D) or (wk is not None and wk.numel() != D):
+            raise ValueError(f"[hip] norm_rope_axes: a norm weight holds head_dim = {D} values")
+        self._call("btb_hip_norm_rope_axes", qkv.data_ptr(), None if wq is None else wq.data_ptr(),
+                   None if wk is None else wk.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(), tables is f32, positions, width,
+                   pos.data_ptr(), A, axes.data_ptr(), slots.data_ptr(), K.data_ptr(), V.data_ptr(), q.data_ptr(), T, Hq, Hk, D, cap,
+                   hs, rs, bool(centered), _stream())
 
     @staticmethod
     def shared_layout(off: int, n: int, rows: Sequence[tuple[int, int]], pad_to: int = 0, device: Any = "cuda") -> torch.Tensor:
@@ -1118,52 +1121,49 @@ class HipCard(CardLaunch):
         """att [T, Hq D] = attention of T rows over a prefix they share, read once for all of them, and keys of their own,
         both as `shared_layout` lays them out in one layer's cache; lse (float32 [T, Hq]): the rows' log-sum-exp. The
         lengths are read on the device; prefix_cap and own_cap are the most they may be."""
-        self._need(q, torch.bfloat16, "q")
-        self._need(att, torch.bfloat16, "att")
-        self._need(lay, torch.int32, "lay")
-        self._need(scratch, torch.float32, "scratch")
-        self._cache_views(K, V, Hk, D, "attn_shared")
-        T = int(lay.numel()) // 2 - 1
-        if T < 1 or lay.numel() != 2 + 2 * T or q.numel() != T * Hq * D or att.numel() != T * Hq * D:
+        if not (self._plain(q, torch.bfloat16) and self._plain(att, torch.bfloat16) and self._plain(lay, torch.int32)
+                and self._plain(scratch, torch.float32) and (lse is None or self._plain(lse, torch.float32))):
+            raise ValueError("[hip] attn_shared: q and att are bfloat16, lay int32, scratch and lse float32, all contiguous on the GPU")
+        hs, rs, cap = self._cache_strides(K, V, Hk, D, "attn_shared")
+        words = lay.numel()
+        T = words // 2 - 1
+        if T < 1 or words != 2 + 2 * T or q.numel() != T * Hq * D or att.numel() != T * Hq * D:
             raise ValueError("[hip] attn_shared: the layout holds 2 + 2 T words, q and att are [T, Hq D]")
-        if lse is not None:
-            self._need(lse, torch.float32, "lse")
-            if lse.numel() != T * Hq:
-                raise ValueError(f"[hip] attn_shared: lse holds {lse.numel()} values, the rows have {T * Hq} heads")
-        cap = K.shape[1]
+        if lse is not None and lse.numel() != T * Hq:
+            raise ValueError(f"[hip] attn_shared: lse holds {lse.numel()} values, the rows have {T * Hq} heads")
         if not (0 <= prefix_cap <= cap and 0 <= own_cap <= cap):
             raise ValueError(f"[hip] attn_shared: the lengths' bounds {prefix_cap} and {own_cap} lie within the cache's {cap} rows")
         need = self.lib.btb_hip_attn_shared_floats(T, Hq, Hk, D, prefix_cap, own_cap)
         if scratch.numel() < need:
             raise ValueError(f"[hip] attn_shared: scratch holds {scratch.numel()} floats, {need} are needed")
-        self._call("btb_hip_attn_shared", _p(q), _p(K), _p(V), _p(att), None if lse is None else _p(lse), _p(lay), T, Hq, Hk, D,
-                   cap, K.stride(0), K.stride(1), float(scale), prefix_cap, own_cap, _p(scratch), _stream())
+        self._call("btb_hip_attn_shared", q.data_ptr(), K.data_ptr(), V.data_ptr(), att.data_ptr(),
+                   None if lse is None else lse.data_ptr(), lay.data_ptr(), T, Hq, Hk, D, cap, hs, rs, scale, prefix_cap, own_cap,
+                   scratch.data_ptr(), _stream())
 
     def attn_mass(self, q: torch.Tensor, K: torch.Tensor, lse: torch.Tensor, seen: torch.Tensor, mass: torch.Tensor | None,
                   Hq: int, Hk: int, D: int, scale: float, n: int, out: torch.Tensor | None = None) -> torch.Tensor:
         """out [Hk, >= n] = mass + the attention weight that each of the first n keys received from the pass's rows q
         [T, Hq D], row t seeing keys 0 .. seen[t] - 1 (int32 [T]) with log-sum-exp lse (float32 [T, Hq], `attn_shared`'s).
         mass None: zeros; out None: mass itself."""
-        self._need(q, torch.bfloat16, "q")
-        self._need(lse, torch.float32, "lse")
-        self._need(seen, torch.int32, "seen")
-        self._cache_views(K, K, Hk, D, "attn_mass")
+        if not (self._plain(q, torch.bfloat16) and self._plain(lse, torch.float32) and self._plain(seen, torch.int32)):
+            raise ValueError("[hip] attn_mass: q is bfloat16, lse float32, seen int32, all contiguous on the GPU")
+        hs, rs, cap = self._cache_strides(K, K, Hk, D, "attn_mass")
         if out is None:
             out = mass if mass is not None else torch.empty(Hk, n, dtype=torch.float32, device=q.device)
-        T = int(seen.numel())
+        T = seen.numel()
         if T < 1 or q.numel() != T * Hq * D or lse.numel() != T * Hq:
             raise ValueError("[hip] attn_mass: q is [T, Hq D], lse [T, Hq], seen [T]")
-        if not 0 < n <= K.shape[1]:
-            raise ValueError(f"[hip] attn_mass: n is 1 .. the cache's {K.shape[1]} rows, got {n}")
-        for t, what in ((mass, "mass"), (out, "out")):
-            if t is not None and (not isinstance(t, _Tensor) or t.dtype is not torch.float32 or not t.is_cuda or t.dim() != 2
-                                  or t.shape[0] != Hk or t.shape[1] < n or t.stride(1) != 1):
-                raise ValueError(f"[hip] attn_mass: {what} is float32 [{Hk}, >= {n}] on the GPU, a head's values together")
+        if not 0 < n <= cap:
+            raise ValueError(f"[hip] attn_mass: n is 1 .. the cache's {cap} rows, got {n}")
+        for t in (out,) if mass is None or mass is out else (out, mass):
+            if not (isinstance(t, _Tensor) and t.dtype is torch.float32 and t.is_cuda and t.dim() == 2 and t.shape[0] == Hk
+                    and t.shape[1] >= n and t.stride(1) == 1):
+                raise ValueError(f"[hip] attn_mass: mass and out are float32 [{Hk}, >= {n}] on the GPU, a head's values together")
         floats = self.lib.btb_hip_attn_mass_floats(T, Hq, Hk, D, n)
         ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-        self._call("btb_hip_attn_mass", _p(q), _p(K), _p(lse), _p(seen), None if mass is None else _p(mass), _p(out), T, Hq, Hk,
-                   D, n, K.stride(0), K.stride(1), 0 if mass is None else mass.stride(0), out.stride(0), float(scale),
-                   None if ws is None else _p(ws), _stream())
+        self._call("btb_hip_attn_mass", q.data_ptr(), K.data_ptr(), lse.data_ptr(), seen.data_ptr(),
+                   None if mass is None else mass.data_ptr(), out.data_ptr(), T, Hq, Hk, D, n, hs, rs,
+                   0 if mass is None else mass.stride(0), out.stride(0), scale, None if ws is None else ws.data_ptr(), _stream())
         return out
 
     def kv_evict(self, mass: torch.Tensor, pos: torch.Tensor, K: torch.Tensor, V: torch.Tensor, n: int, budget: int,
@@ -1173,39 +1173,41 @@ class HipCard(CardLaunch):
         mass (float32 [L, Hk, cap]); keys of position (pos, int32 [L, Hk, cap]) below `sinks` or from `recent_from` on come
         first. What stays below the new length stays in its slot, the rest fills the slots in between; idx (int32 [L, Hk,
         kept]): the slot each came from. The outputs may be the inputs. Returns how many keys a head holds now."""
-        four = lambda t: t if t.dim() == 4 else t.unsqueeze(0)
-        three = lambda t: t if t.dim() == 3 else t.unsqueeze(0)
+        bf = torch.bfloat16
         for t in (K, V, K_out, V_out):
-            if not isinstance(t, _Tensor) or t.dtype is not torch.bfloat16 or not t.is_cuda or t.dim() not in (3, 4):
+            if not (isinstance(t, _Tensor) and t.dtype is bf and t.is_cuda and 3 <= t.dim() <= 4):
                 raise ValueError("[hip] kv_evict: K and V are bf16 [L, Hk, cap, D] views on the GPU")
-        k4, ko = four(K), four(K_out)
-        L, Hk, cap, D = k4.shape
+        shape, strides, out_shape, out_strides = K.shape, K.stride(), K_out.shape, K_out.stride()
+        if V.shape != shape or V.stride() != strides or V_out.shape != out_shape or V_out.stride() != out_strides \
+                or strides[-1] != 1 or out_strides[-1] != 1:
+            raise ValueError("[hip] kv_evict: K and V have the same strides, and their outputs, with D contiguous")
+        L, ls = (shape[0], strides[0]) if len(shape) == 4 else (1, 0)
+        lo = out_strides[0] if len(out_shape) == 4 else 0
+        Hk, cap, D = shape[-3:]
         kept = min(n, budget)
         if not 0 < n <= cap or budget < 1:
             raise ValueError(f"[hip] kv_evict: n is 1 .. the cache's {cap} rows and the budget 1 or more, got {n} and {budget}")
-        if K.shape != V.shape or K.stride() != V.stride() or K_out.shape != V_out.shape or K_out.stride() != V_out.stride() \
-                or k4.stride(3) != 1 or ko.stride(3) != 1:
-            raise ValueError("[hip] kv_evict: K and V have the same strides, and their outputs, with D contiguous")
-        if (ko.shape[0], ko.shape[1], ko.shape[3]) != (L, Hk, D) or ko.shape[2] < kept:
+        if (out_shape[0] if len(out_shape) == 4 else 1) != L or out_shape[-3] != Hk or out_shape[-1] != D or out_shape[-2] < kept:
             raise ValueError(f"[hip] kv_evict: the outputs are [{L}, {Hk}, >= {kept}, {D}]")
-        strides = []
-        for t, dtype, rows, what in ((mass, torch.float32, n, "mass"), (pos, torch.int32, n, "pos"),
-                                     (mass_out, torch.float32, kept, "mass_out"), (pos_out, torch.int32, kept, "pos_out")):
-            if not isinstance(t, _Tensor) or t.dtype is not dtype or not t.is_cuda or t.dim() not in (2, 3):
-                raise ValueError(f"[hip] kv_evict: {what} is a {dtype} tensor [L, Hk, >= {rows}] on the GPU")
-            t = three(t)
-            if t.shape[:2] != (L, Hk) or t.shape[2] < rows or t.stride(2) != 1 or (L > 1 and t.stride(0) != Hk * t.stride(1)):
-                raise ValueError(f"[hip] kv_evict: {what} is [{L}, {Hk}, >= {rows}], its heads evenly apart")
-            strides.append(t.stride(1))
-        self._need(idx, torch.int32, "idx")
-        if idx.numel() != L * Hk * kept:
-            raise ValueError(f"[hip] kv_evict: idx names {idx.numel()} slots, {L * Hk * kept} stay")
+
+        def head_stride(t: torch.Tensor, dtype: torch.dtype, rows: int, what: str) -> int:
+            if isinstance(t, _Tensor) and t.dtype is dtype and t.is_cuda:
+                s, st = t.shape, t.stride()
+                if 2 <= len(s) <= 3 and s[-2] == Hk and s[-1] >= rows and st[-1] == 1 and (
+                        L == 1 if len(s) == 2 else s[0] == L and (L == 1 or st[0] == Hk * st[1])):
+                    return st[-2]
+            raise ValueError(f"[hip] kv_evict: {what} is a {dtype} tensor [{L}, {Hk}, >= {rows}] on the GPU, its heads evenly apart")
+
+        ms, ps = head_stride(mass, torch.float32, n, "mass"), head_stride(pos, torch.int32, n, "pos")
+        mo, po = head_stride(mass_out, torch.float32, kept, "mass_out"), head_stride(pos_out, torch.int32, kept, "pos_out")
+        if not self._plain(idx, torch.int32) or idx.numel() != L * Hk * kept:
+            raise ValueError(f"[hip] kv_evict: idx is a contiguous int32 tensor on the GPU of the {L * Hk * kept} slots that stay")
         words = self.lib.btb_hip_kv_evict_words(L, Hk, n)
         ws = torch.empty(words, dtype=torch.int32, device=K.device) if words else None
-        self._call("btb_hip_kv_evict", _p(mass), strides[0], _p(pos), strides[1], _p(K), _p(V), k4.stride(0), k4.stride(1),
-                   k4.stride(2), L, Hk, D, n, budget, int(sinks), int(recent_from), _p(K_out), _p(V_out), ko.stride(0),
-                   ko.stride(1), ko.stride(2), _p(mass_out), strides[2], _p(pos_out), strides[3], _p(idx),
-                   None if ws is None else _p(ws), _stream())
+        self._call("btb_hip_kv_evict", mass.data_ptr(), ms, pos.data_ptr(), ps, K.data_ptr(), V.data_ptr(), ls, strides[-3],
+                   strides[-2], L, Hk, D, n, budget, sinks, recent_from, K_out.data_ptr(), V_out.data_ptr(), lo, out_strides[-3],
+                   out_strides[-2], mass_out.data_ptr(), mo, pos_out.data_ptr(), po, idx.data_ptr(),
+                   None if ws is None else ws.data_ptr(), _stream())
         return kept
 
     def silu_mul(self, gu: torch.Tensor, m: torch.Tensor) -> torch.Tensor:
