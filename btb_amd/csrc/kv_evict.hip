@@ -34,7 +34,7 @@ struct EvictWork {
 };
 __host__ __device__ inline size_t evict_words(size_t n) {
     const size_t blocks = (n + EV_KEYS - 1) / EV_KEYS;
-    return n + blocks * (EV_BINS / 2) + 2 * EV_BINS + 8 + 4 * blocks + n / 2;
+    return ((n + 3) / 4 * 4 + blocks * (EV_BINS / 2) + 2 * EV_BINS + 8 + 4 * blocks + n / 2 + 3) / 4 * 4;
 }
 
 struct EvictArgs {
@@ -49,7 +49,7 @@ __device__ __forceinline__ EvictWork work_of(const EvictArgs& p, int head) {
     const size_t blocks = (p.n + EV_KEYS - 1) / EV_KEYS;
     EvictWork w;
     w.rank = p.work + (size_t)head * evict_words(p.n);
-    w.first = w.rank + p.n;
+    w.first = w.rank + (p.n + 3) / 4 * 4;
     w.later = reinterpret_cast<int*>(w.first + blocks * (EV_BINS / 2));
     w.state = w.later + 2 * EV_BINS;
     w.counts = w.state + 8;
@@ -66,19 +66,25 @@ __device__ __forceinline__ uint32_t rank_bits(float m, int pos, int sinks, int r
 }
 
 // One more in the bin of every lane that counts. Many keys share one rank - those that received nothing, those that stay
-// whatever they weigh - and additions to one word wait for one another, so the lanes of two bins a wave are added at once.
+// whatever they weigh - and most others a few exponents, and additions to one word wait for one another: one bin's lanes a wave are
+// added at once, and a bin is COPIES words that neighbouring lanes take in turn.
+template <int COPIES>
 __device__ __forceinline__ void count(int* hist, int bin, bool counts, int lane) {
-    unsigned long long todo = __ballot(counts);
+    const unsigned long long todo = __ballot(counts);
+    if (todo == 0) return;
+    const int leader = __builtin_ctzll(todo);
+    const int theirs = __builtin_amdgcn_readlane(bin, leader);
+    const bool same = counts && bin == theirs;
+    const unsigned long long all = __ballot(same);
+    if (lane == leader) atomicAdd(&hist[COPIES * theirs], __popcll(all));
+    if (counts && !same) atomicAdd(&hist[COPIES * bin + lane % COPIES], 1);
+}
+template <int COPIES>
+__device__ __forceinline__ int counted(const int* hist, int bin) {
+    int n = 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        if (todo == 0) return;
-        const int leader = __builtin_ctzll(todo);
-        const int theirs = __builtin_amdgcn_readlane(bin, leader);
-        const unsigned long long same = __ballot(counts && bin == theirs) & todo;
-        if (lane == leader) atomicAdd(&hist[theirs], __popcll(same));
-        todo &= ~same;
-    }
-    if ((todo >> lane) & 1) atomicAdd(&hist[bin], 1);
+    for (int i = 0; i < COPIES; ++i) n += hist[COPIES * bin + i];
+    return n;
 }
 __device__ __forceinline__ int digit(uint32_t r, int round) {
     return (int)(round == 0 ? r >> 21 : round == 1 ? (r >> 10) & 2047u : r & 1023u);
@@ -146,7 +152,8 @@ __device__ __forceinline__ void share(int begin, int end, int wv, int& from, int
 // a head of up to EV_KEYS keys
 __global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(EvictArgs p) {
     extern __shared__ __align__(16) uint32_t rank[];  // [n], then the list [n / 2]
-    __shared__ int hist[EV_BINS], waves[EV_WAVES], pick[2], counts[2][2][EV_WAVES];
+    __shared__ __align__(16) int hist[2 * EV_BINS];
+    __shared__ int waves[EV_WAVES], pick[2], counts[2][2][EV_WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float* mass = p.mass + (size_t)blockIdx.x * p.ms;
     const int32_t* pos = p.pos + (size_t)blockIdx.x * p.ps;
@@ -162,16 +169,16 @@ __global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(EvictArgs p) {
     uint32_t last = 0;
     int left = p.kept;
     for (int round = 0; round < 3; ++round) {
-        hist[tid] = hist[tid + EV_THREADS] = 0;
+        reinterpret_cast<int4*>(hist)[tid] = make_int4(0, 0, 0, 0);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < EV_PER; ++i) {
             if (EV_THREADS * i >= p.n) break;  // uniform
-            count(hist, digit(r[i], round), EV_THREADS * i + tid < p.n && with(r[i], last, round), lane);
+            count<2>(hist, digit(r[i], round), EV_THREADS * i + tid < p.n && with(r[i], last, round), lane);
         }
         __syncthreads();
         uint32_t bin;
-        find(hist[EV_BINS - 1 - 2 * tid], hist[EV_BINS - 2 - 2 * tid], left, bin, waves, pick, tid, lane, wv);
+        find(counted<2>(hist, EV_BINS - 1 - 2 * tid), counted<2>(hist, EV_BINS - 2 - 2 * tid), left, bin, waves, pick, tid, lane, wv);
         last |= bin << (round == 0 ? 21 : round == 1 ? 10 : 0);
     }
     int from[2], to[2];
@@ -227,7 +234,8 @@ __global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(EvictArgs p) {
 // and before it what the last one's says. Round 3: how many keys stay.
 template <int ROUND>
 __global__ void __launch_bounds__(EV_THREADS) evict_round_kernel(EvictArgs p) {
-    __shared__ int hist[EV_BINS], waves[EV_WAVES], pick[2];
+    __shared__ __align__(16) int hist[4 * EV_BINS];
+    __shared__ int waves[EV_WAVES], pick[2];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), block = blockIdx.x;
     const EvictWork w = work_of(p, blockIdx.y);
     const int j0 = block * EV_KEYS + wv * (EV_KEYS / EV_WAVES) + lane;
@@ -242,12 +250,13 @@ __global__ void __launch_bounds__(EV_THREADS) evict_round_kernel(EvictArgs p) {
         else
             r[i] = j < p.n ? w.rank[j] : 0u;
     }
-    hist[tid] = hist[tid + EV_THREADS] = 0;
+    reinterpret_cast<int4*>(hist)[tid] = reinterpret_cast<int4*>(hist)[tid + EV_THREADS] = make_int4(0, 0, 0, 0);
     uint32_t last = 0;
     if constexpr (ROUND > 0) {
         int left = ROUND == 1 ? p.kept : w.state[2 * (ROUND - 1) + 1];
         int h0 = 0, h1 = 0;
         if constexpr (ROUND == 1) {
+#pragma unroll 16
             for (int b = 0; b < (int)gridDim.x; ++b) {
                 const uint32_t two = w.first[(size_t)b * (EV_BINS / 2) + EV_BINS / 2 - 1 - tid];
                 h0 += two >> 16;
@@ -272,18 +281,19 @@ __global__ void __launch_bounds__(EV_THREADS) evict_round_kernel(EvictArgs p) {
         for (int i = 0; i < EV_PER; ++i) {
             const bool in = j0 + 64 * i < p.n;
             if (ROUND == 0 && in) w.rank[j0 + 64 * i] = r[i];
-            count(hist, digit(r[i], ROUND), in && with(r[i], last, ROUND), lane);
+            count<4>(hist, digit(r[i], ROUND), in && with(r[i], last, ROUND), lane);
         }
         __syncthreads();
         if constexpr (ROUND == 0) {
-            w.first[(size_t)block * (EV_BINS / 2) + tid] = (uint32_t)hist[2 * tid] | (uint32_t)hist[2 * tid + 1] << 16;
+            w.first[(size_t)block * (EV_BINS / 2) + tid] = (uint32_t)counted<4>(hist, 2 * tid) | (uint32_t)counted<4>(hist, 2 * tid + 1) << 16;
             if (block == 0)
                 for (int i = tid; i < 2 * EV_BINS; i += EV_THREADS) w.later[i] = 0;
         } else {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int b = tid + EV_THREADS * i;
-                if (hist[b] != 0) atomicAdd(&w.later[(ROUND - 1) * EV_BINS + b], hist[b]);
+                const int n = counted<4>(hist, b);
+                if (n != 0) atomicAdd(&w.later[(ROUND - 1) * EV_BINS + b], n);
             }
         }
     } else {
@@ -304,80 +314,64 @@ __global__ void __launch_bounds__(EV_THREADS) evict_round_kernel(EvictArgs p) {
     }
 }
 
-// MOVERS: the kept keys past slot `kept` into the list; else the slots below, whose holes take them
-template <bool MOVERS>
-__global__ void __launch_bounds__(EV_THREADS) evict_order_kernel(EvictArgs p, int blocks, int first_block) {
-    __shared__ int waves[EV_WAVES], got[2], tallies[2][EV_WAVES];
-    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int block = blockIdx.x + first_block;
+// The order: the kept keys past slot `kept` into the list, and for the slots below, idx: themselves, or -1 - i the i-th hole, which
+// takes the list's i-th key (the move looks it up). Every wave adds up the counts of the workgroups ahead for itself.
+__global__ void __launch_bounds__(EV_THREADS) evict_order_kernel(EvictArgs p) {
+    __shared__ int tallies[4][EV_WAVES];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), block = blockIdx.x, blocks = gridDim.x;
     const EvictWork w = work_of(p, blockIdx.y);
-    const int begin = max(block * EV_KEYS, MOVERS ? p.kept : 0), end = min(min(block * EV_KEYS + EV_KEYS, p.n), MOVERS ? p.n : p.kept);
     const int j0 = block * EV_KEYS + wv * (EV_KEYS / EV_WAVES) + lane;
     uint32_t r[EV_PER];
 #pragma unroll
     for (int i = 0; i < EV_PER; ++i) r[i] = j0 + 64 * i < p.n ? w.rank[j0 + 64 * i] : 0u;
     const uint32_t last = (uint32_t)w.state[6];
     const int left = w.state[7];
-    // ties ahead of this workgroup's stretch - the slots below `kept` come first - and holes or movers ahead
-    int low[2] = {0, 0}, high[2] = {0, 0};
-    if (tid < blocks) {
-        low[0] = w.counts[4 * tid];
-        low[1] = w.counts[4 * tid + 1];
-        high[0] = w.counts[4 * tid + 2];
-        high[1] = w.counts[4 * tid + 3];
-    }
-    const int low_ties = before(low[1], waves, lane, wv);
-    if (tid == EV_THREADS - 1) got[0] = low_ties + low[1];
-    __syncthreads();
-    const int all_low = got[0];
-    int ties = low_ties, stay = low[0] + min(max(left - ties, 0), low[1]);
-    int units = tid < blocks ? max(min(tid * EV_KEYS + EV_KEYS, p.kept) - tid * EV_KEYS, 0) - stay : 0;  // holes
-    if (MOVERS) {
-        ties = all_low + before(high[1], waves, lane, wv);
-        units = high[0] + min(max(left - ties, 0), high[1]);
-        __syncthreads();
-    }
-    const int ahead = before(units, waves, lane, wv);
-    if (tid == block) {
-        got[0] = ties;
-        got[1] = ahead;
-    }
-    // and ahead of the wave's own within the workgroup
-    int above = 0, same = 0;
+    int c[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < EV_PER; ++i) {
         const int j = j0 + 64 * i;
-        tally(r[i], j >= begin && j < end, last, above, same);
+        tally(r[i], j < p.kept, last, c[0], c[1]);
+        tally(r[i], j >= p.kept && j < p.n, last, c[2], c[3]);
     }
-    if (lane == 0) {
-        tallies[0][wv] = above;
-        tallies[1][wv] = same;
+    if (lane < 4) tallies[lane][wv] = lane == 0 ? c[0] : lane == 1 ? c[1] : lane == 2 ? c[2] : c[3];
+    // all ties below `kept` come before those past it
+    int low = 0;
+    for (int b = lane; b < blocks; b += 64) low += w.counts[4 * b + 1];
+    int tie[2] = {0, __builtin_amdgcn_readlane(wave_running(low), 63)}, at[2] = {0, 0};  // ties, then holes and movers, ahead
+    // moves the four on by stretches, a lane each - `n` keys below `kept`, what `v` says of them and of those past it -, up to `upto`
+    auto advance = [&](int4 v, int n, int upto) {
+        const int run[2] = {wave_running(v.y), wave_running(v.w)};
+        const int t[2] = {tie[0] + run[0] - v.y, tie[1] + run[1] - v.w};
+        const int holes = n - v.x - min(max(left - t[0], 0), v.y), movers = v.z + min(max(left - t[1], 0), v.w);
+        const int ran[2] = {wave_running(holes), wave_running(movers)};
+        if (upto == 0) return;
+        tie[0] += __builtin_amdgcn_readlane(run[0], upto - 1);
+        tie[1] += __builtin_amdgcn_readlane(run[1], upto - 1);
+        at[0] += __builtin_amdgcn_readlane(ran[0], upto - 1);
+        at[1] += __builtin_amdgcn_readlane(ran[1], upto - 1);
+    };
+    auto below = [&](int from, int keys) { return max(min(from + keys, p.kept) - from, 0); };
+    for (int b = 0; b < block; b += 64) {
+        const bool live = b + lane < blocks;
+        const int4 v = live ? *reinterpret_cast<const int4*>(w.counts + 4 * (b + lane)) : make_int4(0, 0, 0, 0);
+        advance(v, live ? below((b + lane) * EV_KEYS, EV_KEYS) : 0, min(block - b, 64));
     }
     __syncthreads();
-    const int base_ties = got[0], base_units = got[1];
-    int tie, at;
     {
         const bool live = lane < EV_WAVES;
-        const int mine = live ? tallies[1][lane] : 0, f = block * EV_KEYS + lane * (EV_KEYS / EV_WAVES);
-        const int t = base_ties + wave_running(mine) - mine;
-        const int st = live ? tallies[0][lane] + min(max(left - t, 0), mine) : 0;
-        const int length = live ? max(min(f + EV_KEYS / EV_WAVES, end) - max(f, begin), 0) : 0;
-        const int u = MOVERS ? st : length - st;
-        tie = __builtin_amdgcn_readlane(t, wv);
-        at = base_units + __builtin_amdgcn_readlane(wave_running(u) - u, wv);
+        const int4 v = live ? make_int4(tallies[0][lane], tallies[1][lane], tallies[2][lane], tallies[3][lane]) : make_int4(0, 0, 0, 0);
+        advance(v, live ? below(block * EV_KEYS + lane * (EV_KEYS / EV_WAVES), EV_KEYS / EV_WAVES) : 0, wv);
     }
 #pragma unroll
     for (int i = 0; i < EV_PER; ++i) {
         const int j = j0 + 64 * i;
-        const bool in = j >= begin && j < end, s = stays(r[i], in, last, left, tie, lane);
-        const unsigned long long all = __ballot(MOVERS ? s : in && !s);
-        const int place = at + lanes_before(all, lane);
-        if (MOVERS) {
-            if (s) w.list[place] = j;
-        } else if (in) {
-            p.idx[(size_t)blockIdx.y * p.kept + j] = s ? j : w.list[place];
-        }
-        at += __popcll(all);
+        const bool low_j = j < p.kept, high_j = j >= p.kept && j < p.n;
+        const bool s0 = stays(r[i], low_j, last, left, tie[0], lane), s1 = stays(r[i], high_j, last, left, tie[1], lane);
+        const unsigned long long holes = __ballot(low_j && !s0), movers = __ballot(s1);
+        if (low_j) p.idx[(size_t)blockIdx.y * p.kept + j] = s0 ? j : -1 - (at[0] + lanes_before(holes, lane));
+        if (s1) w.list[at[1] + lanes_before(movers, lane)] = j;
+        at[0] += __popcll(holes);
+        at[1] += __popcll(movers);
     }
 }
 
@@ -390,7 +384,9 @@ struct MoveArgs {
     const int32_t* pos;
     float* mass_out;
     int32_t* pos_out;
-    const int32_t* idx;
+    int32_t* idx;
+    const int* list;  // of head 0, `per` words a head: what idx's negative numbers name
+    long long per;
     long long ls, hs, rs, lo, ho, ro;  // strides of the layers, heads and rows, in and out
     long long ms, ps, mo, po;
     int Hk, kept, in_place;
@@ -405,14 +401,23 @@ __global__ void __launch_bounds__(256) evict_move_kernel(MoveArgs p) {
     const int head = blockIdx.y, layer = head / p.Hk, g = head % p.Hk, c = threadIdx.x % CHUNKS;
     const int j0 = blockIdx.x * EV_MOVE + threadIdx.x / CHUNKS;
     const size_t src = (size_t)layer * p.ls + (size_t)g * p.hs + 8 * c, dst = (size_t)layer * p.lo + (size_t)g * p.ho + 8 * c;
-    const int32_t* idx = p.idx + (size_t)head * p.kept;
+    int32_t* idx = p.idx + (size_t)head * p.kept;
     int from[ROWS];
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        const int j = j0 + STEP * i;
-        from[i] = j < p.kept ? idx[j] : -1;
-        if (p.in_place && from[i] == j) from[i] = -1;
+    for (int i = 0; i < ROWS; ++i) from[i] = j0 + STEP * i < p.kept ? idx[j0 + STEP * i] : 0;
+    if (p.list != nullptr) {  // uniform
+        int named[ROWS];
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) named[i] = from[i] < 0 ? p.list[(size_t)head * p.per - 1 - from[i]] : from[i];
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            if (from[i] < 0 && c == 0) idx[j0 + STEP * i] = named[i];  // (this row's lanes, all of this wave, have read it)
+            from[i] = named[i];
+        }
     }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+        if (j0 + STEP * i >= p.kept || (p.in_place && from[i] == j0 + STEP * i)) from[i] = -1;
     uint4 k[ROWS], v[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)
@@ -453,7 +458,7 @@ extern "C" int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t
     const bool in_place = K == K_out;
     if (L == 0 || Hk == 0 || L > 65535 || Hk > 65535 || L * Hk > 65535 || (D != 64 && D != 128 && D != 256) || n == 0 ||
         n > (size_t)EV_KEYS * EV_BLOCKS || budget == 0 || ms < 0 || ps < 0 || mo < 0 || po < 0 || odd(ls) || odd(hs) || odd(rs) || odd(lo) ||
-        odd(ho) || odd(ro) || loose(K) || loose(V) || loose(K_out) || loose(V_out) || in_place != (V == V_out) ||
+        odd(ho) || odd(ro) || loose(K) || loose(V) || loose(K_out) || loose(V_out) || loose(workspace) || in_place != (V == V_out) ||
         in_place != (mass == mass_out) || in_place != (pos == pos_out) ||
         (in_place && (ls != lo || hs != ho || rs != ro || ms != mo || ps != po))) {
         set_error("kv_evict: at most 65535 heads in all of at most 2^23 keys, head_dim 64, 128 or 256, K and V 16-byte aligned with strides in "
@@ -474,18 +479,21 @@ extern "C" int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t
     e.work = workspace;
     const unsigned heads = (unsigned)(L * Hk);
     if (n <= (size_t)EV_KEYS) {
-        hipLaunchKernelGGL(evict_choose_kernel, dim3(heads), dim3(EV_THREADS), 4 * (n + n / 2), st, e);
+        const size_t lds = 4 * (n + n / 2);
+        if (lds > 44 * 1024) {
+            const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(evict_choose_kernel),
+                                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (rc != hipSuccess) return hip_status(rc, "hipFuncSetAttribute");
+        }
+        hipLaunchKernelGGL(evict_choose_kernel, dim3(heads), dim3(EV_THREADS), lds, st, e);
     } else {
-        const int blocks = (int)((n + EV_KEYS - 1) / EV_KEYS), below = (e.kept + EV_KEYS - 1) / EV_KEYS;
+        const int blocks = (int)((n + EV_KEYS - 1) / EV_KEYS);
         const dim3 grid((unsigned)blocks, heads), threads(EV_THREADS);
         hipLaunchKernelGGL(evict_round_kernel<0>, grid, threads, 0, st, e);
         hipLaunchKernelGGL(evict_round_kernel<1>, grid, threads, 0, st, e);
         hipLaunchKernelGGL(evict_round_kernel<2>, grid, threads, 0, st, e);
         hipLaunchKernelGGL(evict_round_kernel<3>, grid, threads, 0, st, e);
-        if (e.kept < e.n)
-            hipLaunchKernelGGL(evict_order_kernel<true>, dim3((unsigned)(blocks - e.kept / EV_KEYS), heads), threads, 0, st, e,
-                               blocks, e.kept / EV_KEYS);
-        hipLaunchKernelGGL(evict_order_kernel<false>, dim3((unsigned)below, heads), threads, 0, st, e, blocks, 0);
+        hipLaunchKernelGGL(evict_order_kernel, grid, threads, 0, st, e);
     }
     MoveArgs m;
     m.K = static_cast<const uint16_t*>(K);
@@ -497,6 +505,8 @@ extern "C" int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t
     m.mass_out = mass_out;
     m.pos_out = pos_out;
     m.idx = idx;
+    m.list = n <= (size_t)EV_KEYS ? nullptr : reinterpret_cast<const int*>(workspace) + ((n + 3) / 4 * 4 + (n + EV_KEYS - 1) / EV_KEYS * (EV_BINS / 2 + 4) + 2 * EV_BINS + 8);
+    m.per = (long long)evict_words(n);
     m.ls = ls;
     m.hs = hs;
     m.rs = rs;

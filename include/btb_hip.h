@@ -507,7 +507,7 @@ int32_t btb_hip_attn_mass(const void* q, const void* K, const float* lse, const 
  * and pos of slot idx[j] go to slot j of the outputs; idx: i32 [L Hk][kept], dense. Strides: ls / hs / rs (lo / ho / ro) of
  * a layer, head and row of K and V, ms / ps (mo / po) of a head of mass and pos. The outputs may be the inputs, all four
  * with the same strides (only what moves is then written), or must not overlap them. workspace: btb_hip_kv_evict_words(L, Hk,
- * n) words, this call's own (0: NULL will do). n at most 2^23, D 64, 128 or 256; K and V 16-byte aligned, their strides multiples of 8. */
+ * n) words, 16-byte aligned, this call's own (0: NULL will do). n at most 2^23, D 64, 128 or 256; K and V 16-byte aligned, their strides multiples of 8. */
 size_t btb_hip_kv_evict_words(size_t L, size_t Hk, size_t n);
 int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t* pos, int64_t ps, const void* K, const void* V,
                          int64_t ls, int64_t hs, int64_t rs, size_t L, size_t Hk, size_t D, size_t n, size_t budget,
