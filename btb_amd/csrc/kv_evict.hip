@@ -21,6 +21,7 @@ namespace btb {
 
 constexpr int EV_THREADS = 1024, EV_WAVES = EV_THREADS / 64, EV_BINS = 2048;
 constexpr int EV_KEYS = 8192, EV_PER = EV_KEYS / EV_THREADS;  // keys a workgroup, and a thread
+constexpr int EV_COPIES = 8;                                  // words a bin of a long head's histograms
 constexpr int EV_BLOCKS = 1024;                               // workgroups a head: their counts meet in one scan
 
 // what a long head keeps between the launches, in the call's workspace
@@ -66,18 +67,11 @@ __device__ __forceinline__ uint32_t rank_bits(float m, int pos, int sinks, int r
 }
 
 // One more in the bin of every lane that counts. Many keys share one rank - those that received nothing, those that stay
-// whatever they weigh - and most others a few exponents, and additions to one word wait for one another: one bin's lanes a wave are
-// added at once, and a bin is COPIES words that neighbouring lanes take in turn.
+// whatever they weigh - and most others a few exponents, and additions to one word wait for one another: a bin is COPIES words that
+// neighbouring lanes take in turn.
 template <int COPIES>
 __device__ __forceinline__ void count(int* hist, int bin, bool counts, int lane) {
-    const unsigned long long todo = __ballot(counts);
-    if (todo == 0) return;
-    const int leader = __builtin_ctzll(todo);
-    const int theirs = __builtin_amdgcn_readlane(bin, leader);
-    const bool same = counts && bin == theirs;
-    const unsigned long long all = __ballot(same);
-    if (lane == leader) atomicAdd(&hist[COPIES * theirs], __popcll(all));
-    if (counts && !same) atomicAdd(&hist[COPIES * bin + lane % COPIES], 1);
+    if (counts) atomicAdd(&hist[COPIES * bin + lane % COPIES], 1);
 }
 template <int COPIES>
 __device__ __forceinline__ int counted(const int* hist, int bin) {
@@ -152,7 +146,7 @@ __device__ __forceinline__ void share(int begin, int end, int wv, int& from, int
 // a head of up to EV_KEYS keys
 __global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(EvictArgs p) {
     extern __shared__ __align__(16) uint32_t rank[];  // [n], then the list [n / 2]
-    __shared__ __align__(16) int hist[2 * EV_BINS];
+    __shared__ __align__(16) int hist[4 * EV_BINS];
     __shared__ int waves[EV_WAVES], pick[2], counts[2][2][EV_WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float* mass = p.mass + (size_t)blockIdx.x * p.ms;
@@ -169,16 +163,16 @@ __global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(EvictArgs p) {
     uint32_t last = 0;
     int left = p.kept;
     for (int round = 0; round < 3; ++round) {
-        reinterpret_cast<int4*>(hist)[tid] = make_int4(0, 0, 0, 0);
+        reinterpret_cast<int4*>(hist)[tid] = reinterpret_cast<int4*>(hist)[tid + EV_THREADS] = make_int4(0, 0, 0, 0);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < EV_PER; ++i) {
             if (EV_THREADS * i >= p.n) break;  // uniform
-            count<2>(hist, digit(r[i], round), EV_THREADS * i + tid < p.n && with(r[i], last, round), lane);
+            count<4>(hist, digit(r[i], round), EV_THREADS * i + tid < p.n && with(r[i], last, round), lane);
         }
         __syncthreads();
         uint32_t bin;
-        find(counted<2>(hist, EV_BINS - 1 - 2 * tid), counted<2>(hist, EV_BINS - 2 - 2 * tid), left, bin, waves, pick, tid, lane, wv);
+        find(counted<4>(hist, EV_BINS - 1 - 2 * tid), counted<4>(hist, EV_BINS - 2 - 2 * tid), left, bin, waves, pick, tid, lane, wv);
         last |= bin << (round == 0 ? 21 : round == 1 ? 10 : 0);
     }
     int from[2], to[2];
@@ -230,11 +224,23 @@ __global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(EvictArgs p) {
     }
 }
 
+// the four tallies of a wave's keys from slot f on; all of them lie on one side of `kept` but for one wave a head
+__device__ __forceinline__ void tallies_of(const uint32_t (&r)[EV_PER], int f, const EvictArgs& p, uint32_t last, int lane, int (&c)[4]) {
+    if (f < p.kept) {
+#pragma unroll
+        for (int i = 0; i < EV_PER; ++i) tally(r[i], f + 64 * i + lane < p.kept, last, c[0], c[1]);
+    }
+    if (f + 64 * EV_PER > p.kept) {
+#pragma unroll
+        for (int i = 0; i < EV_PER; ++i) tally(r[i], f + 64 * i + lane >= p.kept && f + 64 * i + lane < p.n, last, c[2], c[3]);
+    }
+}
+
 // A longer head, a workgroup EV_KEYS of its keys; wave w takes 512 of them in a row. Rounds 0, 1 and 2: this round's histogram,
 // and before it what the last one's says. Round 3: how many keys stay.
 template <int ROUND>
 __global__ void __launch_bounds__(EV_THREADS) evict_round_kernel(EvictArgs p) {
-    __shared__ __align__(16) int hist[4 * EV_BINS];
+    extern __shared__ __align__(16) int hist[];  // [EV_BINS][EV_COPIES]
     __shared__ int waves[EV_WAVES], pick[2];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), block = blockIdx.x;
     const EvictWork w = work_of(p, blockIdx.y);
@@ -250,7 +256,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_round_kernel(EvictArgs p) {
         else
             r[i] = j < p.n ? w.rank[j] : 0u;
     }
-    reinterpret_cast<int4*>(hist)[tid] = reinterpret_cast<int4*>(hist)[tid + EV_THREADS] = make_int4(0, 0, 0, 0);
+    for (int i = tid; i < EV_COPIES * EV_BINS / 4; i += EV_THREADS) reinterpret_cast<int4*>(hist)[i] = make_int4(0, 0, 0, 0);
     uint32_t last = 0;
     if constexpr (ROUND > 0) {
         int left = ROUND == 1 ? p.kept : w.state[2 * (ROUND - 1) + 1];
@@ -281,29 +287,24 @@ __global__ void __launch_bounds__(EV_THREADS) evict_round_kernel(EvictArgs p) {
         for (int i = 0; i < EV_PER; ++i) {
             const bool in = j0 + 64 * i < p.n;
             if (ROUND == 0 && in) w.rank[j0 + 64 * i] = r[i];
-            count<4>(hist, digit(r[i], ROUND), in && with(r[i], last, ROUND), lane);
+            count<EV_COPIES>(hist, digit(r[i], ROUND), in && with(r[i], last, ROUND), lane);
         }
         __syncthreads();
         if constexpr (ROUND == 0) {
-            w.first[(size_t)block * (EV_BINS / 2) + tid] = (uint32_t)counted<4>(hist, 2 * tid) | (uint32_t)counted<4>(hist, 2 * tid + 1) << 16;
+            w.first[(size_t)block * (EV_BINS / 2) + tid] = (uint32_t)counted<EV_COPIES>(hist, 2 * tid) | (uint32_t)counted<EV_COPIES>(hist, 2 * tid + 1) << 16;
             if (block == 0)
                 for (int i = tid; i < 2 * EV_BINS; i += EV_THREADS) w.later[i] = 0;
         } else {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int b = tid + EV_THREADS * i;
-                const int n = counted<4>(hist, b);
+                const int n = counted<EV_COPIES>(hist, b);
                 if (n != 0) atomicAdd(&w.later[(ROUND - 1) * EV_BINS + b], n);
             }
         }
     } else {
         int c[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < EV_PER; ++i) {
-            const int j = j0 + 64 * i;
-            tally(r[i], j < min(p.kept, p.n), last, c[0], c[1]);
-            tally(r[i], j >= p.kept && j < p.n, last, c[2], c[3]);
-        }
+        tallies_of(r, j0 - lane, p, last, lane, c);
         if (lane < 4) hist[4 * wv + lane] = lane == 0 ? c[0] : lane == 1 ? c[1] : lane == 2 ? c[2] : c[3];
         __syncthreads();
         if (tid < 4) {
@@ -327,12 +328,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_order_kernel(EvictArgs p) {
     const uint32_t last = (uint32_t)w.state[6];
     const int left = w.state[7];
     int c[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < EV_PER; ++i) {
-        const int j = j0 + 64 * i;
-        tally(r[i], j < p.kept, last, c[0], c[1]);
-        tally(r[i], j >= p.kept && j < p.n, last, c[2], c[3]);
-    }
+    tallies_of(r, j0 - lane, p, last, lane, c);
     if (lane < 4) tallies[lane][wv] = lane == 0 ? c[0] : lane == 1 ? c[1] : lane == 2 ? c[2] : c[3];
     // all ties below `kept` come before those past it
     int low = 0;
@@ -362,16 +358,25 @@ __global__ void __launch_bounds__(EV_THREADS) evict_order_kernel(EvictArgs p) {
         const int4 v = live ? make_int4(tallies[0][lane], tallies[1][lane], tallies[2][lane], tallies[3][lane]) : make_int4(0, 0, 0, 0);
         advance(v, live ? below(block * EV_KEYS + lane * (EV_KEYS / EV_WAVES), EV_KEYS / EV_WAVES) : 0, wv);
     }
+    if (j0 - lane < p.kept) {  // uniform
 #pragma unroll
-    for (int i = 0; i < EV_PER; ++i) {
-        const int j = j0 + 64 * i;
-        const bool low_j = j < p.kept, high_j = j >= p.kept && j < p.n;
-        const bool s0 = stays(r[i], low_j, last, left, tie[0], lane), s1 = stays(r[i], high_j, last, left, tie[1], lane);
-        const unsigned long long holes = __ballot(low_j && !s0), movers = __ballot(s1);
-        if (low_j) p.idx[(size_t)blockIdx.y * p.kept + j] = s0 ? j : -1 - (at[0] + lanes_before(holes, lane));
-        if (s1) w.list[at[1] + lanes_before(movers, lane)] = j;
-        at[0] += __popcll(holes);
-        at[1] += __popcll(movers);
+        for (int i = 0; i < EV_PER; ++i) {
+            const int j = j0 + 64 * i;
+            const bool in = j < p.kept, s = stays(r[i], in, last, left, tie[0], lane);
+            const unsigned long long holes = __ballot(in && !s);
+            if (in) p.idx[(size_t)blockIdx.y * p.kept + j] = s ? j : -1 - (at[0] + lanes_before(holes, lane));
+            at[0] += __popcll(holes);
+        }
+    }
+    if (j0 - lane + 64 * EV_PER > p.kept) {
+#pragma unroll
+        for (int i = 0; i < EV_PER; ++i) {
+            const int j = j0 + 64 * i;
+            const bool s = stays(r[i], j >= p.kept && j < p.n, last, left, tie[1], lane);
+            const unsigned long long movers = __ballot(s);
+            if (s) w.list[at[1] + lanes_before(movers, lane)] = j;
+            at[1] += __popcll(movers);
+        }
     }
 }
 
@@ -438,6 +443,16 @@ __global__ void __launch_bounds__(256) evict_move_kernel(MoveArgs p) {
         }
 }
 
+template <int ROUND>
+static int32_t launch_round(const dim3& grid, const EvictArgs& e, hipStream_t st) {
+    constexpr int lds = 4 * EV_COPIES * EV_BINS;
+    const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(evict_round_kernel<ROUND>),
+                                              hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (rc != hipSuccess) return hip_status(rc, "hipFuncSetAttribute");
+    hipLaunchKernelGGL(evict_round_kernel<ROUND>, grid, dim3(EV_THREADS), lds, st, e);
+    return OK;
+}
+
 }  // namespace btb
 
 using namespace btb;
@@ -480,7 +495,7 @@ extern "C" int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t
     const unsigned heads = (unsigned)(L * Hk);
     if (n <= (size_t)EV_KEYS) {
         const size_t lds = 4 * (n + n / 2);
-        if (lds > 44 * 1024) {
+        if (lds > 28 * 1024) {
             const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(evict_choose_kernel),
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
             if (rc != hipSuccess) return hip_status(rc, "hipFuncSetAttribute");
@@ -489,10 +504,8 @@ extern "C" int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t
     } else {
         const int blocks = (int)((n + EV_KEYS - 1) / EV_KEYS);
         const dim3 grid((unsigned)blocks, heads), threads(EV_THREADS);
-        hipLaunchKernelGGL(evict_round_kernel<0>, grid, threads, 0, st, e);
-        hipLaunchKernelGGL(evict_round_kernel<1>, grid, threads, 0, st, e);
-        hipLaunchKernelGGL(evict_round_kernel<2>, grid, threads, 0, st, e);
-        hipLaunchKernelGGL(evict_round_kernel<3>, grid, threads, 0, st, e);
+        const int32_t rc = launch_round<0>(grid, e, st) | launch_round<1>(grid, e, st) | launch_round<2>(grid, e, st) | launch_round<3>(grid, e, st);
+        if (rc != OK) return ERR_PANIC;
         hipLaunchKernelGGL(evict_order_kernel, grid, threads, 0, st, e);
     }
     MoveArgs m;
