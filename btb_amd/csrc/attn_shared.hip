@@ -306,11 +306,232 @@ __device__ __forceinline__ void walk(const SharedArgs& p, const uint16_t* Kg, co
     }
 }
 
+// 128 pairs against a stretch of keys, every wave 32 of them and all the keys: the prefix of many rows, whose products are what
+// it costs. Stages of 64 keys, three of K and two of V in LDS, every wave bringing half a tile of each. A stage's weights are made
+// between the products of the next one's scores, and that one's maxima between the products of its outputs: no stretch of a stage
+// is vector arithmetic alone. Two barriers a stage where walk has four.
+// For head_dim 64, where the exponentials cost as much as the products and so are worth hiding; at 128 one tile's chain of eight
+// dependent products sets the pace and walk is as fast or faster. us, walk / this: 256 rows of 40 heads x 64 over 32768 keys 159 /
+// 139, 41 rows over 6001 and 485 own 21.6 / 19.5; 256 rows of 32 heads x 128 over 32768 keys 160 / 159, and 640 own 232 / 252.
+template <int D, int QW>
+constexpr bool overlaps() {
+    return D == 64 && QW == 4;
+}
+template <int D, class Row, class State>
+__device__ __forceinline__ void walk_many(const SharedArgs& p, const uint16_t* Kg, const uint16_t* Vg, const Keys& keys, uint8_t* lds,
+                                          Row row, State state) {
+    constexpr int STEPS = D / 16, DT = D / 32, TILE = TK * 2 * D, STAGE = 2 * TILE, AHEAD = 4, H = TileLoads<D>::N / 2;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 31, h = lane >> 5;
+    const float ninf = bits_f32(0xff800000u);
+    const int stages = (keys.count + 63) / 64;
+    TileLoads<D> loads;
+    loads.make(p.rs, lane);
+    const uint16_t* Kb = Kg + (size_t)keys.first * p.rs;
+    const uint16_t* Vb = Vg + (size_t)keys.first * p.rs;
+    uint8_t* v_lds = lds + 3 * STAGE;
+    // (`ln` is the lane again, made unknown to the compiler stage by stage: what is rare comes from it and is not kept in registers)
+    int ln = lane;
+    auto issue_k = [&](int s, int slot) {
+        const int k0 = min(64 * s + 16 * wv, keys.count - 1);
+        loads.template issue<true, H>(Kb + (size_t)k0 * p.rs, p.rs, keys.count - k0, lds + slot * STAGE + wv * (TILE / 2), ln);
+    };
+    auto issue_v = [&](int s) {
+        const int k0 = min(64 * s + 16 * wv, keys.count - 1);
+        loads.template issue<false, H>(Vb + (size_t)k0 * p.rs, p.rs, keys.count - k0, v_lds + (s & 1) * STAGE + wv * (TILE / 2), ln);
+    };
+    // all but the youngest n stages' loads have landed
+    auto wait = [&](int n, uint32_t& at) {
+        if (n == 3)
+            wait_loads<3 * H>(at);
+        else if (n == 2)
+            wait_loads<2 * H>(at);
+        else if (n == 1)
+            wait_loads<H>(at);
+        else
+            wait_loads<0>(at);
+    };
+    auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
+    auto barrier = [&] {
+        fence();
+        asm volatile("s_barrier" ::: "memory");
+        fence();
+    };
+    f32x16 o[DT];
+    float m = ninf, l = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = zero16();
+    bf16x8 qf[STEPS];
+    {
+        const uint16_t* qr = row(32 * wv + c) + 8 * h;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) qf[s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(qr + 16 * s));
+    }
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): q is here, and no register of the loop waits for a load
+    fence();
+    const uint32_t k_at = k_place<D>(lane), v_at = v_place<D>(lane);
+    f32x16 st[2];    // a stage's scores
+    u32x4 pw[2][2];  // its weights
+    // the scores of tile `tile` of a stage; work(i) after each of the STEPS
+    auto scores = [&](uint32_t at, int slot, int tile, f32x16& to, auto work) {
+        bf16x8 kf[STEPS];
+        const uint8_t* tiles = lds + slot * STAGE;
+        to = zero16();
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) kf[i] = k_fragment(tiles, at, tile * TILE, i);
+        fence();
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            if (i + AHEAD < STEPS) kf[i + AHEAD] = k_fragment(tiles, at, tile * TILE, i + AHEAD);
+            to = mfma32(kf[i], qf[i], to);
+            work(i);
+            fence();
+        }
+    };
+    // its outputs; work(r) after every second product
+    auto outputs = [&](uint32_t at, int s, auto work) {
+        constexpr int ALL = 4 * DT;
+        bf16x8 vf[ALL];
+        const uint8_t* tiles = v_lds + (s & 1) * STAGE;
+        auto read = [&](int e) { return v_fragment<D>(tiles, at, e / (2 * DT) * TILE, e % DT, e / DT % 2); };
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) vf[e] = read(e);
+        fence();
+#pragma unroll
+        for (int e = 0; e < ALL; ++e) {
+            if (e + AHEAD < ALL) vf[e + AHEAD] = read(e + AHEAD);
+            o[e % DT] = mfma32(vf[e], __builtin_bit_cast(bf16x8, pw[e / (2 * DT)][e / DT % 2]), o[e % DT]);
+            if (e % 2 == 1) {
+                work(e / 2);
+                fence();
+            }
+        }
+    };
+    auto mask = [&](int s) {  // keys past the end
+        if (64 * s + 64 <= keys.count) return;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (8 * (i / 4) + i % 4 >= keys.count - 64 * s - TK * j - 4 * (ln >> 5)) st[j][i] = ninf;
+    };
+    auto settle = [&](float top) {  // as in walk
+        top = fmaxf(top, xor32(top)) * p.scale_log2;
+        const bool moves = top > m + 8.f || m == ninf;
+        if (__any(moves)) {
+            const float mn = moves ? top : m;
+            const float corr = m == ninf ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= corr;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= corr;
+        }
+    };
+    if (stages > 0) {
+        issue_k(0, 0);
+        if (stages > 1) issue_k(1, 1);
+        issue_v(0);
+        if (stages > 2) issue_k(2, 2);
+        uint32_t ak = k_at;
+        wait(stages > 2 ? 3 : stages > 1 ? 2 : 1, ak);
+        barrier();
+        scores(ak, 0, 0, st[0], [](int) {});
+        scores(ak, 0, 1, st[1], [](int) {});
+        mask(0);
+        float top = st[0][0];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(st[0][i], st[1][i]));
+        settle(top);
+    }
+    int slot = 0;  // of stage s's K
+    for (int s = 0; s < stages; ++s) {
+        const int left = stages - 1 - s;  // stages behind this one
+        uint32_t ak = k_at, av = v_at;
+        asm volatile("" : "+v"(ln));
+        if (left > 0) wait(left > 1 ? 2 : 1, ak);  // the next one's K; behind it this one's V and the K after
+        barrier();
+        if (left > 0) issue_v(s + 1);
+        if (left > 2) issue_k(s + 3, slot);
+        slot = slot == 2 ? 0 : slot + 1;
+        const float ref = m == ninf ? 0.f : m;
+        float sum = 0.f;
+        constexpr int EACH = 16 / STEPS;
+        auto weigh = [&](int j, int step) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 2)
+                if (e / EACH == step) {
+                    const float w0 = __builtin_amdgcn_exp2f(fmaf(st[j][e], p.scale_log2, -ref));
+                    const float w1 = __builtin_amdgcn_exp2f(fmaf(st[j][e + 1], p.scale_log2, -ref));
+                    sum += w0;
+                    sum += w1;
+                    pw[j][e / 8][e % 8 / 2] = f32x2_bf16(w0, w1);
+                    if (e % 8 == 6) asm volatile("" : "+v"(pw[j][e / 8]));  // made here, not where they are used
+                }
+        };
+        f32x16 next[2];
+        if (left > 0) {
+            scores(ak, slot, 0, next[0], [&](int i) { weigh(0, i); });
+            scores(ak, slot, 1, next[1], [&](int i) { weigh(1, i); });
+            st[0] = next[0];
+            st[1] = next[1];
+            mask(s + 1);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2 * STEPS; ++i) weigh(i / STEPS, i % STEPS);
+        }
+        l += sum;
+        wait(left > 2 ? 3 : left > 1 ? 2 : left > 0 ? 1 : 0, av);  // this one's V; behind it K, V and K
+        if (64 * s + 64 > keys.count) {
+            const int mine = keys.count - 64 * s - 16 * wv;
+            if (mine < 16) TileLoads<D>::template clear_past<H>(v_lds + (s & 1) * STAGE + wv * (TILE / 2), mine, ln);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+        barrier();
+        // (after the last stage st holds its own scores still: their maximum moves nothing that matters)
+        float top = st[0][0], other = st[1][0];
+        constexpr int EACH_MAX = 16 / (2 * DT);
+        outputs(av, s, [&](int r) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (i / EACH_MAX == r) {
+                    top = fmaxf(top, st[0][i]);
+                    other = fmaxf(other, st[1][i]);
+                }
+        });
+        if (left > 0) settle(fmaxf(top, other));
+    }
+    l += xor32(l);
+    // the outputs through LDS, a pair's 16-byte chunks permuted, so that they are written in whole rows
+    __syncthreads();
+    float* all = reinterpret_cast<float*>(lds) + (size_t)(wv * 32) * D;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+            *reinterpret_cast<float4*>(all + c * D + 4 * ((8 * d + 2 * b + h) ^ (c & (D / 4 - 1)))) =
+                make_float4(o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]);
+    const long long mine = state(32 * wv + c);
+    if (h == 0 && mine >= 0) {
+        p.part_m[mine] = m;
+        p.part_l[mine] = l;
+    }
+#pragma unroll 4
+    for (int e = lane; e < 32 * (D / 4); e += 64) {
+        const int r = e / (D / 4), chunk = e % (D / 4);
+        const long long to = state(32 * wv + r);
+        if (to >= 0)
+            *reinterpret_cast<float4*>(p.part_acc + (size_t)to * D + 4 * chunk) =
+                *reinterpret_cast<const float4*>(all + r * D + 4 * (chunk ^ (r & (D / 4 - 1))));
+    }
+}
+
 // The prefix's workgroups come first, the long ones; the rows' own take what room is left beside them and after them.
 template <int D, int QW>
 __global__ void __launch_bounds__(256, 2) attn_shared_kernel(SharedArgs p) {
-    extern __shared__ __align__(16) uint8_t lds[];  // a stage
-    __shared__ float meet[2 * 4 * 32];
+    extern __shared__ __align__(16) uint8_t lds[];  // a stage and where the waves meet, or walk_many's five
+    float* meet = reinterpret_cast<float*>(lds + 8 * TK * 2 * D);
     const int pairs = p.T * p.G;
     const int prefix = p.Hk * p.pair_tiles * p.prefix_spans;
     int id = blockIdx.x;
@@ -326,7 +547,10 @@ __global__ void __launch_bounds__(256, 2) attn_shared_kernel(SharedArgs p) {
             const int r = r0 + i, t = r / p.G;
             return r < pairs ? ((long long)t * p.Hq + g * p.G + (r - t * p.G)) * p.states + sp : -1;
         };
-        walk<D, QW>(p, p.K + (size_t)g * p.hs, p.V + (size_t)g * p.hs, keys, lds, meet, row, state);
+        if constexpr (overlaps<D, QW>())
+            walk_many<D>(p, p.K + (size_t)g * p.hs, p.V + (size_t)g * p.hs, keys, lds, row, state);
+        else
+            walk<D, QW>(p, p.K + (size_t)g * p.hs, p.V + (size_t)g * p.hs, keys, lds, meet, row, state);
         return;
     }
     id -= prefix;
@@ -414,8 +638,8 @@ static SharedPlan shared_plan(size_t T, size_t Hq, size_t Hk, size_t prefix_cap,
 }
 template <int D, int QW>
 static int32_t launch_one(const dim3& grid, const SharedArgs& p, hipStream_t st) {
-    constexpr int lds = 8 * TK * 2 * D, most = 64 * 1024 - 1024;
-    if (lds > most) {
+    constexpr int lds = overlaps<D, QW>() ? 10 * TK * 2 * D : 8 * TK * 2 * D + 1024;
+    if (lds > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_shared_kernel<D, QW>),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return hip_status(e, "hipFuncSetAttribute");

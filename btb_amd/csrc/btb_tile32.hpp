@@ -75,6 +75,17 @@ __device__ __forceinline__ void load4_to_lds(const char* base, size_t step, uint
         : "s"(to), "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "s"(base + step), "s"(base + 2 * step), "s"(base + 3 * step)
         : "memory", "scc");
 }
+// two of them
+__device__ __forceinline__ void load2_to_lds(const char* base, size_t step, uint32_t o0, uint32_t o1, uint32_t to) {
+    uint32_t kept;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %4\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %5\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(kept)
+        : "s"(to), "v"(o0), "v"(o1), "s"(base), "s"(base + step)
+        : "memory", "scc");
+}
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
     return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }
@@ -100,33 +111,37 @@ struct TileLoads {
         for (int i = 0; i < KP; ++i) k[i] = row + 16 * k_chunk<D>(KPI * i + lane / CH, lane % CH);
         v = row + 16 * v_chunk(lane / CH, lane % CH);
     }
-    // the tile of `left` >= 1 keys at `from` (uniform) into LDS: K's, or V's; keys past the last are the last again
-    template <bool IS_K>
+    // COUNT instructions' keys at `from` (uniform), a whole tile or half of one, into LDS: K's, or V's. `left` >= 1 keys are there;
+    // those past the last are the last again.
+    template <bool IS_K, int COUNT = N>
     __device__ __forceinline__ void issue(const uint16_t* from, long long rs, int left, uint8_t* tile, int lane) const {
+        static_assert(COUNT == N || (2 * COUNT == N && COUNT % KP == 0), "a tile or half of one, whose permutation starts over");
         const char* base = reinterpret_cast<const char*>(uniform(from));
         const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_address(tile));
-        if (left >= TK) {
-            const size_t step = (size_t)KPI * rs * 2;
+        const bool whole = left >= COUNT * KPI;
+        const size_t step = whole ? (size_t)KPI * rs * 2 : 0;
+        auto at = [&](int i) {
+            if (whole) return IS_K ? k[i % KP] : v;
+            const int key = KPI * i + lane / CH;
+            return (uint32_t)(min(key, left - 1) * rs * 2) + 16 * (IS_K ? k_chunk<D>(key, lane % CH) : v_chunk(key, lane % CH));
+        };
+        if (whole) {
 #pragma unroll
-            for (int i = 0; i < N; i += 4) {
-                auto at = [&](int j) { return IS_K ? k[(i + j) % KP] : v; };
-                load4_to_lds(base + i * step, step, at(0), at(1), at(2), at(3), to + 1024 * i);
-            }
+            for (int i = 0; i + 3 < COUNT; i += 4)
+                load4_to_lds(base + i * step, step, IS_K ? k[i % KP] : v, IS_K ? k[(i + 1) % KP] : v, IS_K ? k[(i + 2) % KP] : v,
+                             IS_K ? k[(i + 3) % KP] : v, to + 1024 * i);
+            if constexpr (COUNT == 2) load2_to_lds(base, step, IS_K ? k[0] : v, IS_K ? k[1 % KP] : v, to);
         } else {
 #pragma unroll
-            for (int i = 0; i < N; i += 4) {
-                auto at = [&](int j) {
-                    const int key = KPI * (i + j) + lane / CH;
-                    return (uint32_t)(min(key, left - 1) * rs * 2) + 16 * (IS_K ? k_chunk<D>(key, lane % CH) : v_chunk(key, lane % CH));
-                };
-                load4_to_lds(base, 0, at(0), at(1), at(2), at(3), to + 1024 * i);
-            }
+            for (int i = 0; i + 3 < COUNT; i += 4) load4_to_lds(base, 0, at(i), at(i + 1), at(i + 2), at(i + 3), to + 1024 * i);
+            if constexpr (COUNT == 2) load2_to_lds(base, 0, at(0), at(1), to);
         }
     }
     // V's rows past the last key as zeros, once the tile has landed: weight 0 times what lies there must not make a NaN
+    template <int COUNT = N>
     __device__ __forceinline__ static void clear_past(uint8_t* v_lds, int left, int lane) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
+        for (int i = 0; i < COUNT; ++i)
             if (KPI * i + lane / CH >= left) *reinterpret_cast<uint4*>(v_lds + 1024 * i + 16 * lane) = make_uint4(0u, 0u, 0u, 0u);
     }
 };
