@@ -8,10 +8,12 @@
 //
 //   many pairs: a wave holds 64 keys as stationary operands and takes the pass's (row, head) pairs 32 at a time out of LDS, where the
 //     workgroup's four waves bring them a stage ahead. A tile's weights are made between the next tile's products. Where keys are
-//     few, the pairs are cut over workgroups too, whose sums a second launch adds in order. Bound: the exponentials, sixteen of
-//     a quarter's rate a lane beside sixteen multiply-adds and additions a tile, against eight products of head_dim 128.
+//     few, the pairs are cut over workgroups too, whose sums a second launch adds in order. Bound: the products and the exponentials, a
+//     multiply-add, a quarter-rate exponential and an addition a score beside a thirty-second of a product of 32 clocks a lane. 500 rows of
+//     32 heads x 128 over 16384 keys 87 us (760 TFLOP/s), of which 13 bring the keys into registers; 4096 rows 544 us (1010 TFLOP/s), 507
+//     without the stages' loads and 398 (1384 TFLOP/s, the chip's rate for bare products) with no exponential either.
 //   few pairs (64 and less): they lie in LDS and the keys go by, a tile of 32 a wave ahead of the one at work. Bound: K's
-//     trip from memory.
+//     trip from memory. 4 rows of 32 heads x 128 over 32000 keys 14.0 us (4.8 TB/s).
 
 #include "btb_common.hpp"
 #include "btb_tile32.hpp"
@@ -23,7 +25,9 @@ namespace btb {
 
 constexpr int MA_KEYS = 256;   // many pairs: keys a workgroup, four waves of two tiles
 constexpr int MA_META = 1024;  // pairs whose log-sums and limits lie in LDS at a time
-constexpr int MA_FEW = 64;     // few pairs, at most
+// few pairs, at most: two tiles, the most whose log-sums and limits fit a wave's registers. 64 pairs of 8 heads, us, few / many: over 32000 keys
+// 16.4 / 26.3, over 2000 9.0 / 9.6; 72 pairs (many) over 32000: 26.0
+constexpr int MA_FEW = 64;
 
 struct MassArgs {
     const uint16_t* q;
@@ -332,7 +336,8 @@ __global__ void __launch_bounds__(256) attn_mass_add_kernel(MassArgs p) {
     p.out[(size_t)g * p.os + key] = v + (p.mass != nullptr ? p.mass[(size_t)g * p.ms + key] : 0.f);
 }
 
-// workgroups the pairs are cut over: until there are two a CU, each with two stages and more
+// Workgroups the pairs are cut over: until there are two a CU, each with two stages and more. 8 heads of 128, us, cut / whole: 500 rows over
+// 2000 keys 21.5 / 60, over 512 13.1 / 43; 100 rows over 4000 16.0 / 18.9.
 static int mass_parts(size_t T, size_t Hq, size_t Hk, size_t D, size_t n) {
     if (T * (Hq / Hk) <= (size_t)MA_FEW) return 1;
     const size_t wgs = Hk * ((n + MA_KEYS - 1) / MA_KEYS), stages = (T * (Hq / Hk) * D / 64 + 127) / 128;

@@ -4,14 +4,19 @@
 //   s_j = scale q . k_j over the prefix's and the row's own keys;  lse = log sum_j exp s_j;  att = sum_j exp(s_j - lse) v_j
 //
 // in one pass over the keys with a running maximum and sum. A workgroup is four waves and one of two kinds of work:
-//   prefix: one kv head, one span of the prefix, a tile of (row, query head) pairs - a wave takes 32 pairs and every key,
-//           or, where the head has no more than 32 pairs, all the pairs and a quarter of the keys
+//   prefix: one kv head, one span of the prefix, a tile of 32, 64 or 128 (row, query head) pairs, of which a wave takes 32 - with
+//           128 pairs every key, else the half or the quarter of the keys that the waves of the same pairs share out
 //   own:    one row, one kv head, one span of the row's own keys; a wave a quarter of them
 // and leaves states (maximum, sum, output) in the scratch, which a second launch folds in a fixed order. The spans are
 // cut from the keys there are (the layout lies on the device), so a recorded launch holds while the rows grow.
 //
 // Sums and outputs are f32; a weight is rounded to bf16 for the product with V, as the matrix cores take it (relative
-// 2-norm against 64 bits 2.1e-3 where rounding the output alone makes 1.7e-3), and the sum takes the unrounded weight.
+// 2-norm against 64 bits 2.3e-3 where rounding the output alone makes 1.7e-3), and the sum takes the unrounded weight.
+//
+// Bound: memory where few rows share the prefix (16 rows of 32 heads x 128 over 131072 keys, 100 own: 104 us, 5.2 TB/s), the products and
+// what stands between them where many do (256 rows over 32768: 156 us, 880 TFLOP/s, the fold included; bare products reach 1384), and
+// both at once where many rows have many own keys (640 each: 235 us, 3.4 TB/s and 590 TFLOP/s): there a prefix workgroup a CU takes 204 us of
+// 8192 keys, 167 with no own keys beside it, 139 without its loads, 130 without its barriers and 94 for the products alone.
 
 #include "btb_common.hpp"
 #include "btb_tile32.hpp"
@@ -564,7 +569,8 @@ __global__ void __launch_bounds__(256, 2) attn_shared_kernel(SharedArgs p) {
 }
 
 // WAVES waves a (row, head): the states' common maximum, their factors, their outputs in a fixed order - a lane two dims, at
-// head_dim 64 the halves of a wave in turn. One wave where there are heads enough to fill the chip, else four.
+// head_dim 64 the halves of a wave in turn. One wave where there are heads enough to fill the chip, else four: the whole call, us, one
+// / four: 16 rows of 32 heads 14.9 / 13.0 (over 700 keys), 64 rows 24.0 / 24.3 (over 4096), 128 rows 33.3 / 35.4, 256 rows 50.5 / 55.3.
 template <int D, int WAVES>
 __global__ void __launch_bounds__(256) attn_shared_fold_kernel(SharedArgs p, uint16_t* att, float* lse) {
     constexpr int HEADS = 4 / WAVES, PART = 128 / D * WAVES;  // heads a workgroup, parts that the states are taken in
@@ -617,7 +623,7 @@ struct SharedPlan {
 // A prefix workgroup a CU, the rows' own beside them; two a CU where the products are what the prefix costs - 128 pairs of a head and
 // more, spans of eight stages and more - and the rows' own keys, read at 5.1 TB/s, cost less than half of that (at 900 TFLOP/s).
 // us, one a CU / two: 16 rows x 131072 keys, 100 own 107 / 119; 4 rows 102 / 107; 256 x 32768, 640 own 235 / 273, 64 own 192 /
-// 172, 64 x 131072, 640 own 212 / 196; 41 rows of 40 heads x 64 over 6001, 485 own 22.7 / 27.0, none 17.6 / 19.3.
+// 172, 64 x 131072, 640 own 212 / 196.
 static SharedPlan shared_plan(size_t T, size_t Hq, size_t Hk, size_t prefix_cap, size_t own_cap) {
     const size_t G = Hq / Hk, pairs = T * G, cus = (size_t)device_info().cus;
     auto spans = [&](size_t groups, size_t cap, size_t wgs) {

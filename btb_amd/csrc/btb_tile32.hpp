@@ -58,8 +58,9 @@ __device__ __forceinline__ bf16x8 v_fragment(const uint8_t* tiles, uint32_t plac
 // global_load_lds_dwordx4 writes lane l's 16 bytes at a wave's LDS base plus 16 l: the place in the tile is fixed, so the
 // permutation of a key's chunks is made on the way out of memory, within the key's own row.
 
-// Four such loads, 16 bytes a lane each: from base, base + step, + 2 step and + 3 step (uniform) + the lane's offsets to LDS bytes `to` (uniform) + 16 lane and 1, 2 and 3 KB on. Written out, because behind the builtin the
-// compiler makes every transposing read of LDS wait for all such loads there are, the next stage's among them. They write no
+// Four such loads, 16 bytes a lane each: from base, base + step, + 2 step and + 3 step (uniform) + the lane's offsets to LDS bytes
+// `to` (uniform) + 16 lane and 1, 2 and 3 KB on. Written out, because behind the builtin the compiler makes every transposing
+// read of LDS wait for all such loads there are, the next stage's among them. They write no
 // register; what they write is waited for by count (wait_loads), and a wait of the compiler's own for another load can only come out
 // longer. M0 is left as it was.
 __device__ __forceinline__ void load4_to_lds(const char* base, size_t step, uint32_t o0, uint32_t o1, uint32_t o2, uint32_t o3,

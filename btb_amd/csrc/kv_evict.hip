@@ -8,9 +8,12 @@
 // ten bits at a time from the top (histograms in LDS), counts what stays and then writes the order. A wave takes a stretch of
 // the slots below `kept` and one of those above, so its own running count is all that its keys' order needs, and the waves
 // meet in one scan. A workgroup takes a head of up to 8192 keys alone, ranks in LDS, one launch; a longer one is cut over
-// workgroups of 8192 keys and the rounds are launches (six), since what a key costs is arithmetic: 131072 keys x 32 heads
-// took one workgroup a head 358 us.
-// Bound: memory: mass and pos read, the moved rows read and written.
+// workgroups of 8192 keys and the rounds are launches (six), since what a key costs is arithmetic.
+//
+// us, a workgroup a head / the rounds: 8192 keys to 4096 x 8 heads 18.9 / 30.7, x 32 39.4 / 51.6, x 288 260 / 274; the choice alone of
+// 131072 keys x 32 358 / 49. Bound: memory, mass and pos read, the moved rows read and written: 4608 keys to 4096 x 288 heads 245 us
+// (5.0 TB/s); 131072 to 16384 x 32 heads 153 us, of which the move 104 and the first round, additions in LDS, 19; 700 to 512 x 8 heads
+// 13.5 us, two launches of 6 and 4.
 
 #include "btb_common.hpp"
 #include "btb_tuning.hpp"
@@ -21,7 +24,7 @@ namespace btb {
 
 constexpr int EV_THREADS = 1024, EV_WAVES = EV_THREADS / 64, EV_BINS = 2048;
 constexpr int EV_KEYS = 8192, EV_PER = EV_KEYS / EV_THREADS;  // keys a workgroup, and a thread
-constexpr int EV_COPIES = 8;                                  // words a bin of a long head's histograms
+constexpr int EV_COPIES = 8;  // words a bin of a long head's histograms (131072 keys x 32 heads: 4 words 158 us a call, 8 153)
 constexpr int EV_BLOCKS = 1024;                               // workgroups a head: their counts meet in one scan
 
 // what a long head keeps between the launches, in the call's workspace
@@ -518,7 +521,9 @@ extern "C" int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t
     m.mass_out = mass_out;
     m.pos_out = pos_out;
     m.idx = idx;
-    m.list = n <= (size_t)EV_KEYS ? nullptr : reinterpret_cast<const int*>(workspace) + ((n + 3) / 4 * 4 + (n + EV_KEYS - 1) / EV_KEYS * (EV_BINS / 2 + 4) + 2 * EV_BINS + 8);
+    m.list = nullptr;
+    if (n > (size_t)EV_KEYS)
+        m.list = reinterpret_cast<const int*>(workspace) + (n + 3) / 4 * 4 + (n + EV_KEYS - 1) / EV_KEYS * (EV_BINS / 2 + 4) + 2 * EV_BINS + 8;
     m.per = (long long)evict_words(n);
     m.ls = ls;
     m.hs = hs;
