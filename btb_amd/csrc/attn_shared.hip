@@ -682,11 +682,10 @@ int32_t btb_hip_attn_shared(const void* q, const void* K, const void* V, void* a
                             size_t prefix_cap, size_t own_cap, float* workspace, void* stream) {
     if (!q || !K || !V || !att || !layout || !workspace) return ERR_NULL;
     auto loose = [](const void* a) { return ((uintptr_t)a & 15u) != 0; };
-    if (!shared_sizes_fit(T, Hq, Hk, D, prefix_cap, own_cap) || cap == 0 || cap > 0x7FFFFFFFu || prefix_cap > cap ||
-        own_cap > cap || hs < 0 || rs < 0 || rs > (1 << 25) || hs % 8 || rs % 8 || !(scale > 0.f) || !(scale < __builtin_inff()) || loose(q) ||
+    if (!shared_sizes_fit(T, Hq, Hk, D, prefix_cap, own_cap) || cap == 0 || cap > 0x7FFFFFFFu || hs < 0 || rs < 0 || rs > (1 << 25) || hs % 8 || rs % 8 || !(scale > 0.f) || !(scale < __builtin_inff()) || loose(q) ||
         loose(K) || loose(V) || loose(att) || loose(workspace)) {
-        set_error("attn_shared: head_dim 64 or 128, up to 32 query heads a kv head, capacities within the cache's, a positive "
-                  "scale, q, K, V, att and the workspace 16-byte aligned with strides in multiples of 8, a row's up to 2^25");
+        set_error("attn_shared: head_dim 64 or 128, up to 32 query heads a kv head, a positive scale, q, K, V, att "
+                  "and the workspace 16-byte aligned with strides in multiples of 8, a row's up to 2^25");
         return ERR_DOMAIN;
     }
     const SharedPlan s = shared_plan(T, Hq, Hk, prefix_cap, own_cap);

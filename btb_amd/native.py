@@ -1120,7 +1120,7 @@ class HipCard(CardLaunch):
                     lse: torch.Tensor | None = None) -> None:
         """att [T, Hq D] = attention of T rows over a prefix they share, read once for all of them, and keys of their own,
         both as `shared_layout` lays them out in one layer's cache; lse (float32 [T, Hq]): the rows' log-sum-exp. The
-        lengths are read on the device; prefix_cap and own_cap are the most they may be."""
+        lengths are read on the device; prefix_cap and own_cap are the most they may be (the cache's rows bound them too)."""
         if not (self._plain(q, torch.bfloat16) and self._plain(att, torch.bfloat16) and self._plain(lay, torch.int32)
                 and self._plain(scratch, torch.float32) and (lse is None or self._plain(lse, torch.float32))):
             raise ValueError("[hip] attn_shared: q and att are bfloat16, lay int32, scratch and lse float32, all contiguous on the GPU")
@@ -1131,8 +1131,8 @@ class HipCard(CardLaunch):
             raise ValueError("[hip] attn_shared: the layout holds 2 + 2 T words, q and att are [T, Hq D]")
         if lse is not None and lse.numel() != T * Hq:
             raise ValueError(f"[hip] attn_shared: lse holds {lse.numel()} values, the rows have {T * Hq} heads")
-        if not (0 <= prefix_cap <= cap and 0 <= own_cap <= cap):
-            raise ValueError(f"[hip] attn_shared: the lengths' bounds {prefix_cap} and {own_cap} lie within the cache's {cap} rows")
+        if prefix_cap < 0 or own_cap < 0:
+            raise ValueError(f"[hip] attn_shared: the lengths' bounds are 0 or more, got {prefix_cap} and {own_cap}")
         need = self.lib.btb_hip_attn_shared_floats(T, Hq, Hk, D, prefix_cap, own_cap)
         if scratch.numel() < need:
             raise ValueError(f"[hip] attn_shared: scratch holds {scratch.numel()} floats, {need} are needed")

@@ -199,6 +199,24 @@ def test_attn_shared(card, T, Hq, Hk, D, P, lens, slot_major):
     _hold_shared(att2, lse2, q, K, V, off, P, own, scale)
 
 
+@pytest.mark.parametrize("D,T", [(64, 3), (128, 50)])
+def test_attn_shared_bounds_past_the_cache(card, D, T):
+    """rows of unlike lengths in a cache that holds no more than they need: the longest may be more than all of its rows"""
+    g = gen(5215 + T)
+    q, K, V, off, offs = _shared_case(g, T, 8, 2, D, 4, [2] * T)
+    own = [(o, 2) for o in offs]
+    for prefix_cap, own_cap in ((4, 4 * K.shape[1]), (4 * K.shape[1], 2), (1 << 20, 1 << 20)):
+        att, lse = _run_shared(card, q, K, V, off, 4, own, 0.1, prefix_cap, own_cap)
+        _hold_shared(att, lse, q, K, V, off, 4, own, 0.1)
+    # lengths that run past the cache are cut at its last row
+    K, V = K.nan_to_num(nan=0.5), V.nan_to_num(nan=0.5)
+    lay = card.shared_layout(off, 1 << 20, [(o, -1) for o in offs[1:]] + [(offs[0], 2)])
+    att, lse = torch.zeros(T, 8 * D, dtype=torch.bfloat16, device="cuda"), torch.zeros(T, 8, device="cuda")
+    card.attn_shared(q.view(T, -1), K, V, att, lay, 8, 2, D, 0.1, 1 << 20, 1 << 20, card.attn_shared_scratch(T, 8, 2, D, 1 << 20, 1 << 20), lse=lse)
+    torch.cuda.synchronize()
+    _hold_shared(att.view(T, 8, D)[-1:], lse[-1:], q[-1:], K, V, off, K.shape[1] - off, [(offs[0], 2)], 0.1)
+
+
 def test_attn_shared_scores_far_apart(card):
     """maxima that grow along the keys, by hundreds, and keys whose weight underflows"""
     g = gen(5300)
@@ -447,7 +465,7 @@ def test_refusals(card):
     shared_ = lambda **k: card.attn_shared(*[k.get(n, v) for n, v in dict(
         q=q, K=K, V=V, att=att, lay=lay, Hq=Hq, Hk=Hk, D=D, scale=0.1, prefix_cap=20, own_cap=4, scratch=scratch, lse=None).items()])
     shared_()
-    for bad in (dict(prefix_cap=cap + 1), dict(own_cap=-1), dict(scratch=scratch[:-1]), dict(lay=lay[:5].contiguous()),
+    for bad in (dict(own_cap=-1), dict(scratch=scratch[:-1]), dict(lay=lay[:5].contiguous()),
                 dict(lse=z(T, Hq + 1, dt=f32)), dict(q=q.float()), dict(K=K.transpose(1, 2)), dict(att=z(T, D))):
         with pytest.raises(ValueError):
             shared_(**bad)
