@@ -32,12 +32,12 @@ constexpr int MA_FEW = 64;
 struct MassArgs {
     const uint16_t* q;
     const uint16_t* K;
-    const float* lse;      // [T, Hq]
+    const float* lse;      // [T, Hq], strides lr and lh
     const int32_t* seen;   // [T]
     const float* mass;     // rows of `ms` floats, or none
     float* out;            // rows of `os` floats
     float* work;           // [parts][Hk][n] where parts > 1
-    long long hs, rs, ms, os;
+    long long hs, rs, ms, os, lr, lh;
     float scale_log2;
     int T, Hq, Hk, G, n, parts;
 };
@@ -47,7 +47,7 @@ __device__ __forceinline__ void pair_facts(const MassArgs& p, int g, int r, int 
     z = 0.f;
     seen = 0;
     if (r < pairs) {
-        const float raw = p.lse[(size_t)row * p.Hq + g * p.G + (r - row * p.G)];
+        const float raw = p.lse[row * p.lr + (g * p.G + (r - row * p.G)) * p.lh];
         if (raw != -__builtin_inff()) {
             z = raw * 1.44269504088896341f;
             seen = p.seen[row];
@@ -379,10 +379,10 @@ size_t btb_hip_attn_mass_floats(size_t T, size_t Hq, size_t Hk, size_t D, size_t
 
 int32_t btb_hip_attn_mass(const void* q, const void* K, const float* lse, const int32_t* seen, const float* mass, float* out,
                           size_t T, size_t Hq, size_t Hk, size_t D, size_t n, int64_t hs, int64_t rs, int64_t mass_stride,
-                          int64_t out_stride, float scale, float* workspace, void* stream) {
+                          int64_t out_stride, int64_t lse_row, int64_t lse_head, float scale, float* workspace, void* stream) {
     if (!q || !K || !lse || !seen || !out) return ERR_NULL;
     auto loose = [](const void* a) { return ((uintptr_t)a & 15u) != 0; };
-    if (!mass_sizes_fit(T, Hq, Hk, D, n) || hs < 0 || rs < 0 || rs > (1 << 25) || hs % 8 || rs % 8 || mass_stride < 0 || out_stride < 0 ||
+    if (!mass_sizes_fit(T, Hq, Hk, D, n) || hs < 0 || rs < 0 || rs > (1 << 25) || hs % 8 || rs % 8 || mass_stride < 0 || out_stride < 0 || lse_row < 0 || lse_head < 0 ||
         !(scale > 0.f) || !(scale < __builtin_inff()) || loose(q) || loose(K)) {
         set_error("attn_mass: head_dim 64 or 128, up to 32 query heads a kv head, a positive scale, q and K 16-byte aligned "
                   "with strides in multiples of 8, a row's up to 2^25");
@@ -404,6 +404,8 @@ int32_t btb_hip_attn_mass(const void* q, const void* K, const float* lse, const 
     p.rs = rs;
     p.ms = mass_stride;
     p.os = out_stride;
+    p.lr = lse_row;
+    p.lh = lse_head;
     p.scale_log2 = scale * 1.44269504088896341f;
     p.T = (int)T;
     p.Hq = (int)Hq;

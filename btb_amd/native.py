@@ -113,7 +113,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "btb_hip_attn_shared_floats": (_sz, [_sz, _sz, _sz, _sz, _sz, _sz]),
     "btb_hip_attn_shared": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, ctypes.c_int64, ctypes.c_int64,
                                    ctypes.c_float, _sz, _sz, _vp, _vp]),
-    "btb_hip_attn_mass": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz] + [ctypes.c_int64] * 4 +
+    "btb_hip_attn_mass": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz] + [ctypes.c_int64] * 6 +
                           [ctypes.c_float, _vp, _vp]),
     "btb_hip_attn_mass_floats": (_sz, [_sz] * 5),
     "btb_hip_kv_evict": (_i32, [_vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp] + [ctypes.c_int64] * 3 + [_sz] * 5 +
@@ -1143,15 +1143,16 @@ class HipCard(CardLaunch):
     def attn_mass(self, q: torch.Tensor, K: torch.Tensor, lse: torch.Tensor, seen: torch.Tensor, mass: torch.Tensor | None,
                   Hq: int, Hk: int, D: int, scale: float, n: int, out: torch.Tensor | None = None) -> torch.Tensor:
         """out [Hk, >= n] = mass + the attention weight that each of the first n keys received from the pass's rows q
-        [T, Hq D], row t seeing keys 0 .. seen[t] - 1 (int32 [T]) with log-sum-exp lse (float32 [T, Hq], `attn_shared`'s).
-        mass None: zeros; out None: mass itself."""
-        if not (self._plain(q, torch.bfloat16) and self._plain(lse, torch.float32) and self._plain(seen, torch.int32)):
-            raise ValueError("[hip] attn_mass: q is bfloat16, lse float32, seen int32, all contiguous on the GPU")
+        [T, Hq D], row t seeing keys 0 .. seen[t] - 1 (int32 [T]) with log-sum-exp lse (float32 [T, Hq] of any strides,
+        `attn_shared`'s). mass None: zeros; out None: mass itself."""
+        if not (self._plain(q, torch.bfloat16) and self._plain(seen, torch.int32) and isinstance(lse, _Tensor)
+                and lse.dtype is torch.float32 and lse.is_cuda):
+            raise ValueError("[hip] attn_mass: q is bfloat16, lse float32, seen int32, on the GPU, q and seen contiguous")
         hs, rs, cap = self._cache_strides(K, K, Hk, D, "attn_mass")
         if out is None:
             out = mass if mass is not None else torch.empty(Hk, n, dtype=torch.float32, device=q.device)
         T = seen.numel()
-        if T < 1 or q.numel() != T * Hq * D or lse.numel() != T * Hq:
+        if T < 1 or q.numel() != T * Hq * D or lse.shape != (T, Hq):
             raise ValueError("[hip] attn_mass: q is [T, Hq D], lse [T, Hq], seen [T]")
         if not 0 < n <= cap:
             raise ValueError(f"[hip] attn_mass: n is 1 .. the cache's {cap} rows, got {n}")
@@ -1163,7 +1164,7 @@ class HipCard(CardLaunch):
         ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
         self._call("btb_hip_attn_mass", q.data_ptr(), K.data_ptr(), lse.data_ptr(), seen.data_ptr(),
                    None if mass is None else mass.data_ptr(), out.data_ptr(), T, Hq, Hk, D, n, hs, rs,
-                   0 if mass is None else mass.stride(0), out.stride(0), scale, None if ws is None else ws.data_ptr(), _stream())
+                   0 if mass is None else mass.stride(0), out.stride(0), lse.stride(0), lse.stride(1), scale, None if ws is None else ws.data_ptr(), _stream())
         return out
 
     def kv_evict(self, mass: torch.Tensor, pos: torch.Tensor, K: torch.Tensor, V: torch.Tensor, n: int, budget: int,

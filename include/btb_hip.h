@@ -492,14 +492,14 @@ int32_t btb_hip_attn_shared(const void* q, const void* K, const void* V, void* a
 
 /* The attention weight every key received from a pass, added to what it had: for kv head g and key j < n
  *     out[g][j] = mass[g][j] + sum over rows t with j < seen[t] and g's query heads h of exp(scale q[t][h] . K[g][j] - lse[t][h])
- * with lse [T, Hq] as btb_hip_attn_shared leaves it (a row whose lse is -inf adds nothing). seen: i32 [T]. mass and out:
- * f32 rows mass_stride / out_stride apart; mass NULL: zeros; out may be mass. workspace: btb_hip_attn_mass_floats of
+ * with lse [T, Hq] as btb_hip_attn_shared leaves it, its rows lse_row and its heads lse_head values apart (a row whose lse is
+ * -inf adds nothing). seen: i32 [T]. mass and out: f32 rows mass_stride / out_stride apart; mass NULL: zeros; out may be mass. workspace: btb_hip_attn_mass_floats of
  * them, this call's own (0: NULL will do). The additions' order is fixed. D 64 or 128, Hq / Hk up to 32, T Hq at most 2^23, scale > 0;
  * q and K 16-byte aligned, hs and rs multiples of 8. */
 size_t btb_hip_attn_mass_floats(size_t T, size_t Hq, size_t Hk, size_t D, size_t n);
 int32_t btb_hip_attn_mass(const void* q, const void* K, const float* lse, const int32_t* seen, const float* mass, float* out,
                           size_t T, size_t Hq, size_t Hk, size_t D, size_t n, int64_t hs, int64_t rs, int64_t mass_stride,
-                          int64_t out_stride, float scale, float* workspace, void* stream);
+                          int64_t out_stride, int64_t lse_row, int64_t lse_head, float scale, float* workspace, void* stream);
 
 /* A cache of L layers x Hk heads cut to its heaviest keys. Of a head's n keys the first kept = min(n, budget) in the order
  * (mass descending, slot ascending) stay, where a key with pos < sinks or pos >= recent_from counts as +inf and a NaN as

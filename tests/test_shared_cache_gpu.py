@@ -346,6 +346,22 @@ def test_attn_mass(card, T, Hq, Hk, D, n, chain, slot_major):
     assert torch.equal(out[:, :n], mass[:, :n]) and bool((out[:, n:] == 7.0).all()) and torch.equal(mass[:, n:], kept[:, n:])
 
 
+@pytest.mark.parametrize("T,Hq,Hk,D,n", [(5, 3, 3, 128, 70), (9, 8, 2, 64, 300), (90, 6, 6, 128, 400), (70, 12, 3, 64, 257)])
+def test_attn_mass_log_sums_of_any_strides(card, T, Hq, Hk, D, n):
+    """the log-sums head by head, in a wider array, or one for all rows: the bits of the dense ones"""
+    g = gen(5440 + T)
+    q, K = torch.randn(T, Hq * D, generator=g).to(torch.bfloat16).cuda(), _cache(g, Hk, n, D, False)
+    seen = torch.randint(0, n + 1, (T,), generator=g).to(torch.int32).cuda()
+    lse = torch.rand(T, Hq, generator=g).cuda() * 4
+    wide = torch.full((T, 2 * Hq + 3), NAN, device="cuda")
+    wide[:, 1:2 * Hq:2] = lse
+    call = lambda z: card.attn_mass(q, K, z, seen, None, Hq, Hk, D, 0.1, n)
+    want = call(lse)
+    for z in (lse.t().contiguous().t(), wide[:, 1:2 * Hq:2]):
+        assert z.shape == (T, Hq) and (T == 1 or not z.is_contiguous()) and torch.equal(call(z), want)
+    assert torch.equal(call(lse[:1].expand(T, Hq)), call(lse[:1].repeat(T, 1)))
+
+
 def test_attn_mass_takes_attentions_own_log_sums(card):
     """after attn_shared, the weights over prefix and own keys come to one a head"""
     g = gen(5450)
@@ -496,7 +512,7 @@ def test_refusals(card):
     lib, p = card.lib, lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())
     assert lib.btb_hip_attn_shared(None, p(K), p(V), p(att), None, p(lay), T, Hq, Hk, D, cap, 1, 1, 0.1, 20, 4, p(scratch), None) == -1
     assert lib.btb_hip_attn_shared(p(q), p(K), p(V), p(att), None, p(lay), T, 7, 2, D, cap, 8, 8, 0.1, 20, 4, p(scratch), None) == -6
-    assert lib.btb_hip_attn_mass(p(q), p(K), p(lse), None, None, p(lse), T, Hq, Hk, D, 10, 8, 8, 0, 0, 0.1, None, None) == -1
+    assert lib.btb_hip_attn_mass(p(q), p(K), p(lse), None, None, p(lse), T, Hq, Hk, D, 10, 8, 8, 0, 0, Hq, 1, 0.1, None, None) == -1
     assert lib.btb_hip_kv_evict(p(mass), 1, None, 1, p(K), p(V), 0, 8, 8, 1, Hk, D, 16, 8, 0, 0, p(K), p(V), 0, 8, 8, p(mass), 1, p(p32), 1,
                                 p(idx), None, None) == -1
     assert lib.btb_hip_norm_rope_axes(p(qkv), None, None, 1e-6, p(cos), p(cos), 0, 16, D, p(pos), 3, p(axes), None, p(K), p(V), p(q), T, Hq,
