@@ -621,10 +621,11 @@ struct SharedPlan {
     int pair_tiles, prefix_spans, own_spans, states;
 };
 // A prefix workgroup a CU, the rows' own beside them; two a CU where the products are what the prefix costs - 128 pairs of a head and
-// more, spans of eight stages and more - and the rows' own keys, read at 5.1 TB/s, cost less than half of that (at 900 TFLOP/s).
+// more, spans of eight stages and more (three at head_dim 64) - and the rows' own keys, read at 5.1 TB/s, cost less than half of that (at 900 TFLOP/s).
 // us, one a CU / two: 16 rows x 131072 keys, 100 own 107 / 119; 4 rows 102 / 107; 256 x 32768, 640 own 235 / 273, 64 own 192 /
-// 172, 64 x 131072, 640 own 212 / 196.
-static SharedPlan shared_plan(size_t T, size_t Hq, size_t Hk, size_t prefix_cap, size_t own_cap) {
+// 172, 64 x 131072, 640 own 212 / 196; 60 rows of 48 heads x 12000 (spans of six) 42 / 45; head_dim 64, 2 kv heads of 8, 200 rows x 20000
+// (of five) 50 / 41, of 4, 36 x 98126 (of six) 37.7 / 36.6.
+static SharedPlan shared_plan(size_t T, size_t Hq, size_t Hk, size_t D, size_t prefix_cap, size_t own_cap) {
     const size_t G = Hq / Hk, pairs = T * G, cus = (size_t)device_info().cus;
     auto spans = [&](size_t groups, size_t cap, size_t wgs) {
         const size_t most = (cap + SH_KEYS - 1) / SH_KEYS, want = (wgs + groups - 1) / groups;
@@ -635,7 +636,7 @@ static SharedPlan shared_plan(size_t T, size_t Hq, size_t Hk, size_t prefix_cap,
     const size_t wide = 32 * (size_t)r.qw;
     r.pair_tiles = (int)((pairs + wide - 1) / wide);
     const size_t groups = Hk * r.pair_tiles;
-    const bool twice = pairs >= 128 && prefix_cap * groups >= 2 * cus * 8 * SH_KEYS && own_cap * 352 < G * prefix_cap;
+    const bool twice = pairs >= 128 && prefix_cap * groups >= 2 * cus * (D == 64 ? 3 : 8) * SH_KEYS && own_cap * 352 < G * prefix_cap;
     r.prefix_spans = spans(groups, prefix_cap, (twice ? 2 : 1) * cus);
     r.own_spans = spans(Hk * T, own_cap, cus);
     if (r.prefix_spans + r.own_spans == 0) r.own_spans = 1;  // no key anywhere: states that say so
@@ -672,7 +673,7 @@ extern "C" {
 
 size_t btb_hip_attn_shared_floats(size_t T, size_t Hq, size_t Hk, size_t D, size_t prefix_cap, size_t own_cap) {
     if (!shared_sizes_fit(T, Hq, Hk, D, prefix_cap, own_cap)) return 0;
-    const SharedPlan s = shared_plan(T, Hq, Hk, prefix_cap, own_cap);
+    const SharedPlan s = shared_plan(T, Hq, Hk, D, prefix_cap, own_cap);
     const size_t n = T * Hq * (size_t)s.states;
     return (2 * n + 3) / 4 * 4 + n * D;
 }
@@ -688,7 +689,7 @@ int32_t btb_hip_attn_shared(const void* q, const void* K, const void* V, void* a
                   "and the workspace 16-byte aligned with strides in multiples of 8, a row's up to 2^25");
         return ERR_DOMAIN;
     }
-    const SharedPlan s = shared_plan(T, Hq, Hk, prefix_cap, own_cap);
+    const SharedPlan s = shared_plan(T, Hq, Hk, D, prefix_cap, own_cap);
     const size_t n = T * Hq * (size_t)s.states;
     SharedArgs p;
     p.q = static_cast<const uint16_t*>(q);
