@@ -70,9 +70,9 @@ __device__ __forceinline__ void table_run(const float* t, float (&v)[8]) {
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 
-template <int D, class TT>
+template <int D, class TT, int AT_ONCE>
 __global__ void __launch_bounds__(256) rope_axes_kernel(RopeAxes p) {
-    constexpr int LPH = D / 16, HPW = 64 / LPH, HALF = D / 2, AT_ONCE = 3;
+    constexpr int LPH = D / 16, HPW = 64 / LPH, HALF = D / 2;
     const int lane = threadIdx.x & 63, l = lane % LPH, heads = p.Hq + 2 * p.Hk;
     const long long wave = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t = (int)(wave / p.split), part = (int)(wave % p.split);
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(RopeAxes p) {
             *reinterpret_cast<uint4*>(dst) = narrow8(x);
             *reinterpret_cast<uint4*>(dst + HALF) = narrow8(y);
         }
-        request(head + AT_ONCE * p.split * HPW);
+        if (__any(head + AT_ONCE * p.split * HPW < heads)) request(head + AT_ONCE * p.split * HPW);
     }
 }
 
@@ -198,10 +198,11 @@ static void launch_rope_axes(RopeAxes& p, bool wide_table, hipStream_t st) {
     const int groups = (p.Hq + 2 * p.Hk + 1024 / D - 1) / (1024 / D), want = (8 * device_info().cus + p.T - 1) / p.T;
     p.split = want < groups ? want : groups;
     const dim3 grid((unsigned)(((long long)p.T * p.split + 3) / 4));
+    const bool once = p.split == groups;  // a wave has one group of heads
     if (wide_table)
-        hipLaunchKernelGGL((rope_axes_kernel<D, float>), grid, dim3(256), 0, st, p);
+        hipLaunchKernelGGL((once ? rope_axes_kernel<D, float, 1> : rope_axes_kernel<D, float, 3>), grid, dim3(256), 0, st, p);
     else
-        hipLaunchKernelGGL((rope_axes_kernel<D, uint16_t>), grid, dim3(256), 0, st, p);
+        hipLaunchKernelGGL((once ? rope_axes_kernel<D, uint16_t, 1> : rope_axes_kernel<D, uint16_t, 3>), grid, dim3(256), 0, st, p);
 }
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
