@@ -7,11 +7,12 @@
 //   out[i + D/2]   = y[i + D/2] c_i + y[i] s_i
 //
 // in f32 throughout, rounded to bf16 once. Bound: memory, the qkv rows read once and q, K and V written once: 16384 rows of 48 heads x 128 take
-// 92 us (4.4 TB/s); one row takes 9.2, the launch.
+// 89 us (4.6 TB/s); one row takes 9.1, the launch.
 //
 // A head by D / 16 lanes: lane l holds dims 8 l .. + 7 and their partners D / 2 further on, so the rotation stays within a lane and
 // loads and stores are 16 bytes. A wave takes 1024 / D heads of one row at a time and keeps the row's sixteen cosines and sines;
-// many rows: a row a wave, few: a row's heads over several.
+// many rows: a row a wave, few: a row's heads over several. AT_ONCE groups of heads are on their way at a time: three, or one where
+// a wave has no more (16122 rows of 7 + 1 heads x 64: three 42 us, one 35: fewer registers, more waves).
 
 #include "btb_common.hpp"
 #include "btb_tuning.hpp"
