@@ -10,13 +10,14 @@
 // and leaves states (maximum, sum, output) in the scratch, which a second launch folds in a fixed order. The spans are
 // cut from the keys there are (the layout lies on the device), so a recorded launch holds while the rows grow.
 //
-// Sums and outputs are f32; a weight is rounded to bf16 for the product with V, as the matrix cores take it (relative
-// 2-norm against 64 bits 2.3e-3 where rounding the output alone makes 1.7e-3), and the sum takes the unrounded weight.
+// Sums and outputs are f32; a weight goes to the matrix cores as two bf16 terms, since one leaves the outputs of wide passes 1.9e-3 off
+// (relative 2-norm against 64 bits; 40 rows of 16 / 2 heads, normal values, scores of deviation 3) and two 1.65e-3, what rounding
+// the outputs alone makes. us, one / two: 16 rows of 32 heads x 128 over 131072 keys, 100 own 104 / 105; 256 rows over 32768 160 / 211,
+// and 640 own 239 / 284; 256 rows of 40 heads x 64 over 32768 141 / 196; 41 rows over 6001, 485 own 19.5 / 21.3.
 //
-// Bound: memory where few rows share the prefix (16 rows of 32 heads x 128 over 131072 keys, 100 own: 104 us, 5.2 TB/s), the products and
-// what stands between them where many do (256 rows over 32768: 156 us, 880 TFLOP/s, the fold included; bare products reach 1384), and
-// both at once where many rows have many own keys (640 each: 235 us, 3.4 TB/s and 590 TFLOP/s): there a prefix workgroup a CU takes 204 us of
-// 8192 keys, 167 with no own keys beside it, 139 without its loads, 130 without its barriers and 94 for the products alone.
+// Bound: memory where few rows share the prefix (16 rows of 32 heads x 128 over 131072 keys, 100 own: 105 us, 5.2 TB/s), the products
+// where many do (256 rows over 32768: 211 us, the fold included; three products for every two of the formula, 975 TFLOP/s of bare
+// products' 1384), and both at once where many rows have many own keys (640 each: 284 us, 2.8 TB/s and 495 TFLOP/s).
 
 #include "btb_common.hpp"
 #include "btb_tile32.hpp"
@@ -118,8 +119,7 @@ __device__ __forceinline__ void walk(const SharedArgs& p, const uint16_t* Kg, co
     // and what vector arithmetic there is to do meanwhile - a group's weights under the next one's scores, that one's maximum
     // under the first one's outputs - is dealt out between the products.
     constexpr int GT = TPW < 2 ? TPW : 2, GROUPS = TPW / GT, AHEAD = 4;
-    f32x16 st[GROUPS][GT];
-    bf16x8 pf[GT][2];
+    f32x16 st[GROUPS][GT];  // scores, then weights
     auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
     // products GT STEPS; work(i) after each of the STEPS
     auto scores = [&](uint32_t at, int group, f32x16(&to)[GT], auto work) {
@@ -168,41 +168,23 @@ __device__ __forceinline__ void walk(const SharedArgs& p, const uint16_t* Kg, co
                 for (int i = 0; i < 16; ++i) o[d][i] *= corr;
         }
     };
-    // scores [from, to) of a group as weights
-    float w[GT][16];
+    // scores [from, to) of a group as weights, in their place
     auto weigh = [&](int group, float ref, int from, int to) {
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < GT * 16; ++e)
             if (e >= from && e < to) {
-                w[e / 16][e % 16] = __builtin_amdgcn_exp2f(fmaf(st[group][e / 16][e % 16], p.scale_log2, -ref));
-                sum += w[e / 16][e % 16];
-                if (e % 8 == 7) {
-                    pf[e / 16][e % 16 / 8] = weight_fragment(&w[e / 16][e % 16 - 7]);
-                    made(pf[e / 16][e % 16 / 8]);
-                }
+                const float w = __builtin_amdgcn_exp2f(fmaf(st[group][e / 16][e % 16], p.scale_log2, -ref));
+                st[group][e / 16][e % 16] = w;
+                sum += w;
             }
         l += sum;
     };
-    // products GT 2 DT; work(r) after every second
+    // products GT 4 DT; work(r), GT DT of them
     auto outputs = [&](uint32_t at, int group, auto work) {
-        constexpr int ALL = GT * 2 * DT;
-        bf16x8 vf[ALL];
-        auto read = [&](int e) {
-            return v_fragment<D>(lds + (4 + kw) * TILE, at, KW * (GT * group + e / (2 * DT)) * TILE, e % DT, e / DT % 2);
-        };
-#pragma unroll
-        for (int e = 0; e < AHEAD; ++e) vf[e] = read(e);
-        fence();
-#pragma unroll
-        for (int e = 0; e < ALL; ++e) {
-            if (e + AHEAD < ALL) vf[e + AHEAD] = read(e + AHEAD);
-            o[e % DT] = mfma32(vf[e], pf[e / (2 * DT)][e / DT % 2], o[e % DT]);
-            if (e % 2 == 1) {
-                work(e / 2);
-                fence();
-            }
-        }
+        weighted_sums<DT, 2 * GT>(
+            o, [&](int u, int d) { return v_fragment<D>(lds + (4 + kw) * TILE, at, KW * (GT * group + u / 2) * TILE, d, u % 2); },
+            [&](int u, int i) { return st[group][u / 2][8 * (u % 2) + i]; }, work);
     };
     auto nothing = [](int) {};
     const uint32_t k_at = k_place<D>(lane), v_at = v_place<D>(lane);
@@ -315,9 +297,10 @@ __device__ __forceinline__ void walk(const SharedArgs& p, const uint16_t* Kg, co
 // it costs. Stages of 64 keys, three of K and two of V in LDS, every wave bringing half a tile of each. A stage's weights are made
 // between the products of the next one's scores, and that one's maxima between the products of its outputs: no stretch of a stage
 // is vector arithmetic alone. Two barriers a stage where walk has four.
-// For head_dim 64, where the exponentials cost as much as the products and so are worth hiding; at 128 one tile's chain of eight
-// dependent products sets the pace and walk is as fast or faster. us, walk / this: 256 rows of 40 heads x 64 over 32768 keys 159 /
-// 139, 41 rows over 6001 and 485 own 21.6 / 19.5; 256 rows of 32 heads x 128 over 32768 keys 160 / 159, and 640 own 232 / 252.
+// For head_dim 64, where the vector arithmetic costs as much as the products and so is worth hiding; at 128 one tile's chain of eight
+// dependent products sets the pace and walk is faster. us, walk / this: head_dim 64, 41 rows of 40 / 8 heads over 6001 and 485 own 23.2 /
+// 21.3, 200 rows of 16 / 2 over 20000 54 / 48, 256 of 40 / 8 over 32768 212 / 209; 256 rows of 32 / 8 heads x 128 over 32768 keys 217 /
+// 223, and 640 own 285 / 317.
 template <int D, int QW>
 constexpr bool overlaps() {
     return D == 64 && QW == 4;
@@ -375,9 +358,9 @@ __device__ __forceinline__ void walk_many(const SharedArgs& p, const uint16_t* K
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): q is here, and no register of the loop waits for a load
     fence();
     const uint32_t k_at = k_place<D>(lane), v_at = v_place<D>(lane);
-    f32x16 st[2];    // a stage's scores
-    u32x4 pw[2][2];  // its weights
+    f32x16 st[2], next[2];  // a stage's scores, then weights; the next one's scores
     // the scores of tile `tile` of a stage; work(i) after each of the STEPS
+    next[0] = next[1] = zero16();
     auto scores = [&](uint32_t at, int slot, int tile, f32x16& to, auto work) {
         bf16x8 kf[STEPS];
         const uint8_t* tiles = lds + slot * STAGE;
@@ -393,32 +376,20 @@ __device__ __forceinline__ void walk_many(const SharedArgs& p, const uint16_t* K
             fence();
         }
     };
-    // its outputs; work(r) after every second product
+    // its outputs; work(r), 2 DT of them
     auto outputs = [&](uint32_t at, int s, auto work) {
-        constexpr int ALL = 4 * DT;
-        bf16x8 vf[ALL];
         const uint8_t* tiles = v_lds + (s & 1) * STAGE;
-        auto read = [&](int e) { return v_fragment<D>(tiles, at, e / (2 * DT) * TILE, e % DT, e / DT % 2); };
-#pragma unroll
-        for (int e = 0; e < AHEAD; ++e) vf[e] = read(e);
-        fence();
-#pragma unroll
-        for (int e = 0; e < ALL; ++e) {
-            if (e + AHEAD < ALL) vf[e + AHEAD] = read(e + AHEAD);
-            o[e % DT] = mfma32(vf[e], __builtin_bit_cast(bf16x8, pw[e / (2 * DT)][e / DT % 2]), o[e % DT]);
-            if (e % 2 == 1) {
-                work(e / 2);
-                fence();
-            }
-        }
+        weighted_sums<DT, 4>(
+            o, [&](int u, int d) { return v_fragment<D>(tiles, at, u / 2 * TILE, d, u % 2); },
+            [&](int u, int i) { return st[u / 2][8 * (u % 2) + i]; }, work);
     };
-    auto mask = [&](int s) {  // keys past the end
+    auto mask = [&](int s, f32x16(&of)[2]) {  // keys past the end
         if (64 * s + 64 <= keys.count) return;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                if (8 * (i / 4) + i % 4 >= keys.count - 64 * s - TK * j - 4 * (ln >> 5)) st[j][i] = ninf;
+                if (8 * (i / 4) + i % 4 >= keys.count - 64 * s - TK * j - 4 * (ln >> 5)) of[j][i] = ninf;
     };
     auto settle = [&](float top) {  // as in walk
         top = fmaxf(top, xor32(top)) * p.scale_log2;
@@ -444,7 +415,7 @@ __device__ __forceinline__ void walk_many(const SharedArgs& p, const uint16_t* K
         barrier();
         scores(ak, 0, 0, st[0], [](int) {});
         scores(ak, 0, 1, st[1], [](int) {});
-        mask(0);
+        mask(0, st);
         float top = st[0][0];
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(st[0][i], st[1][i]));
@@ -465,23 +436,16 @@ __device__ __forceinline__ void walk_many(const SharedArgs& p, const uint16_t* K
         constexpr int EACH = 16 / STEPS;
         auto weigh = [&](int j, int step) {
 #pragma unroll
-            for (int e = 0; e < 16; e += 2)
+            for (int e = 0; e < 16; ++e)
                 if (e / EACH == step) {
-                    const float w0 = __builtin_amdgcn_exp2f(fmaf(st[j][e], p.scale_log2, -ref));
-                    const float w1 = __builtin_amdgcn_exp2f(fmaf(st[j][e + 1], p.scale_log2, -ref));
-                    sum += w0;
-                    sum += w1;
-                    pw[j][e / 8][e % 8 / 2] = f32x2_bf16(w0, w1);
-                    if (e % 8 == 6) asm volatile("" : "+v"(pw[j][e / 8]));  // made here, not where they are used
+                    st[j][e] = __builtin_amdgcn_exp2f(fmaf(st[j][e], p.scale_log2, -ref));
+                    sum += st[j][e];
                 }
         };
-        f32x16 next[2];
         if (left > 0) {
             scores(ak, slot, 0, next[0], [&](int i) { weigh(0, i); });
             scores(ak, slot, 1, next[1], [&](int i) { weigh(1, i); });
-            st[0] = next[0];
-            st[1] = next[1];
-            mask(s + 1);
+            mask(s + 1, next);
         } else {
 #pragma unroll
             for (int i = 0; i < 2 * STEPS; ++i) weigh(i / STEPS, i % STEPS);
@@ -494,18 +458,20 @@ __device__ __forceinline__ void walk_many(const SharedArgs& p, const uint16_t* K
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
         barrier();
-        // (after the last stage st holds its own scores still: their maximum moves nothing that matters)
-        float top = st[0][0], other = st[1][0];
+        // (after the last stage `next` holds the last one's scores or none: their maximum goes nowhere)
+        float top = next[0][0], other = next[1][0];
         constexpr int EACH_MAX = 16 / (2 * DT);
         outputs(av, s, [&](int r) {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 if (i / EACH_MAX == r) {
-                    top = fmaxf(top, st[0][i]);
-                    other = fmaxf(other, st[1][i]);
+                    top = fmaxf(top, next[0][i]);
+                    other = fmaxf(other, next[1][i]);
                 }
         });
         if (left > 0) settle(fmaxf(top, other));
+        st[0] = next[0];
+        st[1] = next[1];
     }
     l += xor32(l);
     // the outputs through LDS, a pair's 16-byte chunks permuted, so that they are written in whole rows
@@ -621,10 +587,11 @@ struct SharedPlan {
     int pair_tiles, prefix_spans, own_spans, states;
 };
 // A prefix workgroup a CU, the rows' own beside them; two a CU where the products are what the prefix costs - 128 pairs of a head and
-// more, spans of eight stages and more (three at head_dim 64) - and the rows' own keys, read at 5.1 TB/s, cost less than half of that (at 900 TFLOP/s).
-// us, one a CU / two: 16 rows x 131072 keys, 100 own 107 / 119; 4 rows 102 / 107; 256 x 32768, 640 own 235 / 273, 64 own 192 /
-// 172, 64 x 131072, 640 own 212 / 196; 60 rows of 48 heads x 12000 (spans of six) 42 / 45; head_dim 64, 2 kv heads of 8, 200 rows x 20000
-// (of five) 50 / 41, of 4, 36 x 98126 (of six) 37.7 / 36.6.
+// more, spans of eight stages and more (three at head_dim 64) - and the rows' own keys, read at 5.1 TB/s, cost less than half of that (at
+// 640 TFLOP/s). us, one a CU / two: 16 rows x 131072 keys, 100 own 105 / 114; 4 rows 98 / 102; 256 x 32768, 640 own 286 / 306, 400 own
+// 273 / 266, 64 own 253 / 218, 64 x 131072, 640 own 269 / 240; 48 heads, 60 rows x 12000 (spans of five) 51 / 53, x 24000 (of nine) 82 / 78;
+// 128 x 10000 (of five) 51 / 59, x 17000 (of nine) 76 / 79.5; 24 heads, 200 x 20000 (of thirteen) 117 / 107. Head_dim 64, 2 kv heads of 8, 200
+// rows x 8000 (of four) 34 / 32, x 20000 (of eight) 63 / 49, of 4, 36 x 98126 (of six) 46 / 39.5.
 static SharedPlan shared_plan(size_t T, size_t Hq, size_t Hk, size_t D, size_t prefix_cap, size_t own_cap) {
     const size_t G = Hq / Hk, pairs = T * G, cus = (size_t)device_info().cus;
     auto spans = [&](size_t groups, size_t cap, size_t wgs) {
@@ -636,7 +603,7 @@ static SharedPlan shared_plan(size_t T, size_t Hq, size_t Hk, size_t D, size_t p
     const size_t wide = 32 * (size_t)r.qw;
     r.pair_tiles = (int)((pairs + wide - 1) / wide);
     const size_t groups = Hk * r.pair_tiles;
-    const bool twice = pairs >= 128 && prefix_cap * groups >= 2 * cus * (D == 64 ? 3 : 8) * SH_KEYS && own_cap * 352 < G * prefix_cap;
+    const bool twice = pairs >= 128 && prefix_cap * groups >= 2 * cus * (D == 64 ? 3 : 8) * SH_KEYS && own_cap * 250 < G * prefix_cap;
     r.prefix_spans = spans(groups, prefix_cap, (twice ? 2 : 1) * cus);
     r.own_spans = spans(Hk * T, own_cap, cus);
     if (r.prefix_spans + r.own_spans == 0) r.own_spans = 1;  // no key anywhere: states that say so

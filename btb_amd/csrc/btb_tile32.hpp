@@ -154,10 +154,16 @@ __device__ __forceinline__ void wait_loads(uint32_t& at) {
     asm volatile("s_waitcnt vmcnt(%1)" : "+v"(at) : "n"(N) : "memory");
 }
 
-// eight weights as an operand
-__device__ __forceinline__ bf16x8 weight_fragment(const float* p) {
-    return __builtin_bit_cast(bf16x8, make_uint4(f32x2_bf16(p[0], p[1]), f32x2_bf16(p[2], p[3]), f32x2_bf16(p[4], p[5]),
-                                                 f32x2_bf16(p[6], p[7])));
+// A weight (0 or more) as two bf16 terms: its upper half, and the upper half of what that leaves; 2^-15 of it at most stays out.
+// Neither term has another sign than the weight, nor is the second zero where the weight is 2^-100 and more (its lowest bit is
+// set, 2^-23 of it), so that an infinite value stays infinite in both products. Two weights at a time.
+__device__ __forceinline__ uint32_t first_terms(float a, float b) {
+    return __builtin_amdgcn_perm(f32_bits(b), f32_bits(a), 0x07060302u);
+}
+__device__ __forceinline__ uint32_t second_terms(float a, float b) {
+    const float ra = bits_f32(f32_bits(a) | 1u) - bits_f32(f32_bits(a) & 0xFFFF0000u);
+    const float rb = bits_f32(f32_bits(b) | 1u) - bits_f32(f32_bits(b) & 0xFFFF0000u);
+    return first_terms(ra, rb);
 }
 
 __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
@@ -172,10 +178,51 @@ __device__ __forceinline__ f32x16 zero16() {
 }
 
 // the value is made here, not where it is first used
-__device__ __forceinline__ void made(bf16x8& v) {
-    u32x4 w = __builtin_bit_cast(u32x4, v);
-    asm volatile("" : "+v"(w));
-    v = __builtin_bit_cast(bf16x8, w);
+__device__ __forceinline__ void made(uint32_t& v) { asm volatile("" : "+v"(v)); }
+
+// DT outputs of 32 dims += V^T times a tile's weights, as two terms, against V's fragments as they are asked for: 16 keys and DT
+// fragments a unit, UNITS of them. The next unit's fragments come in and a unit's second terms are made between the products of
+// its first; what else there is to do - `work`, numbered - goes between those of its second. read(unit, dt): a fragment;
+// weight(unit, i): the i-th of a unit's eight weights a lane.
+template <int DT, int UNITS, class Read, class Weight, class Work>
+__device__ __forceinline__ void weighted_sums(f32x16 (&o)[DT], Read read, Weight weight, Work work) {
+    auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
+    bf16x8 vf[UNITS + 1][DT];
+    u32x4 first[UNITS + 1], second;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) vf[0][d] = read(0, d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) first[0][i] = first_terms(weight(0, 2 * i), weight(0, 2 * i + 1));
+    fence();
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            if (u + 1 < UNITS) vf[u + 1][d] = read(u + 1, d);
+            o[d] = mfma32(vf[u][d], __builtin_bit_cast(bf16x8, first[u]), o[d]);
+#pragma unroll
+            for (int i = 4 * d / DT; i < 4 * (d + 1) / DT; ++i) {
+                uint32_t w = second_terms(weight(u, 2 * i), weight(u, 2 * i + 1));
+                made(w);
+                second[i] = w;
+            }
+            fence();
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            o[d] = mfma32(vf[u][d], __builtin_bit_cast(bf16x8, second), o[d]);
+            if (u + 1 < UNITS) {
+#pragma unroll
+                for (int i = 4 * d / DT; i < 4 * (d + 1) / DT; ++i) {
+                    uint32_t w = first_terms(weight(u + 1, 2 * i), weight(u + 1, 2 * i + 1));
+                    made(w);
+                    first[u + 1][i] = w;
+                }
+            }
+            if (d % 2 == 1) work((u * DT + d) / 2);
+            fence();
+        }
+    }
 }
 
 }  // namespace btb
