@@ -20,7 +20,7 @@ from .decode import StackConfig, recording, rope_axes, rope_tables
 
 class Forks:
     """`rows` continuations of up to `steps` tokens each over at most `budget` keys a head of one prompt, which goes in `chunk` tokens
-    at a time and may be of any length up to `positions` less `steps`. Of its keys the first `sinks` and the newest `recent` always
+    at a time and stands on any places up to `positions` less `steps`. Of its keys the first `sinks` and the newest `recent` always
     stay. `sections`: how many frequencies each position axis turns (one axis: all of them), `interleaved` as in `rope_axes`."""
 
     def __init__(self, card: Any, cfg: StackConfig, weights: dict[str, Any], rows: int, budget: int, steps: int, chunk: int = 32,
@@ -45,18 +45,29 @@ class Forks:
         self.axes = rope_axes(sections, dev, interleaved)
         self.n = 0      # keys of the prompt a head holds
         self.seen = 0   # tokens of the prompt so far
+        self.place = 0  # where the next token stands on every axis: one past the largest place so far
         self.taken = 0  # steps the rows have taken
         self._pass = _Pass(self, chunk, self.held, chunk)
         self._step = _Pass(self, rows, self.held, steps)
         self.graph: torch.cuda.CUDAGraph | None = None
 
     def prompt(self, tokens: Sequence[int], places: torch.Tensor | None = None) -> torch.Tensor:
-        """the prompt's next tokens, at `places` (int32 [axes, tokens] on the GPU) or one after the other on every axis; the last
-        one's logits [vocab]"""
+        """the prompt's next tokens, at `places` (integers [axes, tokens]) or one after the other on every axis, from one
+        past the largest place so far; the last one's logits [vocab]"""
         if self.taken:
             raise RuntimeError("[forks] the rows have begun: the prompt is closed")
-        if not tokens or self.seen + len(tokens) + self.steps > self.positions:
-            raise ValueError(f"[forks] {len(tokens)} tokens after {self.seen}: the tables hold {self.positions} positions")
+        if not tokens:
+            raise ValueError("[forks] no tokens")
+        low, end = self.place, self.place + len(tokens)
+        if places is not None:
+            axes = self._pass.pos.shape[0]
+            if places.is_floating_point() or places.shape != (axes, len(tokens)):
+                raise ValueError(f"[forks] places are integers [{axes}, {len(tokens)}], got {places.dtype} {list(places.shape)}")
+            low, top = (int(v) for v in places.aminmax())
+            end = max(self.place, top + 1)
+        if low < 0 or end + self.steps > self.positions:
+            raise ValueError(f"[forks] {len(tokens)} tokens on places from {low}, {self.steps} steps from {end} on: the tables hold "
+                             f"{self.positions} positions")
         p, logits = self._pass, None
         for at in range(0, len(tokens), self.chunk):
             part = tokens[at:at + self.chunk]
@@ -65,7 +76,7 @@ class Forks:
                 p = _Pass(self, T, self.held, T)
             first = torch.arange(T, dtype=torch.int32, device="cuda")
             p.ids.copy_(torch.tensor(list(part), dtype=torch.int32))
-            p.pos.copy_(first + self.seen if places is None else places[:, at:at + T])
+            p.pos.copy_(first + self.place + at if places is None else places[:, at:at + T])
             p.slots.copy_(first + self.n)
             # a chain: every row sees the keys there are and the pass's own up to itself
             p.lay.copy_(self.card.shared_layout(0, self.n, [(self.n, t + 1) for t in range(T)]))
@@ -76,6 +87,7 @@ class Forks:
             self.seen += T
             if self.n > self.budget:
                 self.cut()
+        self.place = end
         return logits[-1]
 
     def cut(self) -> None:
@@ -91,7 +103,7 @@ class Forks:
         p = self._step
         base = [self.held + t * self.steps for t in range(self.rows)]
         p.ids.copy_(torch.tensor(list(tokens), dtype=torch.int32))
-        p.pos.fill_(self.seen)
+        p.pos.fill_(self.place)
         p.slots.copy_(torch.tensor(base, dtype=torch.int32))
         p.lay.copy_(self.card.shared_layout(0, self.n, [(b, 1) for b in base]))
         self.taken = 0
