@@ -47,6 +47,7 @@ class Forks:
         self.seen = 0   # tokens of the prompt so far
         self.place = 0  # where the next token stands on every axis: one past the largest place so far
         self.taken = 0  # steps the rows have taken
+        self.begun = False  # whether the rows' tokens and slots describe the cache
         self._pass = _Pass(self, chunk, self.held, chunk)
         self._step = _Pass(self, rows, self.held, steps)
         self.graph: torch.cuda.CUDAGraph | None = None
@@ -106,10 +107,11 @@ class Forks:
         p.pos.fill_(self.place)
         p.slots.copy_(torch.tensor(base, dtype=torch.int32))
         p.lay.copy_(self.card.shared_layout(0, self.n, [(b, 1) for b in base]))
-        self.taken = 0
+        self.taken, self.begun = 0, True
 
     def step(self) -> torch.Tensor:
         """a token more in every row, the greedy picks fed forward; the logits [rows, vocab]. Recorded by `capture`: replayed."""
+        self._need_rows()
         if self.taken >= self.steps:
             raise RuntimeError(f"[forks] the rows have room for {self.steps} tokens")
         self.taken += 1
@@ -117,6 +119,10 @@ class Forks:
             self.graph.replay()
             return self._step.logits
         return self._body()
+
+    def _need_rows(self) -> None:
+        if not self.begun:  # their slots are the prompt's
+            raise RuntimeError("[forks] the rows have no tokens yet: begin first")
 
     def _body(self) -> torch.Tensor:
         p = self._step
@@ -129,6 +135,7 @@ class Forks:
 
     def capture(self) -> None:
         """records a step; the rows' state is as before (`begin` first)"""
+        self._need_rows()
         p = self._step
         state = [t.clone() for t in (p.ids, p.pos, p.slots, p.lay)]
         side = torch.cuda.Stream()

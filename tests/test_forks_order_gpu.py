@@ -1,0 +1,50 @@
+"""`Forks` called out of order: what cannot be answered rightly is refused and leaves the cache and the rows as they were."""
+
+from __future__ import annotations
+
+import os
+
+import pytest
+import torch
+
+from btb_amd.forks import Forks
+from btb_amd.load import load_stack
+
+from .helpers import GOLDEN
+
+pytestmark = pytest.mark.gpu
+
+PROMPT = [3, 17, 42, 5, 99, 120, 7, 7, 200, 12]
+
+
+@pytest.fixture(scope="module")
+def stack(card):
+    return load_stack(card, os.path.join(GOLDEN, "tiny_qwen3"))
+
+
+def _forks(card, stack, rows=3, steps=4, budget=32):
+    cfg, w = stack
+    return Forks(card, cfg, w, rows, budget=budget, steps=steps, chunk=8, sinks=1, recent=4, positions=128)
+
+
+def _held(f):
+    torch.cuda.synchronize()
+    return [t.clone() for t in (f.kv, f.mass, f.pos, f._step.ids, f._step.pos, f._step.slots, f._step.lay)] + [f.n, f.seen, f.taken]
+
+
+def _same(a, b):
+    return all(torch.equal(x, y) if isinstance(x, torch.Tensor) else x == y for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("prompted", [False, True])
+def test_no_step_and_no_recording_before_the_rows_begin(card, stack, prompted):
+    """the rows' slots are the prompt's first one then: a pass would write all of them there"""
+    f = _forks(card, stack)
+    if prompted:
+        f.prompt(PROMPT)
+    before = _held(f)
+    with pytest.raises(RuntimeError):
+        f.step()
+    with pytest.raises(RuntimeError):
+        f.capture()
+    assert f.graph is None and _same(_held(f), before)
