@@ -54,7 +54,7 @@ class Forks:
 
     def prompt(self, tokens: Sequence[int], places: torch.Tensor | None = None) -> torch.Tensor:
         """the prompt's next tokens, at `places` (integers [axes, tokens]) or one after the other on every axis, from one
-        past the largest place so far; the last one's logits [vocab]"""
+        past the largest place so far; the last one's logits [vocab]. Rows that had begun, with no step yet, begin again."""
         if self.taken:
             raise RuntimeError("[forks] the rows have begun: the prompt is closed")
         if not tokens:
@@ -69,6 +69,7 @@ class Forks:
         if low < 0 or end + self.steps > self.positions:
             raise ValueError(f"[forks] {len(tokens)} tokens on places from {low}, {self.steps} steps from {end} on: the tables hold "
                              f"{self.positions} positions")
+        self.begun = False  # rows that had begun begin again, behind these tokens
         p, logits = self._pass, None
         for at in range(0, len(tokens), self.chunk):
             part = tokens[at:at + self.chunk]
@@ -121,8 +122,8 @@ class Forks:
         return self._body()
 
     def _need_rows(self) -> None:
-        if not self.begun:  # their slots are the prompt's
-            raise RuntimeError("[forks] the rows have no tokens yet: begin first")
+        if not self.begun:  # their slots are the prompt's first, or their layout that of a prompt before its last tokens
+            raise RuntimeError("[forks] the rows have not begun behind the prompt as it is: begin first")
 
     def _body(self) -> torch.Tensor:
         p = self._step

@@ -48,3 +48,32 @@ def test_no_step_and_no_recording_before_the_rows_begin(card, stack, prompted):
     with pytest.raises(RuntimeError):
         f.capture()
     assert f.graph is None and _same(_held(f), before)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_longer_prompt_is_what_the_rows_begin_behind(card, stack, captured):
+    """tokens between `begin` and the first step: the rows begin again, and are then those of the whole prompt"""
+    whole, f = _forks(card, stack, budget=12), _forks(card, stack, budget=12)
+    for t in (PROMPT, [60, 61, 8, 45, 3]):
+        whole.prompt(t)
+    f.prompt(PROMPT)
+    f.begin([5, 6, 7])
+    if captured:
+        f.capture()
+    with pytest.raises(ValueError):
+        f.prompt([1] * 128)  # refused: the rows stand as they did
+    f.prompt([60, 61, 8, 45, 3])
+    before = _held(f)
+    for call in (f.step, f.capture):
+        with pytest.raises(RuntimeError):
+            call()
+    assert _same(_held(f), before)
+    for g in (whole, f):
+        g.begin([5, 6, 7])
+    for _ in range(4):
+        a, b = whole.step().clone(), f.step().clone()
+        torch.cuda.synchronize()
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError):
+        f.prompt([1])
+    assert f.begun and f.taken == 4
