@@ -113,8 +113,6 @@ class Forks:
     def step(self) -> torch.Tensor:
         """a token more in every row, the greedy picks fed forward; the logits [rows, vocab]. Recorded by `capture`: replayed."""
         self._need_rows()
-        if self.taken >= self.steps:
-            raise RuntimeError(f"[forks] the rows have room for {self.steps} tokens")
         self.taken += 1
         if self.graph is not None:
             self.graph.replay()
@@ -124,6 +122,8 @@ class Forks:
     def _need_rows(self) -> None:
         if not self.begun:  # their slots are the prompt's first, or their layout that of a prompt before its last tokens
             raise RuntimeError("[forks] the rows have not begun behind the prompt as it is: begin first")
+        if self.taken >= self.steps:  # the next slot is another row's
+            raise RuntimeError(f"[forks] the rows have room for {self.steps} tokens")
 
     def _body(self) -> torch.Tensor:
         p = self._step
@@ -135,7 +135,7 @@ class Forks:
         return p.logits
 
     def capture(self) -> None:
-        """records a step; the rows' state is as before (`begin` first)"""
+        """records a step, for which the rows have room; their state is as before (`begin` first)"""
         self._need_rows()
         p = self._step
         state = [t.clone() for t in (p.ids, p.pos, p.slots, p.lay)]

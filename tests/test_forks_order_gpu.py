@@ -77,3 +77,20 @@ def test_a_longer_prompt_is_what_the_rows_begin_behind(card, stack, captured):
     with pytest.raises(RuntimeError):
         f.prompt([1])
     assert f.begun and f.taken == 4
+
+
+def test_no_recording_without_room(card, stack):
+    """with all steps taken, the pass that warms a recording up would write each row's next slot: the next row's first"""
+    f = _forks(card, stack, steps=2)
+    f.prompt(PROMPT)
+    f.begin([5, 6, 7])
+    f.step()
+    f.step()
+    before = _held(f)
+    with pytest.raises(RuntimeError):
+        f.capture()
+    assert f.graph is None and _same(_held(f), before)
+    f.begin([8, 9, 10])
+    f.capture()
+    f.step()
+    f.step()
