@@ -87,13 +87,14 @@ class Forks:
             self.pos[:, :, self.n:self.n + T] = first + self.seen
             self.n += T
             self.seen += T
-            if self.n > self.budget:
-                self.cut()
+            self.cut()
         self.place = end
         return logits[-1]
 
     def cut(self) -> None:
-        """every layer's cache back to the budget, in place"""
+        """every layer's cache back to the budget, in place; one within it stays as it is"""
+        if self.n <= self.budget:
+            return
         K, V = self.kv[:, 0], self.kv[:, 1]
         self.n = self.card.kv_evict(self.mass, self.pos, K, V, self.n, self.budget, K, V, self.mass, self.pos, self.idx,
                                     sinks=self.sinks, recent_from=self.seen - self.recent)

@@ -94,3 +94,14 @@ def test_no_recording_without_room(card, stack):
     f.capture()
     f.step()
     f.step()
+
+
+def test_a_cut_within_the_budget_moves_nothing(card, stack):
+    f = _forks(card, stack, budget=12)
+    f.cut()
+    f.prompt(PROMPT)
+    f.begin([5, 6, 7])
+    before = _held(f)
+    f.cut()
+    assert _same(_held(f), before) and f.n == len(PROMPT)
+    f.step()
