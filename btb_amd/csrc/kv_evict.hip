@@ -453,7 +453,7 @@ static int32_t launch_round(const dim3& grid, const EvictArgs& e, hipStream_t st
                                               hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (rc != hipSuccess) return hip_status(rc, "hipFuncSetAttribute");
     hipLaunchKernelGGL(evict_round_kernel<ROUND>, grid, dim3(EV_THREADS), lds, st, e);
-    return OK;
+    return hip_status(hipGetLastError(), "kv_evict launch");
 }
 
 }  // namespace btb
@@ -496,6 +496,7 @@ extern "C" int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t
     hipStream_t st = static_cast<hipStream_t>(stream);
     e.work = workspace;
     const unsigned heads = (unsigned)(L * Hk);
+    int32_t rc = OK;
     if (n <= (size_t)EV_KEYS) {
         const size_t lds = 4 * (n + n / 2);
         if (lds > 28 * 1024) {
@@ -504,13 +505,21 @@ extern "C" int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t
             if (rc != hipSuccess) return hip_status(rc, "hipFuncSetAttribute");
         }
         hipLaunchKernelGGL(evict_choose_kernel, dim3(heads), dim3(EV_THREADS), lds, st, e);
+        rc = hip_status(hipGetLastError(), "kv_evict launch");
     } else {
         const int blocks = (int)((n + EV_KEYS - 1) / EV_KEYS);
         const dim3 grid((unsigned)blocks, heads), threads(EV_THREADS);
-        const int32_t rc = launch_round<0>(grid, e, st) | launch_round<1>(grid, e, st) | launch_round<2>(grid, e, st) | launch_round<3>(grid, e, st);
-        if (rc != OK) return ERR_PANIC;
-        hipLaunchKernelGGL(evict_order_kernel, grid, threads, 0, st, e);
+        // one statement each: a round reads what the one before it left
+        rc = launch_round<0>(grid, e, st);
+        if (rc == OK) rc = launch_round<1>(grid, e, st);
+        if (rc == OK) rc = launch_round<2>(grid, e, st);
+        if (rc == OK) rc = launch_round<3>(grid, e, st);
+        if (rc == OK) {
+            hipLaunchKernelGGL(evict_order_kernel, grid, threads, 0, st, e);
+            rc = hip_status(hipGetLastError(), "kv_evict launch");
+        }
     }
+    if (rc != OK) return rc;  // (the move goes by what the choice wrote)
     MoveArgs m;
     m.K = static_cast<const uint16_t*>(K);
     m.V = static_cast<const uint16_t*>(V);
