@@ -24,6 +24,7 @@
 namespace btb {
 
 constexpr int MA_KEYS = 256;   // many pairs: keys a workgroup, four waves of two tiles
+constexpr int mass_stage(int D) { return 16384 / D; }  // pairs a stage: eight loads a wave
 constexpr int MA_META = 1024;  // pairs whose log-sums and limits lie in LDS at a time
 // few pairs, at most: two tiles, the most whose log-sums and limits fit a wave's registers. 64 pairs of 8 heads, us, few / many: over 32000 keys
 // 16.4 / 26.3, over 2000 9.0 / 9.6; 72 pairs (many) over 32000: 26.0
@@ -75,7 +76,8 @@ __device__ __forceinline__ void of_pairs(const float* from, int h, float (&v)[16
 template <int D>
 __global__ void __launch_bounds__(256, 2) attn_mass_kernel(MassArgs p) {
     constexpr int STEPS = D / 16, CH = D / 8, KPI = 64 / CH;
-    constexpr int STAGE = 32 * KPI, TILES = STAGE / 32, TILE = TK * 2 * D, AHEAD = 4;  // pairs a stage (eight loads a wave), its tiles
+    constexpr int STAGE = mass_stage(D), TILES = STAGE / 32, TILE = TK * 2 * D, AHEAD = 4;
+    static_assert(STAGE == 32 * KPI, "a wave's eight loads bring a quarter of the stage");
     __shared__ __align__(16) uint8_t q_lds[2][TILES * TILE];
     __shared__ __align__(16) float logs[MA_META];
     __shared__ __align__(16) int limits[MA_META];
@@ -336,14 +338,18 @@ __global__ void __launch_bounds__(256) attn_mass_add_kernel(MassArgs p) {
     p.out[(size_t)g * p.os + key] = v + (p.mass != nullptr ? p.mass[(size_t)g * p.ms + key] : 0.f);
 }
 
-// Workgroups the pairs are cut over: until there are two a CU, each with two stages and more. 8 heads of 128, us, cut / whole: 500 rows over
-// 2000 keys 21.5 / 60, over 512 13.1 / 43; 100 rows over 4000 16.0 / 18.9.
+// Workgroups the pairs are cut over, a stage each or more: until there are two a CU, and from more than 256 pairs on, whose second
+// launch costs less than their stages one after the other. 8 heads of 128, us, cut / whole: 500 rows over 512 keys 13.5 / 43, over 2000
+// 22.3 / 60, over 8000 53 / 54; 96 rows over 4000 15.5 / 15.5, 90 over 700 14.2 / 16; 64 rows (256 pairs) over 4000 14.8 / 12.1. Heads of
+// 64: 500 rows over 512 14.1 with a stage each, 15.2 with two; 70 rows over 4000 14.3 / 15.5.
 static int mass_parts(size_t T, size_t Hq, size_t Hk, size_t D, size_t n) {
-    if (T * (Hq / Hk) <= (size_t)MA_FEW) return 1;
-    const size_t wgs = Hk * ((n + MA_KEYS - 1) / MA_KEYS), stages = (T * (Hq / Hk) * D / 64 + 127) / 128;
-    const size_t want = 2 * (size_t)device_info().cus / wgs, most = stages / 2;
-    const size_t parts = want < most ? want : most;
-    return (int)(parts > 1 ? parts : 1);
+    const size_t pairs = T * (Hq / Hk), stage = (size_t)mass_stage((int)D);
+    if (pairs <= 256) return 1;
+    const size_t wgs = Hk * ((n + MA_KEYS - 1) / MA_KEYS), stages = (pairs + stage - 1) / stage;
+    const size_t want = 2 * (size_t)device_info().cus / wgs, parts = want < stages ? want : stages;
+    if (parts < 2) return 1;
+    const size_t per = (stages + parts - 1) / parts;
+    return (int)((stages + per - 1) / per);  // none without a stage
 }
 static bool mass_sizes_fit(size_t T, size_t Hq, size_t Hk, size_t D, size_t n) {
     return T > 0 && Hk > 0 && Hk <= 1024 && Hq > 0 && Hq % Hk == 0 && Hq / Hk <= 32 && T <= (1u << 23) / Hq && (D == 64 || D == 128) &&
