@@ -1160,6 +1160,8 @@ class HipCard(CardLaunch):
             if not (isinstance(t, _Tensor) and t.dtype is torch.float32 and t.is_cuda and t.dim() == 2 and t.shape[0] == Hk
                     and t.shape[1] >= n and t.stride(1) == 1):
                 raise ValueError(f"[hip] attn_mass: mass and out are float32 [{Hk}, >= {n}] on the GPU, a head's values together")
+        if Hk > 1 and out.stride(0) < n:
+            raise ValueError("[hip] attn_mass: out's heads share memory")
         floats = self.lib.btb_hip_attn_mass_floats(T, Hq, Hk, D, n)
         ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
         self._call("btb_hip_attn_mass", q.data_ptr(), K.data_ptr(), lse.data_ptr(), seen.data_ptr(),
@@ -1201,6 +1203,8 @@ class HipCard(CardLaunch):
 
         ms, ps = head_stride(mass, torch.float32, n, "mass"), head_stride(pos, torch.int32, n, "pos")
         mo, po = head_stride(mass_out, torch.float32, kept, "mass_out"), head_stride(pos_out, torch.int32, kept, "pos_out")
+        if L * Hk > 1 and (mo < kept or po < kept):
+            raise ValueError("[hip] kv_evict: heads of mass_out or pos_out share memory")
         if not self._plain(idx, torch.int32) or idx.numel() != L * Hk * kept:
             raise ValueError(f"[hip] kv_evict: idx is a contiguous int32 tensor on the GPU of the {L * Hk * kept} slots that stay")
         words = self.lib.btb_hip_kv_evict_words(L, Hk, n)

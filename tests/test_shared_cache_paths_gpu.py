@@ -274,3 +274,34 @@ def test_evict_outputs_stay_inside(card, L, Hk, D, n, budget):
     for o in inside:
         o.check("kv_evict in place")
     assert torch.equal(idx, outs[4].t) and torch.equal(k[:, :, :budget], outs[0].t) and torch.equal(m[..., :budget], outs[2].t)
+
+
+# ---- refusals ---------------------------------------------------------------------------------------------------------
+
+
+def test_outputs_whose_heads_share_memory(card):
+    """one mass for all heads may be read, and not written: their workgroups would race for it"""
+    T, Hq, Hk, D, n = 2, 8, 4, 64, 40
+    g = gen(5990)
+    q, K = (torch.randn(*s, generator=g).to(torch.bfloat16).cuda() for s in ((T, Hq * D), (Hk, n, D)))
+    lse, seen = torch.full((T, Hq), 3.0, device="cuda"), torch.full((T,), n, dtype=torch.int32, device="cuda")
+    one = torch.rand(1, n, generator=g).cuda().expand(Hk, n)
+    call = lambda mass, out: card.attn_mass(q, K, lse, seen, mass, Hq, Hk, D, 0.1, n, out=out)
+    assert torch.equal(call(one, torch.empty(Hk, n, device="cuda")), call(one.contiguous(), None))
+    half = torch.zeros(Hk * n, device="cuda").as_strided((Hk, n), (n // 2, 1))
+    for mass, out in ((one, None), (None, one), (None, half)):
+        with pytest.raises(ValueError):
+            call(mass, out)
+    pos, i32 = torch.arange(n, dtype=torch.int32, device="cuda"), torch.int32
+    kept = 8
+    outs = lambda **k: [k.get(a, v) for a, v in dict(
+        K=torch.empty(Hk, kept, D, dtype=torch.bfloat16, device="cuda"), V=torch.empty(Hk, kept, D, dtype=torch.bfloat16, device="cuda"),
+        mass=torch.empty(Hk, kept, device="cuda"), pos=torch.empty(Hk, kept, dtype=i32, device="cuda"),
+        idx=torch.empty(Hk, kept, dtype=i32, device="cuda")).items()]
+    assert card.kv_evict(one, pos.expand(Hk, n), K, K, n, kept, *outs()) == kept
+    for bad in (dict(mass=torch.empty(1, kept, device="cuda").expand(Hk, kept)), dict(pos=torch.empty(1, kept, dtype=i32, device="cuda").expand(Hk, kept))):
+        with pytest.raises(ValueError):
+            card.kv_evict(one, pos.expand(Hk, n), K, K, n, kept, *outs(**bad))
+    # one head has no other to share with
+    assert card.kv_evict(one[:1], pos[None], K[:1], K[:1], n, kept, *(t[:1].contiguous() for t in outs())) == kept
+    torch.cuda.synchronize()
