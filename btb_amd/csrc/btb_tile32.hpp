@@ -154,16 +154,15 @@ __device__ __forceinline__ void wait_loads(uint32_t& at) {
     asm volatile("s_waitcnt vmcnt(%1)" : "+v"(at) : "n"(N) : "memory");
 }
 
-// A weight (0 or more) as two bf16 terms: its upper half, and the upper half of what that leaves; 2^-15 of it at most stays out.
-// Neither term has another sign than the weight, nor is the second zero where the weight is 2^-100 and more (its lowest bit is
+// A weight (0 or more) as two bf16 terms: its upper half, and what that leaves, rounded; 2^-16 of it at most stays out, up as often as
+// down. Neither term has another sign than the weight, nor is the second zero where the weight is 2^-100 and more (its lowest bit is
 // set, 2^-23 of it), so that an infinite value stays infinite in both products. Two weights at a time.
 __device__ __forceinline__ uint32_t first_terms(float a, float b) {
     return __builtin_amdgcn_perm(f32_bits(b), f32_bits(a), 0x07060302u);
 }
 __device__ __forceinline__ uint32_t second_terms(float a, float b) {
-    const float ra = bits_f32(f32_bits(a) | 1u) - bits_f32(f32_bits(a) & 0xFFFF0000u);
-    const float rb = bits_f32(f32_bits(b) | 1u) - bits_f32(f32_bits(b) & 0xFFFF0000u);
-    return first_terms(ra, rb);
+    return f32x2_bf16(bits_f32(f32_bits(a) | 1u) - bits_f32(f32_bits(a) & 0xFFFF0000u),
+                      bits_f32(f32_bits(b) | 1u) - bits_f32(f32_bits(b) & 0xFFFF0000u));
 }
 
 __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
