@@ -10,8 +10,9 @@
 //     workgroup's four waves bring them a stage ahead. A tile's weights are made between the next tile's products. Where keys are
 //     few, the pairs are cut over workgroups too, whose sums a second launch adds in order. Bound: the products and the exponentials, a
 //     multiply-add, a quarter-rate exponential and an addition a score beside a thirty-second of a product of 32 clocks a lane. 500 rows of
-//     32 heads x 128 over 16384 keys 87 us (760 TFLOP/s), of which 13 bring the keys into registers; 4096 rows 544 us (1010 TFLOP/s), 507
-//     without the stages' loads and 398 (1384 TFLOP/s, the chip's rate for bare products) with no exponential either.
+//     32 heads x 128 over 16384 keys 82 to 92 us by the chip (720 to 815 TFLOP/s), of which 13 bring the keys into registers; 4096 rows 544
+//     to 566 us (970 to 1010 TFLOP/s), of 544 507 without the stages' loads and 398 (1384 TFLOP/s, the chip's rate for bare products) with no
+//     exponential either.
 //   few pairs (64 and less): they lie in LDS and the keys go by, a tile of 32 a wave ahead of the one at work. Bound: K's
 //     trip from memory. 4 rows of 32 heads x 128 over 32000 keys 14.0 us (4.8 TB/s).
 

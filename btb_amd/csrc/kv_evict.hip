@@ -8,7 +8,8 @@
 // ten bits at a time from the top (histograms in LDS), counts what stays and then writes the order. A wave takes a stretch of
 // the slots below `kept` and one of those above, so its own running count is all that its keys' order needs, and the waves
 // meet in one scan. A workgroup takes a head of up to 8192 keys alone, ranks in LDS, one launch; a longer one is cut over
-// workgroups of 8192 keys and the rounds are launches (six), since what a key costs is arithmetic.
+// workgroups of 8192 keys and the rounds are launches (six), since what a key costs is arithmetic. The second round reads every
+// workgroup's histogram in every workgroup, 4 KB times the square of their number a head: 1 MB at 131072 keys, 4 GB at 2^23.
 //
 // us, a workgroup a head / the rounds: 8192 keys to 4096 x 8 heads 18.9 / 30.7, x 32 39.4 / 51.6, x 288 260 / 274; the choice alone of
 // 131072 keys x 32 358 / 49. Bound: memory, mass and pos read, the moved rows read and written: 4608 keys to 4096 x 288 heads 245 us
@@ -500,9 +501,9 @@ extern "C" int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t
     if (n <= (size_t)EV_KEYS) {
         const size_t lds = 4 * (n + n / 2);
         if (lds > 28 * 1024) {
-            const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(evict_choose_kernel),
-                                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-            if (rc != hipSuccess) return hip_status(rc, "hipFuncSetAttribute");
+            const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(evict_choose_kernel),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (set != hipSuccess) return hip_status(set, "hipFuncSetAttribute");
         }
         hipLaunchKernelGGL(evict_choose_kernel, dim3(heads), dim3(EV_THREADS), lds, st, e);
         rc = hip_status(hipGetLastError(), "kv_evict launch");

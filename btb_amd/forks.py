@@ -3,9 +3,9 @@ least are dropped whenever the cache holds more than its budget, and rows of the
 pass reads once for all of them.
 
 `Forks` runs a dense stack (`DecodeStep`'s weights) through `HipCard.norm_rope_axes`, `attn_shared`, `attn_mass` and `kv_evict`. A
-layer's cache is one arena [Hk, slots, D]: the prompt's keys first, then a stretch of `steps` slots a row. After a cut a key's slot
-is no longer its position and differs from head to head, so positions travel beside the cache (`pos`) and new keys are roped at
-their own places. No counterpart in the reference.
+layer's cache is one arena [Hk, slots, D]: the prompt's keys first, then a stretch of `steps` slots a row, which are neither weighed
+nor cut: the budget is the prompt's. After a cut a key's slot is no longer its token's number and differs from head to head, so the
+numbers travel beside the cache (`pos`) and new keys are roped at their own places. No counterpart in the reference.
 """
 
 from __future__ import annotations

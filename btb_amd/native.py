@@ -1175,7 +1175,8 @@ class HipCard(CardLaunch):
         """the cache K, V [L, Hk, cap, D] (or one layer's [Hk, cap, D]), n keys a head, cut to its min(n, budget) heaviest by
         mass (float32 [L, Hk, cap]); keys of position (pos, int32 [L, Hk, cap]) below `sinks` or from `recent_from` on come
         first. What stays below the new length stays in its slot, the rest fills the slots in between; idx (int32 [L, Hk,
-        kept]): the slot each came from. The outputs may be the inputs. Returns how many keys a head holds now."""
+        kept]): the slot each came from. The outputs may be the inputs, all four, and overlap them in no other way. Returns how
+        many keys a head holds now."""
         bf = torch.bfloat16
         for t in (K, V, K_out, V_out):
             if not (isinstance(t, _Tensor) and t.dtype is bf and t.is_cuda and 3 <= t.dim() <= 4):

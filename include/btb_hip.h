@@ -470,7 +470,8 @@ int32_t btb_hip_attn_decode_qkv_span(const void* qkv, const void* wq, const void
  * axis that turns each frequency (an axis past A - 1 is A - 1); slots: i32 [T], distinct, the cache rows that the new k and
  * v go to - a slot outside 0 .. cap - 1 is not written. cos_t / sin_t: [positions] rows `table_stride` values apart,
  * of which the first D / 2 are read; bf16, or f32 where table_f32 is 1. q [T, Hq D]. K, V: one layer's, `cap` rows a head, strides hs
- * and rs in values. D 64, 128 or 256; qkv, q, K and V 16-byte aligned, hs and rs multiples of 8. */
+ * and rs in values. T up to 2^24, A up to 255, D 64, 128 or 256; qkv, q, K and V 16-byte aligned,
+ * hs and rs multiples of 8. */
 int32_t btb_hip_norm_rope_axes(const void* qkv, const void* wq, const void* wk, float eps, const void* cos_t,
                                const void* sin_t, int32_t table_f32, size_t positions, size_t table_stride,
                                const int32_t* pos, size_t A, const uint8_t* axes, const int32_t* slots, void* K, void* V,
@@ -483,8 +484,9 @@ int32_t btb_hip_norm_rope_axes(const void* qkv, const void* wq, const void* wk, 
  * chain name growing stretches of the same slots). A row of own length < 0 is padding, left as it was; a row with no
  * key at all gets zeros and -inf. prefix_cap and own_cap bound the lengths (a longer stretch is cut there, and at the
  * cache's `cap` rows): they size the launch and the workspace (btb_hip_attn_shared_floats, this call's own), the lengths
- * are read on the device. The prefix's keys are read once for all the rows. D 64 or 128, Hq / Hk up to 32, scale > 0; q,
- * K, V, att and workspace 16-byte aligned, hs and rs multiples of 8. */
+ * are read on the device. The prefix's keys are read once for all the rows, a row's own once for that row, also where rows
+ * name the same. Sums are f32, a weight goes to the product with V as two bf16 terms. T up to 65536, T Hq up to 2^24, D 64 or 128, Hq / Hk up
+ * to 32, scale > 0; q, K, V, att and workspace 16-byte aligned, hs and rs multiples of 8, rs up to 2^25. */
 size_t btb_hip_attn_shared_floats(size_t T, size_t Hq, size_t Hk, size_t D, size_t prefix_cap, size_t own_cap);
 int32_t btb_hip_attn_shared(const void* q, const void* K, const void* V, void* att, float* lse, const int32_t* layout,
                             size_t T, size_t Hq, size_t Hk, size_t D, size_t cap, int64_t hs, int64_t rs, float scale,
@@ -495,7 +497,7 @@ int32_t btb_hip_attn_shared(const void* q, const void* K, const void* V, void* a
  * with lse [T, Hq] as btb_hip_attn_shared leaves it, its rows lse_row and its heads lse_head values apart (a row whose lse is
  * -inf adds nothing). seen: i32 [T]. mass and out: f32 rows mass_stride / out_stride apart; mass NULL: zeros; out may be mass. workspace: btb_hip_attn_mass_floats of
  * them, this call's own (0: NULL will do). The additions' order is fixed. D 64 or 128, Hq / Hk up to 32, T Hq at most 2^23, scale > 0;
- * q and K 16-byte aligned, hs and rs multiples of 8. */
+ * q and K 16-byte aligned, hs and rs multiples of 8, rs up to 2^25; out's heads must not share memory. */
 size_t btb_hip_attn_mass_floats(size_t T, size_t Hq, size_t Hk, size_t D, size_t n);
 int32_t btb_hip_attn_mass(const void* q, const void* K, const float* lse, const int32_t* seen, const float* mass, float* out,
                           size_t T, size_t Hq, size_t Hk, size_t D, size_t n, int64_t hs, int64_t rs, int64_t mass_stride,
@@ -507,7 +509,8 @@ int32_t btb_hip_attn_mass(const void* q, const void* K, const float* lse, const 
  * and pos of slot idx[j] go to slot j of the outputs; idx: i32 [L Hk][kept], dense. Strides: ls / hs / rs (lo / ho / ro) of
  * a layer, head and row of K and V, ms / ps (mo / po) of a head of mass and pos. The outputs may be the inputs, all four
  * with the same strides (only what moves is then written), or must not overlap them. workspace: btb_hip_kv_evict_words(L, Hk,
- * n) words, 16-byte aligned, this call's own (0: NULL will do). n at most 2^23, D 64, 128 or 256; K and V 16-byte aligned, their strides multiples of 8. */
+ * n) words, 16-byte aligned, this call's own (0: NULL will do). n at most 2^23, L Hk at most 65535, D 64, 128 or 256; K
+ * and V 16-byte aligned, their strides multiples of 8; heads of the outputs must not share memory. */
 size_t btb_hip_kv_evict_words(size_t L, size_t Hk, size_t n);
 int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t* pos, int64_t ps, const void* K, const void* V,
                          int64_t ls, int64_t hs, int64_t rs, size_t L, size_t Hk, size_t D, size_t n, size_t budget,
