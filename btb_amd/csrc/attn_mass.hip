@@ -389,10 +389,10 @@ int32_t btb_hip_attn_mass(const void* q, const void* K, const float* lse, const 
                           int64_t out_stride, int64_t lse_row, int64_t lse_head, float scale, float* workspace, void* stream) {
     if (!q || !K || !lse || !seen || !out) return ERR_NULL;
     auto loose = [](const void* a) { return ((uintptr_t)a & 15u) != 0; };
-    if (!mass_sizes_fit(T, Hq, Hk, D, n) || hs < 0 || rs < 0 || rs > (1 << 25) || hs % 8 || rs % 8 || mass_stride < 0 || out_stride < 0 || lse_row < 0 || lse_head < 0 ||
+    if (!mass_sizes_fit(T, Hq, Hk, D, n) || hs < 0 || rs < 0 || rs > (1 << 25) || hs % 8 || rs % 8 || mass_stride < 0 || out_stride < 0 || (Hk > 1 && (size_t)out_stride < n) || lse_row < 0 || lse_head < 0 ||
         !(scale > 0.f) || !(scale < __builtin_inff()) || loose(q) || loose(K)) {
         set_error("attn_mass: head_dim 64 or 128, up to 32 query heads a kv head, a positive scale, q and K 16-byte aligned "
-                  "with strides in multiples of 8, a row's up to 2^25");
+                  "with strides in multiples of 8, a row's up to 2^25, out's heads apart");
         return ERR_DOMAIN;
     }
     const int parts = mass_parts(T, Hq, Hk, D, n);

@@ -475,13 +475,17 @@ extern "C" int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t
     auto loose = [](const void* a) { return ((uintptr_t)a & 15u) != 0; };
     auto odd = [](int64_t s) { return s < 0 || s % 8 != 0; };
     const bool in_place = K == K_out;
+    const size_t kept = budget < n ? budget : n;
+    // rows, or a head's numbers, that several workgroups would write
+    const bool shared = (lo == 0 && L > 1) || (ho == 0 && Hk > 1) || (ro == 0 && kept > 1) ||
+                        (L * Hk > 1 && ((size_t)mo < kept || (size_t)po < kept));
     if (L == 0 || Hk == 0 || L > 65535 || Hk > 65535 || L * Hk > 65535 || (D != 64 && D != 128 && D != 256) || n == 0 ||
-        n > (size_t)EV_KEYS * EV_BLOCKS || budget == 0 || ms < 0 || ps < 0 || mo < 0 || po < 0 || odd(ls) || odd(hs) || odd(rs) || odd(lo) ||
+        n > (size_t)EV_KEYS * EV_BLOCKS || budget == 0 || shared || ms < 0 || ps < 0 || mo < 0 || po < 0 || odd(ls) || odd(hs) || odd(rs) || odd(lo) ||
         odd(ho) || odd(ro) || loose(K) || loose(V) || loose(K_out) || loose(V_out) || loose(workspace) || in_place != (V == V_out) ||
         in_place != (mass == mass_out) || in_place != (pos == pos_out) ||
         (in_place && (ls != lo || hs != ho || rs != ro || ms != mo || ps != po))) {
         set_error("kv_evict: at most 65535 heads in all of at most 2^23 keys, head_dim 64, 128 or 256, K and V 16-byte aligned with strides in "
-                  "multiples of 8; in place: all four outputs the inputs with their strides, or none");
+                  "multiples of 8, no two outputs in one place; in place: all four outputs the inputs with their strides, or none");
         return ERR_DOMAIN;
     }
     EvictArgs e;
@@ -491,7 +495,7 @@ extern "C" int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t
     e.ms = ms;
     e.ps = ps;
     e.n = (int)n;
-    e.kept = (int)(budget < n ? budget : n);
+    e.kept = (int)kept;
     e.sinks = sinks;
     e.recent_from = recent_from;
     hipStream_t st = static_cast<hipStream_t>(stream);

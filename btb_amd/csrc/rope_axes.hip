@@ -220,10 +220,10 @@ extern "C" int32_t btb_hip_norm_rope_axes(const void* qkv, const void* wq, const
     if (!qkv || !cos_t || !sin_t || !pos || !axes || !slots || !K || !V || !q) return ERR_NULL;
     if (T == 0 || T > (1u << 24) || Hq == 0 || Hk == 0 || Hq + 2 * Hk > 65535 || (D != 64 && D != 128 && D != 256) || A == 0 ||
         A > 255 || positions == 0 || positions > 0x7FFFFFFFu || cap == 0 || cap > 0x7FFFFFFFu || table_stride < D / 2 ||
-        table_stride > 0x7FFFFFFFu || hs < 0 || rs < 0 || hs % 8 || rs % 8 || !aligned16(qkv) || !aligned16(q) ||
+        table_stride > 0x7FFFFFFFu || hs < 0 || rs < 0 || (hs == 0 && Hk > 1) || (rs == 0 && cap > 1) || hs % 8 || rs % 8 || !aligned16(qkv) || !aligned16(q) ||
         !aligned16(K) || !aligned16(V)) {
         set_error("norm_rope_axes: 1 .. 2^24 rows, head_dim 64, 128 or 256, 1 .. 255 axes, tables at least D / 2 wide, qkv, q, "
-                  "K and V 16-byte aligned with strides in multiples of 8");
+                  "K and V 16-byte aligned with strides in multiples of 8, no two rows of K in one place");
         return ERR_DOMAIN;
     }
     RopeAxes p;

@@ -471,7 +471,7 @@ int32_t btb_hip_attn_decode_qkv_span(const void* qkv, const void* wq, const void
  * v go to - a slot outside 0 .. cap - 1 is not written. cos_t / sin_t: [positions] rows `table_stride` values apart,
  * of which the first D / 2 are read; bf16, or f32 where table_f32 is 1. q [T, Hq D]. K, V: one layer's, `cap` rows a head, strides hs
  * and rs in values. T up to 2^24, A up to 255, D 64, 128 or 256; qkv, q, K and V 16-byte aligned,
- * hs and rs multiples of 8. */
+ * hs and rs multiples of 8 and, of several heads and rows, not 0. */
 int32_t btb_hip_norm_rope_axes(const void* qkv, const void* wq, const void* wk, float eps, const void* cos_t,
                                const void* sin_t, int32_t table_f32, size_t positions, size_t table_stride,
                                const int32_t* pos, size_t A, const uint8_t* axes, const int32_t* slots, void* K, void* V,
@@ -510,7 +510,7 @@ int32_t btb_hip_attn_mass(const void* q, const void* K, const float* lse, const 
  * a layer, head and row of K and V, ms / ps (mo / po) of a head of mass and pos. The outputs may be the inputs, all four
  * with the same strides (only what moves is then written), or must not overlap them. workspace: btb_hip_kv_evict_words(L, Hk,
  * n) words, 16-byte aligned, this call's own (0: NULL will do). n at most 2^23, L Hk at most 65535, D 64, 128 or 256; K
- * and V 16-byte aligned, their strides multiples of 8; heads of the outputs must not share memory. */
+ * and V 16-byte aligned, their strides multiples of 8; rows and heads of the outputs must not share memory. */
 size_t btb_hip_kv_evict_words(size_t L, size_t Hk, size_t n);
 int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t* pos, int64_t ps, const void* K, const void* V,
                          int64_t ls, int64_t hs, int64_t rs, size_t L, size_t Hk, size_t D, size_t n, size_t budget,

@@ -15,6 +15,7 @@ import pytest
 import torch
 
 from btb_amd.decode import StackConfig, rope_axes, rope_tables
+from btb_amd.native import HipError
 from oracle import shared
 
 from . import test_shared_cache_gpu as base
@@ -304,4 +305,31 @@ def test_outputs_whose_heads_share_memory(card):
             card.kv_evict(one, pos.expand(Hk, n), K, K, n, kept, *outs(**bad))
     # one head has no other to share with
     assert card.kv_evict(one[:1], pos[None], K[:1], K[:1], n, kept, *(t[:1].contiguous() for t in outs())) == kept
+    torch.cuda.synchronize()
+
+
+def test_caches_whose_rows_share_memory_are_not_written(card):
+    """an expanded cache may be read; written, its heads or slots would race for one place"""
+    T, Hq, Hk, D, cap, kept = 2, 4, 2, 64, 16, 8
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt, device="cuda")
+    i32 = torch.int32
+    cos, axes = z(8, D), z(D // 2, dt=torch.uint8)
+    heads, slots = z(1, cap, D).expand(Hk, cap, D), z(Hk, 1, D).expand(Hk, cap, D)
+    rope = lambda K, V, hq, hk: card.norm_rope_axes(z(T, (hq + 2 * hk) * D), None, None, 1e-6, cos, cos, z(1, T, dt=i32), axes,
+                                                 torch.arange(T, dtype=i32, device="cuda"), K, V, z(T, hq * D), hq, hk, D)
+    rope(z(Hk, cap, D), z(Hk, cap, D), Hq, Hk)
+    rope(heads[:1], z(1, cap, D).expand(Hk, cap, D)[:1], Hq, 1)  # one head: no other to share with
+    for K in (heads, slots):
+        with pytest.raises(HipError):
+            rope(K, K, Hq, Hk)
+    K, mass, pos = z(2, Hk, cap, D), z(2, Hk, cap, dt=torch.float32), z(2, Hk, cap, dt=i32)
+    evict = lambda K_out, V_out: card.kv_evict(mass, pos, K, K, cap, kept, K_out, V_out, z(2, Hk, kept, dt=torch.float32), z(2, Hk, kept, dt=i32),
+                                        z(2, Hk, kept, dt=i32))
+    for bad in (z(1, Hk, kept, D).expand(2, Hk, kept, D), z(2, 1, kept, D).expand(2, Hk, kept, D), z(2, Hk, 1, D).expand(2, Hk, kept, D)):
+        with pytest.raises(HipError):
+            evict(bad, bad)
+    assert evict(z(2, Hk, kept, D), z(2, Hk, kept, D)) == kept
+    lib, p = card.lib, lambda t: t.data_ptr()
+    q, f = z(T, Hq * D), z(64, dt=torch.float32)
+    assert lib.btb_hip_attn_mass(p(q), p(K), p(f), p(pos), None, p(f), T, Hq, Hk, D, 8, cap * D, D, 0, 7, Hq, 1, 0.1, None, None) == -6
     torch.cuda.synchronize()
