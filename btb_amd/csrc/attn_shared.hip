@@ -15,7 +15,7 @@
 // the outputs alone makes. us, one / two: 16 rows of 32 heads x 128 over 131072 keys, 100 own 104 / 105; 256 rows over 32768 160 / 211,
 // and 640 own 239 / 284; 256 rows of 40 heads x 64 over 32768 141 / 196; 41 rows over 6001, 485 own 19.5 / 21.3.
 //
-// Bound: memory where few rows share the prefix (16 rows of 32 heads x 128 over 131072 keys, 100 own: 105 to 112 us, 4.8 to 5.2 TB/s), the products
+// Bound: memory where few rows share the prefix (16 rows of 32 heads x 128 over 131072 keys, 100 own: 105 to 115 us, 4.7 to 5.2 TB/s), the products
 // where many do (256 rows over 32768: 211 us, the fold included; three products for every two of the formula, 975 TFLOP/s of bare
 // products' 1384), and both at once where many rows have many own keys (640 each: 284 us, 2.8 TB/s and 495 TFLOP/s).
 
