@@ -46,6 +46,7 @@ HIPCC_FLAGS = [
 FILE_FLAGS = {
     "attn_shared.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "attn_mass.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "attn_kv4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

@@ -119,6 +119,14 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "btb_hip_kv_evict": (_i32, [_vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp] + [ctypes.c_int64] * 3 + [_sz] * 5 +
                          [_i32, _i32, _vp, _vp] + [ctypes.c_int64] * 3 + [_vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp, _vp]),
     "btb_hip_kv_evict_words": (_sz, [_sz, _sz, _sz]),
+    "btb_hip_kv4_tile_bytes": (_sz, [_sz]),
+    "btb_hip_kv4_write": (_i32, [_vp] * 6 + [_sz] * 4 + [ctypes.c_int64] + [_sz] * 3 + [ctypes.c_int64] * 4 + [_vp]),
+    "btb_hip_kv4_read": (_i32, [_vp] * 4 + [_sz] * 4 + [ctypes.c_int64] + [_sz] * 3 + [_vp, _vp, _i32] + [ctypes.c_int64] * 4 + [_vp]),
+    "btb_hip_attn_kv4_floats": (_sz, [_sz] * 6),
+    "btb_hip_attn_kv4": (_i32, [_vp] * 7 + [_sz] * 4 + [ctypes.c_int64] + [_sz] * 4 + [ctypes.c_float, _sz, _vp, _vp]),
+    "btb_hip_pages_fork": (_i32, [_vp] + [_sz] * 3 + [ctypes.c_int64] * 2 + [_vp, _vp] + [_sz] * 3 + [_vp] * 3 + [_sz, _vp]),
+    "btb_hip_pages_compact_words": (_sz, [_sz]),
+    "btb_hip_pages_compact": (_i32, [_vp] + [_sz] * 3 + [ctypes.c_int64] * 2 + [_vp, _vp] + [_sz] * 3 + [_vp] * 4),
     "btb_hip_silu_mul": (_i32, [_vp, _vp, _sz, _sz, _vp]),
     "btb_hip_argmax": (_i32, [_vp, _vp, _sz, _sz, _vp]),
     "btb_hip_publish": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
@@ -1215,6 +1223,137 @@ class HipCard(CardLaunch):
                    out_strides[-2], mass_out.data_ptr(), mo, pos_out.data_ptr(), po, idx.data_ptr(),
                    None if ws is None else ws.data_ptr(), _stream())
         return kept
+
+    # -- a paged cache held in 4 bits -----------------------------------------------------------------------------------
+
+    def kv4_pool(self, pages: int, Hk: int, D: int, page: int = 64, layers: int | None = None, device: Any = "cuda") -> torch.Tensor:
+        """an empty pool for `kv4_write`: uint8 [pages, Hk, page / 32, tile bytes], with `layers` of them in front where given"""
+        tile = int(self.lib.btb_hip_kv4_tile_bytes(D))
+        if tile == 0 or page < 32 or page % 32 or pages < 1 or Hk < 1:
+            raise ValueError(f"[hip] kv4_pool: head_dim 64 or 128, pages of a multiple of 32 tokens, got {D} and {page}")
+        shape = (pages, Hk, page // 32, tile)
+        return torch.zeros(shape if layers is None else (layers, *shape), dtype=torch.uint8, device=device)
+
+    def _kv4_seqs(self, what: str, cache: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, first: torch.Tensor | None, T: int,
+                  Hk: int, D: int) -> tuple[int, int, int, int, int]:
+        """a layer's pool, the tables and the lengths of a call: sequences, entries each, pages, tokens a page, bytes between pages"""
+        i32 = torch.int32
+        if not (self._plain(tables, i32) and tables.dim() == 2 and self._plain(lens, i32) and lens.numel() == tables.shape[0]
+                and (first is None or (self._plain(first, i32) and first.numel() == tables.shape[0] + 1))):
+            raise ValueError(f"[hip] {what}: tables int32 [sequences, entries], lens [sequences] and first [sequences + 1] or None, "
+                             "contiguous on the GPU")
+        if not (isinstance(cache, _Tensor) and cache.dtype is torch.uint8 and cache.is_cuda and cache.dim() == 4
+                and cache.shape[1] == Hk and cache.shape[3] == self.lib.btb_hip_kv4_tile_bytes(D) and cache[0].is_contiguous()):
+            raise ValueError(f"[hip] {what}: the cache is one layer's pool, uint8 [pages, {Hk}, page / 32, tile bytes] (kv4_pool), whole "
+                             "pages contiguous")
+        B, W = tables.shape
+        if T < 1 or (first is None and T % B):
+            raise ValueError(f"[hip] {what}: {T} rows are not as many for each of {B} sequences: say which with first")
+        pages = cache.shape[0]
+        return B, W, pages, 32 * cache.shape[2], cache.stride(0) if pages > 1 else cache[0].numel()
+
+    @staticmethod
+    def _kv4_rows(what: str, k: torch.Tensor, v: torch.Tensor, dtypes: tuple[torch.dtype, ...]) -> tuple[int, int, int]:
+        for t in (k, v):
+            if not (isinstance(t, _Tensor) and t.dtype is k.dtype and t.dtype in dtypes and t.is_cuda and t.dim() == 3
+                    and t.shape == k.shape and t.stride(2) == 1):
+                raise ValueError(f"[hip] {what}: k and v are [rows, kv heads, head_dim] views of one type on the GPU, {dtypes}, head_dim "
+                                 "contiguous")
+        return k.shape[0], k.shape[1], k.shape[2]
+
+    def kv4_write(self, k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor,
+                  first: torch.Tensor | None = None) -> None:
+        """the pass's rows k, v (bfloat16 [T, Hk, D] views) into a layer's pool (`kv4_pool`) in 4 bits: rows first[b] .. first[b + 1] - 1
+        (None: T / B each) are the last ones of sequence b, which has lens[b] tokens with them in pages tables[b]. A row whose page is
+        not the pool's is not written; two sequences write to no common page."""
+        T, Hk, D = self._kv4_rows("kv4_write", k, v, (torch.bfloat16,))
+        B, W, pages, page, stride = self._kv4_seqs("kv4_write", cache, tables, lens, first, T, Hk, D)
+        self._call("btb_hip_kv4_write", k.data_ptr(), v.data_ptr(), cache.data_ptr(), tables.data_ptr(), lens.data_ptr(),
+                   None if first is None else first.data_ptr(), B, W, pages, page, stride, T, Hk, D, k.stride(0), k.stride(1),
+                   v.stride(0), v.stride(1), _stream())
+
+    def kv4_read(self, cache: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                 first: torch.Tensor | None = None) -> None:
+        """the pass's rows as the cache holds them, into k and v [T, Hk, D] (views; float32, exact, or bfloat16): `kv4_write`'s
+        other way round. Zeros where the page is not the pool's."""
+        T, Hk, D = self._kv4_rows("kv4_read", k, v, (torch.float32, torch.bfloat16))
+        B, W, pages, page, stride = self._kv4_seqs("kv4_read", cache, tables, lens, first, T, Hk, D)
+        for t in (k, v):
+            if (t.stride(0) == 0 and T > 1) or (t.stride(1) == 0 and Hk > 1):
+                raise ValueError("[hip] kv4_read: rows or heads of k or v share memory")
+        self._call("btb_hip_kv4_read", cache.data_ptr(), tables.data_ptr(), lens.data_ptr(),
+                   None if first is None else first.data_ptr(), B, W, pages, page, stride, T, Hk, D, k.data_ptr(), v.data_ptr(),
+                   k.dtype is torch.float32, k.stride(0), k.stride(1), v.stride(0), v.stride(1), _stream())
+
+    def attn_kv4_scratch(self, T: int, B: int, Hq: int, Hk: int, D: int, keys_cap: int, device: Any = "cuda") -> torch.Tensor:
+        """the f32 scratch `attn_kv4` leaves its states in, at these sizes"""
+        n = int(self.lib.btb_hip_attn_kv4_floats(T, B, Hq, Hk, D, keys_cap))
+        if n == 0:
+            raise ValueError("[hip] attn_kv4 takes head_dim 64 or 128, 1 .. 64 query heads a kv head and keys_cap 1 .. 2^30")
+        return torch.empty(n, dtype=torch.float32, device=device)
+
+    def attn_kv4(self, q: torch.Tensor, cache: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, att: torch.Tensor, Hq: int, Hk: int,
+                 D: int, scale: float, scratch: torch.Tensor, first: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                 keys_cap: int = 0) -> None:
+        """att [T, Hq D] = attention of the pass's rows q [T, Hq D], which are their sequences' last ones as in `kv4_write`, each over
+        its sequence's tokens up to itself, out of a layer's pool in 4 bits; lse (float32 [T, Hq]): the rows' log-sum-exp.
+        keys_cap: about how long the longest sequence is (0: as long as the tables allow); it goes into the launch's
+        shape and the scratch's size only."""
+        if not (self._plain(q, torch.bfloat16) and self._plain(att, torch.bfloat16) and self._plain(scratch, torch.float32)
+                and (lse is None or self._plain(lse, torch.float32))):
+            raise ValueError("[hip] attn_kv4: q and att are bfloat16, scratch and lse float32, all contiguous on the GPU")
+        T = q.numel() // (Hq * D)
+        if q.numel() != T * Hq * D or att.numel() != q.numel() or (lse is not None and lse.numel() != T * Hq):
+            raise ValueError("[hip] attn_kv4: q and att are [T, Hq D], lse [T, Hq]")
+        B, W, pages, page, stride = self._kv4_seqs("attn_kv4", cache, tables, lens, first, T, Hk, D)
+        keys = keys_cap if keys_cap > 0 else W * page
+        need = self.lib.btb_hip_attn_kv4_floats(T, B, Hq, Hk, D, keys)
+        if scratch.numel() < need:
+            raise ValueError(f"[hip] attn_kv4: scratch holds {scratch.numel()} floats, {need} are needed")
+        self._call("btb_hip_attn_kv4", q.data_ptr(), cache.data_ptr(), tables.data_ptr(), lens.data_ptr(),
+                   None if first is None else first.data_ptr(), att.data_ptr(), None if lse is None else lse.data_ptr(), B, W, pages, page,
+                   stride, T, Hq, Hk, D, scale, keys, scratch.data_ptr(), _stream())
+
+    def _pages_of(self, what: str, pool: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor) -> tuple[int, ...]:
+        """the pool's address, layers, pages, bytes a page and the strides of both, in bytes; sequences and entries"""
+        if not (isinstance(pool, _Tensor) and pool.is_cuda and pool.dim() >= 3 and pool[0, 0].is_contiguous()):
+            raise ValueError(f"[hip] {what}: the pool is [layers, pages, ...] on the GPU, a page's values together")
+        if not (self._plain(tables, torch.int32) and tables.dim() == 2 and self._plain(lens, torch.int32)
+                and lens.numel() == tables.shape[0]):
+            raise ValueError(f"[hip] {what}: tables int32 [sequences, entries] and lens int32 [sequences], contiguous on the GPU")
+        L, pages, size = pool.shape[0], pool.shape[1], pool.element_size()
+        nb = pool[0, 0].numel() * size
+        stride = pool.stride(1) * size if pages > 1 else nb
+        return (pool.data_ptr(), L, pages, nb, pool.stride(0) * size if L > 1 else 0, stride, *tables.shape)
+
+    def pages_fork(self, pool: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
+                   fresh: torch.Tensor, page: int) -> None:
+        """sequences dst[f] go on from src[f] (int32 [F] on the GPU): they take over its length and whole pages of `page` tokens, and
+        page fresh[f] becomes a copy of its last, partial one in every layer of the pool [layers, pages, ...] (any type). No dst is
+        a src or named twice, a fresh page is in nobody's table. A fork that names a sequence or page that is not there is not made."""
+        at, L, pages, nb, layer, stride, B, W = self._pages_of("pages_fork", pool, tables, lens)
+        F = src.numel()
+        for t in (src, dst, fresh):
+            if not self._plain(t, torch.int32) or t.numel() != F:
+                raise ValueError("[hip] pages_fork: src, dst and fresh are int32, as many of each, contiguous on the GPU")
+        self._call("btb_hip_pages_fork", at, L, pages, nb, layer, stride, tables.data_ptr(), lens.data_ptr(), B, W, page, src.data_ptr(),
+                   dst.data_ptr(), fresh.data_ptr(), F, _stream())
+
+    def pages_compact(self, pool: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, page: int,
+                      tables_out: torch.Tensor | None = None) -> torch.Tensor:
+        """the pages that sequences name closed up to the pool's first ones, in every layer of the pool [layers, pages, ...]: those
+        too far back go, in order, where nobody names a page. tables_out (None: tables itself): the tables as they are then, -1
+        behind a sequence's pages. Returns how many pages are in use (int32 [1] on the GPU)."""
+        at, L, pages, nb, layer, stride, B, W = self._pages_of("pages_compact", pool, tables, lens)
+        out = tables if tables_out is None else tables_out
+        if not self._plain(out, torch.int32) or out.shape != tables.shape:
+            raise ValueError("[hip] pages_compact: tables_out is like tables")
+        words = self.lib.btb_hip_pages_compact_words(pages)
+        ws = torch.empty(words + 1, dtype=torch.int32, device=pool.device)
+        used = ws[words:]
+        self._call("btb_hip_pages_compact", at, L, pages, nb, layer, stride, tables.data_ptr(), lens.data_ptr(), B, W, page,
+                   out.data_ptr(), used.data_ptr(), ws.data_ptr(), _stream())
+        return used
 
     def silu_mul(self, gu: torch.Tensor, m: torch.Tensor) -> torch.Tensor:
         self._need(gu, torch.bfloat16, "gu")

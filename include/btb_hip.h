@@ -518,6 +518,61 @@ int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t* pos, int6
                          float* mass_out, int64_t mo, int32_t* pos_out, int64_t po, int32_t* idx, uint32_t* workspace,
                          void* stream);
 
+/* ---- a paged cache held in 4 bits -------------------------------------------------------------------------
+ * Pages of `page` tokens (a multiple of 32) of all Hk kv heads of one layer, in a pool of `pages` of them, `stride` bytes from one to
+ * the next: page / 32 tiles of btb_hip_kv4_tile_bytes(D) bytes a head, one head after another. Sequence b's tokens 0 .. lens[b] - 1 lie in
+ * pages tables[b][0], tables[b][1], ... (i32 [B, W]); a length is cut to 0 .. W page, and tokens whose page is not one of the pool's are not there.
+ * The rows of a pass are its sequences' last ones: rows first[b] .. first[b + 1] - 1 (i32 [B + 1] on the device, ascending) are
+ * sequence b's, T / B a sequence where first is NULL; row i of n stands at lens[b] - n + i, and rows at places below 0 or behind the last
+ * sequence's are left alone. All of it is read on the device: a recorded call replays over longer sequences and other tables.
+ * A key is held as e2m1 codes with a power of two for 32 dims, the smallest e with max |k| <= 7 2^e (MXFP4: btb_hip_mx4_widen), a value as
+ * e2m1 codes with one scale, bf16(max |v| / 6); codes are the nearest, ties to even. An infinity or NaN makes all that its scale is for
+ * NaN. D 64 or 128; cache 16-byte aligned, stride a multiple of 16; B up to 65536, T up to 2^24, Hk up to 1024, W page up to 2^30. No
+ * counterpart in the reference. */
+
+/* bytes of 32 tokens of one kv head, keys and values: 2176 at D 64, 4288 at 128, 0 at others */
+size_t btb_hip_kv4_tile_bytes(size_t D);
+
+/* The pass's rows into the cache: k and v bf16, row t of head g at t * k_row + g * k_head (v_row, v_head) values, 16-byte aligned,
+ * strides multiples of 8. A row in a page outside the pool is not written. No two sequences may write to one page. */
+int32_t btb_hip_kv4_write(const void* k, const void* v, void* cache, const int32_t* tables, const int32_t* lens,
+                          const int32_t* first, size_t B, size_t W, size_t pages, size_t page, int64_t stride, size_t T,
+                          size_t Hk, size_t D, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, void* stream);
+
+/* The pass's rows as the cache holds them: into k and v, laid out as above, f32 (out_f32 != 0) or, rounded, bf16. A row in a page
+ * outside the pool reads as zeros. */
+int32_t btb_hip_kv4_read(const void* cache, const int32_t* tables, const int32_t* lens, const int32_t* first, size_t B,
+                         size_t W, size_t pages, size_t page, int64_t stride, size_t T, size_t Hk, size_t D, void* k, void* v,
+                         int32_t out_f32, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, void* stream);
+
+/* Attention of the pass's rows, q [T, Hq D] bf16, each over its sequence's tokens up to its own place: att [T, Hq D] bf16 and, where lse is
+ * not NULL, the rows' log-sum-exp [T, Hq] f32 (natural units, of scale q . k). A row with no token to see gets zeros and -inf. keys_cap: about how
+ * many tokens the longest sequence has; it sizes the launch and the workspace (btb_hip_attn_kv4_floats of them, this call's own; 0: the sizes are
+ * refused), a longer sequence takes longer. Sums are f32; q goes in to 2^-22 of the largest of its 32 dims, a weight to 2^-12 of itself (or 2^-36
+ * of the largest |weight value| of the tokens). Hq / Hk up to 64, T Hq up to 2^24, scale > 0; q, cache, att and workspace 16-byte aligned. */
+size_t btb_hip_attn_kv4_floats(size_t T, size_t B, size_t Hq, size_t Hk, size_t D, size_t keys_cap);
+int32_t btb_hip_attn_kv4(const void* q, const void* cache, const int32_t* tables, const int32_t* lens, const int32_t* first,
+                         void* att, float* lse, size_t B, size_t W, size_t pages, size_t page, int64_t stride, size_t T, size_t Hq,
+                         size_t Hk, size_t D, float scale, size_t keys_cap, float* workspace, void* stream);
+
+/* Sequences that go on from others, in all L layers of a pool (pages of `bytes` bytes, `stride` apart, `layer` bytes from a layer to the
+ * next; what they hold does not matter): for f < F sequence dst[f] takes over the length of src[f] and the entries of its whole pages; if
+ * tokens are left, its next entry is fresh[f], a copy of that page in every layer; the entries behind are -1. A fork is not made where src or
+ * dst is outside 0 .. B - 1, they are the same, or fresh is needed and outside the pool. dst distinct and none of them a src, fresh
+ * distinct and in nobody's table. src, dst, fresh: i32 [F] on the device. bytes, stride, layer multiples of 16; F up to 65536. */
+int32_t btb_hip_pages_fork(void* pool, size_t L, size_t pages, size_t bytes, int64_t layer, int64_t stride, int32_t* tables,
+                           int32_t* lens, size_t B, size_t W, size_t page, const int32_t* src, const int32_t* dst,
+                           const int32_t* fresh, size_t F, void* stream);
+
+/* The pool closed up: of the n pages that sequences name (the first ceil(lens[b] / page) entries of each), those below n stay, and the
+ * others, ascending, go to the pages below n that nobody names, ascending, in every layer. tables_out [B, W] (may be tables): the entries as
+ * they are then, -1 behind a sequence's and for what is no page of the pool; *used = n. workspace: btb_hip_pages_compact_words of
+ * them, this call's own. Up to 2^19 pages. */
+size_t btb_hip_pages_compact_words(size_t pages);
+int32_t btb_hip_pages_compact(void* pool, size_t L, size_t pages, size_t bytes, int64_t layer, int64_t stride, const int32_t* tables,
+                              const int32_t* lens, size_t B, size_t W, size_t page, int32_t* tables_out, int32_t* used,
+                              int32_t* workspace, void* stream);
+
 /* m [T, I] = bf16(bf16(silu(g)) * u) over gu [T, 2I] (gate then up). Replaces btb_silu_mul
  * (native/cuda/btb_kernels.cu:467-484); the matvec btb_hip_gemv_silu_bf16 folds the same values into its x load. */
 int32_t btb_hip_silu_mul(const void* gu, void* m, size_t T, size_t I, void* stream);
