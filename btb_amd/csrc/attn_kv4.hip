@@ -3,9 +3,9 @@
 //   s_j = scale q . k_j for j = 0 .. the row's position,  lse = log sum_j exp s_j,  att = sum_j exp(s_j - lse) v_j
 //
 // A wave has 32 (row, query head) pairs of a sequence and kv head, and walks tiles of 32 tokens with a running maximum and sum.
-// S^T = K Q^T by v_mfma_scale_f32_32x32x64_f8f6f4: the keys' codes go in as they lie, with their blocks' exponents, q as two
-// e4m3 terms with an exponent for 32 dims each: the second is what the first leaves, and together they are q to 2^-22 of the block's
-// largest value (bf16's eight bits are two times e4m3's four). A pair's scores against keys 8 (i / 4) + 4 h + i % 4 are then lane
+// S^T = K Q^T by v_mfma_f32_32x32x16_bf16, a key's codes times their power of two as bf16, which they are exactly, two a conversion. (The
+// products that take the codes as they lie, v_mfma_scale_f32_32x32x64_f8f6f4, lose what is 2^-13 of the largest term: with q as two e4m3
+// terms that was 5e-6 of lse.) A pair's scores against keys 8 (i / 4) + 4 h + i % 4 are then lane
 // (pair, h)'s own, and V lies in the same order: out^T += V^T P by v_mfma_f32_32x32x16_f16, the codes as f16, which they are exactly,
 // a value's scale in its weight.
 //
@@ -21,7 +21,6 @@
 namespace btb {
 
 typedef __attribute__((ext_vector_type(16))) float f32x16;
-typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
@@ -46,66 +45,21 @@ struct AttnKv4 {
 // spans of a sequence of `tiles` tiles: how many, and how long
 __device__ __forceinline__ int kv4_span(const AttnKv4& p, int tiles) { return max(p.span, (tiles + p.S - 1) / p.S); }
 
-// q's fragment: two e4m3 terms of the pair's dims, and the exponents of both, biased by 127 (NaN: 255). Of a step's 64 dims lane
-// (pair, h) holds 16 h .. + 15 of the first 32 and then of the last 32, and the exponent of the h-th 32.
+// q's fragment, exact: 8 dims a product, lane (pair, h) dims 64 step + 32 h + 8 j .. + 7 of the pair's row for product j of a step, as K's
+// codes lie (the order of the dims is free as long as both operands have it)
 template <int D>
 struct QueryFragment {
-    i32x8 hi[D / 64], lo[D / 64];
-    int e[D / 64];
+    bf16x8 x[D / 16];
 
     __device__ __forceinline__ void make(const uint16_t* q, bool there, int h) {
 #pragma unroll
-        for (int s = 0; s < D / 64; ++s) {
-            uint4 w[2][2];
-            uint32_t top[2];
+        for (int s = 0; s < D / 64; ++s)
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                top[b] = 0;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    w[b][i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (there) w[b][i] = *reinterpret_cast<const uint4*>(q + 64 * s + 32 * b + 16 * h + 8 * i);
-                    const uint32_t x[4] = {w[b][i].x, w[b][i].y, w[b][i].z, w[b][i].w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        top[b] = max(top[b], x[j] & 0x7FFFu);
-                        top[b] = max(top[b], x[j] >> 16 & 0x7FFFu);
-                    }
-                }
-                top[b] = max(top[b], f32_bits(xor32(bits_f32(top[b]))));
+            for (int j = 0; j < 4; ++j) {
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (there) w = *reinterpret_cast<const uint4*>(q + 64 * s + 32 * h + 8 * j);
+                x[4 * s + j] = __builtin_bit_cast(bf16x8, w);
             }
-            int es[2];
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                // the block's largest value becomes 2^7 .. 2^8; the second term's exponent, four less, stays one too
-                es[b] = max((int)(top[b] >> 7) - 7, 4);
-                const bool lost = top[b] >= 0x7F80u;
-                const float down = lost ? 0.f : bits_f32((uint32_t)(254 - es[b]) << 23);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t x[4] = {w[b][i].x, w[b][i].y, w[b][i].z, w[b][i].w};
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float y[4];
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            y[2 * k] = lost ? 0.f : bf16lo_f32(x[2 * j + k]) * down;
-                            y[2 * k + 1] = lost ? 0.f : bf16hi_f32(x[2 * j + k]) * down;
-                        }
-                        int a = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-                        a = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], a, true);
-                        const f32x2 b0 = __builtin_amdgcn_cvt_pk_f32_fp8(a, false), b1 = __builtin_amdgcn_cvt_pk_f32_fp8(a, true);
-                        int r = __builtin_amdgcn_cvt_pk_fp8_f32((y[0] - b0.x) * 16.f, (y[1] - b0.y) * 16.f, 0, false);
-                        r = __builtin_amdgcn_cvt_pk_fp8_f32((y[2] - b1.x) * 16.f, (y[3] - b1.y) * 16.f, r, true);
-                        hi[s][4 * b + 2 * i + j] = a;
-                        lo[s][4 * b + 2 * i + j] = r;
-                    }
-                }
-                if (lost) es[b] = 255;
-            }
-            const int mine = h ? es[1] : es[0];
-            e[s] = mine == 255 ? 0xFFFF : mine | (mine - 4) << 8;  // the first term's, the second's
-        }
     }
 };
 
@@ -137,6 +91,12 @@ __device__ __forceinline__ f16x8 codes_f16(uint32_t w) {
     return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+__device__ __forceinline__ bf16x8 codes_bf16(uint32_t w, float scale) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
 // a wave's pairs over the tiles it has been given
 template <int D>
 struct Walk {
@@ -162,14 +122,11 @@ struct Walk {
         for (int i = 0; i < 16; ++i) z[i] = 0.f;
 #pragma unroll
         for (int s = 0; s < D / 64; ++s) {
-            const i32x8 k = {(int)f.k[s].x, (int)f.k[s].y, (int)f.k[s].z, (int)f.k[s].w, 0, 0, 0, 0};
-            if (s == 0) {
-                z = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q.lo[s], z, 4, 0, 0, (int)f.e, 1, q.e[s]);
-                z = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q.hi[s], z, 4, 0, 0, (int)f.e, 0, q.e[s]);
-            } else {
-                z = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q.lo[s], z, 4, 0, 1, (int)f.e, 1, q.e[s]);
-                z = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q.hi[s], z, 4, 0, 1, (int)f.e, 0, q.e[s]);
-            }
+            // (the conversion reads the exponent's field alone: 0 is 2^-127, 255 makes of the zeros that go with it NaN)
+            const float scale = bits_f32((s ? f.e >> 8 : f.e & 0xFFu) << 23);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(codes_bf16(dword(f.k[s], j), scale), q.x[4 * s + j], z, 0, 0, 0);
         }
         uint32_t sc[8] = {f.s[0].x, f.s[0].y, f.s[0].z, f.s[0].w, f.s[1].x, f.s[1].y, f.s[1].z, f.s[1].w};
         if (MASKED) {

@@ -3,7 +3,7 @@
 // A tile is 32 tokens of one kv head, laid out as the matrix cores' operands, so that attention reads it in whole 16-byte pieces a
 // lane, straight into registers, and nothing passes through LDS:
 //   K codes   D / 64 steps x 64 lanes x 16 bytes: lane (c, h) = (lane & 31, lane >> 5) has token c's dims 64 step + 32 h .. + 31,
-//             the lower dim of a pair in a byte's low half: the operand of v_mfma_scale_f32_32x32x64_f8f6f4
+//             the lower dim of a pair in a byte's low half: one block of 32 dims, with one exponent
 //   V codes   D / 64 parts x 64 lanes x 16 bytes: dword 2 d + u of lane (c, h) has dim 64 part + 32 d + c of the 8 tokens
 //             16 u + 8 (e / 4) + 4 h + e % 4, e = 0 .. 7: where scores made as K Q^T lie, which are thus the second product's operand
 //   K scales  D / 64 bytes a lane in the same order: the exponent of the lane's 32 dims, biased by 127 (255: NaN)

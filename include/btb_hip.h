@@ -548,8 +548,8 @@ int32_t btb_hip_kv4_read(const void* cache, const int32_t* tables, const int32_t
 /* Attention of the pass's rows, q [T, Hq D] bf16, each over its sequence's tokens up to its own place: att [T, Hq D] bf16 and, where lse is
  * not NULL, the rows' log-sum-exp [T, Hq] f32 (natural units, of scale q . k). A row with no token to see gets zeros and -inf. keys_cap: about how
  * many tokens the longest sequence has; it sizes the launch and the workspace (btb_hip_attn_kv4_floats of them, this call's own; 0: the sizes are
- * refused), a longer sequence takes longer. Sums are f32; q goes in to 2^-22 of the largest of its 32 dims, a weight to 2^-12 of itself (or 2^-36
- * of the largest |weight value| of the tokens). Hq / Hk up to 64, T Hq up to 2^24, scale > 0; q, cache, att and workspace 16-byte aligned. */
+ * refused), a longer sequence takes longer. Sums are f32; a weight goes to the product with V to 2^-12 of itself (or 2^-36 of the largest, times
+ * their values' scales). Hq / Hk up to 64, T Hq up to 2^24, scale > 0; q, cache, att and workspace 16-byte aligned. */
 size_t btb_hip_attn_kv4_floats(size_t T, size_t B, size_t Hq, size_t Hk, size_t D, size_t keys_cap);
 int32_t btb_hip_attn_kv4(const void* q, const void* cache, const int32_t* tables, const int32_t* lens, const int32_t* first,
                          void* att, float* lse, size_t B, size_t W, size_t pages, size_t page, int64_t stride, size_t T, size_t Hq,
