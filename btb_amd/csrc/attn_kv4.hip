@@ -11,7 +11,8 @@
 //
 // Weights are f16, off by 2^-12 of themselves at most: e^(s - maximum) times 2^11 times the value's scale over the power of two `unit`, the
 // largest one so far: at most 2^15 (the maximum may lag by 2^4), in full precision down to 2^-25 of the largest, and 2^-36 of it is lost at most. A
-// bf16 weight would be off by 2^-9, two of them cost twice the products.
+// bf16 weight would be off by 2^-9, two of them cost twice the products. The unit in the maximum instead of in the scales would save a product
+// a weight (1 % of the time), but not the last bits of lse.
 
 #include "btb_kv4.hpp"
 #include "btb_tuning.hpp"
@@ -26,8 +27,12 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float NONE = -3.0e38f;   // a maximum of nothing: what is subtracted from it underflows to weight 0
-constexpr float LAG = 4.f;         // how far, in powers of two, scores may pass the maximum in use
-constexpr int PAIRS = 32;          // (row, query head) pairs a wave
+constexpr int ROOM = 11;           // a weight of 1 times the largest scale, in units of the power of two above that, as f16
+constexpr float LAG = 4.f;         // how far, in powers of two, scores may pass the maximum in use: f16 ends at 2^16
+constexpr int PAIRS = 32;          // (row, query head) pairs a workgroup
+#ifndef KV4_ROUNDS
+#define KV4_ROUNDS 2
+#endif
 
 struct AttnKv4 {
     Kv4Seqs seqs;
@@ -43,7 +48,7 @@ struct AttnKv4 {
 };
 
 // spans of a sequence of `tiles` tiles: how many, and how long
-__device__ __forceinline__ int kv4_span(const AttnKv4& p, int tiles) { return max(p.span, (tiles + p.S - 1) / p.S); }
+__device__ __forceinline__ int kv4_span_tiles(const AttnKv4& p, int tiles) { return max(p.span, (tiles + p.S - 1) / p.S); }
 
 // q's fragment, exact: 8 dims a product, lane (pair, h) dims 64 step + 32 h + 8 j .. + 7 of the pair's row for product j of a step, as K's
 // codes lie (the order of the dims is free as long as both operands have it)
@@ -63,26 +68,6 @@ struct QueryFragment {
     }
 };
 
-// a tile as a lane holds it
-template <int D>
-struct Kv4Fragment {
-    uint4 k[D / 64], v[D / 64];
-    uint32_t e;     // D / 64 exponents
-    uint4 s[2];     // the half's sixteen scales
-
-    __device__ __forceinline__ void load(const uint8_t* tile, int lane) {
-        using Tile = Kv4Tile<D>;
-#pragma unroll
-        for (int i = 0; i < D / 64; ++i) {
-            k[i] = load_stream16(reinterpret_cast<const uint4*>(tile) + 64 * i + lane);
-            v[i] = load_stream16(reinterpret_cast<const uint4*>(tile + Tile::V) + 64 * i + lane);
-        }
-        e = D == 128 ? reinterpret_cast<const uint16_t*>(tile + Tile::KS)[lane] : tile[Tile::KS + lane];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) s[i] = reinterpret_cast<const uint4*>(tile + Tile::VS + 32 * (lane >> 5))[i];
-    }
-};
-
 __device__ __forceinline__ uint32_t dword(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
 
 __device__ __forceinline__ f16x8 codes_f16(uint32_t w) {
@@ -97,12 +82,19 @@ __device__ __forceinline__ bf16x8 codes_bf16(uint32_t w, float scale) {
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// a wave's pairs over the tiles it has been given
-template <int D>
+// A wave's walk over the tiles it has been given, NG at a time: lane (column, h)'s pair is column % (32 / NG), and of each NG tiles it
+// weighs tile column / (32 / NG) alone. The products of K with q give every column the scores of every tile, of which it keeps
+// its own tile's; V's products get weights of zero in the other columns. So the softmax's work is done once for NG tiles where a sequence has few pairs,
+// and a column is a running softmax of its own; the columns of a pair meet at the end.
+template <int D, int NG>
 struct Walk {
-    static constexpr int DT = D / 32;
+    static constexpr int DT = D / 32, STEPS = D / 64, COLUMNS = PAIRS / NG;
+    using Tile = Kv4Tile<D>;
     f32x16 o[DT];
     float m, l, unit;
+    QueryFragment<D> q;
+    uint4 k[NG][STEPS], v[NG][STEPS], s[2];
+    uint32_t e[NG];
 
     __device__ __forceinline__ void begin() {
 #pragma unroll
@@ -112,44 +104,65 @@ struct Walk {
         m = NONE, l = 0.f;
         unit = bits_f32(27u << 23);  // 2^-100
     }
+    __device__ __forceinline__ static int group(int lane) { return NG == 1 ? 0 : (lane & 31) / COLUMNS; }
 
-    // `left`: tokens of the tile the lane's pair sees; `there`: that any pair does; MASKED: some pair does not see all 32
-    template <bool MASKED>
-    __device__ __forceinline__ void tile(const Kv4Fragment<D>& f, const QueryFragment<D>& q, float c, int left, int there, int lane) {
-        const int h = lane >> 5;
-        f32x16 z;
+    __device__ __forceinline__ void load_k(int t, const uint8_t* tile, int lane) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) z[i] = 0.f;
+        for (int i = 0; i < STEPS; ++i) k[t][i] = reinterpret_cast<const uint4*>(tile)[64 * i + lane];
+        e[t] = D == 128 ? reinterpret_cast<const uint16_t*>(tile + Tile::KS)[lane] : tile[Tile::KS + lane];
+    }
+    __device__ __forceinline__ void load_v(int t, const uint8_t* tile, int lane) {
 #pragma unroll
-        for (int s = 0; s < D / 64; ++s) {
-            // (the conversion reads the exponent's field alone: 0 is 2^-127, 255 makes of the zeros that go with it NaN)
-            const float scale = bits_f32((s ? f.e >> 8 : f.e & 0xFFu) << 23);
+        for (int i = 0; i < STEPS; ++i) v[t][i] = reinterpret_cast<const uint4*>(tile + Tile::V)[64 * i + lane];
+    }
+    __device__ __forceinline__ void load_s(const uint8_t* tile, int lane) {  // the lane's own tile
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(codes_bf16(dword(f.k[s], j), scale), q.x[4 * s + j], z, 0, 0, 0);
-        }
-        uint32_t sc[8] = {f.s[0].x, f.s[0].y, f.s[0].z, f.s[0].w, f.s[1].x, f.s[1].y, f.s[1].z, f.s[1].w};
-        if (MASKED) {
+        for (int i = 0; i < 2; ++i) s[i] = reinterpret_cast<const uint4*>(tile + Tile::VS + 32 * (lane >> 5))[i];
+    }
+
+    __device__ __forceinline__ void scores(f32x16& z, int lane) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int token = kv4_token(h, i);
-                if (token >= left) z[i] = -__builtin_inff();
-                if (token >= there) sc[i / 2] &= i % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+        for (int t = 0; t < NG; ++t) {
+            f32x16 x;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = 0.f;
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) {
+                // (the conversion reads the exponent's field alone: 0 is 2^-127, 255 makes of the zeros that go with it NaN)
+                const float scale = bits_f32((st ? e[t] >> 8 : e[t] & 0xFFu) << 23);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(codes_bf16(dword(k[t][st], j), scale), q.x[4 * st + j], x, 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            if (t == 0) {
+                z = x;
+            } else {
+                const bool own = group(lane) == t;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) z[i] = own ? x[i] : z[i];
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
+    }
+
+    // tokens of its tile that the lane's pair does not see, from `left` on: no score, and no scale (what lies there may be anything)
+    __device__ __forceinline__ void hide(f32x16& z, int left, int lane) {
+        uint32_t* sc = reinterpret_cast<uint32_t*>(s);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (kv4_token(lane >> 5, i) >= left) {
+                z[i] = -__builtin_inff();
+                sc[i / 2] &= i % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+            }
+    }
+
+    __device__ __forceinline__ void weights(f32x16& z, f16x8 (&w)[2], float c) {
+        const uint32_t sc[8] = {s[0].x, s[0].y, s[0].z, s[0].w, s[1].x, s[1].y, s[1].z, s[1].w};
         float top = z[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = fmaxf(top, z[i]);
         top = fmaxf(top, xor32(top)) * c;
-        if (__any(top > m + LAG)) {
-            const float to = fmaxf(m, top), by = __builtin_amdgcn_exp2f(m - to);
-            l *= by;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[d][i] *= by;
-            m = to;
-        }
         // the largest scale: as signed 16-bit numbers, of which NaN is the least
         typedef __attribute__((ext_vector_type(2))) short i16x2;
         i16x2 big = __builtin_bit_cast(i16x2, sc[0]);
@@ -157,180 +170,217 @@ struct Walk {
         for (int i = 1; i < 8; ++i) big = __builtin_elementwise_max(big, __builtin_bit_cast(i16x2, sc[i]));
         int most = max((int)big[0], (int)big[1]);
         most = max(most, __builtin_bit_cast(int, xor32(__builtin_bit_cast(float, most))));
-        most = __builtin_amdgcn_readfirstlane(most);
         const float power = bits_f32(((uint32_t)(max(most, 0) & 0x7F80) + 0x80u) << 16);  // the power of two above it
-        if (power > unit) {
-            const float by = unit / power;
+        if (__any(top > m + LAG || power > unit)) {
+            const float to = fmaxf(m, top), above = fmaxf(power, unit);
+            const float by = __builtin_amdgcn_exp2f(m - to);
+            l *= by;
+            const float both = by * (unit / above);
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[d][i] *= by;
-            unit = power;
+                for (int i = 0; i < 16; ++i) o[d][i] *= both;
+            m = to, unit = above;
         }
-        const float inv = bits_f32((265u << 23) - f32_bits(unit));  // 2^11 / unit
-        f16x8 w[2];
+        const float inv = bits_f32((uint32_t)(254 + ROOM) * (1u << 23) - f32_bits(unit));  // 2^ROOM / unit
+        float ps[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float p = __builtin_amdgcn_exp2f(fmaf(z[i], c, -m));
             l += p;
-            const float sv = (i % 2 ? bf16hi_f32(sc[i / 2]) : bf16lo_f32(sc[i / 2])) * inv;
-            float ps = p * sv;
-            if (MASKED && kv4_token(h, i) >= left) ps = 0.f;
-            w[i / 8][i % 8] = (_Float16)ps;
+            ps[i] = p * ((i % 2 ? bf16hi_f32(sc[i / 2]) : bf16lo_f32(sc[i / 2])) * inv);
         }
+        // (two to an instruction: left to itself the compiler folds each product into a conversion of its own, at half the rate)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < 2; ++u) {
+            u32x4 x;
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_f16(dword(f.v[d / 2], 2 * (d % 2) + u)), w[u], o[d], 0, 0, 0);
+            for (int i = 0; i < 4; ++i) {
+                uint32_t y;
+                asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(y) : "v"(ps[8 * u + 2 * i]), "v"(ps[8 * u + 2 * i + 1]));
+                x[i] = y;
+            }
+            w[u] = __builtin_bit_cast(f16x8, x);
+        }
+    }
+
+    __device__ __forceinline__ void outputs(const f16x8 (&w)[2], int lane) {
+#pragma unroll
+        for (int t = 0; t < NG; ++t) {
+            const bool own = group(lane) == t;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                f16x8 x = w[u];
+                if (NG > 1) {
+                    u32x4 y = __builtin_bit_cast(u32x4, x);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[i] = own ? y[i] : 0u;
+                    x = __builtin_bit_cast(f16x8, y);
+                }
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_f16(dword(v[t][d / 2], 2 * (d % 2) + u)), x, o[d], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
     }
 };
 
-// SHARE: the workgroup's four waves have a tile of pairs each and the same span; else one tile of pairs, its span dealt out among them
-template <int D, bool SHARE>
-__global__ void __launch_bounds__(256, 2) attn_kv4_kernel(AttnKv4 p) {
-    constexpr int DT = D / 32, PITCH = D + 4;
-    __shared__ float meet[SHARE ? 1 : 2][SHARE ? 1 : PAIRS][SHARE ? 1 : PITCH];
-    __shared__ float meet_m[2][PAIRS], meet_l[2][PAIRS];
-    const int lane = threadIdx.x & 63, pair = lane & 31, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int hk = blockIdx.x % p.Hk, rest = blockIdx.x / p.Hk, span = rest % p.S;
-    const int per_group = SHARE ? 4 * PAIRS : PAIRS;
-    auto groups = [&](int b) {
-        int row0, n;
-        p.seqs.of(b, row0, n);
-        return (int)(((long long)n * p.G + per_group - 1) / per_group);
-    };
-    int b, item;
-    if (p.seqs.first == nullptr)
-        b = rest / p.S / p.items, item = rest / p.S % p.items;
-    else
-        kv4_find(rest / p.S, p.seqs.B, b, item, groups);
-    if (b < 0) return;
-    b = __builtin_amdgcn_readfirstlane(b), item = __builtin_amdgcn_readfirstlane(item);
-    int row0, n;
-    p.seqs.of(b, row0, n);
-    const int len = p.seqs.len(b), tiles = (len + KV4_TOKENS - 1) / KV4_TOKENS, length = kv4_span(p, tiles);
-    const int spans = max(1, (tiles + length - 1) / length);
-    if (span >= spans) return;
-    const int pairs = n * p.G, pair0 = item * per_group + (SHARE ? wave * PAIRS : 0);
-    if (SHARE && pair0 >= pairs) return;  // (no barrier follows in this form)
-    const int mine = pair0 + pair;
-    const bool there = mine < pairs;
-    const int row = there ? mine / p.G : 0, head = hk * p.G + (there ? mine % p.G : 0);
-    const size_t place = (size_t)(row0 + row) * p.Hq + head;  // the pair's row and head in q, att and lse
-    QueryFragment<D> q;
-    q.make(p.q + place * D, there, h);
-    // tokens the pair sees, and what every pair of the wave sees
-    const int sees = there ? len - n + row + 1 : 0;
-    const int last = min(pair0 + PAIRS, pairs) - 1;
-    const int all = len - n + pair0 / p.G + 1, any = len - n + last / p.G + 1;
-    const int from = span * length + (SHARE ? 0 : wave), to = min(min((span + 1) * length, tiles), (any + KV4_TOKENS - 1) / KV4_TOKENS);
-    constexpr int STEP = SHARE ? 1 : 4;
+// A workgroup's span of tiles for up to 32 pairs of a sequence and kv head
+struct KvSpan {
+    int b, hk, span, spans, from, to;  // its tiles
+    int row0, n, len;                  // the sequence's rows and tokens
+    int pair0, pairs;                  // the first pair, and how many the sequence has
+};
 
-    Walk<D> w;
+template <int D>
+struct Meet {  // the columns of the four waves
+    float o[4 * PAIRS][D + 4];
+    float m[4 * PAIRS], l[4 * PAIRS];
+};
+
+// its four waves' batches of NG tiles, dealt out in turn; the columns meet in LDS
+template <int D, int NG>
+__device__ __forceinline__ void kv4_span(const AttnKv4& p, const KvSpan& a, Meet<D>& meet) {
+    constexpr int DT = D / 32, COLUMNS = PAIRS / NG;
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int mine = a.pair0 + (lane & (COLUMNS - 1)), here = min(a.pairs - a.pair0, COLUMNS);
+    const bool there = mine < a.pairs;
+    const int row = there ? mine / p.G : 0, head = a.hk * p.G + (there ? mine % p.G : 0);
+    Walk<D, NG> w;
+    w.q.make(p.q + ((size_t)(a.row0 + row) * p.Hq + head) * D, there, h);
     w.begin();
-    const uint8_t* cache = p.cache;
-    // places of the next 64 tiles, one a lane
+    const int sees = there ? a.len - a.n + row + 1 : 0;            // tokens the pair sees
+    const int all = a.len - a.n + a.pair0 / p.G + 1;               // what every pair sees
+    const int own = Walk<D, NG>::group(lane);
+    // places of the wave's next 64 tiles, one a lane; -1: no tile, or no page of the pool
+    const int from = a.from + wave * NG;
     long long at = -1, ahead = -1;
-    auto places = [&](int j) { return j + STEP * lane < to ? p.seqs.at(b, j + STEP * lane, hk) : -1; };
+    auto places = [&](int base) {
+        const int j = base + lane / NG * 4 * NG + lane % NG;
+        return j < a.to ? p.seqs.at(a.b, j, a.hk) : -1;
+    };
     auto take = [&](int i) {
         const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, i);
         const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)at >> 32), i);
         return (long long)((uint64_t)hi << 32 | lo);
     };
-    auto step = [&](const Kv4Fragment<D>& f, long long where, int j) {
-        if (where < 0) return;  // no page of the pool: its tokens are not there
-        const int first = j * KV4_TOKENS;
-        if (first + KV4_TOKENS <= all)
-            w.template tile<false>(f, q, p.c, 32, 32, lane);
-        else
-            w.template tile<true>(f, q, p.c, sees - first, len - first, lane);
+    auto give = [&](long long x, int i) {  // lane i's number in the lanes that ask for it
+        const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)x, i, WAVE), hi = (uint32_t)__shfl((int)(uint32_t)((uint64_t)x >> 32), i, WAVE);
+        return (long long)((uint64_t)hi << 32 | lo);
     };
-    for (int base = from; base < to; base += 64 * STEP) {
-        at = base == from ? places(base) : ahead;
-        ahead = places(base + 64 * STEP);
-        const int count = min((to - base + STEP - 1) / STEP, 64);
-        Kv4Fragment<D> f[2];
-        long long where[2];
-        where[0] = take(0);
-        f[0].load(cache + max(where[0], 0ll), lane);
-        for (int i = 0; i < count; i += 2) {
-            where[1] = -1;
-            if (i + 1 < count) {
-                where[1] = take(i + 1);
-                f[1].load(cache + max(where[1], 0ll), lane);
+    auto request_k = [&](int i) {
+#pragma unroll
+        for (int t = 0; t < NG; ++t) w.load_k(t, p.cache + max(take(i + t), 0ll), lane);
+    };
+    auto request_v = [&](int i) {
+#pragma unroll
+        for (int t = 0; t < NG; ++t) w.load_v(t, p.cache + max(take(i + t), 0ll), lane);
+        w.load_s(p.cache + max(NG == 1 ? take(i) : give(at, i + own), 0ll), lane);
+    };
+    constexpr int STRIDE = 4 * NG, REFILL = 64 / NG * STRIDE;
+    if (from < a.to) {
+        at = places(from);
+        ahead = places(from + REFILL);
+        request_k(0);
+        request_v(0);
+        int i = 0;  // of the 64 places
+        for (int j = from; j < a.to; j += STRIDE) {
+            // (the places of this batch, before those behind it take over)
+            const long long place = NG == 1 ? take(i) : give(at, i + own);
+            f32x16 z;
+            w.scores(z, lane);
+            i += NG;
+            if (i == 64) {
+                i = 0, at = ahead;
+                ahead = places(j + STRIDE + REFILL);
             }
-            step(f[0], where[0], base + STEP * i);
-            if (i + 2 < count) {
-                where[0] = take(i + 2);
-                f[0].load(cache + max(where[0], 0ll), lane);
-            }
-            if (i + 1 < count) step(f[1], where[1], base + STEP * (i + 1));
+            const bool more = j + STRIDE < a.to;
+            if (more) request_k(i);
+            const int first = (j + own) * KV4_TOKENS;
+            f16x8 weight[2];
+            if ((j + NG) * KV4_TOKENS > all || j + NG > a.to || __any(place < 0)) w.hide(z, place < 0 ? 0 : sees - first, lane);
+            w.weights(z, weight, p.c);
+            w.outputs(weight, lane);
+            if (more) request_v(i);
         }
     }
-    float l = w.l + xor32(w.l), m = w.m;
-    const float real = w.unit * bits_f32(116u << 23);  // unit / 2^11
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) w.o[d][i] *= real;
-    if constexpr (!SHARE) {
-        // the four waves' states, two and two
-        for (int half = 2; half >= 1; half /= 2) {
-            if (half == 1) __syncthreads();
-            if (wave >= half && wave < 2 * half) {
-                if (h == 0) meet_m[wave - half][pair] = m, meet_l[wave - half][pair] = l;
-                if (there)
-#pragma unroll
-                    for (int d = 0; d < DT; ++d)
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4)
-                            *reinterpret_cast<float4*>(&meet[wave - half][pair][32 * d + 2 * i + 4 * h]) =
-                                make_float4(w.o[d][i], w.o[d][i + 1], w.o[d][i + 2], w.o[d][i + 3]);
-            }
-            __syncthreads();
-            if (wave < half) {
-                const float m2 = meet_m[wave][pair], l2 = meet_l[wave][pair], to_m = fmaxf(m, m2);
-                const float a = __builtin_amdgcn_exp2f(m - to_m), a2 = __builtin_amdgcn_exp2f(m2 - to_m);
-                l = l * a + l2 * a2;
-                m = to_m;
-                if (there)
-#pragma unroll
-                    for (int d = 0; d < DT; ++d)
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            const float4 x = *reinterpret_cast<const float4*>(&meet[wave][pair][32 * d + 2 * i + 4 * h]);
-                            w.o[d][i] = fmaf(w.o[d][i], a, x.x * a2);
-                            w.o[d][i + 1] = fmaf(w.o[d][i + 1], a, x.y * a2);
-                            w.o[d][i + 2] = fmaf(w.o[d][i + 2], a, x.z * a2);
-                            w.o[d][i + 3] = fmaf(w.o[d][i + 3], a, x.w * a2);
-                        }
-            }
-        }
-        if (wave != 0) return;
-    }
-    if (!there) return;
-    if (spans == 1) {
-        const float by = l == 0.f ? 0.f : 1.f / l;
-        uint16_t* out = p.att + place * D;
+    const float l = w.l + xor32(w.l), real = w.unit * bits_f32((127u - ROOM) << 23);
+    const int column = wave * PAIRS + (lane & 31);
+    if (h == 0) meet.m[column] = w.m, meet.l[column] = l;
+    if (there)
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<uint2*>(out + 32 * d + 2 * i + 4 * h) =
-                    make_uint2(f32x2_bf16(w.o[d][i] * by, w.o[d][i + 1] * by), f32x2_bf16(w.o[d][i + 2] * by, w.o[d][i + 3] * by));
-        if (p.lse != nullptr && h == 0) p.lse[place] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * LN2;
-        return;
+                *reinterpret_cast<float4*>(&meet.o[column][32 * d + 2 * i + 4 * h]) =
+                    make_float4(w.o[d][i] * real, w.o[d][i + 1] * real, w.o[d][i + 2] * real, w.o[d][i + 3] * real);
+    __syncthreads();
+    // a thread four dims of a pair, over its 4 NG columns
+    for (int task = threadIdx.x; task < here * (D / 4); task += 256) {
+        const int pair = task / (D / 4), dim = 4 * (task % (D / 4));
+        float to = NONE, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4 * NG; ++i) to = fmaxf(to, meet.m[i / NG * PAIRS + i % NG * COLUMNS + pair]);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 4 * NG; ++i) {
+            const int from_column = i / NG * PAIRS + i % NG * COLUMNS + pair;
+            const float by = __builtin_amdgcn_exp2f(meet.m[from_column] - to);
+            sum = fmaf(meet.l[from_column], by, sum);
+            const float4 y = *reinterpret_cast<const float4*>(&meet.o[from_column][dim]);
+            x = make_float4(fmaf(y.x, by, x.x), fmaf(y.y, by, x.y), fmaf(y.z, by, x.z), fmaf(y.w, by, x.w));
+        }
+        const int r = (a.pair0 + pair) / p.G, hd = a.hk * p.G + (a.pair0 + pair) % p.G;
+        const size_t at_pair = (size_t)(a.row0 + r) * p.Hq + hd;
+        if (a.spans == 1) {
+            const float by = sum == 0.f ? 0.f : 1.f / sum;
+            *reinterpret_cast<uint2*>(p.att + at_pair * D + dim) = make_uint2(f32x2_bf16(x.x * by, x.y * by), f32x2_bf16(x.z * by, x.w * by));
+            if (p.lse != nullptr && dim == 0) p.lse[at_pair] = sum == 0.f ? -__builtin_inff() : (to + __builtin_amdgcn_logf(sum)) * LN2;
+        } else {
+            const size_t slot = at_pair * p.S + a.span;
+            if (dim == 0) reinterpret_cast<float2*>(p.part)[slot] = make_float2(to, sum);
+            *reinterpret_cast<float4*>(p.part + 2 * (size_t)p.seqs.T * p.Hq * p.S + slot * D + dim) = x;
+        }
     }
-    const size_t slot = place * p.S + span;
-    if (h == 0) reinterpret_cast<float2*>(p.part)[slot] = make_float2(m, l);
-    float* out = p.part + 2 * (size_t)p.seqs.T * p.Hq * p.S + slot * D;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<float4*>(out + 32 * d + 2 * i + 4 * h) =
-                make_float4(w.o[d][i], w.o[d][i + 1], w.o[d][i + 2], w.o[d][i + 3]);
+}
+
+template <int D>
+__global__ void __launch_bounds__(256, 2) attn_kv4_kernel(AttnKv4 p) {
+    extern __shared__ float4 lds[];
+    Meet<D>& meet = *reinterpret_cast<Meet<D>*>(lds);
+    KvSpan a;
+    a.hk = blockIdx.x % p.Hk;
+    const int rest = blockIdx.x / p.Hk;
+    a.span = rest % p.S;
+    int item;
+    if (p.seqs.first == nullptr)
+        a.b = rest / p.S / p.items, item = rest / p.S % p.items;
+    else
+        kv4_find(rest / p.S, p.seqs.B, a.b, item, [&](int b) {
+            int row0, n;
+            p.seqs.of(b, row0, n);
+            return (int)(((long long)n * p.G + PAIRS - 1) / PAIRS);
+        });
+    if (a.b < 0) return;
+    a.b = __builtin_amdgcn_readfirstlane(a.b), item = __builtin_amdgcn_readfirstlane(item);
+    p.seqs.of(a.b, a.row0, a.n);
+    a.len = p.seqs.len(a.b);
+    const int tiles = (a.len + KV4_TOKENS - 1) / KV4_TOKENS, length = kv4_span_tiles(p, tiles);
+    a.spans = max(1, (tiles + length - 1) / length);
+    if (a.span >= a.spans) return;
+    a.pairs = a.n * p.G, a.pair0 = item * PAIRS;
+    const int last = min(a.pair0 + PAIRS, a.pairs) - 1;  // the pair that sees most
+    const int any = a.len - a.n + last / p.G + 1;
+    a.from = a.span * length;
+    a.to = min(min(a.from + length, tiles), (any + KV4_TOKENS - 1) / KV4_TOKENS);
+    // few pairs: several tiles at a time. At head_dim 128 four of them do not fit the registers: 131072 tokens of one row 33 us by two,
+    // 37 by one, 51 by four; 56 rows of 5 + 8 heads x 64 over 3001 15.2 by four, 16.4 by two, 17.0 by one
+    constexpr int NG = D == 64 ? 4 : 2;
+    if (a.pairs - a.pair0 <= PAIRS / NG)
+        kv4_span<D, NG>(p, a, meet);
+    else
+        kv4_span<D, 1>(p, a, meet);
 }
 
 // The spans of a row and head, in their order: a workgroup each, its waves a quarter of them each.
@@ -355,7 +405,7 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(AttnKv4 p) {
         }
         if (b < 0) return;
     }
-    const int tiles = (p.seqs.len(b) + KV4_TOKENS - 1) / KV4_TOKENS, length = kv4_span(p, tiles);
+    const int tiles = (p.seqs.len(b) + KV4_TOKENS - 1) / KV4_TOKENS, length = kv4_span_tiles(p, tiles);
     const int spans = (tiles + length - 1) / length;
     if (spans <= 1) return;
     const size_t place = blockIdx.x;
@@ -419,23 +469,19 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(AttnKv4 p) {
     if (p.lse != nullptr && lane == 0) p.lse[place] = total == 0.f ? -__builtin_inff() : (to + __builtin_amdgcn_logf(total)) * LN2;
 }
 
-// How a call is cut, from what the host knows: tiles of pairs a sequence, one or four a workgroup, and spans.
+// How a call is cut, from what the host knows: tiles of pairs a sequence, and spans.
 struct Kv4Plan {
-    bool share;
     int items;        // workgroups a sequence, where each has as many rows
     long long groups; // workgroups a kv head and span
     int S, span;
 };
 static Kv4Plan kv4_plan(size_t T, size_t B, size_t Hk, size_t G, size_t keys_cap, bool ragged) {
     Kv4Plan plan;
-    const size_t R = T / B;
-    plan.share = (T + B - 1) / B * G > 2 * PAIRS;
-    const size_t per = plan.share ? 4 * PAIRS : PAIRS;
-    plan.items = (int)((R * G + per - 1) / per);
-    plan.groups = (long long)(ragged ? T * G / per + B : B * plan.items);
+    plan.items = (int)((T / B * G + PAIRS - 1) / PAIRS);
+    plan.groups = (long long)(ragged ? T * G / PAIRS + B : B * plan.items);
     const size_t tiles = (keys_cap + KV4_TOKENS - 1) / KV4_TOKENS;
-    const size_t least = 8;  // tiles a span at least: two a wave
-    const size_t want = ((size_t)4 * device_info().cus + plan.groups * Hk - 1) / (plan.groups * Hk);
+    const size_t least = 16;  // tiles a span at least: a batch a wave
+    const size_t want = ((size_t)KV4_ROUNDS * device_info().cus + plan.groups * Hk - 1) / (plan.groups * Hk);
     size_t S = want < 1 ? 1 : want;
     const size_t most = tiles < least ? 1 : tiles / least;
     if (S > most) S = most;
@@ -444,6 +490,18 @@ static Kv4Plan kv4_plan(size_t T, size_t B, size_t Hk, size_t G, size_t keys_cap
     plan.span = (int)((tiles + S - 1) / S);
     if (plan.span < (int)least) plan.span = (int)least;
     return plan;
+}
+
+template <int D>
+static int32_t launch_attn_kv4(const AttnKv4& p, const Kv4Plan& plan, hipStream_t st) {
+    constexpr int lds = (int)sizeof(Meet<D>);
+    const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_kv4_kernel<D>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (rc != hipSuccess) return hip_status(rc, "hipFuncSetAttribute");
+    hipLaunchKernelGGL(attn_kv4_kernel<D>, dim3((unsigned)(plan.groups * plan.S * (long long)p.Hk)), dim3(256), lds, st, p);
+    const int32_t done = hip_status(hipGetLastError(), "attn_kv4 launch");
+    if (done != OK || plan.S == 1) return done;
+    hipLaunchKernelGGL(attn_kv4_join_kernel<D>, dim3((unsigned)(p.seqs.T * p.Hq)), dim3(256), 0, st, p);
+    return hip_status(hipGetLastError(), "attn_kv4 join launch");
 }
 
 }  // namespace btb
@@ -487,16 +545,5 @@ extern "C" int32_t btb_hip_attn_kv4(const void* q, const void* cache, const int3
     p.Hq = (int)Hq, p.Hk = (int)Hk, p.G = (int)(Hq / Hk);
     p.items = plan.items, p.S = plan.S, p.span = plan.span;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const dim3 grid((unsigned)(plan.groups * plan.S * (long long)Hk)), threads(256);
-    if (D == 64)
-        hipLaunchKernelGGL((plan.share ? attn_kv4_kernel<64, true> : attn_kv4_kernel<64, false>), grid, threads, 0, st, p);
-    else
-        hipLaunchKernelGGL((plan.share ? attn_kv4_kernel<128, true> : attn_kv4_kernel<128, false>), grid, threads, 0, st, p);
-    int32_t rc = hip_status(hipGetLastError(), "attn_kv4 launch");
-    if (rc != OK || plan.S == 1) return rc;
-    if (D == 64)
-        hipLaunchKernelGGL(attn_kv4_join_kernel<64>, dim3((unsigned)(T * Hq)), threads, 0, st, p);
-    else
-        hipLaunchKernelGGL(attn_kv4_join_kernel<128>, dim3((unsigned)(T * Hq)), threads, 0, st, p);
-    return hip_status(hipGetLastError(), "attn_kv4 join launch");
+    return D == 64 ? launch_attn_kv4<64>(p, plan, st) : launch_attn_kv4<128>(p, plan, st);
 }

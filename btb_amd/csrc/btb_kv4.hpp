@@ -38,7 +38,7 @@ struct Kv4Seqs {
     int B, W, T, rows, pages;
     int per;                // tiles a page
     long long stride;       // bytes from a page to the next
-    long long head;         // bytes of a page's head
+    int tile;               // bytes of a tile
 
     // what the device arrays say is cut to what there is
     __device__ __forceinline__ int len(int b) const {
@@ -55,7 +55,7 @@ struct Kv4Seqs {
     // the bytes of tile j of a sequence's head, -1 where the table names no page of the pool
     __device__ __forceinline__ long long at(int b, int j, int hk) const {
         const int page = tables[(size_t)b * W + j / per];
-        return page < 0 || page >= pages ? -1 : page * stride + hk * head + (long long)(j % per) * (head / per);
+        return page < 0 || page >= pages ? -1 : page * stride + ((long long)hk * per + j % per) * tile;
     }
 };
 
@@ -93,9 +93,9 @@ inline bool kv4_seqs(Kv4Seqs& s, const int32_t* tables, const int32_t* lens, con
         (first == nullptr && T % B != 0))
         return false;
     s.per = (int)(page / KV4_TOKENS);
-    s.head = (long long)(s.per * kv4_tile_bytes(D));
+    s.tile = (int)kv4_tile_bytes(D);
     s.stride = stride;
-    if (stride < (long long)Hk * s.head || stride % 16 != 0 || stride > ((int64_t)1 << 46) / (int64_t)pages) return false;
+    if (stride < (long long)Hk * s.per * s.tile || stride % 16 != 0 || stride > ((int64_t)1 << 46) / (int64_t)pages) return false;
     s.tables = tables, s.lens = lens, s.first = first;
     s.B = (int)B, s.W = (int)W, s.T = (int)T, s.rows = (int)(T / B), s.pages = (int)pages;
     return true;
