@@ -383,12 +383,15 @@ __global__ void __launch_bounds__(256, 2) attn_kv4_kernel(AttnKv4 p) {
         kv4_span<D, 1>(p, a, meet);
 }
 
-// The spans of a row and head, in their order: a workgroup each, its waves a quarter of them each.
-template <int D>
+// The spans of a row and head, in their order: a wave each, or (WAVES 4) a workgroup, its waves a quarter of them each.
+template <int D, int WAVES>
 __global__ void __launch_bounds__(256) attn_kv4_join_kernel(AttnKv4 p) {
     constexpr int V = D / 64;
     __shared__ float sum_o[4][D], sum_m[4], sum_l[4];
-    const int t = blockIdx.x / p.Hq, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = WAVES == 1 ? 0 : threadIdx.x >> 6;
+    const unsigned mine = WAVES == 1 ? 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
+    if (mine >= (unsigned)p.seqs.T * p.Hq) return;
+    const int t = mine / p.Hq;
     int b = -1;
     if (p.seqs.first == nullptr) {
         b = t / p.seqs.rows;
@@ -408,10 +411,10 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(AttnKv4 p) {
     const int tiles = (p.seqs.len(b) + KV4_TOKENS - 1) / KV4_TOKENS, length = kv4_span_tiles(p, tiles);
     const int spans = (tiles + length - 1) / length;
     if (spans <= 1) return;
-    const size_t place = blockIdx.x;
+    const size_t place = mine;
     const float2* ml = reinterpret_cast<const float2*>(p.part) + place * p.S;
     const float* o = p.part + 2 * (size_t)p.seqs.T * p.Hq * p.S + place * p.S * D + V * lane;
-    const int quarter = (spans + 3) / 4, first = wave * quarter, end = min(first + quarter, spans);
+    const int quarter = (spans + WAVES - 1) / WAVES, first = wave * quarter, end = min(first + quarter, spans);
     float m = NONE, l = 0.f, sum[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.f;
@@ -443,22 +446,27 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(AttnKv4 p) {
         }
         m = to;
     }
-    if (lane == 0) sum_m[wave] = m, sum_l[wave] = l;
+    float to = m, total = l, out[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) sum_o[wave][V * lane + i] = sum[i];
-    __syncthreads();
-    if (wave != 0) return;
-    float to = NONE, total = 0.f, out[V];
+    for (int i = 0; i < V; ++i) out[i] = sum[i];
+    if constexpr (WAVES == 4) {
+        if (lane == 0) sum_m[wave] = m, sum_l[wave] = l;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) to = fmaxf(to, sum_m[u]);
+        for (int i = 0; i < V; ++i) sum_o[wave][V * lane + i] = sum[i];
+        __syncthreads();
+        if (wave != 0) return;
+        to = NONE, total = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = 0.f;
+        for (int u = 0; u < 4; ++u) to = fmaxf(to, sum_m[u]);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const float a = __builtin_amdgcn_exp2f(sum_m[u] - to);
-        total = fmaf(sum_l[u], a, total);
+        for (int i = 0; i < V; ++i) out[i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) out[i] = fmaf(sum_o[u][V * lane + i], a, out[i]);
+        for (int u = 0; u < 4; ++u) {
+            const float a = __builtin_amdgcn_exp2f(sum_m[u] - to);
+            total = fmaf(sum_l[u], a, total);
+#pragma unroll
+            for (int i = 0; i < V; ++i) out[i] = fmaf(sum_o[u][V * lane + i], a, out[i]);
+        }
     }
     const float by = total == 0.f ? 0.f : 1.f / total;
     uint16_t* att = p.att + place * D + V * lane;
@@ -481,7 +489,7 @@ static Kv4Plan kv4_plan(size_t T, size_t B, size_t Hk, size_t G, size_t keys_cap
     plan.groups = (long long)(ragged ? T * G / PAIRS + B : B * plan.items);
     const size_t tiles = (keys_cap + KV4_TOKENS - 1) / KV4_TOKENS;
     const size_t least = 16;  // tiles a span at least: a batch a wave
-    const size_t want = ((size_t)KV4_ROUNDS * device_info().cus + plan.groups * Hk - 1) / (plan.groups * Hk);
+    const size_t want = (size_t)KV4_ROUNDS * device_info().cus / (plan.groups * Hk);
     size_t S = want < 1 ? 1 : want;
     const size_t most = tiles < least ? 1 : tiles / least;
     if (S > most) S = most;
@@ -500,7 +508,11 @@ static int32_t launch_attn_kv4(const AttnKv4& p, const Kv4Plan& plan, hipStream_
     hipLaunchKernelGGL(attn_kv4_kernel<D>, dim3((unsigned)(plan.groups * plan.S * (long long)p.Hk)), dim3(256), lds, st, p);
     const int32_t done = hip_status(hipGetLastError(), "attn_kv4 launch");
     if (done != OK || plan.S == 1) return done;
-    hipLaunchKernelGGL(attn_kv4_join_kernel<D>, dim3((unsigned)(p.seqs.T * p.Hq)), dim3(256), 0, st, p);
+    const unsigned pairs = (unsigned)(p.seqs.T * p.Hq);
+    if (plan.S >= 16)  // (one wave a pair takes its spans four at a time)
+        hipLaunchKernelGGL((attn_kv4_join_kernel<D, 4>), dim3(pairs), dim3(256), 0, st, p);
+    else
+        hipLaunchKernelGGL((attn_kv4_join_kernel<D, 1>), dim3((pairs + 3) / 4), dim3(256), 0, st, p);
     return hip_status(hipGetLastError(), "attn_kv4 join launch");
 }
 
