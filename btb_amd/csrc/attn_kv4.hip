@@ -30,9 +30,6 @@ constexpr float NONE = -3.0e38f;   // a maximum of nothing: what is subtracted f
 constexpr int ROOM = 11;           // a weight of 1 times the largest scale, in units of the power of two above that, as f16
 constexpr float LAG = 4.f;         // how far, in powers of two, scores may pass the maximum in use: f16 ends at 2^16
 constexpr int PAIRS = 32;          // (row, query head) pairs a workgroup
-#ifndef KV4_ROUNDS
-#define KV4_ROUNDS 2
-#endif
 
 struct AttnKv4 {
     Kv4Seqs seqs;
@@ -82,19 +79,12 @@ __device__ __forceinline__ bf16x8 codes_bf16(uint32_t w, float scale) {
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// A wave's walk over the tiles it has been given, NG at a time: lane (column, h)'s pair is column % (32 / NG), and of each NG tiles it
-// weighs tile column / (32 / NG) alone. The products of K with q give every column the scores of every tile, of which it keeps
-// its own tile's; V's products get weights of zero in the other columns. So the softmax's work is done once for NG tiles where a sequence has few pairs,
-// and a column is a running softmax of its own; the columns of a pair meet at the end.
-template <int D, int NG>
-struct Walk {
-    static constexpr int DT = D / 32, STEPS = D / 64, COLUMNS = PAIRS / NG;
-    using Tile = Kv4Tile<D>;
+// A pair's running softmax, in the lanes (column, 0) and (column, 1)
+template <int D>
+struct Softmax {
+    static constexpr int DT = D / 32;
     f32x16 o[DT];
     float m, l, unit;
-    QueryFragment<D> q;
-    uint4 k[NG][STEPS], v[NG][STEPS], s[2];
-    uint32_t e[NG];
 
     __device__ __forceinline__ void begin() {
 #pragma unroll
@@ -104,70 +94,18 @@ struct Walk {
         m = NONE, l = 0.f;
         unit = bits_f32(27u << 23);  // 2^-100
     }
-    __device__ __forceinline__ static int group(int lane) { return NG == 1 ? 0 : (lane & 31) / COLUMNS; }
 
-    __device__ __forceinline__ void load_k(int t, const uint8_t* tile, int lane) {
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) k[t][i] = reinterpret_cast<const uint4*>(tile)[64 * i + lane];
-        e[t] = D == 128 ? reinterpret_cast<const uint16_t*>(tile + Tile::KS)[lane] : tile[Tile::KS + lane];
-    }
-    __device__ __forceinline__ void load_v(int t, const uint8_t* tile, int lane) {
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) v[t][i] = reinterpret_cast<const uint4*>(tile + Tile::V)[64 * i + lane];
-    }
-    __device__ __forceinline__ void load_s(const uint8_t* tile, int lane) {  // the lane's own tile
-#pragma unroll
-        for (int i = 0; i < 2; ++i) s[i] = reinterpret_cast<const uint4*>(tile + Tile::VS + 32 * (lane >> 5))[i];
-    }
-
-    __device__ __forceinline__ void scores(f32x16& z, int lane) {
-#pragma unroll
-        for (int t = 0; t < NG; ++t) {
-            f32x16 x;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = 0.f;
-#pragma unroll
-            for (int st = 0; st < STEPS; ++st) {
-                // (the conversion reads the exponent's field alone: 0 is 2^-127, 255 makes of the zeros that go with it NaN)
-                const float scale = bits_f32((st ? e[t] >> 8 : e[t] & 0xFFu) << 23);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(codes_bf16(dword(k[t][st], j), scale), q.x[4 * st + j], x, 0, 0, 0);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            if (t == 0) {
-                z = x;
-            } else {
-                const bool own = group(lane) == t;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) z[i] = own ? x[i] : z[i];
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
-
-    // tokens of its tile that the lane's pair does not see, from `left` on: no score, and no scale (what lies there may be anything)
-    __device__ __forceinline__ void hide(f32x16& z, int left, int lane) {
-        uint32_t* sc = reinterpret_cast<uint32_t*>(s);
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (kv4_token(lane >> 5, i) >= left) {
-                z[i] = -__builtin_inff();
-                sc[i / 2] &= i % 2 ? 0x0000FFFFu : 0xFFFF0000u;
-            }
-    }
-
-    __device__ __forceinline__ void weights(f32x16& z, f16x8 (&w)[2], float c) {
-        const uint32_t sc[8] = {s[0].x, s[0].y, s[0].z, s[0].w, s[1].x, s[1].y, s[1].z, s[1].w};
+    // the maximum and the unit moved to where a tile's scores z and scales s need them
+    __device__ __forceinline__ void move(const f32x16& z, const uint32_t (&s)[8], float c) {
         float top = z[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = fmaxf(top, z[i]);
         top = fmaxf(top, xor32(top)) * c;
         // the largest scale: as signed 16-bit numbers, of which NaN is the least
         typedef __attribute__((ext_vector_type(2))) short i16x2;
-        i16x2 big = __builtin_bit_cast(i16x2, sc[0]);
+        i16x2 big = __builtin_bit_cast(i16x2, s[0]);
 #pragma unroll
-        for (int i = 1; i < 8; ++i) big = __builtin_elementwise_max(big, __builtin_bit_cast(i16x2, sc[i]));
+        for (int i = 1; i < 8; ++i) big = __builtin_elementwise_max(big, __builtin_bit_cast(i16x2, s[i]));
         int most = max((int)big[0], (int)big[1]);
         most = max(most, __builtin_bit_cast(int, xor32(__builtin_bit_cast(float, most))));
         const float power = bits_f32(((uint32_t)(max(most, 0) & 0x7F80) + 0x80u) << 16);  // the power of two above it
@@ -182,47 +120,152 @@ struct Walk {
                 for (int i = 0; i < 16; ++i) o[d][i] *= both;
             m = to, unit = above;
         }
-        const float inv = bits_f32((uint32_t)(254 + ROOM) * (1u << 23) - f32_bits(unit));  // 2^ROOM / unit
-        float ps[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(z[i], c, -m));
-            l += p;
-            ps[i] = p * ((i % 2 ? bf16hi_f32(sc[i / 2]) : bf16lo_f32(sc[i / 2])) * inv);
-        }
-        // (two to an instruction: left to itself the compiler folds each product into a conversion of its own, at half the rate)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            u32x4 x;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t y;
-                asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(y) : "v"(ps[8 * u + 2 * i]), "v"(ps[8 * u + 2 * i + 1]));
-                x[i] = y;
-            }
-            w[u] = __builtin_bit_cast(f16x8, x);
-        }
     }
 
-    __device__ __forceinline__ void outputs(const f16x8 (&w)[2], int lane) {
+    // scores 2 i and 2 i + 1 to weights
+    __device__ __forceinline__ void weigh(const f32x16& z, const uint32_t (&s)[8], u32x4 (&w)[2], float c, int i) {
+        const float inv = bits_f32((uint32_t)(254 + ROOM) * (1u << 23) - f32_bits(unit));  // 2^ROOM / unit
+        const float a = __builtin_amdgcn_exp2f(fmaf(z[2 * i], c, -m)), b = __builtin_amdgcn_exp2f(fmaf(z[2 * i + 1], c, -m));
+        l += a;
+        l += b;
+        const float x = a * (bf16lo_f32(s[i]) * inv), y = b * (bf16hi_f32(s[i]) * inv);
+        // (two to an instruction: left to itself the compiler folds each product into a conversion of its own, at half the rate)
+        uint32_t both;
+        asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(both) : "v"(x), "v"(y));
+        w[i / 4][i % 4] = both;
+    }
+};
+
+// a tile's operands as a lane holds them
+template <int D>
+struct TileWords {
+    static constexpr int STEPS = D / 64;
+    using Tile = Kv4Tile<D>;
+    uint4 k[STEPS], v[STEPS];
+    uint32_t e;
+
+    __device__ __forceinline__ void load_k(const uint8_t* tile, int lane) {
 #pragma unroll
-        for (int t = 0; t < NG; ++t) {
-            const bool own = group(lane) == t;
+        for (int i = 0; i < STEPS; ++i) k[i] = reinterpret_cast<const uint4*>(tile)[64 * i + lane];
+        e = D == 128 ? reinterpret_cast<const uint16_t*>(tile + Tile::KS)[lane] : tile[Tile::KS + lane];
+    }
+    __device__ __forceinline__ void load_v(const uint8_t* tile, int lane) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                f16x8 x = w[u];
-                if (NG > 1) {
-                    u32x4 y = __builtin_bit_cast(u32x4, x);
+        for (int i = 0; i < STEPS; ++i) v[i] = reinterpret_cast<const uint4*>(tile + Tile::V)[64 * i + lane];
+    }
+    // K's operand of product j: 8 dims of the lane's 32. (The conversion reads the exponent's field alone: 0 is 2^-127, 255 makes of
+    // the zeros that go with it NaN.)
+    __device__ __forceinline__ bf16x8 wide_k(int j) const {
+        return codes_bf16(dword(k[j / 4], j % 4), bits_f32((j / 4 ? e >> 8 : e & 0xFFu) << 23));
+    }
+    // V's operand of 32 dims against the u-th 16 tokens
+    __device__ __forceinline__ f16x8 wide_v(int d, int u) const { return codes_f16(dword(v[d / 2], 2 * (d % 2) + u)); }
+};
+
+// the scales of a lane's half of a tile
+struct TileScales {
+    uint4 s[2];
+    __device__ __forceinline__ void load(const uint8_t* scales, int lane) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) y[i] = own ? y[i] : 0u;
-                    x = __builtin_bit_cast(f16x8, y);
-                }
+        for (int i = 0; i < 2; ++i) s[i] = reinterpret_cast<const uint4*>(scales + 32 * (lane >> 5))[i];
+    }
+    __device__ __forceinline__ void get(uint32_t (&x)[8]) const {
 #pragma unroll
-                for (int d = 0; d < DT; ++d)
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_f16(dword(v[t][d / 2], 2 * (d % 2) + u)), x, o[d], 0, 0, 0);
-                __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < 8; ++i) x[i] = dword(s[i / 4], i % 4);
+    }
+};
+
+// tokens of a tile from `left` on, which the lane's pair does not see: no score, and no scale (what lies there may be anything)
+__device__ __forceinline__ void hide(f32x16& z, uint32_t (&s)[8], int left, int lane) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (kv4_token(lane >> 5, i) >= left) {
+            z[i] = -__builtin_inff();
+            s[i / 2] &= i % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+        }
+}
+
+__device__ __forceinline__ f32x16 zeros() {
+    f32x16 z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+    return z;
+}
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// Up to 32 pairs over tiles NG at a time: lane (column, h)'s pair is column % (32 / NG), and of each NG tiles it weighs tile
+// column / (32 / NG) alone. The products of K with q give every column the scores of every tile, of which it keeps
+// its own tile's; V's products get weights of zero in the other columns. So the softmax's work is done once for NG tiles where a sequence has few pairs,
+// and a column is a running softmax of its own; the columns of a pair meet at the end. A batch's weights are made between the products of
+// the next one's scores.
+template <int D, int NG>
+struct Walk {
+    static constexpr int DT = D / 32, COLUMNS = PAIRS / NG, PRODUCTS = NG * D / 16;
+    Softmax<D> to;
+    QueryFragment<D> q;
+    TileWords<D> t[NG];
+    TileScales s;
+    f32x16 z;
+
+    __device__ __forceinline__ static int group(int lane) { return NG == 1 ? 0 : (lane & 31) / COLUMNS; }
+
+    // `between`(n) is done behind product n of PRODUCTS
+    template <class Between>
+    __device__ __forceinline__ f32x16 scores(int lane, Between between) {
+        f32x16 all;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            f32x16 x = zeros();
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+                x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(t[g].wide_k(j), q.x[j], x, 0, 0, 0);
+                between(g * D / 16 + j);
+                fence();
+            }
+            if (g == 0) {
+                all = x;
+            } else {
+                const bool own = group(lane) == g;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) all[i] = own ? x[i] : all[i];
             }
         }
+        return all;
+    }
+
+    // a batch whose K has been multiplied: `hidden` and left as for `hide`; next_k() asks for the K behind the next batch's, next_v() for the
+    // next batch's V
+    template <class NextK, class NextV>
+    __device__ __forceinline__ void batch(bool hidden, int left, float c, int lane, NextK next_k, NextV next_v) {
+        uint32_t sc[8];
+        s.get(sc);
+        if (hidden) hide(z, sc, left, lane);
+        to.move(z, sc, c);
+        u32x4 w[2];
+        // ahead of the CU's other workgroup meanwhile: two waves in step would multiply together and then wait for the vector unit together
+        __builtin_amdgcn_s_setprio(1);
+        const f32x16 ahead = scores(lane, [&](int n) {
+#pragma unroll
+            for (int i = 8 * n / PRODUCTS; i < 8 * (n + 1) / PRODUCTS; ++i) to.weigh(z, sc, w, c, i);
+        });
+        __builtin_amdgcn_s_setprio(0);
+        next_k();
+        f16x8 wide = t[0].wide_v(0, 0);
+#pragma unroll
+        for (int n = 0; n < NG * 2 * DT; ++n) {
+            const int d = n % DT, u = n / DT % 2, g = n / DT / 2;
+            u32x4 x = w[u];
+            if (NG > 1) {
+                const bool own = group(lane) == g;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = own ? x[i] : 0u;
+            }
+            to.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wide, __builtin_bit_cast(f16x8, x), to.o[d], 0, 0, 0);
+            if (n + 1 < NG * 2 * DT) wide = t[(n + 1) / DT / 2].wide_v((n + 1) % DT, (n + 1) / DT % 2);
+            fence();
+        }
+        next_v();
+        z = ahead;
     }
 };
 
@@ -239,83 +282,10 @@ struct Meet {  // the columns of the four waves
     float m[4 * PAIRS], l[4 * PAIRS];
 };
 
-// its four waves' batches of NG tiles, dealt out in turn; the columns meet in LDS
+// a tile of pairs' columns, of which `here` are pairs, added up; behind a barrier
 template <int D, int NG>
-__device__ __forceinline__ void kv4_span(const AttnKv4& p, const KvSpan& a, Meet<D>& meet) {
-    constexpr int DT = D / 32, COLUMNS = PAIRS / NG;
-    const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int mine = a.pair0 + (lane & (COLUMNS - 1)), here = min(a.pairs - a.pair0, COLUMNS);
-    const bool there = mine < a.pairs;
-    const int row = there ? mine / p.G : 0, head = a.hk * p.G + (there ? mine % p.G : 0);
-    Walk<D, NG> w;
-    w.q.make(p.q + ((size_t)(a.row0 + row) * p.Hq + head) * D, there, h);
-    w.begin();
-    const int sees = there ? a.len - a.n + row + 1 : 0;            // tokens the pair sees
-    const int all = a.len - a.n + a.pair0 / p.G + 1;               // what every pair sees
-    const int own = Walk<D, NG>::group(lane);
-    // places of the wave's next 64 tiles, one a lane; -1: no tile, or no page of the pool
-    const int from = a.from + wave * NG;
-    long long at = -1, ahead = -1;
-    auto places = [&](int base) {
-        const int j = base + lane / NG * 4 * NG + lane % NG;
-        return j < a.to ? p.seqs.at(a.b, j, a.hk) : -1;
-    };
-    auto take = [&](int i) {
-        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, i);
-        const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)at >> 32), i);
-        return (long long)((uint64_t)hi << 32 | lo);
-    };
-    auto give = [&](long long x, int i) {  // lane i's number in the lanes that ask for it
-        const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)x, i, WAVE), hi = (uint32_t)__shfl((int)(uint32_t)((uint64_t)x >> 32), i, WAVE);
-        return (long long)((uint64_t)hi << 32 | lo);
-    };
-    auto request_k = [&](int i) {
-#pragma unroll
-        for (int t = 0; t < NG; ++t) w.load_k(t, p.cache + max(take(i + t), 0ll), lane);
-    };
-    auto request_v = [&](int i) {
-#pragma unroll
-        for (int t = 0; t < NG; ++t) w.load_v(t, p.cache + max(take(i + t), 0ll), lane);
-        w.load_s(p.cache + max(NG == 1 ? take(i) : give(at, i + own), 0ll), lane);
-    };
-    constexpr int STRIDE = 4 * NG, REFILL = 64 / NG * STRIDE;
-    if (from < a.to) {
-        at = places(from);
-        ahead = places(from + REFILL);
-        request_k(0);
-        request_v(0);
-        int i = 0;  // of the 64 places
-        for (int j = from; j < a.to; j += STRIDE) {
-            // (the places of this batch, before those behind it take over)
-            const long long place = NG == 1 ? take(i) : give(at, i + own);
-            f32x16 z;
-            w.scores(z, lane);
-            i += NG;
-            if (i == 64) {
-                i = 0, at = ahead;
-                ahead = places(j + STRIDE + REFILL);
-            }
-            const bool more = j + STRIDE < a.to;
-            if (more) request_k(i);
-            const int first = (j + own) * KV4_TOKENS;
-            f16x8 weight[2];
-            if ((j + NG) * KV4_TOKENS > all || j + NG > a.to || __any(place < 0)) w.hide(z, place < 0 ? 0 : sees - first, lane);
-            w.weights(z, weight, p.c);
-            w.outputs(weight, lane);
-            if (more) request_v(i);
-        }
-    }
-    const float l = w.l + xor32(w.l), real = w.unit * bits_f32((127u - ROOM) << 23);
-    const int column = wave * PAIRS + (lane & 31);
-    if (h == 0) meet.m[column] = w.m, meet.l[column] = l;
-    if (there)
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<float4*>(&meet.o[column][32 * d + 2 * i + 4 * h]) =
-                    make_float4(w.o[d][i] * real, w.o[d][i + 1] * real, w.o[d][i + 2] * real, w.o[d][i + 3] * real);
-    __syncthreads();
+__device__ __forceinline__ void kv4_meet(const AttnKv4& p, const KvSpan& a, const Meet<D>& meet, int pair0, int here) {
+    constexpr int COLUMNS = PAIRS / NG;
     // a thread four dims of a pair, over its 4 NG columns
     for (int task = threadIdx.x; task < here * (D / 4); task += 256) {
         const int pair = task / (D / 4), dim = 4 * (task % (D / 4));
@@ -331,7 +301,7 @@ __device__ __forceinline__ void kv4_span(const AttnKv4& p, const KvSpan& a, Meet
             const float4 y = *reinterpret_cast<const float4*>(&meet.o[from_column][dim]);
             x = make_float4(fmaf(y.x, by, x.x), fmaf(y.y, by, x.y), fmaf(y.z, by, x.z), fmaf(y.w, by, x.w));
         }
-        const int r = (a.pair0 + pair) / p.G, hd = a.hk * p.G + (a.pair0 + pair) % p.G;
+        const int r = (pair0 + pair) / p.G, hd = a.hk * p.G + (pair0 + pair) % p.G;
         const size_t at_pair = (size_t)(a.row0 + r) * p.Hq + hd;
         if (a.spans == 1) {
             const float by = sum == 0.f ? 0.f : 1.f / sum;
@@ -343,6 +313,96 @@ __device__ __forceinline__ void kv4_span(const AttnKv4& p, const KvSpan& a, Meet
             *reinterpret_cast<float4*>(p.part + 2 * (size_t)p.seqs.T * p.Hq * p.S + slot * D + dim) = x;
         }
     }
+}
+
+// its four waves' batches of NG tiles, dealt out in turn; the columns meet in LDS
+template <int D, int NG>
+__device__ __forceinline__ void kv4_span(const AttnKv4& p, const KvSpan& a, Meet<D>& meet) {
+    constexpr int DT = D / 32, COLUMNS = PAIRS / NG;
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int mine = a.pair0 + (lane & (COLUMNS - 1)), here = min(a.pairs - a.pair0, COLUMNS);
+    const bool there = mine < a.pairs;
+    const int row = there ? mine / p.G : 0, head = a.hk * p.G + (there ? mine % p.G : 0);
+    Walk<D, NG> w;
+    w.to.begin();
+    w.q.make(p.q + ((size_t)(a.row0 + row) * p.Hq + head) * D, there, h);
+    const int sees = there ? a.len - a.n + row + 1 : 0;  // tokens the lane's pair sees
+    const int all = a.len - a.n + a.pair0 / p.G + 1;     // and every pair
+    const int own = Walk<D, NG>::group(lane);
+    // places of the wave's next 64 tiles, one a lane; -1: no tile, or no page of the pool
+    const int from = a.from + wave * NG;
+    constexpr int STRIDE = 4 * NG, REFILL = 64 / NG * STRIDE;
+    auto places = [&](int base) {
+        const int j = base + lane / NG * STRIDE + lane % NG;
+        return j < a.to ? p.seqs.at(a.b, j, a.hk) : -1;
+    };
+    auto take = [&](long long x, int i) {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, i);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)x >> 32), i);
+        return (long long)((uint64_t)hi << 32 | lo);
+    };
+    auto give = [&](long long x, int i) {  // the place of the lane's own tile
+        if (NG == 1) return take(x, i);
+        const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)x, i + own, WAVE);
+        const uint32_t hi = (uint32_t)__shfl((int)(uint32_t)((uint64_t)x >> 32), i + own, WAVE);
+        return (long long)((uint64_t)hi << 32 | lo);
+    };
+    auto request_k = [&](long long x, int i) {
+#pragma unroll
+        for (int t = 0; t < NG; ++t) w.t[t].load_k(p.cache + max(take(x, i + t), 0ll), lane);
+    };
+    auto request_v = [&](long long x, int i) {
+#pragma unroll
+        for (int t = 0; t < NG; ++t) w.t[t].load_v(p.cache + max(take(x, i + t), 0ll), lane);
+        w.s.load(p.cache + max(give(x, i), 0ll) + Kv4Tile<D>::VS, lane);
+    };
+    if (from < a.to) {
+        // (behind the last tile what is asked for is the pool's first, for nobody)
+        long long at = places(from), ahead = places(from + REFILL);
+        int i = 0, base = from;  // of the 64 places `at`, and the first one's tile
+        auto on = [&] {
+            i += NG;
+            if (i == 64) {
+                i = 0, base += REFILL;
+                at = ahead;
+                ahead = places(base + REFILL);
+            }
+        };
+        request_k(at, 0);
+        request_v(at, 0);
+        long long place = give(at, 0);
+        w.z = w.scores(lane, [](int) {});
+        on();
+        request_k(at, i);
+        for (int j = from; j < a.to; j += STRIDE) {
+            const int left = place < 0 ? 0 : sees - (j + own) * KV4_TOKENS;
+            const bool hidden = (j + NG) * KV4_TOKENS > all || j + NG > a.to || __any(place < 0);
+            const long long next = at;
+            const int next_i = i;
+            place = give(next, next_i);
+            w.batch(
+                hidden, left, p.c, lane,
+                [&] {
+                    on();
+                    request_k(at, i);
+                },
+                [&] { request_v(next, next_i); });
+        }
+    }
+    const int column = wave * PAIRS + (lane & 31);
+    const float l = w.to.l + xor32(w.to.l), real = w.to.unit * bits_f32((127u - ROOM) << 23);
+    if (h == 0) meet.m[column] = w.to.m, meet.l[column] = l;
+    if (there)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const f32x16& o = w.to.o[d];
+                *reinterpret_cast<float4*>(&meet.o[column][32 * d + 2 * i + 4 * h]) =
+                    make_float4(o[i] * real, o[i + 1] * real, o[i + 2] * real, o[i + 3] * real);
+            }
+    __syncthreads();
+    kv4_meet<D, NG>(p, a, meet, a.pair0, here);
 }
 
 template <int D>
@@ -489,7 +549,9 @@ static Kv4Plan kv4_plan(size_t T, size_t B, size_t Hk, size_t G, size_t keys_cap
     plan.groups = (long long)(ragged ? T * G / PAIRS + B : B * plan.items);
     const size_t tiles = (keys_cap + KV4_TOKENS - 1) / KV4_TOKENS;
     const size_t least = 16;  // tiles a span at least: a batch a wave
-    const size_t want = (size_t)KV4_ROUNDS * device_info().cus / (plan.groups * Hk);
+    // two workgroups a CU, as many as fit (131072 tokens of one row: 32 us, 37 with three, 44 with six; without a second round 500 rows over
+    // 16384 are 175 instead of 183)
+    const size_t want = (size_t)2 * device_info().cus / (plan.groups * Hk);
     size_t S = want < 1 ? 1 : want;
     const size_t most = tiles < least ? 1 : tiles / least;
     if (S > most) S = most;
