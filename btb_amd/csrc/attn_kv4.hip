@@ -25,6 +25,7 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
+constexpr int MOST_SPANS = 256;    // a thread each where they are joined
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float NONE = -3.0e38f;   // a maximum of nothing: what is subtracted from it underflows to weight 0
 constexpr int ROOM = 11;           // a weight of 1 times the largest scale, in units of the power of two above that, as f16
@@ -443,15 +444,14 @@ __global__ void __launch_bounds__(256, 2) attn_kv4_kernel(AttnKv4 p) {
         kv4_span<D, 1>(p, a, meet);
 }
 
-// The spans of a row and head, in their order: a wave each, or (WAVES 4) a workgroup, its waves a quarter of them each.
-template <int D, int WAVES>
-__global__ void __launch_bounds__(256) attn_kv4_join_kernel(AttnKv4 p) {
-    constexpr int V = D / 64;
-    __shared__ float sum_o[4][D], sum_m[4], sum_l[4];
-    const int lane = threadIdx.x & 63, wave = WAVES == 1 ? 0 : threadIdx.x >> 6;
-    const unsigned mine = WAVES == 1 ? 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
-    if (mine >= (unsigned)p.seqs.T * p.Hq) return;
-    const int t = mine / p.Hq;
+// A row's spans, and where they lie: false where it has none, or one, which has made its outputs itself
+struct KvParts {
+    int spans;
+    const float2* ml;
+    const float* o;
+};
+__device__ __forceinline__ bool kv4_parts(const AttnKv4& p, unsigned pair, int D, KvParts& parts) {
+    const int t = pair / p.Hq, lane = threadIdx.x & 63;
     int b = -1;
     if (p.seqs.first == nullptr) {
         b = t / p.seqs.rows;
@@ -466,28 +466,39 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(AttnKv4 p) {
             const uint64_t found = __ballot(mine);
             if (found != 0) b = b0 + __ffsll((unsigned long long)found) - 1;
         }
-        if (b < 0) return;
+        if (b < 0) return false;
     }
     const int tiles = (p.seqs.len(b) + KV4_TOKENS - 1) / KV4_TOKENS, length = kv4_span_tiles(p, tiles);
-    const int spans = (tiles + length - 1) / length;
-    if (spans <= 1) return;
-    const size_t place = mine;
-    const float2* ml = reinterpret_cast<const float2*>(p.part) + place * p.S;
-    const float* o = p.part + 2 * (size_t)p.seqs.T * p.Hq * p.S + place * p.S * D + V * lane;
-    const int quarter = (spans + WAVES - 1) / WAVES, first = wave * quarter, end = min(first + quarter, spans);
+    parts.spans = (tiles + length - 1) / length;
+    parts.ml = reinterpret_cast<const float2*>(p.part) + (size_t)pair * p.S;
+    parts.o = p.part + 2 * (size_t)p.seqs.T * p.Hq * p.S + (size_t)pair * p.S * D;
+    return parts.spans > 1;
+}
+__device__ __forceinline__ void kv4_lse(const AttnKv4& p, unsigned pair, float m, float l) {
+    if (p.lse != nullptr) p.lse[pair] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+// Few spans: a wave a row and head, the spans four at a time.
+template <int D>
+__global__ void __launch_bounds__(256) attn_kv4_join_few(AttnKv4 p) {
+    constexpr int V = D / 64;
+    const int lane = threadIdx.x & 63;
+    const unsigned pair = 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    KvParts parts;
+    if (pair >= (unsigned)p.seqs.T * p.Hq || !kv4_parts(p, pair, D, parts)) return;
     float m = NONE, l = 0.f, sum[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.f;
-    for (int j = first; j < end; j += 4) {
+    for (int j = 0; j < parts.spans; j += 4) {
         float2 x[4];
         float y[4][V];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const int at = min(j + u, end - 1);
-            x[u] = ml[at];
+            const int at = min(j + u, parts.spans - 1);
+            x[u] = parts.ml[at];
 #pragma unroll
-            for (int i = 0; i < V; ++i) y[u][i] = o[(size_t)at * D + i];
-            if (j + u >= end) x[u] = make_float2(NONE, 0.f);
+            for (int i = 0; i < V; ++i) y[u][i] = parts.o[(size_t)at * D + V * lane + i];
+            if (j + u >= parts.spans) x[u] = make_float2(NONE, 0.f);
         }
         float to = m;
 #pragma unroll
@@ -498,7 +509,7 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(AttnKv4 p) {
         for (int i = 0; i < V; ++i) sum[i] *= by;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            if (j + u >= end) continue;
+            if (j + u >= parts.spans) continue;
             const float a = __builtin_amdgcn_exp2f(x[u].x - to);
             l = fmaf(x[u].y, a, l);
 #pragma unroll
@@ -506,35 +517,65 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(AttnKv4 p) {
         }
         m = to;
     }
-    float to = m, total = l, out[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = sum[i];
-    if constexpr (WAVES == 4) {
-        if (lane == 0) sum_m[wave] = m, sum_l[wave] = l;
-#pragma unroll
-        for (int i = 0; i < V; ++i) sum_o[wave][V * lane + i] = sum[i];
-        __syncthreads();
-        if (wave != 0) return;
-        to = NONE, total = 0.f;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) to = fmaxf(to, sum_m[u]);
-#pragma unroll
-        for (int i = 0; i < V; ++i) out[i] = 0.f;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const float a = __builtin_amdgcn_exp2f(sum_m[u] - to);
-            total = fmaf(sum_l[u], a, total);
-#pragma unroll
-            for (int i = 0; i < V; ++i) out[i] = fmaf(sum_o[u][V * lane + i], a, out[i]);
-        }
-    }
-    const float by = total == 0.f ? 0.f : 1.f / total;
-    uint16_t* att = p.att + place * D + V * lane;
+    const float by = l == 0.f ? 0.f : 1.f / l;
+    uint16_t* att = p.att + (size_t)pair * D + V * lane;
     if constexpr (V == 2)
-        *reinterpret_cast<uint32_t*>(att) = f32x2_bf16(out[0] * by, out[1] * by);
+        *reinterpret_cast<uint32_t*>(att) = f32x2_bf16(sum[0] * by, sum[1] * by);
     else
-        *att = f32_bf16(out[0] * by);
-    if (p.lse != nullptr && lane == 0) p.lse[place] = total == 0.f ? -__builtin_inff() : (to + __builtin_amdgcn_logf(total)) * LN2;
+        *att = f32_bf16(sum[0] * by);
+    if (lane == 0) kv4_lse(p, pair, m, l);
+}
+
+// Many spans: a workgroup a row and head. All that it reads is asked for at once; the spans' weights are made meanwhile.
+constexpr int JOIN_AT_ONCE = 8;
+template <int D>
+__global__ void __launch_bounds__(256) attn_kv4_join_many(AttnKv4 p) {
+    constexpr int GROUPS = 1024 / D;  // of threads, a span each at a time
+    __shared__ float by[MOST_SPANS], tops[4], sums[4];
+    __shared__ float4 part[GROUPS][D / 4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = tid / (D / 4), dim = tid % (D / 4);
+    KvParts parts;
+    if (!kv4_parts(p, blockIdx.x, D, parts)) return;
+    const float4* o = reinterpret_cast<const float4*>(parts.o) + dim;
+    float4 y[JOIN_AT_ONCE];
+    const float2 ml = tid < parts.spans ? parts.ml[tid] : make_float2(NONE, 0.f);
+#pragma unroll
+    for (int u = 0; u < JOIN_AT_ONCE; ++u) {
+        const int j = group + GROUPS * u;
+        y[u] = j < parts.spans ? o[(size_t)j * (D / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float top = ml.x;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d, WAVE));
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const float a = __builtin_amdgcn_exp2f(ml.x - top);
+    by[tid] = a;
+    const float mine = wave_sum(ml.y * a);
+    if (lane == 0) sums[wave] = mine;
+    __syncthreads();
+    const float total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](const float4& v, int j) {
+        const float f = by[j];
+        x = make_float4(fmaf(v.x, f, x.x), fmaf(v.y, f, x.y), fmaf(v.z, f, x.z), fmaf(v.w, f, x.w));
+    };
+#pragma unroll
+    for (int u = 0; u < JOIN_AT_ONCE; ++u)
+        if (group + GROUPS * u < parts.spans) add(y[u], group + GROUPS * u);
+    for (int j = group + GROUPS * JOIN_AT_ONCE; j < parts.spans; j += GROUPS) add(o[(size_t)j * (D / 4)], j);
+    part[group][dim] = x;
+    __syncthreads();
+    if (group != 0) return;
+#pragma unroll
+    for (int g = 1; g < GROUPS; ++g) {
+        const float4 v = part[g][dim];
+        x = make_float4(x.x + v.x, x.y + v.y, x.z + v.z, x.w + v.w);
+    }
+    const float f = total == 0.f ? 0.f : 1.f / total;
+    *reinterpret_cast<uint2*>(p.att + (size_t)blockIdx.x * D + 4 * dim) = make_uint2(f32x2_bf16(x.x * f, x.y * f), f32x2_bf16(x.z * f, x.w * f));
+    if (dim == 0) kv4_lse(p, blockIdx.x, top, total);
 }
 
 // How a call is cut, from what the host knows: tiles of pairs a sequence, and spans.
@@ -555,7 +596,7 @@ static Kv4Plan kv4_plan(size_t T, size_t B, size_t Hk, size_t G, size_t keys_cap
     size_t S = want < 1 ? 1 : want;
     const size_t most = tiles < least ? 1 : tiles / least;
     if (S > most) S = most;
-    if (S > 256) S = 256;
+    if (S > (size_t)MOST_SPANS) S = MOST_SPANS;
     plan.S = (int)S;
     plan.span = (int)((tiles + S - 1) / S);
     if (plan.span < (int)least) plan.span = (int)least;
@@ -571,10 +612,10 @@ static int32_t launch_attn_kv4(const AttnKv4& p, const Kv4Plan& plan, hipStream_
     const int32_t done = hip_status(hipGetLastError(), "attn_kv4 launch");
     if (done != OK || plan.S == 1) return done;
     const unsigned pairs = (unsigned)(p.seqs.T * p.Hq);
-    if (plan.S >= 16)  // (one wave a pair takes its spans four at a time)
-        hipLaunchKernelGGL((attn_kv4_join_kernel<D, 4>), dim3(pairs), dim3(256), 0, st, p);
+    if (plan.S >= 16)
+        hipLaunchKernelGGL(attn_kv4_join_many<D>, dim3(pairs), dim3(256), 0, st, p);
     else
-        hipLaunchKernelGGL((attn_kv4_join_kernel<D, 1>), dim3((pairs + 3) / 4), dim3(256), 0, st, p);
+        hipLaunchKernelGGL(attn_kv4_join_few<D>, dim3((pairs + 3) / 4), dim3(256), 0, st, p);
     return hip_status(hipGetLastError(), "attn_kv4 join launch");
 }
 
