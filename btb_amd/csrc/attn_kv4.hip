@@ -145,14 +145,22 @@ struct TileWords {
     uint4 k[STEPS], v[STEPS];
     uint32_t e;
 
+    // ONCE: no other workgroup reads the tile
+    template <bool ONCE>
+    __device__ __forceinline__ static uint4 piece(const uint8_t* at, int i) {
+        const uint4* from = reinterpret_cast<const uint4*>(at) + i;
+        return ONCE ? load_stream16(from) : *from;
+    }
+    template <bool ONCE>
     __device__ __forceinline__ void load_k(const uint8_t* tile, int lane) {
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) k[i] = reinterpret_cast<const uint4*>(tile)[64 * i + lane];
+        for (int i = 0; i < STEPS; ++i) k[i] = piece<ONCE>(tile, 64 * i + lane);
         e = D == 128 ? reinterpret_cast<const uint16_t*>(tile + Tile::KS)[lane] : tile[Tile::KS + lane];
     }
+    template <bool ONCE>
     __device__ __forceinline__ void load_v(const uint8_t* tile, int lane) {
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) v[i] = reinterpret_cast<const uint4*>(tile + Tile::V)[64 * i + lane];
+        for (int i = 0; i < STEPS; ++i) v[i] = piece<ONCE>(tile + Tile::V, 64 * i + lane);
     }
     // K's operand of product j: 8 dims of the lane's 32. (The conversion reads the exponent's field alone: 0 is 2^-127, 255 makes of
     // the zeros that go with it NaN.)
@@ -317,7 +325,7 @@ __device__ __forceinline__ void kv4_meet(const AttnKv4& p, const KvSpan& a, cons
 }
 
 // its four waves' batches of NG tiles, dealt out in turn; the columns meet in LDS
-template <int D, int NG>
+template <int D, int NG, bool ONCE>
 __device__ __forceinline__ void kv4_span(const AttnKv4& p, const KvSpan& a, Meet<D>& meet) {
     constexpr int DT = D / 32, COLUMNS = PAIRS / NG;
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -350,11 +358,11 @@ __device__ __forceinline__ void kv4_span(const AttnKv4& p, const KvSpan& a, Meet
     };
     auto request_k = [&](long long x, int i) {
 #pragma unroll
-        for (int t = 0; t < NG; ++t) w.t[t].load_k(p.cache + max(take(x, i + t), 0ll), lane);
+        for (int t = 0; t < NG; ++t) w.t[t].template load_k<ONCE>(p.cache + max(take(x, i + t), 0ll), lane);
     };
     auto request_v = [&](long long x, int i) {
 #pragma unroll
-        for (int t = 0; t < NG; ++t) w.t[t].load_v(p.cache + max(take(x, i + t), 0ll), lane);
+        for (int t = 0; t < NG; ++t) w.t[t].template load_v<ONCE>(p.cache + max(take(x, i + t), 0ll), lane);
         w.s.load(p.cache + max(give(x, i), 0ll) + Kv4Tile<D>::VS, lane);
     };
     if (from < a.to) {
@@ -435,13 +443,16 @@ __global__ void __launch_bounds__(256, 2) attn_kv4_kernel(AttnKv4 p) {
     const int any = a.len - a.n + last / p.G + 1;
     a.from = a.span * length;
     a.to = min(min(a.from + length, tiles), (any + KV4_TOKENS - 1) / KV4_TOKENS);
-    // few pairs: several tiles at a time. At head_dim 128 four of them do not fit the registers: 131072 tokens of one row 33 us by two,
-    // 37 by one, 51 by four; 56 rows of 5 + 8 heads x 64 over 3001 15.2 by four, 16.4 by two, 17.0 by one
+    // Few pairs: several tiles at a time. At head_dim 128 four of them do not fit the registers: 131072 tokens of one row 36 us by two,
+    // 38 by one, 62 by four; 64 sequences of up to 8192 80, 96 and 137. Tiles that this workgroup alone reads are not kept in the caches: 36 -> 33 and
+    // 80 -> 76, but 61 -> 65 for prompts beside single tokens where others read them too.
     constexpr int NG = D == 64 ? 4 : 2;
-    if (a.pairs - a.pair0 <= PAIRS / NG)
-        kv4_span<D, NG>(p, a, meet);
+    if (a.pairs <= PAIRS / NG)
+        kv4_span<D, NG, true>(p, a, meet);
+    else if (a.pairs - a.pair0 <= PAIRS / NG)
+        kv4_span<D, NG, false>(p, a, meet);
     else
-        kv4_span<D, 1>(p, a, meet);
+        kv4_span<D, 1, false>(p, a, meet);
 }
 
 // A row's spans, and where they lie: false where it has none, or one, which has made its outputs itself
