@@ -9,9 +9,9 @@
 // (pair, h)'s own, and V lies in the same order: out^T += V^T P by v_mfma_f32_32x32x16_f16, the codes as f16, which they are exactly,
 // a value's scale in its weight.
 //
-// Weights are f16, off by 2^-12 of themselves at most: e^(s - maximum) times 2^11 times the value's scale over the power of two `unit`, the
+// Weights are f16, off by 2^-11 of themselves at most: e^(s - maximum) times 2^11 times the value's scale over the power of two `unit`, the
 // largest one so far: at most 2^15 (the maximum may lag by 2^4), in full precision down to 2^-25 of the largest, and 2^-36 of it is lost at most. A
-// bf16 weight would be off by 2^-9, two of them cost twice the products. The unit in the maximum instead of in the scales would save a product
+// bf16 weight would be off by 2^-8, two of them cost twice the products. The unit in the maximum instead of in the scales would save a product
 // a weight (1 % of the time), but not the last bits of lse.
 
 #include "btb_kv4.hpp"
@@ -655,7 +655,7 @@ extern "C" int32_t btb_hip_attn_kv4(const void* q, const void* cache, const int3
     auto loose = [](const void* a) { return ((uintptr_t)a & 15u) != 0; };
     AttnKv4 p{};
     if (!kv4_seqs(p.seqs, tables, lens, first, B, W, pages, page, stride, T, Hk, D) ||
-        btb_hip_attn_kv4_floats(T, B, Hq, Hk, D, keys_cap) == 0 || T * Hq > (1u << 24) || !(scale > 0.f) || loose(q) || loose(cache) || loose(att) ||
+        btb_hip_attn_kv4_floats(T, B, Hq, Hk, D, keys_cap) == 0 || T * Hq > (1u << 24) || !(scale > 0.f) || scale > 3.4e38f || loose(q) || loose(cache) || loose(att) ||
         loose(workspace)) {
         set_error("attn_kv4: " KV4_DOMAIN ", up to 64 query heads a kv head, 2^24 rows times query heads, scale > 0, keys_cap 1 .. 2^30; "
                   "q, cache, att and workspace 16-byte aligned");

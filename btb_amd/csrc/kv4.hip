@@ -1,6 +1,6 @@
 // New rows of keys and values into a paged cache held in 4 bits (btb_kv4.hpp), and cached rows back as the values they stand for.
 //
-//   K, 32 dims of a token and head:  e = the smallest with max |k| <= 7 2^e, code = e2m1(k / 2^e)    (an infinity or NaN: all 32 NaN)
+//   K, 32 dims of a token and head:  e = the smallest with max |k| <= 7 2^e (-127 .. 125), code = e2m1(k / 2^e)    (an infinity or NaN: all 32 NaN)
 //   V, a token and head:             s = bf16(max |v| / 6), code = e2m1(v / s), s = 0: 0             (an infinity or NaN: all of it NaN)
 //
 // e2m1: 0, 1/2, 1, 3/2, 2, 3, 4, 6, the nearest, a tie to the even code, 7 to 6. Keys keep a power of two a block, which the
@@ -120,10 +120,11 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(Kv4Rows p) {
         top = umax(top, dpp_u32<0xB1>(top));
         top = umax(top, dpp_u32<0x4E>(top));
         const bool lost = top >= 0x7F80u;
-        // the exponent of bf16's own field; 1 3/4 is the largest mantissa that the power two below it still holds
-        const int e = max((int)(top >> 7) - 2 + ((top & 0x7Fu) > 0x60u ? 1 : 0), 0);
+        // the exponent of bf16's own field; 1 3/4 is the largest mantissa that the power two below it still holds (up to 2^125: six of
+        // it are a number yet)
+        const int e = min(max((int)(top >> 7) - 2 + ((top & 0x7Fu) > 0x60u ? 1 : 0), 0), 252);
         widen8(k, y);
-        const float down = bits_f32((uint32_t)(254 - min(e, 253)) << 23);
+        const float down = bits_f32((uint32_t)(254 - e) << 23);
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] *= down;
         const int piece = c / 8 * 64 + c / 4 % 2 * 32 + token;
@@ -294,6 +295,15 @@ extern "C" int32_t btb_hip_kv4_read(const void* cache, const int32_t* tables, co
     const int32_t rc = kv4_rows(p, cache, tables, lens, first, B, W, pages, page, stride, T, Hk, D, k_row, k_head, v_row, v_head, k, v,
                                 "kv4_read: " KV4_DOMAIN "; k, v and cache 16-byte aligned, strides in multiples of 8");
     if (rc != OK) return rc;
+    // rows or heads in one place
+    auto shared = [&](int64_t row, int64_t head) {
+        return (T > 1 && row < (int64_t)D) || (Hk > 1 && head < (int64_t)D) ||
+               (T > 1 && Hk > 1 && row < (int64_t)Hk * head && head < (int64_t)T * row);
+    };
+    if (shared(k_row, k_head) || shared(v_row, v_head)) {
+        set_error("kv4_read: rows or heads of an output share memory");
+        return ERR_DOMAIN;
+    }
     p.k_out = k;
     p.v_out = v;
     hipStream_t st = static_cast<hipStream_t>(stream);

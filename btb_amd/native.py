@@ -1234,6 +1234,14 @@ class HipCard(CardLaunch):
         shape = (pages, Hk, page // 32, tile)
         return torch.zeros(shape if layers is None else (layers, *shape), dtype=torch.uint8, device=device)
 
+    @staticmethod
+    def _here(what: str, *tensors: torch.Tensor | None) -> None:
+        """the tensors lie on the current device, whose stream the kernels go to"""
+        dev = torch._C._cuda_getDevice()
+        for t in tensors:
+            if t is not None and t.get_device() != dev:
+                raise ValueError(f"[hip] {what}: the tensors are on the current device, {dev}, not on {t.get_device()}")
+
     def _kv4_seqs(self, what: str, cache: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, first: torch.Tensor | None, T: int,
                   Hk: int, D: int) -> tuple[int, int, int, int, int]:
         """a layer's pool, the tables and the lengths of a call: sequences, entries each, pages, tokens a page, bytes between pages"""
@@ -1246,6 +1254,7 @@ class HipCard(CardLaunch):
                 and cache.shape[1] == Hk and cache.shape[3] == self.lib.btb_hip_kv4_tile_bytes(D) and cache[0].is_contiguous()):
             raise ValueError(f"[hip] {what}: the cache is one layer's pool, uint8 [pages, {Hk}, page / 32, tile bytes] (kv4_pool), whole "
                              "pages contiguous")
+        self._here(what, cache, tables, lens, first)
         B, W = tables.shape
         if T < 1 or (first is None and T % B):
             raise ValueError(f"[hip] {what}: {T} rows are not as many for each of {B} sequences: say which with first")
@@ -1268,6 +1277,7 @@ class HipCard(CardLaunch):
         not the pool's is not written; two sequences write to no common page."""
         T, Hk, D = self._kv4_rows("kv4_write", k, v, (torch.bfloat16,))
         B, W, pages, page, stride = self._kv4_seqs("kv4_write", cache, tables, lens, first, T, Hk, D)
+        self._here("kv4_write", k, v)
         self._call("btb_hip_kv4_write", k.data_ptr(), v.data_ptr(), cache.data_ptr(), tables.data_ptr(), lens.data_ptr(),
                    None if first is None else first.data_ptr(), B, W, pages, page, stride, T, Hk, D, k.stride(0), k.stride(1),
                    v.stride(0), v.stride(1), _stream())
@@ -1278,9 +1288,7 @@ class HipCard(CardLaunch):
         other way round. Zeros where the page is not the pool's."""
         T, Hk, D = self._kv4_rows("kv4_read", k, v, (torch.float32, torch.bfloat16))
         B, W, pages, page, stride = self._kv4_seqs("kv4_read", cache, tables, lens, first, T, Hk, D)
-        for t in (k, v):
-            if (t.stride(0) == 0 and T > 1) or (t.stride(1) == 0 and Hk > 1):
-                raise ValueError("[hip] kv4_read: rows or heads of k or v share memory")
+        self._here("kv4_read", k, v)
         self._call("btb_hip_kv4_read", cache.data_ptr(), tables.data_ptr(), lens.data_ptr(),
                    None if first is None else first.data_ptr(), B, W, pages, page, stride, T, Hk, D, k.data_ptr(), v.data_ptr(),
                    k.dtype is torch.float32, k.stride(0), k.stride(1), v.stride(0), v.stride(1), _stream())
@@ -1306,6 +1314,7 @@ class HipCard(CardLaunch):
         if q.numel() != T * Hq * D or att.numel() != q.numel() or (lse is not None and lse.numel() != T * Hq):
             raise ValueError("[hip] attn_kv4: q and att are [T, Hq D], lse [T, Hq]")
         B, W, pages, page, stride = self._kv4_seqs("attn_kv4", cache, tables, lens, first, T, Hk, D)
+        self._here("attn_kv4", q, att, lse, scratch)
         keys = keys_cap if keys_cap > 0 else W * page
         need = self.lib.btb_hip_attn_kv4_floats(T, B, Hq, Hk, D, keys)
         if scratch.numel() < need:
@@ -1321,6 +1330,7 @@ class HipCard(CardLaunch):
         if not (self._plain(tables, torch.int32) and tables.dim() == 2 and self._plain(lens, torch.int32)
                 and lens.numel() == tables.shape[0]):
             raise ValueError(f"[hip] {what}: tables int32 [sequences, entries] and lens int32 [sequences], contiguous on the GPU")
+        self._here(what, pool, tables, lens)
         L, pages, size = pool.shape[0], pool.shape[1], pool.element_size()
         nb = pool[0, 0].numel() * size
         stride = pool.stride(1) * size if pages > 1 else nb
@@ -1336,6 +1346,7 @@ class HipCard(CardLaunch):
         for t in (src, dst, fresh):
             if not self._plain(t, torch.int32) or t.numel() != F:
                 raise ValueError("[hip] pages_fork: src, dst and fresh are int32, as many of each, contiguous on the GPU")
+        self._here("pages_fork", src, dst, fresh)
         self._call("btb_hip_pages_fork", at, L, pages, nb, layer, stride, tables.data_ptr(), lens.data_ptr(), B, W, page, src.data_ptr(),
                    dst.data_ptr(), fresh.data_ptr(), F, _stream())
 
@@ -1348,6 +1359,7 @@ class HipCard(CardLaunch):
         out = tables if tables_out is None else tables_out
         if not self._plain(out, torch.int32) or out.shape != tables.shape:
             raise ValueError("[hip] pages_compact: tables_out is like tables")
+        self._here("pages_compact", out)
         words = self.lib.btb_hip_pages_compact_words(pages)
         ws = torch.empty(words + 1, dtype=torch.int32, device=pool.device)
         used = ws[words:]

@@ -525,7 +525,7 @@ int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t* pos, int6
  * The rows of a pass are its sequences' last ones: rows first[b] .. first[b + 1] - 1 (i32 [B + 1] on the device, ascending) are
  * sequence b's, T / B a sequence where first is NULL; row i of n stands at lens[b] - n + i, and rows at places below 0 or behind the last
  * sequence's are left alone. All of it is read on the device: a recorded call replays over longer sequences and other tables.
- * A key is held as e2m1 codes with a power of two for 32 dims, the smallest e with max |k| <= 7 2^e (MXFP4: btb_hip_mx4_widen), a value as
+ * A key is held as e2m1 codes with a power of two for 32 dims, the smallest e of -127 .. 125 with max |k| <= 7 2^e (MXFP4: btb_hip_mx4_widen), a value as
  * e2m1 codes with one scale, bf16(max |v| / 6); codes are the nearest, ties to even. An infinity or NaN makes all that its scale is for
  * NaN. D 64 or 128; cache 16-byte aligned, stride a multiple of 16; B up to 65536, T up to 2^24, Hk up to 1024, W page up to 2^30. No
  * counterpart in the reference. */
@@ -540,7 +540,7 @@ int32_t btb_hip_kv4_write(const void* k, const void* v, void* cache, const int32
                           size_t Hk, size_t D, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, void* stream);
 
 /* The pass's rows as the cache holds them: into k and v, laid out as above, f32 (out_f32 != 0) or, rounded, bf16. A row in a page
- * outside the pool reads as zeros. */
+ * outside the pool reads as zeros. Rows and heads of an output must not share memory. */
 int32_t btb_hip_kv4_read(const void* cache, const int32_t* tables, const int32_t* lens, const int32_t* first, size_t B,
                          size_t W, size_t pages, size_t page, int64_t stride, size_t T, size_t Hk, size_t D, void* k, void* v,
                          int32_t out_f32, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, void* stream);
@@ -548,8 +548,8 @@ int32_t btb_hip_kv4_read(const void* cache, const int32_t* tables, const int32_t
 /* Attention of the pass's rows, q [T, Hq D] bf16, each over its sequence's tokens up to its own place: att [T, Hq D] bf16 and, where lse is
  * not NULL, the rows' log-sum-exp [T, Hq] f32 (natural units, of scale q . k). A row with no token to see gets zeros and -inf. keys_cap: about how
  * many tokens the longest sequence has; it sizes the launch and the workspace (btb_hip_attn_kv4_floats of them, this call's own; 0: the sizes are
- * refused), a longer sequence takes longer. Sums are f32; a weight goes to the product with V to 2^-12 of itself (or 2^-36 of the largest, times
- * their values' scales). Hq / Hk up to 64, T Hq up to 2^24, scale > 0; q, cache, att and workspace 16-byte aligned. */
+ * refused), a longer sequence takes longer. Sums are f32; a weight goes to the product with V as f16, to 2^-11 of itself (or 2^-36 of the largest,
+ * both times their values' scales). Hq / Hk up to 64, T Hq up to 2^24, scale > 0; q, cache, att and workspace 16-byte aligned. */
 size_t btb_hip_attn_kv4_floats(size_t T, size_t B, size_t Hq, size_t Hk, size_t D, size_t keys_cap);
 int32_t btb_hip_attn_kv4(const void* q, const void* cache, const int32_t* tables, const int32_t* lens, const int32_t* first,
                          void* att, float* lse, size_t B, size_t W, size_t pages, size_t page, int64_t stride, size_t T, size_t Hq,
