@@ -42,11 +42,12 @@ struct AttnKv4 {
     float c;         // scale log2(e)
     int Hq, Hk, G;
     int items;       // tiles of pairs a sequence, where each has as many rows
-    int S, span;     // spans a sequence at most, tiles a span at least
+    int S;           // spans a sequence at most
 };
 
-// spans of a sequence of `tiles` tiles: how many, and how long
-__device__ __forceinline__ int kv4_span_tiles(const AttnKv4& p, int tiles) { return max(p.span, (tiles + p.S - 1) / p.S); }
+// tiles a span of a sequence of `tiles`, each span but the last: what S spans come to, a batch a wave at least
+constexpr int LEAST = 16;
+__device__ __forceinline__ int kv4_span_tiles(const AttnKv4& p, int tiles) { return max(LEAST, (tiles + p.S - 1) / p.S); }
 
 // q's fragment, exact: 8 dims a product, lane (pair, h) dims 64 step + 32 h + 8 j .. + 7 of the pair's row for product j of a step, as K's
 // codes lie (the order of the dims is free as long as both operands have it)
@@ -593,24 +594,21 @@ __global__ void __launch_bounds__(256) attn_kv4_join_many(AttnKv4 p) {
 struct Kv4Plan {
     int items;        // workgroups a sequence, where each has as many rows
     long long groups; // workgroups a kv head and span
-    int S, span;
+    int S;
 };
 static Kv4Plan kv4_plan(size_t T, size_t B, size_t Hk, size_t G, size_t keys_cap, bool ragged) {
     Kv4Plan plan;
     plan.items = (int)((T / B * G + PAIRS - 1) / PAIRS);
     plan.groups = (long long)(ragged ? T * G / PAIRS + B : B * plan.items);
     const size_t tiles = (keys_cap + KV4_TOKENS - 1) / KV4_TOKENS;
-    const size_t least = 16;  // tiles a span at least: a batch a wave
     // two workgroups a CU, as many as fit (131072 tokens of one row: 32 us, 37 with three, 44 with six; without a second round 500 rows over
     // 16384 are 175 instead of 183)
     const size_t want = (size_t)2 * device_info().cus / (plan.groups * Hk);
     size_t S = want < 1 ? 1 : want;
-    const size_t most = tiles < least ? 1 : tiles / least;
+    const size_t most = tiles < LEAST ? 1 : tiles / LEAST;
     if (S > most) S = most;
     if (S > (size_t)MOST_SPANS) S = MOST_SPANS;
     plan.S = (int)S;
-    plan.span = (int)((tiles + S - 1) / S);
-    if (plan.span < (int)least) plan.span = (int)least;
     return plan;
 }
 
@@ -669,7 +667,7 @@ extern "C" int32_t btb_hip_attn_kv4(const void* q, const void* cache, const int3
     p.part = workspace;
     p.c = scale * LOG2E;
     p.Hq = (int)Hq, p.Hk = (int)Hk, p.G = (int)(Hq / Hk);
-    p.items = plan.items, p.S = plan.S, p.span = plan.span;
+    p.items = plan.items, p.S = plan.S;
     hipStream_t st = static_cast<hipStream_t>(stream);
     return D == 64 ? launch_attn_kv4<64>(p, plan, st) : launch_attn_kv4<128>(p, plan, st);
 }

@@ -5,7 +5,7 @@
 //
 // e2m1: 0, 1/2, 1, 3/2, 2, 3, 4, 6, the nearest, a tie to the even code, 7 to 6. Keys keep a power of two a block, which the
 // matrix cores apply; a value's scale is a whole token's and goes into its weight, and with bf16's eight bits nothing of the codes' range is
-// lost to a power of two. Quotients are f32's: two bf16 numbers' quotient is on the same side of every border as the exact one.
+// lost to a power of two.
 //
 // A workgroup a tile of 32 tokens and a head: whoever writes one of two tokens that share V's bytes writes both. Bound: memory for many rows,
 // the launch for few.
@@ -137,8 +137,14 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(Kv4Rows p) {
         if (CH == 16) top = umax(top, dpp_u32<0x140>(top));
         const uint16_t s = top >= 0x7F80u ? KV4_NAN : f32_bf16(bf16_f32((uint16_t)top) / 6.f);
         widen8(v, y);
+        // the quotient by the reciprocal, and what that leaves by it once more: a tie comes out as one, and no other quotient of two bf16 numbers is
+        // nearer to one than 2^-12 of it (small scales times 2^64, for their reciprocals' sake)
+        const float up = (s & 0x7FFFu) < 0x2000u ? bits_f32(191u << 23) : 1.f, scale = bf16_f32(s) * up, by = __builtin_amdgcn_rcpf(scale);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = y[j] / bf16_f32(s);
+        for (int j = 0; j < 8; ++j) {
+            const float x = y[j] * up, z = x * by;
+            y[j] = fmaf(fmaf(-z, scale, x), by, z);
+        }
         v_code[token][c] = s == 0 || s == KV4_NAN ? 0u : codes8(y);
         if (c == 0) v_scale[kv4_half(token) * 16 + kv4_index(token)] = s;
     }
