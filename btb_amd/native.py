@@ -185,6 +185,7 @@ def _split_pays(R: int, C: int, M: int) -> bool:
     return M * C >= (122880 if C <= 4096 else 86016) or (M > 16 and C > 4096) or R * C >= 1 << 24
 
 
+_KV4_TILE = {64: 2176, 128: 4288}  # btb_hip_kv4_tile_bytes
 _ARGMAX_EAGER = 163840  # logits a row from which an eager argmax gains by the many workgroups
 
 
@@ -1228,7 +1229,7 @@ class HipCard(CardLaunch):
 
     def kv4_pool(self, pages: int, Hk: int, D: int, page: int = 64, layers: int | None = None, device: Any = "cuda") -> torch.Tensor:
         """an empty pool for `kv4_write`: uint8 [pages, Hk, page / 32, tile bytes], with `layers` of them in front where given"""
-        tile = int(self.lib.btb_hip_kv4_tile_bytes(D))
+        tile = _KV4_TILE.get(D, 0)
         if tile == 0 or page < 32 or page % 32 or pages < 1 or Hk < 1:
             raise ValueError(f"[hip] kv4_pool: head_dim 64 or 128, pages of a multiple of 32 tokens, got {D} and {page}")
         shape = (pages, Hk, page // 32, tile)
@@ -1246,29 +1247,33 @@ class HipCard(CardLaunch):
                   Hk: int, D: int) -> tuple[int, int, int, int, int]:
         """a layer's pool, the tables and the lengths of a call: sequences, entries each, pages, tokens a page, bytes between pages"""
         i32 = torch.int32
-        if not (self._plain(tables, i32) and tables.dim() == 2 and self._plain(lens, i32) and lens.numel() == tables.shape[0]
-                and (first is None or (self._plain(first, i32) and first.numel() == tables.shape[0] + 1))):
+        if not (self._plain(tables, i32) and tables.dim() == 2 and self._plain(lens, i32)
+                and (first is None or self._plain(first, i32))):
             raise ValueError(f"[hip] {what}: tables int32 [sequences, entries], lens [sequences] and first [sequences + 1] or None, "
                              "contiguous on the GPU")
-        if not (isinstance(cache, _Tensor) and cache.dtype is torch.uint8 and cache.is_cuda and cache.dim() == 4
-                and cache.shape[1] == Hk and cache.shape[3] == self.lib.btb_hip_kv4_tile_bytes(D) and cache[0].is_contiguous()):
+        B, W = tables.shape
+        if lens.numel() != B or (first is not None and first.numel() != B + 1):
+            raise ValueError(f"[hip] {what}: lens is [{B}] and first [{B + 1}] or None, as tables has them")
+        if not (isinstance(cache, _Tensor) and cache.dtype is torch.uint8 and cache.is_cuda and cache.dim() == 4):
+            raise ValueError(f"[hip] {what}: the cache is a layer's pool, uint8 on the GPU (kv4_pool)")
+        pages, heads, tiles, tile = cache.shape
+        stride, by_head, by_tile, by_byte = cache.stride()
+        if heads != Hk or tile != _KV4_TILE.get(D) or by_byte != 1 or by_tile != tile or by_head != tiles * tile:
             raise ValueError(f"[hip] {what}: the cache is one layer's pool, uint8 [pages, {Hk}, page / 32, tile bytes] (kv4_pool), whole "
                              "pages contiguous")
         self._here(what, cache, tables, lens, first)
-        B, W = tables.shape
         if T < 1 or (first is None and T % B):
             raise ValueError(f"[hip] {what}: {T} rows are not as many for each of {B} sequences: say which with first")
-        pages = cache.shape[0]
-        return B, W, pages, 32 * cache.shape[2], cache.stride(0) if pages > 1 else cache[0].numel()
+        return B, W, pages, 32 * tiles, stride if pages > 1 else heads * by_head
 
     @staticmethod
     def _kv4_rows(what: str, k: torch.Tensor, v: torch.Tensor, dtypes: tuple[torch.dtype, ...]) -> tuple[int, int, int]:
-        for t in (k, v):
-            if not (isinstance(t, _Tensor) and t.dtype is k.dtype and t.dtype in dtypes and t.is_cuda and t.dim() == 3
-                    and t.shape == k.shape and t.stride(2) == 1):
-                raise ValueError(f"[hip] {what}: k and v are [rows, kv heads, head_dim] views of one type on the GPU, {dtypes}, head_dim "
-                                 "contiguous")
-        return k.shape[0], k.shape[1], k.shape[2]
+        if not (isinstance(k, _Tensor) and isinstance(v, _Tensor) and k.dtype in dtypes and v.dtype is k.dtype and k.is_cuda and v.is_cuda
+                and k.dim() == 3 and v.shape == k.shape and k.stride(2) == 1 and v.stride(2) == 1):
+            raise ValueError(f"[hip] {what}: k and v are [rows, kv heads, head_dim] views of one type on the GPU, {dtypes}, head_dim "
+                             "contiguous")
+        T, Hk, D = k.shape
+        return T, Hk, D
 
     def kv4_write(self, k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor,
                   first: torch.Tensor | None = None) -> None:
