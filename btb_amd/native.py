@@ -1235,68 +1235,66 @@ class HipCard(CardLaunch):
         shape = (pages, Hk, page // 32, tile)
         return torch.zeros(shape if layers is None else (layers, *shape), dtype=torch.uint8, device=device)
 
+    # (these checks stand before launches of 3 us: what they read of a tensor is read once, and pages are looked over by their strides)
     @staticmethod
-    def _here(what: str, *tensors: torch.Tensor | None) -> None:
-        """the tensors lie on the current device, whose stream the kernels go to"""
-        dev = torch._C._cuda_getDevice()
-        for t in tensors:
-            if t is not None and t.get_device() != dev:
-                raise ValueError(f"[hip] {what}: the tensors are on the current device, {dev}, not on {t.get_device()}")
+    def _mine(t: Any, dtype: torch.dtype, dev: int) -> bool:
+        """whether t is a contiguous tensor of this type on this GPU"""
+        return isinstance(t, _Tensor) and t.dtype is dtype and t.get_device() == dev and t.is_contiguous()
 
-    def _kv4_seqs(self, what: str, cache: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, first: torch.Tensor | None, T: int,
-                  Hk: int, D: int) -> tuple[int, int, int, int, int]:
+    def _kv4_seqs(self, what: str, dev: int, cache: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, first: torch.Tensor | None,
+                  T: int, Hk: int, D: int) -> tuple[int, int, int, int, int]:
         """a layer's pool, the tables and the lengths of a call: sequences, entries each, pages, tokens a page, bytes between pages"""
-        i32 = torch.int32
-        if not (self._plain(tables, i32) and tables.dim() == 2 and self._plain(lens, i32)
-                and (first is None or self._plain(first, i32))):
+        i32, mine = torch.int32, self._mine
+        if not (mine(tables, i32, dev) and tables.dim() == 2 and mine(lens, i32, dev) and (first is None or mine(first, i32, dev))):
             raise ValueError(f"[hip] {what}: tables int32 [sequences, entries], lens [sequences] and first [sequences + 1] or None, "
-                             "contiguous on the GPU")
+                             "contiguous on the current GPU")
         B, W = tables.shape
         if lens.numel() != B or (first is not None and first.numel() != B + 1):
             raise ValueError(f"[hip] {what}: lens is [{B}] and first [{B + 1}] or None, as tables has them")
-        if not (isinstance(cache, _Tensor) and cache.dtype is torch.uint8 and cache.is_cuda and cache.dim() == 4):
-            raise ValueError(f"[hip] {what}: the cache is a layer's pool, uint8 on the GPU (kv4_pool)")
+        if not (isinstance(cache, _Tensor) and cache.dtype is torch.uint8 and cache.get_device() == dev and cache.dim() == 4):
+            raise ValueError(f"[hip] {what}: the cache is a layer's pool, uint8 on the current GPU (kv4_pool)")
         pages, heads, tiles, tile = cache.shape
         stride, by_head, by_tile, by_byte = cache.stride()
         if heads != Hk or tile != _KV4_TILE.get(D) or by_byte != 1 or by_tile != tile or by_head != tiles * tile:
             raise ValueError(f"[hip] {what}: the cache is one layer's pool, uint8 [pages, {Hk}, page / 32, tile bytes] (kv4_pool), whole "
                              "pages contiguous")
-        self._here(what, cache, tables, lens, first)
         if T < 1 or (first is None and T % B):
             raise ValueError(f"[hip] {what}: {T} rows are not as many for each of {B} sequences: say which with first")
         return B, W, pages, 32 * tiles, stride if pages > 1 else heads * by_head
 
     @staticmethod
-    def _kv4_rows(what: str, k: torch.Tensor, v: torch.Tensor, dtypes: tuple[torch.dtype, ...]) -> tuple[int, int, int]:
-        if not (isinstance(k, _Tensor) and isinstance(v, _Tensor) and k.dtype in dtypes and v.dtype is k.dtype and k.is_cuda and v.is_cuda
-                and k.dim() == 3 and v.shape == k.shape and k.stride(2) == 1 and v.stride(2) == 1):
-            raise ValueError(f"[hip] {what}: k and v are [rows, kv heads, head_dim] views of one type on the GPU, {dtypes}, head_dim "
-                             "contiguous")
-        T, Hk, D = k.shape
-        return T, Hk, D
+    def _kv4_rows(what: str, dev: int, k: torch.Tensor, v: torch.Tensor, f32: bool) -> tuple[tuple[int, ...], tuple[int, ...], tuple[int, ...]]:
+        """k's and v's common shape [rows, kv heads, head_dim] and their strides"""
+        if not (isinstance(k, _Tensor) and isinstance(v, _Tensor) and k.dtype is v.dtype
+                and (k.dtype is torch.bfloat16 or (f32 and k.dtype is torch.float32)) and k.get_device() == dev and v.get_device() == dev):
+            raise ValueError(f"[hip] {what}: k and v are both bfloat16{' or both float32' if f32 else ''}, on the current GPU")
+        shape, ks, vs = k.shape, k.stride(), v.stride()
+        if len(shape) != 3 or v.shape != shape or ks[2] != 1 or vs[2] != 1:
+            raise ValueError(f"[hip] {what}: k and v are [rows, kv heads, head_dim] views of one shape, head_dim contiguous")
+        return shape, ks, vs
 
     def kv4_write(self, k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor,
                   first: torch.Tensor | None = None) -> None:
         """the pass's rows k, v (bfloat16 [T, Hk, D] views) into a layer's pool (`kv4_pool`) in 4 bits: rows first[b] .. first[b + 1] - 1
         (None: T / B each) are the last ones of sequence b, which has lens[b] tokens with them in pages tables[b]. A row whose page is
         not the pool's is not written; two sequences write to no common page."""
-        T, Hk, D = self._kv4_rows("kv4_write", k, v, (torch.bfloat16,))
-        B, W, pages, page, stride = self._kv4_seqs("kv4_write", cache, tables, lens, first, T, Hk, D)
-        self._here("kv4_write", k, v)
+        dev = torch._C._cuda_getDevice()
+        (T, Hk, D), ks, vs = self._kv4_rows("kv4_write", dev, k, v, False)
+        B, W, pages, page, stride = self._kv4_seqs("kv4_write", dev, cache, tables, lens, first, T, Hk, D)
         self._call("btb_hip_kv4_write", k.data_ptr(), v.data_ptr(), cache.data_ptr(), tables.data_ptr(), lens.data_ptr(),
-                   None if first is None else first.data_ptr(), B, W, pages, page, stride, T, Hk, D, k.stride(0), k.stride(1),
-                   v.stride(0), v.stride(1), _stream())
+                   None if first is None else first.data_ptr(), B, W, pages, page, stride, T, Hk, D, ks[0], ks[1], vs[0],
+                   vs[1], torch._C._cuda_getCurrentRawStream(dev))
 
     def kv4_read(self, cache: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                  first: torch.Tensor | None = None) -> None:
         """the pass's rows as the cache holds them, into k and v [T, Hk, D] (views; float32, exact, or bfloat16): `kv4_write`'s
         other way round. Zeros where the page is not the pool's."""
-        T, Hk, D = self._kv4_rows("kv4_read", k, v, (torch.float32, torch.bfloat16))
-        B, W, pages, page, stride = self._kv4_seqs("kv4_read", cache, tables, lens, first, T, Hk, D)
-        self._here("kv4_read", k, v)
+        dev = torch._C._cuda_getDevice()
+        (T, Hk, D), ks, vs = self._kv4_rows("kv4_read", dev, k, v, True)
+        B, W, pages, page, stride = self._kv4_seqs("kv4_read", dev, cache, tables, lens, first, T, Hk, D)
         self._call("btb_hip_kv4_read", cache.data_ptr(), tables.data_ptr(), lens.data_ptr(),
                    None if first is None else first.data_ptr(), B, W, pages, page, stride, T, Hk, D, k.data_ptr(), v.data_ptr(),
-                   k.dtype is torch.float32, k.stride(0), k.stride(1), v.stride(0), v.stride(1), _stream())
+                   k.dtype is torch.float32, ks[0], ks[1], vs[0], vs[1], torch._C._cuda_getCurrentRawStream(dev))
 
     def attn_kv4_scratch(self, T: int, B: int, Hq: int, Hk: int, D: int, keys_cap: int, device: Any = "cuda") -> torch.Tensor:
         """the f32 scratch `attn_kv4` leaves its states in, at these sizes"""
@@ -1312,64 +1310,68 @@ class HipCard(CardLaunch):
         its sequence's tokens up to itself, out of a layer's pool in 4 bits; lse (float32 [T, Hq]): the rows' log-sum-exp.
         keys_cap: about how long the longest sequence is (0: as long as the tables allow); it goes into the launch's
         shape and the scratch's size only."""
-        if not (self._plain(q, torch.bfloat16) and self._plain(att, torch.bfloat16) and self._plain(scratch, torch.float32)
-                and (lse is None or self._plain(lse, torch.float32))):
-            raise ValueError("[hip] attn_kv4: q and att are bfloat16, scratch and lse float32, all contiguous on the GPU")
-        T = q.numel() // (Hq * D)
-        if q.numel() != T * Hq * D or att.numel() != q.numel() or (lse is not None and lse.numel() != T * Hq):
+        dev, mine, bf, f32 = torch._C._cuda_getDevice(), self._mine, torch.bfloat16, torch.float32
+        if not (mine(q, bf, dev) and mine(att, bf, dev) and mine(scratch, f32, dev) and (lse is None or mine(lse, f32, dev))):
+            raise ValueError("[hip] attn_kv4: q and att are bfloat16, scratch and lse float32, all contiguous on the current GPU")
+        n = q.numel()
+        T = n // max(1, Hq * D)
+        if n != T * Hq * D or att.numel() != n or (lse is not None and lse.numel() != T * Hq):
             raise ValueError("[hip] attn_kv4: q and att are [T, Hq D], lse [T, Hq]")
-        B, W, pages, page, stride = self._kv4_seqs("attn_kv4", cache, tables, lens, first, T, Hk, D)
-        self._here("attn_kv4", q, att, lse, scratch)
+        B, W, pages, page, stride = self._kv4_seqs("attn_kv4", dev, cache, tables, lens, first, T, Hk, D)
         keys = keys_cap if keys_cap > 0 else W * page
         need = self.lib.btb_hip_attn_kv4_floats(T, B, Hq, Hk, D, keys)
         if scratch.numel() < need:
             raise ValueError(f"[hip] attn_kv4: scratch holds {scratch.numel()} floats, {need} are needed")
         self._call("btb_hip_attn_kv4", q.data_ptr(), cache.data_ptr(), tables.data_ptr(), lens.data_ptr(),
                    None if first is None else first.data_ptr(), att.data_ptr(), None if lse is None else lse.data_ptr(), B, W, pages, page,
-                   stride, T, Hq, Hk, D, scale, keys, scratch.data_ptr(), _stream())
+                   stride, T, Hq, Hk, D, scale, keys, scratch.data_ptr(), torch._C._cuda_getCurrentRawStream(dev))
 
-    def _pages_of(self, what: str, pool: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor) -> tuple[int, ...]:
+    def _pages_of(self, what: str, dev: int, pool: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor) -> tuple[int, ...]:
         """the pool's address, layers, pages, bytes a page and the strides of both, in bytes; sequences and entries"""
-        if not (isinstance(pool, _Tensor) and pool.is_cuda and pool.dim() >= 3 and pool[0, 0].is_contiguous()):
-            raise ValueError(f"[hip] {what}: the pool is [layers, pages, ...] on the GPU, a page's values together")
-        if not (self._plain(tables, torch.int32) and tables.dim() == 2 and self._plain(lens, torch.int32)
+        if not (isinstance(pool, _Tensor) and pool.get_device() == dev and pool.dim() >= 3):
+            raise ValueError(f"[hip] {what}: the pool is [layers, pages, ...] on the current GPU")
+        shape, strides, size = pool.shape, pool.stride(), pool.element_size()
+        n = 1
+        for i in range(len(shape) - 1, 1, -1):
+            if strides[i] != n and shape[i] != 1:
+                raise ValueError(f"[hip] {what}: a page's values lie together")
+            n *= shape[i]
+        if not (self._mine(tables, torch.int32, dev) and tables.dim() == 2 and self._mine(lens, torch.int32, dev)
                 and lens.numel() == tables.shape[0]):
-            raise ValueError(f"[hip] {what}: tables int32 [sequences, entries] and lens int32 [sequences], contiguous on the GPU")
-        self._here(what, pool, tables, lens)
-        L, pages, size = pool.shape[0], pool.shape[1], pool.element_size()
-        nb = pool[0, 0].numel() * size
-        stride = pool.stride(1) * size if pages > 1 else nb
-        return (pool.data_ptr(), L, pages, nb, pool.stride(0) * size if L > 1 else 0, stride, *tables.shape)
+            raise ValueError(f"[hip] {what}: tables int32 [sequences, entries] and lens int32 [sequences], contiguous on the current GPU")
+        L, pages, nb = shape[0], shape[1], n * size
+        return (pool.data_ptr(), L, pages, nb, strides[0] * size if L > 1 else 0, strides[1] * size if pages > 1 else nb, *tables.shape)
 
     def pages_fork(self, pool: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
                    fresh: torch.Tensor, page: int) -> None:
         """sequences dst[f] go on from src[f] (int32 [F] on the GPU): they take over its length and whole pages of `page` tokens, and
         page fresh[f] becomes a copy of its last, partial one in every layer of the pool [layers, pages, ...] (any type). No dst is
         a src or named twice, a fresh page is in nobody's table. A fork that names a sequence or page that is not there is not made."""
-        at, L, pages, nb, layer, stride, B, W = self._pages_of("pages_fork", pool, tables, lens)
+        dev, mine, i32 = torch._C._cuda_getDevice(), self._mine, torch.int32
+        at, L, pages, nb, layer, stride, B, W = self._pages_of("pages_fork", dev, pool, tables, lens)
+        if not (mine(src, i32, dev) and mine(dst, i32, dev) and mine(fresh, i32, dev)):
+            raise ValueError("[hip] pages_fork: src, dst and fresh are int32, contiguous on the current GPU")
         F = src.numel()
-        for t in (src, dst, fresh):
-            if not self._plain(t, torch.int32) or t.numel() != F:
-                raise ValueError("[hip] pages_fork: src, dst and fresh are int32, as many of each, contiguous on the GPU")
-        self._here("pages_fork", src, dst, fresh)
+        if dst.numel() != F or fresh.numel() != F:
+            raise ValueError(f"[hip] pages_fork: src names {F} sequences, dst {dst.numel()}, fresh {fresh.numel()} pages")
         self._call("btb_hip_pages_fork", at, L, pages, nb, layer, stride, tables.data_ptr(), lens.data_ptr(), B, W, page, src.data_ptr(),
-                   dst.data_ptr(), fresh.data_ptr(), F, _stream())
+                   dst.data_ptr(), fresh.data_ptr(), F, torch._C._cuda_getCurrentRawStream(dev))
 
     def pages_compact(self, pool: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, page: int,
                       tables_out: torch.Tensor | None = None) -> torch.Tensor:
         """the pages that sequences name closed up to the pool's first ones, in every layer of the pool [layers, pages, ...]: those
         too far back go, in order, where nobody names a page. tables_out (None: tables itself): the tables as they are then, -1
         behind a sequence's pages. Returns how many pages are in use (int32 [1] on the GPU)."""
-        at, L, pages, nb, layer, stride, B, W = self._pages_of("pages_compact", pool, tables, lens)
+        dev = torch._C._cuda_getDevice()
+        at, L, pages, nb, layer, stride, B, W = self._pages_of("pages_compact", dev, pool, tables, lens)
         out = tables if tables_out is None else tables_out
-        if not self._plain(out, torch.int32) or out.shape != tables.shape:
+        if out is not tables and not (self._mine(out, torch.int32, dev) and out.shape == tables.shape):
             raise ValueError("[hip] pages_compact: tables_out is like tables")
-        self._here("pages_compact", out)
         words = self.lib.btb_hip_pages_compact_words(pages)
         ws = torch.empty(words + 1, dtype=torch.int32, device=pool.device)
         used = ws[words:]
         self._call("btb_hip_pages_compact", at, L, pages, nb, layer, stride, tables.data_ptr(), lens.data_ptr(), B, W, page,
-                   out.data_ptr(), used.data_ptr(), ws.data_ptr(), _stream())
+                   out.data_ptr(), used.data_ptr(), ws.data_ptr(), torch._C._cuda_getCurrentRawStream(dev))
         return used
 
     def silu_mul(self, gu: torch.Tensor, m: torch.Tensor) -> torch.Tensor:
