@@ -25,6 +25,7 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
+constexpr int WAVES = 4;           // waves a workgroup
 constexpr int MOST_SPANS = 256;    // a thread each where they are joined
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float NONE = -3.0e38f;   // a maximum of nothing: what is subtracted from it underflows to weight 0
@@ -41,12 +42,11 @@ struct AttnKv4 {
     float* part;     // a pair's spans: maximum and sum [T Hq, S, 2], then outputs [T Hq, S, D]
     float c;         // scale log2(e)
     int Hq, Hk, G;
-    int items;       // tiles of pairs a sequence, where each has as many rows
     int S;           // spans a sequence at most
 };
 
 // tiles a span of a sequence of `tiles`, each span but the last: what S spans come to, two a wave at least
-constexpr int LEAST = 8;
+constexpr int LEAST = 2 * WAVES;
 __device__ __forceinline__ int kv4_span_tiles(const AttnKv4& p, int tiles) { return max(LEAST, (tiles + p.S - 1) / p.S); }
 
 // q's fragment, exact: 8 dims a product, lane (pair, h) dims 64 step + 32 h + 8 j .. + 7 of the pair's row for product j of a step, as K's
@@ -288,8 +288,8 @@ struct KvSpan {
 
 template <int D>
 struct Meet {  // the columns of the four waves
-    float o[4 * PAIRS][D + 4];
-    float m[4 * PAIRS], l[4 * PAIRS];
+    float o[WAVES * PAIRS][D + 4];
+    float m[WAVES * PAIRS], l[WAVES * PAIRS];
 };
 
 // a tile of pairs' columns, of which `here` are pairs, added up; behind a barrier
@@ -297,14 +297,14 @@ template <int D, int NG>
 __device__ __forceinline__ void kv4_meet(const AttnKv4& p, const KvSpan& a, const Meet<D>& meet, int pair0, int here) {
     constexpr int COLUMNS = PAIRS / NG;
     // a thread four dims of a pair, over its 4 NG columns
-    for (int task = threadIdx.x; task < here * (D / 4); task += 256) {
+    for (int task = threadIdx.x; task < here * (D / 4); task += 64 * WAVES) {
         const int pair = task / (D / 4), dim = 4 * (task % (D / 4));
         float to = NONE, sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4 * NG; ++i) to = fmaxf(to, meet.m[i / NG * PAIRS + i % NG * COLUMNS + pair]);
+        for (int i = 0; i < WAVES * NG; ++i) to = fmaxf(to, meet.m[i / NG * PAIRS + i % NG * COLUMNS + pair]);
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < 4 * NG; ++i) {
+        for (int i = 0; i < WAVES * NG; ++i) {
             const int from_column = i / NG * PAIRS + i % NG * COLUMNS + pair;
             const float by = __builtin_amdgcn_exp2f(meet.m[from_column] - to);
             sum = fmaf(meet.l[from_column], by, sum);
@@ -341,7 +341,7 @@ __device__ __forceinline__ void kv4_span(const AttnKv4& p, const KvSpan& a, Meet
     const int own = Walk<D, NG>::group(lane);
     // places of the wave's next 64 tiles, one a lane; -1: no tile, or no page of the pool
     const int from = a.from + wave * NG;
-    constexpr int STRIDE = 4 * NG, REFILL = 64 / NG * STRIDE;
+    constexpr int STRIDE = WAVES * NG, REFILL = 64 / NG * STRIDE;
     auto places = [&](int base) {
         const int j = base + lane / NG * STRIDE + lane % NG;
         return j < a.to ? p.seqs.at(a.b, j, a.hk) : -1;
@@ -416,22 +416,32 @@ __device__ __forceinline__ void kv4_span(const AttnKv4& p, const KvSpan& a, Meet
 }
 
 template <int D>
-__global__ void __launch_bounds__(256, 2) attn_kv4_kernel(AttnKv4 p) {
+__global__ void __launch_bounds__(64 * WAVES, 2) attn_kv4_kernel(AttnKv4 p) {
     extern __shared__ float4 lds[];
     Meet<D>& meet = *reinterpret_cast<Meet<D>*>(lds);
     KvSpan a;
     a.hk = blockIdx.x % p.Hk;
     const int rest = blockIdx.x / p.Hk;
     a.span = rest % p.S;
-    int item;
-    if (p.seqs.first == nullptr)
-        a.b = rest / p.S / p.items, item = rest / p.S % p.items;
-    else
-        kv4_find(rest / p.S, p.seqs.B, a.b, item, [&](int b) {
-            int row0, n;
-            p.seqs.of(b, row0, n);
-            return (int)(((long long)n * p.G + PAIRS - 1) / PAIRS);
-        });
+    // whole tiles of pairs come before what is left of each sequence's: they take longest, and a CU gets one of them rather than two
+    // (prompts beside single tokens 58.3 -> 56.9 us; spans that cut the prompts' sequences in two cost 87: the CUs are full as it is)
+    int item, x = rest / p.S;
+    auto pairs = [&](int b) {
+        int row0, n;
+        p.seqs.of(b, row0, n);
+        return (long long)n * p.G;
+    };
+    if (p.seqs.first == nullptr) {
+        const int each = p.seqs.rows * p.G / PAIRS, whole = p.seqs.B * each;
+        a.b = x < whole ? x / each : x - whole, item = x < whole ? x % each : each;
+        if (a.b >= p.seqs.B) a.b = -1;
+    } else {
+        kv4_find(x, p.seqs.B, a.b, item, [&](int b) { return (int)(pairs(b) / PAIRS); });
+        if (a.b < 0) {
+            kv4_find(x, p.seqs.B, a.b, item, [&](int b) { return pairs(b) % PAIRS != 0 ? 1 : 0; });
+            if (a.b >= 0) item = (int)(pairs(a.b) / PAIRS);
+        }
+    }
     if (a.b < 0) return;
     a.b = __builtin_amdgcn_readfirstlane(a.b), item = __builtin_amdgcn_readfirstlane(item);
     p.seqs.of(a.b, a.row0, a.n);
@@ -590,23 +600,21 @@ __global__ void __launch_bounds__(256) attn_kv4_join_many(AttnKv4 p) {
     if (dim == 0) kv4_lse(p, blockIdx.x, top, total);
 }
 
-// How a call is cut, from what the host knows: tiles of pairs a sequence, and spans.
+// How a call is cut, from what the host knows: tiles of pairs, and spans.
 struct Kv4Plan {
-    int items;        // workgroups a sequence, where each has as many rows
     long long groups; // workgroups a kv head and span
     int S;
 };
 static Kv4Plan kv4_plan(size_t T, size_t B, size_t Hk, size_t G, size_t keys_cap, bool ragged) {
     Kv4Plan plan;
-    plan.items = (int)((T / B * G + PAIRS - 1) / PAIRS);
-    plan.groups = (long long)(ragged ? T * G / PAIRS + B : B * plan.items);
+    plan.groups = (long long)(ragged ? T * G / PAIRS + B : B * ((T / B * G + PAIRS - 1) / PAIRS));
     const size_t tiles = (keys_cap + KV4_TOKENS - 1) / KV4_TOKENS;
     // two workgroups a CU, as many as fit (131072 tokens of one row: 32 us, 37 with three, 44 with six; without a second round 500 rows over
-    // 16384 are 175 instead of 183)
-    const size_t want = (size_t)2 * device_info().cus / (plan.groups * Hk);
+    // 16384 are 175 instead of 183). One of eight waves a CU instead: 64 sequences 74 -> 82, prompts beside single tokens 57 -> 64.
+    const size_t want = (size_t)(8 / WAVES) * device_info().cus / (plan.groups * Hk);
     size_t S = want < 1 ? 1 : want;
     // (a second launch, for the join, pays from 32 tiles on: 700 tokens of one row take 12.6 us in two spans, 10.0 in one)
-    const size_t most = tiles < 4 * LEAST ? 1 : tiles / LEAST;
+    const size_t most = tiles < 32 ? 1 : tiles / LEAST;
     if (S > most) S = most;
     if (S > (size_t)MOST_SPANS) S = MOST_SPANS;
     plan.S = (int)S;
@@ -618,7 +626,7 @@ static int32_t launch_attn_kv4(const AttnKv4& p, const Kv4Plan& plan, hipStream_
     constexpr int lds = (int)sizeof(Meet<D>);
     const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_kv4_kernel<D>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (rc != hipSuccess) return hip_status(rc, "hipFuncSetAttribute");
-    hipLaunchKernelGGL(attn_kv4_kernel<D>, dim3((unsigned)(plan.groups * plan.S * (long long)p.Hk)), dim3(256), lds, st, p);
+    hipLaunchKernelGGL(attn_kv4_kernel<D>, dim3((unsigned)(plan.groups * plan.S * (long long)p.Hk)), dim3(64 * WAVES), lds, st, p);
     const int32_t done = hip_status(hipGetLastError(), "attn_kv4 launch");
     if (done != OK || plan.S == 1) return done;
     const unsigned pairs = (unsigned)(p.seqs.T * p.Hq);
@@ -668,7 +676,7 @@ extern "C" int32_t btb_hip_attn_kv4(const void* q, const void* cache, const int3
     p.part = workspace;
     p.c = scale * LOG2E;
     p.Hq = (int)Hq, p.Hk = (int)Hk, p.G = (int)(Hq / Hk);
-    p.items = plan.items, p.S = plan.S;
+    p.S = plan.S;
     hipStream_t st = static_cast<hipStream_t>(stream);
     return D == 64 ? launch_attn_kv4<64>(p, plan, st) : launch_attn_kv4<128>(p, plan, st);
 }

@@ -60,9 +60,9 @@ struct Kv4Seqs {
 };
 
 // Item `x` of a pass whose sequence b has count(b) of them, one sequence after another: its sequence and which of them it is; b = -1
-// behind the last. Each wave looks for itself, 64 sequences at a time.
+// behind the last, and x is then how far. Each wave looks for itself, 64 sequences at a time.
 template <class Count>
-__device__ __forceinline__ void kv4_find(int x, int B, int& b, int& i, Count count) {
+__device__ __forceinline__ void kv4_find(int& x, int B, int& b, int& i, Count count) {
     const int lane = threadIdx.x & 63;
     b = -1, i = 0;
     for (int b0 = 0; b0 < B; b0 += 64) {
