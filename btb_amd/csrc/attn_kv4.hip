@@ -446,14 +446,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attn_kv4_kernel(AttnKv4 p) {
     a.b = __builtin_amdgcn_readfirstlane(a.b), item = __builtin_amdgcn_readfirstlane(item);
     p.seqs.of(a.b, a.row0, a.n);
     a.len = p.seqs.len(a.b);
-    const int tiles = (a.len + KV4_TOKENS - 1) / KV4_TOKENS, length = kv4_span_tiles(p, tiles);
+    const int tiles = (p.seqs.held(a.len) + KV4_TOKENS - 1) / KV4_TOKENS, length = kv4_span_tiles(p, tiles);
     a.spans = max(1, (tiles + length - 1) / length);
     if (a.span >= a.spans) return;
     a.pairs = a.n * p.G, a.pair0 = item * PAIRS;
     const int last = min(a.pair0 + PAIRS, a.pairs) - 1;  // the pair that sees most
     const int any = a.len - a.n + last / p.G + 1;
     a.from = a.span * length;
-    a.to = min(min(a.from + length, tiles), (any + KV4_TOKENS - 1) / KV4_TOKENS);
+    a.to = min(min(a.from + length, tiles), any < 1 ? 0 : (any - 1) / KV4_TOKENS + 1);
     // Few pairs: several tiles at a time. At head_dim 128 four of them do not fit the registers: 131072 tokens of one row 36 us by two,
     // 38 by one, 62 by four; 64 sequences of up to 8192 80, 96 and 137. Tiles that this workgroup alone reads are not kept in the caches: 36 -> 33 and
     // 80 -> 76, but 61 -> 65 for prompts beside single tokens where others read them too.
@@ -490,7 +490,7 @@ __device__ __forceinline__ bool kv4_parts(const AttnKv4& p, unsigned pair, int D
         }
         if (b < 0) return false;
     }
-    const int tiles = (p.seqs.len(b) + KV4_TOKENS - 1) / KV4_TOKENS, length = kv4_span_tiles(p, tiles);
+    const int tiles = (p.seqs.held(p.seqs.len(b)) + KV4_TOKENS - 1) / KV4_TOKENS, length = kv4_span_tiles(p, tiles);
     parts.spans = (tiles + length - 1) / length;
     parts.ml = reinterpret_cast<const float2*>(p.part) + (size_t)pair * p.S;
     parts.o = p.part + 2 * (size_t)p.seqs.T * p.Hq * p.S + (size_t)pair * p.S * D;

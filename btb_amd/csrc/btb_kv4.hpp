@@ -40,10 +40,10 @@ struct Kv4Seqs {
     long long stride;       // bytes from a page to the next
     int tile;               // bytes of a tile
 
-    // what the device arrays say is cut to what there is
-    __device__ __forceinline__ int len(int b) const {
-        return (int)min((long long)max(lens[b], 0), (long long)W * per * KV4_TOKENS);
-    }
+    // what the device arrays say is cut to what there is: a sequence's length, by which its rows stand at their places, and how many of
+    // those places its table has
+    __device__ __forceinline__ int len(int b) const { return max(lens[b], 0); }
+    __device__ __forceinline__ int held(int len) const { return (int)min((long long)len, (long long)W * per * KV4_TOKENS); }
     __device__ __forceinline__ void of(int b, int& row0, int& n) const {
         if (first == nullptr) {
             row0 = b * rows, n = rows;

@@ -32,8 +32,8 @@ struct Kv4Rows {
 __device__ __forceinline__ int kv4_tiles(const Kv4Seqs& s, int b) {
     int row0, n;
     s.of(b, row0, n);
-    const int len = s.len(b), there = min(n, len);
-    return there < 1 ? 0 : (len - 1) / KV4_TOKENS - (len - there) / KV4_TOKENS + 1;
+    const int len = s.len(b), from = len - min(n, len), to = s.held(len);
+    return from >= to ? 0 : (to - 1) / KV4_TOKENS - from / KV4_TOKENS + 1;
 }
 
 // the workgroup's tile: its sequence and number, the pass's row of its first token (below 0: that token is no row of the pass) and which
@@ -55,7 +55,7 @@ __device__ __forceinline__ bool kv4_place(const Kv4Rows& p, int item, Kv4Place& 
     p.seqs.of(at.b, row0, n);
     const int len = p.seqs.len(at.b), from = len - min(n, len);  // the first position that is a row's
     at.tile = from / KV4_TOKENS + i;
-    const int first = at.tile * KV4_TOKENS, low = max(from - first, 0), high = min(len - first, KV4_TOKENS);
+    const int first = at.tile * KV4_TOKENS, low = max(from - first, 0), high = min(p.seqs.held(len) - first, KV4_TOKENS);
     at.row = row0 + n - len + first;
     at.tokens = (high == 32 ? 0xFFFFFFFFu : (1u << high) - 1u) & (0xFFFFFFFFu << low);
     return true;

@@ -202,8 +202,9 @@ extern "C" int32_t btb_hip_pages_compact(void* pool, size_t L, size_t pages, siz
                                          int32_t* tables_out, int32_t* used, int32_t* workspace, void* stream) {
     if (!pool || !tables || !lens || !tables_out || !used || !workspace) return ERR_NULL;
     Pages p{};
-    if (!pages_of(p, pool, L, pages, bytes, layer, stride, B, W, page) || pages > COMPACT_PAGES) {
-        set_error("pages_compact: " PAGES_DOMAIN ", up to 2^19 pages");
+    const bool crossed = tables_out != tables && tables_out < tables + B * W && tables < tables_out + B * W;
+    if (!pages_of(p, pool, L, pages, bytes, layer, stride, B, W, page) || pages > COMPACT_PAGES || crossed) {
+        set_error("pages_compact: " PAGES_DOMAIN ", up to 2^19 pages, tables_out the tables or apart from them");
         return ERR_DOMAIN;
     }
     p.tables = const_cast<int32_t*>(tables), p.lens = const_cast<int32_t*>(lens);

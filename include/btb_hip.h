@@ -521,10 +521,11 @@ int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t* pos, int6
 /* ---- a paged cache held in 4 bits -------------------------------------------------------------------------
  * Pages of `page` tokens (a multiple of 32) of all Hk kv heads of one layer, in a pool of `pages` of them, `stride` bytes from one to
  * the next: page / 32 tiles of btb_hip_kv4_tile_bytes(D) bytes a head, one head after another. Sequence b's tokens 0 .. lens[b] - 1 lie in
- * pages tables[b][0], tables[b][1], ... (i32 [B, W]); a length is cut to 0 .. W page, and tokens whose page is not one of the pool's are not there.
+ * pages tables[b][0], tables[b][1], ... (i32 [B, W]; a length below 0 is 0). Tokens from W page on, and those whose page is not one of the
+ * pool's, are not there.
  * The rows of a pass are its sequences' last ones: rows first[b] .. first[b + 1] - 1 (i32 [B + 1] on the device, ascending) are
- * sequence b's, T / B a sequence where first is NULL; row i of n stands at lens[b] - n + i, and rows at places below 0 or behind the last
- * sequence's are left alone. All of it is read on the device: a recorded call replays over longer sequences and other tables.
+ * sequence b's, T / B a sequence where first is NULL; row i of n stands at lens[b] - n + i, and rows at places below 0 or from W page
+ * on are left alone in the cache, rows behind the last sequence's everywhere. All of it is read on the device: a recorded call replays over longer sequences and other tables.
  * A key is held as e2m1 codes with a power of two for 32 dims, the smallest e of -127 .. 125 with max |k| <= 7 2^e (MXFP4: btb_hip_mx4_widen), a value as
  * e2m1 codes with one scale, bf16(max |v| / 6); codes are the nearest, ties to even. An infinity or NaN makes all that its scale is for
  * NaN. D 64 or 128; cache 16-byte aligned, stride a multiple of 16; B up to 65536, T up to 2^24, Hk up to 1024, W page up to 2^30. No
@@ -556,7 +557,7 @@ int32_t btb_hip_attn_kv4(const void* q, const void* cache, const int32_t* tables
                          size_t Hk, size_t D, float scale, size_t keys_cap, float* workspace, void* stream);
 
 /* Sequences that go on from others, in all L layers of a pool (pages of `bytes` bytes, `stride` apart, `layer` bytes from a layer to the
- * next; what they hold does not matter): for f < F sequence dst[f] takes over the length of src[f] and the entries of its whole pages; if
+ * next; what they hold does not matter): for f < F sequence dst[f] takes over the length of src[f], W page at most, and the entries of its whole pages; if
  * tokens are left, its next entry is fresh[f], a copy of that page in every layer; the entries behind are -1. A fork is not made where src or
  * dst is outside 0 .. B - 1, they are the same, or fresh is needed and outside the pool. dst distinct and none of them a src, fresh
  * distinct and in nobody's table. src, dst, fresh: i32 [F] on the device. bytes, stride, layer multiples of 16; F up to 65536. */
@@ -565,7 +566,7 @@ int32_t btb_hip_pages_fork(void* pool, size_t L, size_t pages, size_t bytes, int
                            const int32_t* fresh, size_t F, void* stream);
 
 /* The pool closed up: of the n pages that sequences name (the first ceil(lens[b] / page) entries of each), those below n stay, and the
- * others, ascending, go to the pages below n that nobody names, ascending, in every layer. tables_out [B, W] (may be tables): the entries as
+ * others, ascending, go to the pages below n that nobody names, ascending, in every layer. tables_out [B, W] (tables themselves, or apart from them): the entries as
  * they are then, -1 behind a sequence's and for what is no page of the pool; *used = n. workspace: btb_hip_pages_compact_words of
  * them, this call's own. Up to 2^19 pages. */
 size_t btb_hip_pages_compact_words(size_t pages);

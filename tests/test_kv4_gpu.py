@@ -218,6 +218,28 @@ def test_rows_that_are_nobodys_and_pages_that_are_not_there(card):
     torch.cuda.synchronize()
 
 
+def test_a_full_table(card):
+    """a sequence longer than its table: rows past it are not written, what stands there stays, attention is over what is held"""
+    g = gen(9450)
+    Hk, G, D, page = 1, 2, 64, 32
+    tables = _i32([[2, 0]])
+    pool = _filled(card, 3, Hk, D, page)
+    k, v = _rows(g, 66, Hk, D), _rows(g, 66, Hk, D)
+    card.kv4_write(k[:64], v[:64], pool, tables, _i32([64]))
+    full = pool.clone()
+    card.kv4_write(k[64:65], v[64:65], pool, tables, _i32([65]))
+    card.kv4_write(k[:1], v[:1], pool, tables, _i32([(1 << 31) - 1]))
+    assert torch.equal(pool, full)
+    card.kv4_write(k[60:66], v[60:66], pool, tables, _i32([66]))  # the first four of them are the last that fit, and the same
+    assert torch.equal(pool, full)
+    a, b = (torch.full((6, Hk, D), 9.0, device="cuda") for _ in range(2))
+    card.kv4_read(pool, tables, _i32([66]), a, b)
+    assert _same(a[:4], kv4.held_k(k[60:64].double().cpu().numpy())[0]) and bool((a[4:] == 9.0).all()) and bool((b[4:] == 9.0).all())
+    q = _rows(g, 3, G, D)
+    att, lse = _attend(card, q, pool, tables, [66], [3], G, page, check=False)  # at 63, 64 and 65
+    _check(q, pool, _i32([[2, 0, -1]]), [66], [3], att, lse, 1.0 / math.sqrt(D), G, page)
+
+
 # ---- attention -----------------------------------------------------------------------------------------------------------------
 
 

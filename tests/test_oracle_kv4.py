@@ -153,6 +153,7 @@ def test_pages_refused(other):
 def test_more_refusals():
     lib = native.load_library()
     assert _fork(lib, F=0) == native.ERR_DOMAIN and _fork(lib, F=65537) == native.ERR_DOMAIN
+    assert _compact(lib, tables=ctypes.c_void_p(0x1000), out=ctypes.c_void_p(0x1010)) == native.ERR_DOMAIN  # four entries on
     assert _compact(lib, pages=(1 << 19) + 1, layer=((1 << 19) + 1) * 4096) == native.ERR_DOMAIN
     for name in ("k", "v", "cache", "tables", "lens"):
         assert _write(lib, **{name: None}) == native.ERR_NULL and _read(lib, **{name: None}) == native.ERR_NULL
