@@ -669,6 +669,11 @@ extern "C" int32_t btb_hip_attn_kv4(const void* q, const void* cache, const int3
         return ERR_DOMAIN;
     }
     const Kv4Plan plan = kv4_plan(T, B, Hk, Hq / Hk, keys_cap, first != nullptr);
+    // (a join's workgroup a pair comes with many spans only, and those with few pairs)
+    if (plan.groups * plan.S * (long long)Hk > MOST_GROUPS) {
+        set_error("attn_kv4: sequences, with tiles of 32 rows and heads, times kv heads below 2^24");
+        return ERR_DOMAIN;
+    }
     p.q = static_cast<const uint16_t*>(q);
     p.cache = static_cast<const uint8_t*>(cache);
     p.att = static_cast<uint16_t*>(att);

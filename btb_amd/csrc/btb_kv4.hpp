@@ -84,6 +84,9 @@ __device__ __forceinline__ void kv4_find(int& x, int B, int& b, int& i, Count co
     }
 }
 
+// workgroups of 256 threads that a launch can have: its threads are counted in 32 bits
+constexpr long long MOST_GROUPS = ((1ll << 32) - 1) / 256;
+
 // What every entry point over such a cache asks of its sizes; false: refused. The words for it:
 #define KV4_DOMAIN "head_dim 64 or 128, pages of a multiple of 32 tokens, 1 .. 65536 sequences of up to 2^30 tokens, up to 2^24 rows (without first: as many a sequence), up to 1024 kv heads"
 inline bool kv4_seqs(Kv4Seqs& s, const int32_t* tables, const int32_t* lens, const int32_t* first, size_t B, size_t W, size_t pages,

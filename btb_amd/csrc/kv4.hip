@@ -26,6 +26,7 @@ struct Kv4Rows {
     void* v_out;
     long long kt, kh, vt, vh;  // values from a row, and from a head, to the next
     int Hk, items;             // items a sequence, where each has as many rows
+    long long groups;
 };
 
 // the tiles a sequence's last rows lie in
@@ -261,15 +262,16 @@ static int32_t kv4_rows(Kv4Rows& p, const void* cache, const int32_t* tables, co
     p.cache = static_cast<uint8_t*>(const_cast<void*>(cache));
     p.kt = kt, p.kh = kh, p.vt = vt, p.vh = vh;
     p.Hk = (int)Hk;
-    return OK;
-}
-
-// workgroups: the tiles that the rows can lie in, each at least one of them, a head each
-static dim3 kv4_grid(Kv4Rows& p) {
-    const long long T = p.seqs.T, B = p.seqs.B, R = p.seqs.rows;
+    // workgroups: the tiles that the rows can lie in, each at least one of them, a head each
+    const long long rows = p.seqs.T, seqs = p.seqs.B, R = p.seqs.rows;
     p.items = (int)(R < (R + 30) / 32 + 1 ? R : (R + 30) / 32 + 1);
-    const long long ragged = T < T / 32 + 2 * B ? T : T / 32 + 2 * B;
-    return dim3((unsigned)((p.seqs.first ? ragged : B * p.items) * p.Hk));
+    const long long ragged = rows < rows / 32 + 2 * seqs ? rows : rows / 32 + 2 * seqs;
+    p.groups = (first ? ragged : seqs * p.items) * p.Hk;
+    if (p.groups > MOST_GROUPS) {
+        set_error(what);
+        return ERR_DOMAIN;
+    }
+    return OK;
 }
 
 }  // namespace btb
@@ -284,12 +286,12 @@ extern "C" int32_t btb_hip_kv4_write(const void* k, const void* v, void* cache, 
     if (!k || !v || !cache || !tables || !lens) return ERR_NULL;
     Kv4Rows p{};
     const int32_t rc = kv4_rows(p, cache, tables, lens, first, B, W, pages, page, stride, T, Hk, D, k_row, k_head, v_row, v_head, k, v,
-                                "kv4_write: " KV4_DOMAIN "; k, v and cache 16-byte aligned, strides in multiples of 8");
+                                "kv4_write: " KV4_DOMAIN "; k, v and cache 16-byte aligned, strides in multiples of 8; tiles and heads of the rows below 2^24");
     if (rc != OK) return rc;
     p.k = static_cast<const uint16_t*>(k);
     p.v = static_cast<const uint16_t*>(v);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const dim3 grid = kv4_grid(p);
+    const dim3 grid((unsigned)p.groups);
     if (D == 64)
         hipLaunchKernelGGL(kv4_write_kernel<64>, grid, dim3(256), 0, st, p);
     else
@@ -304,7 +306,7 @@ extern "C" int32_t btb_hip_kv4_read(const void* cache, const int32_t* tables, co
     if (!k || !v || !cache || !tables || !lens) return ERR_NULL;
     Kv4Rows p{};
     const int32_t rc = kv4_rows(p, cache, tables, lens, first, B, W, pages, page, stride, T, Hk, D, k_row, k_head, v_row, v_head, k, v,
-                                "kv4_read: " KV4_DOMAIN "; k, v and cache 16-byte aligned, strides in multiples of 8");
+                                "kv4_read: " KV4_DOMAIN "; k, v and cache 16-byte aligned, strides in multiples of 8; tiles and heads of the rows below 2^24");
     if (rc != OK) return rc;
     // rows or heads in one place
     auto shared = [&](int64_t row, int64_t head) {
@@ -318,7 +320,7 @@ extern "C" int32_t btb_hip_kv4_read(const void* cache, const int32_t* tables, co
     p.k_out = k;
     p.v_out = v;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const dim3 grid = kv4_grid(p);
+    const dim3 grid((unsigned)p.groups);
     if (D == 64)
         hipLaunchKernelGGL((out_f32 ? kv4_read_kernel<64, float> : kv4_read_kernel<64, uint16_t>), grid, dim3(256), 0, st, p);
     else

@@ -183,8 +183,8 @@ extern "C" int32_t btb_hip_pages_fork(void* pool, size_t L, size_t pages, size_t
     if (!pool || !tables || !lens || !src || !dst || !fresh) return ERR_NULL;
     Pages p{};
     if (!pages_of(p, pool, L, pages, bytes, layer, stride, B, W, page) || F == 0 || F > 65536 ||
-        F * L > 0x7FFFFFFFu / (size_t)p.chunks) {
-        set_error("pages_fork: " PAGES_DOMAIN ", 1 .. 65536 forks");
+        F * L * p.chunks > ((size_t)1 << 24) - 1) {  // (a launch's threads are counted in 32 bits)
+        set_error("pages_fork: " PAGES_DOMAIN ", 1 .. 65536 forks, below 2^24 of 16 KB in all layers");
         return ERR_DOMAIN;
     }
     p.tables = tables, p.lens = lens;

@@ -528,7 +528,8 @@ int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t* pos, int6
  * on are left alone in the cache, rows behind the last sequence's everywhere. All of it is read on the device: a recorded call replays over longer sequences and other tables.
  * A key is held as e2m1 codes with a power of two for 32 dims, the smallest e of -127 .. 125 with max |k| <= 7 2^e (MXFP4: btb_hip_mx4_widen), a value as
  * e2m1 codes with one scale, bf16(max |v| / 6); codes are the nearest, ties to even. An infinity or NaN makes all that its scale is for
- * NaN. D 64 or 128; cache 16-byte aligned, stride a multiple of 16; B up to 65536, T up to 2^24, Hk up to 1024, W page up to 2^30. No
+ * NaN. D 64 or 128; cache 16-byte aligned, stride a multiple of 16; B up to 65536, T up to 2^24, Hk up to 1024, W page up to 2^30, and the tiles of
+ * 32 tokens (for attention: of 32 rows and query heads of a kv head) that the rows can lie in, times Hk, below 2^24. No
  * counterpart in the reference. */
 
 /* bytes of 32 tokens of one kv head, keys and values: 2176 at D 64, 4288 at 128, 0 at others */
@@ -560,7 +561,8 @@ int32_t btb_hip_attn_kv4(const void* q, const void* cache, const int32_t* tables
  * next; what they hold does not matter): for f < F sequence dst[f] takes over the length of src[f], W page at most, and the entries of its whole pages; if
  * tokens are left, its next entry is fresh[f], a copy of that page in every layer; the entries behind are -1. A fork is not made where src or
  * dst is outside 0 .. B - 1, they are the same, or fresh is needed and outside the pool. dst distinct and none of them a src, fresh
- * distinct and in nobody's table. src, dst, fresh: i32 [F] on the device. bytes, stride, layer multiples of 16; F up to 65536. */
+ * distinct and in nobody's table. src, dst, fresh: i32 [F] on the device. bytes, stride, layer multiples of 16; F up to 65536,
+ * F L ceil(bytes / 16384) below 2^24. */
 int32_t btb_hip_pages_fork(void* pool, size_t L, size_t pages, size_t bytes, int64_t layer, int64_t stride, int32_t* tables,
                            int32_t* lens, size_t B, size_t W, size_t page, const int32_t* src, const int32_t* dst,
                            const int32_t* fresh, size_t F, void* stream);

@@ -163,3 +163,16 @@ def test_more_refusals():
         assert _fork(lib, **{name: None}) == native.ERR_NULL
     for name in ("pool", "tables", "lens", "out", "used", "ws"):
         assert _compact(lib, **{name: None}) == native.ERR_NULL
+
+
+@pytest.mark.parametrize("first", [None, P])
+def test_more_workgroups_than_a_launch_has(first):
+    """a launch's threads are counted in 32 bits: 2^24 workgroups of 256 are one too many"""
+    lib = native.load_library()
+    heads = dict(Hk=1024, stride=1024 * 2 * 4288)
+    for T in (1 << 24, 1 << 20):  # 2^19 and 2^15 tiles, 1024 heads
+        assert _write(lib, T=T, first=first, **heads) == native.ERR_DOMAIN
+        assert _read(lib, T=T, first=first, kr=1 << 17, vr=1 << 17, **heads) == native.ERR_DOMAIN
+    assert _attn(lib, B=1 << 16, T=1 << 14, first=P, Hq=1024, **heads) == native.ERR_DOMAIN
+    assert _attn(lib, B=1 << 14, T=1 << 14, Hq=1024, **heads) == native.ERR_DOMAIN
+    assert _fork(lib, F=65536, L=64, bytes=1 << 16, stride=1 << 16, layer=9 << 16) == native.ERR_DOMAIN
