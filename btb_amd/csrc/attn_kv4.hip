@@ -668,6 +668,12 @@ extern "C" int32_t btb_hip_attn_kv4(const void* q, const void* cache, const int3
                   "q, cache, att and workspace 16-byte aligned");
         return ERR_DOMAIN;
     }
+    // (att may be q: a pair's row is read, by the workgroups that write it or before the join, ahead of what is written there)
+    const uintptr_t from = (uintptr_t)q, to = (uintptr_t)att, bytes = 2 * T * Hq * D;
+    if (from != to && from < to + bytes && to < from + bytes) {
+        set_error("attn_kv4: att lies across q");
+        return ERR_DOMAIN;
+    }
     const Kv4Plan plan = kv4_plan(T, B, Hk, Hq / Hk, keys_cap, first != nullptr);
     // (a join's workgroup a pair comes with many spans only, and those with few pairs)
     if (plan.groups * plan.S * (long long)Hk > MOST_GROUPS) {

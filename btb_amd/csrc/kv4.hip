@@ -313,8 +313,8 @@ extern "C" int32_t btb_hip_kv4_read(const void* cache, const int32_t* tables, co
         return (T > 1 && row < (int64_t)D) || (Hk > 1 && head < (int64_t)D) ||
                (T > 1 && Hk > 1 && row < (int64_t)Hk * head && head < (int64_t)T * row);
     };
-    if (shared(k_row, k_head) || shared(v_row, v_head)) {
-        set_error("kv4_read: rows or heads of an output share memory");
+    if (shared(k_row, k_head) || shared(v_row, v_head) || k == v) {
+        set_error("kv4_read: rows or heads of an output, or both outputs, share memory");
         return ERR_DOMAIN;
     }
     p.k_out = k;

@@ -318,6 +318,21 @@ def test_attention(card, lens, rows, Hk, G, D, page, cap):
     assert torch.equal(a[0], again[0]) and torch.equal(a[1], again[1])
 
 
+@pytest.mark.parametrize("lens,rows,Hk,G,D", [([9000], [1], 1, 2, 64), ([1500, 40], [1, 1], 2, 4, 128), ([129, 64, 0, 2000], [100, 64, 2, 1], 2, 5, 128)])
+def test_in_the_place_of_its_rows(card, lens, rows, Hk, G, D):
+    """att is q: many spans, few, none"""
+    g = gen(9550 + D + G)
+    page, scale = 64, 0.1
+    pool, tables, _, _ = _put(card, g, lens, Hk, D, page)
+    q = _rows(g, sum(rows), Hk * G * D)
+    att = torch.zeros_like(q)
+    scratch = card.attn_kv4_scratch(sum(rows), len(lens), Hk * G, Hk, D, max(lens))
+    for out in (att, q):
+        card.attn_kv4(q, pool, tables, _i32(lens), out, Hk * G, Hk, D, scale, scratch, first=_first(rows), keys_cap=max(lens))
+    torch.cuda.synchronize()
+    assert torch.equal(att, q) and bool(att.any())
+
+
 def test_attention_without_anything_to_see(card):
     """lengths of zero and below, rows before the first token, sequences without rows, rows behind the last sequence"""
     g = gen(9600)

@@ -12,6 +12,7 @@ from oracle import kv4
 
 P = ctypes.c_void_p(0x1000)  # an address that no refused call follows
 OFF = ctypes.c_void_p(0x1004)
+FAR = ctypes.c_void_p(0x10000000)  # far from it
 F = ctypes.c_float
 
 
@@ -79,7 +80,7 @@ def test_sizes():
         assert floats(*bad) == 0, bad
 
 
-ROWS = dict(k=P, v=P, cache=P, tables=P, lens=P, first=None, B=2, W=4, pages=9, page=64, stride=8 * 2 * 4288, T=6, Hk=8, D=128, kr=1024,
+ROWS = dict(k=P, v=FAR, cache=P, tables=P, lens=P, first=None, B=2, W=4, pages=9, page=64, stride=8 * 2 * 4288, T=6, Hk=8, D=128, kr=1024,
             kh=128, vr=1024, vh=128)
 # what every operator over such a cache refuses
 SEQS = [dict(B=0), dict(B=65537, first=P), dict(W=0), dict(pages=0), dict(page=0), dict(page=48), dict(page=1 << 21, W=1),
@@ -100,7 +101,7 @@ def _read(lib, **other):
 
 
 def _attn(lib, **other):
-    a = dict(q=P, cache=P, tables=P, lens=P, first=None, att=P, lse=P, B=2, W=4, pages=9, page=64, stride=8 * 2 * 4288, T=6, Hq=32, Hk=8, D=128,
+    a = dict(q=P, cache=P, tables=P, lens=P, first=None, att=FAR, lse=P, B=2, W=4, pages=9, page=64, stride=8 * 2 * 4288, T=6, Hq=32, Hk=8, D=128,
              scale=0.1, keys=200, ws=P)
     a.update(other)
     return lib.btb_hip_attn_kv4(a["q"], a["cache"], a["tables"], a["lens"], a["first"], a["att"], a["lse"], a["B"], a["W"], a["pages"],
@@ -176,3 +177,10 @@ def test_more_workgroups_than_a_launch_has(first):
     assert _attn(lib, B=1 << 16, T=1 << 14, first=P, Hq=1024, **heads) == native.ERR_DOMAIN
     assert _attn(lib, B=1 << 14, T=1 << 14, Hq=1024, **heads) == native.ERR_DOMAIN
     assert _fork(lib, F=65536, L=64, bytes=1 << 16, stride=1 << 16, layer=9 << 16) == native.ERR_DOMAIN
+
+
+def test_outputs_over_each_other_or_the_input():
+    lib = native.load_library()
+    assert _read(lib, v=P) == native.ERR_DOMAIN and b"share memory" in lib.btb_hip_last_error()
+    for at in (0x1010, 0x1000 + 6 * 32 * 128 * 2 - 16, 0x1000 - 16):  # all but the first 16 bytes, the last, all but the last
+        assert _attn(lib, q=P, att=ctypes.c_void_p(at)) == native.ERR_DOMAIN and b"across q" in lib.btb_hip_last_error()
