@@ -195,6 +195,22 @@ def test_strides(card):
     assert torch.equal(pools[1], pools[2])
 
 
+def test_one_row_or_head_of_any_stride(card):
+    """the stride from the only row, or head, to a next one that is not there"""
+    g = gen(9350)
+    D, page = 64, 32
+    for T, Hk in ((1, 2), (2, 1), (1, 1)):
+        pool, tables = card.kv4_pool(1, Hk, D, page), _i32([[0]])
+        k, v = (_rows(g, T, Hk, D) for _ in range(2))
+        strides = 3 if T == 1 else Hk * D, 5 if Hk == 1 else D, 1
+        card.kv4_write(k.as_strided(k.shape, strides), v.as_strided(v.shape, strides), pool, tables, _i32([T]))
+        a, b = torch.zeros_like(k), torch.zeros_like(v)
+        card.kv4_read(pool, tables, _i32([T]), a.as_strided(a.shape, strides), b.as_strided(b.shape, strides))
+        assert _same(a, kv4.held_k(k.double().cpu().numpy())[0])
+        want = kv4.held_v(v.double().cpu().numpy())[0]
+        assert _same(b, torch.from_numpy(want).bfloat16().double().numpy())
+
+
 def test_rows_that_are_nobodys_and_pages_that_are_not_there(card):
     g = gen(9400)
     Hk, D, page, T = 1, 64, 32, 40
