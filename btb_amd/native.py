@@ -1249,8 +1249,8 @@ class HipCard(CardLaunch):
             raise ValueError(f"[hip] {what}: tables int32 [sequences, entries], lens [sequences] and first [sequences + 1] or None, "
                              "contiguous on the current GPU")
         B, W = tables.shape
-        if lens.numel() != B or (first is not None and first.numel() != B + 1):
-            raise ValueError(f"[hip] {what}: lens is [{B}] and first [{B + 1}] or None, as tables has them")
+        if B < 1 or lens.numel() != B or (first is not None and first.numel() != B + 1):
+            raise ValueError(f"[hip] {what}: a sequence or more, lens is [{B}] and first [{B + 1}] or None, as tables has them")
         if not (isinstance(cache, _Tensor) and cache.dtype is torch.uint8 and cache.get_device() == dev and cache.dim() == 4):
             raise ValueError(f"[hip] {what}: the cache is a layer's pool, uint8 on the current GPU (kv4_pool)")
         pages, heads, tiles, tile = cache.shape

@@ -693,6 +693,8 @@ def test_refusals(card):
             card.kv4_write(**{**write, name: bad})
     with pytest.raises(ValueError):
         card.kv4_write(k[:3], v[:3], pool, tables, lens)  # three rows for two sequences
+    with pytest.raises(ValueError):
+        card.kv4_write(k, v, pool, tables[:0], lens[:0])
     f = torch.zeros(T, Hk, D, device="cuda")
     with pytest.raises(ValueError):
         card.kv4_read(pool, tables, lens, f, f.bfloat16(), first=first)
