@@ -9,6 +9,7 @@ at once. A page takes 134 bytes a token, kv head and layer at head_dim 128, wher
 from __future__ import annotations
 
 import math
+from itertools import islice
 from typing import Any, Mapping, Sequence
 
 import torch
@@ -50,17 +51,21 @@ class Paged:
 
     def _take(self, n: int, what: str) -> list[int]:
         """the first n free pages"""
-        found = [p for p, k in enumerate(self.named) if k == 0][:n]
+        found = list(islice((p for p, k in enumerate(self.named) if k == 0), n))
         if len(found) < n:
             raise RuntimeError(f"[paged] {what} needs {n} pages, {len(found)} are free")
         return found
 
     def advance(self, tokens: Mapping[int, Sequence[int]]) -> dict[int, torch.Tensor]:
-        """these sequences' next tokens (a sequence's first ones: its prompt); the logits [vocab] behind each one's last"""
-        for b, part in tokens.items():
-            if not part or self.length[self._seq(b)] + len(part) > self.longest:
+        """these sequences' next tokens (a sequence's first ones: its prompt); the logits [vocab] behind each one's last. Where a pass
+        raises, the sequences keep what the passes before it brought."""
+        left = {b: [int(t) for t in part] for b, part in sorted(tokens.items())}
+        for b, part in left.items():
+            if any(not 0 <= t < self.cfg.vocab for t in part):
+                raise ValueError(f"[paged] sequence {b} was given tokens outside 0 .. {self.cfg.vocab - 1}")
+            if self.length[self._seq(b)] + len(part) > self.longest or not part:
                 raise ValueError(f"[paged] sequence {b} has {self.length[b]} of {self.longest} tokens, {len(part)} more were given")
-        grown = {b: -(-(self.length[b] + len(part)) // self.page) - len(self.held[b]) for b, part in tokens.items()}
+        grown = {b: -(-(self.length[b] + len(part)) // self.page) - len(self.held[b]) for b, part in left.items()}
         fresh = self._take(sum(grown.values()), "a pass")
         for b, n in grown.items():
             for p in fresh[:n]:
@@ -70,20 +75,30 @@ class Paged:
         if any(grown.values()):
             self._books()
         out: dict[int, torch.Tensor] = {}
-        left = {b: list(part) for b, part in sorted(tokens.items())}
-        while left:
-            p = self._narrow if sum(len(part) for part in left.values()) <= self.seqs else self._wide
-            room, now = p.T, {}
-            for i, (b, part) in enumerate(left.items()):  # a row at least for each that is left
-                now[b] = part[:room - (len(left) - 1 - i)]
-                room -= len(now[b])
-            logits = p.run(now)
-            left = {b: part[len(now[b]):] for b, part in left.items() if len(part) > len(now[b])}
-            out.update({b: logits[i].clone() for i, b in enumerate(now) if b not in left})  # (the next pass writes over them)
+        try:
+            while left:
+                p = self._narrow if sum(len(part) for part in left.values()) <= self.seqs else self._wide
+                room, now = p.T, {}
+                for i, (b, part) in enumerate(left.items()):  # a row at least for each that is left
+                    now[b] = part[:room - (len(left) - 1 - i)]
+                    room -= len(now[b])
+                logits = p.run(now)
+                left = {b: part[len(now[b]):] for b, part in left.items() if len(part) > len(now[b])}
+                out.update({b: logits[i].clone() for i, b in enumerate(now) if b not in left})  # (the next pass writes over them)
+        except BaseException:
+            for b in grown:  # pages that it has not come to need
+                whole = -(-self.length[b] // self.page)
+                for p in self.held[b][whole:]:
+                    self.named[p] -= 1
+                del self.held[b][whole:]
+            self._books()
+            raise
         return out
 
     def fork(self, branches: Mapping[int, int]) -> None:
         """sequences branches[dst] = src: each dst, which holds nothing, goes on from src's tokens"""
+        if not branches:
+            return
         for dst, src in branches.items():
             if self.held[self._seq(dst)] or not self.length[self._seq(src)] or src in branches:
                 raise ValueError(f"[paged] sequence {dst} is to be empty and {src} not, for one to go on from the other")
@@ -153,7 +168,7 @@ class _Pass:
     def run(self, tokens: Mapping[int, Sequence[int]]) -> torch.Tensor:
         """the sequences' next tokens, in ascending order of their numbers; the logits behind each one's last, in that order"""
         f = self.f
-        ids, pos, first, last = [], [], [0], []
+        ids, pos, first, last, length = [], [], [0], [], list(f.length)
         for b in range(f.seqs):
             part = tokens.get(b, ())
             ids += part
@@ -161,17 +176,18 @@ class _Pass:
             first.append(len(ids))
             if part:
                 last.append(len(ids) - 1)
-            f.length[b] += len(part)
+            length[b] += len(part)
         n = len(ids)
         for t, values in ((self.ids, ids), (self.pos[0], pos), (self.slots, list(range(n)))):
             t.copy_(torch.tensor(values + [-1 if t is self.slots else 0] * (self.T - n), dtype=torch.int32))
         self.first.copy_(torch.tensor(first, dtype=torch.int32))
         self.last.copy_(torch.tensor(last + [0] * (f.seqs - len(last)), dtype=torch.int32))
-        f.lens.copy_(torch.tensor(f.length, dtype=torch.int32))
+        f.lens.copy_(torch.tensor(length, dtype=torch.int32))
         if self.graph is not None:
             self.graph.replay()
         else:
             self._body()
+        f.length = length
         return self.logits
 
     def _body(self) -> None:

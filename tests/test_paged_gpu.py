@@ -175,7 +175,7 @@ def test_refusals(card, stack):
     with pytest.raises(ValueError):
         Paged(card, cfg, w, 2, 8, page=48)
     f = Paged(card, cfg, w, 2, 3, page=32, rows=8, longest=80)
-    for bad in ({2: [1]}, {-1: [1]}, {0: []}, {0: [1] * 81}):
+    for bad in ({2: [1]}, {2: []}, {-1: [1]}, {0: []}, {0: [1] * 81}):
         with pytest.raises(ValueError):
             f.advance(bad)
     f.advance({0: [1] * 40})
@@ -196,3 +196,36 @@ def test_refusals(card, stack):
     with pytest.raises(RuntimeError):
         f.fork({0: 1}) if f.free == 0 else f.advance({0: [1] * 40})
     _books(f)
+
+
+def test_a_pass_that_raises(card, stack):
+    """the second of three passes: the sequences have the first one's tokens and its pages, and go on from there"""
+    cfg, w = stack
+    one, two = (Paged(card, cfg, w, 2, 12, page=32, rows=40, longest=160) for _ in range(2))
+    for f in (one, two):
+        f.advance({1: _long(20, 3)})
+    body, calls = one._wide._body, []
+
+    def failing():
+        calls.append(0)
+        if len(calls) == 2:
+            raise RuntimeError("no")
+        body()
+
+    one._wide._body = failing
+    with pytest.raises(RuntimeError, match="no"):
+        one.advance({0: _long(90, 7), 1: [5]})
+    assert one.length == [39, 21] and one.free == 12 - 2 - 1
+    _books(one)
+    two.advance({0: _long(90, 7)[:39], 1: [5]})
+    for f in (one, two):
+        f.compact()
+        _books(f)
+    a, b = (f.advance({0: _long(90, 7)[39:], 1: [9]}) for f in (one, two))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    for bad in ([cfg.vocab], [1, -1]):
+        with pytest.raises(ValueError):
+            one.advance({0: bad})
+    assert one.advance({}) == {}
+    one.fork({})
+    _books(one)
