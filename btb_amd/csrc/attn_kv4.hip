@@ -101,23 +101,19 @@ struct Softmax {
         over = -__builtin_inff(), below = 0x0D7F0D7Fu;  // 2^-100
     }
 
-    // the maximum and the unit moved to where a tile's scores z and scales s need them. Whether they do each lane asks of its own scores, and
-    // without working out by how much: 500 rows of 32 heads over 16384 tokens take 161 us instead of 166, at head_dim 64 111 instead of 125
-    __device__ __forceinline__ void move(const f32x16& z, const uint32_t (&s)[8], float c) {
+    // The maximum and the unit moved to where a tile's scores z and its scales need them. Whether they do each lane asks of its own scores and
+    // scales (`past`), and without working out by how much: 500 rows of 32 heads over 16384 tokens take 161 us instead of 166, at head_dim 64 111
+    // instead of 125. most(): the largest of the pair's scales, as bits; NaN is below all.
+    template <class Most>
+    __device__ __forceinline__ void move(const f32x16& z, bool past, float c, Most most) {
         float top = z[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = fmaxf(top, z[i]);
-        // the largest scale: as signed 16-bit numbers, of which NaN is the least
-        typedef __attribute__((ext_vector_type(2))) short i16x2;
-        i16x2 big = __builtin_bit_cast(i16x2, below);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) big = __builtin_elementwise_max(big, __builtin_bit_cast(i16x2, s[i]));
-        if (__any(top > over || __builtin_bit_cast(uint32_t, big) != below)) {
+        if (__any(top > over || past)) {
             top = fmaxf(top, xor32(top)) * c;
-            int most = max((int)big[0], (int)big[1]);
-            most = max(most, __builtin_bit_cast(int, xor32(__builtin_bit_cast(float, most))));
-            // the power of two above the largest scale (2^-100 at least); of what is below the unit, the unit
-            const float was = bits_f32(unit()), to = fmaxf(m, top), above = fmaxf(was, bits_f32(((uint32_t)(most & 0x7F80) + 0x80u) << 16));
+            // the power of two above the largest scale, or the unit as it is
+            const float was = bits_f32(unit()), to = fmaxf(m, top);
+            const float above = fmaxf(was, bits_f32(((uint32_t)(max(most(), 0) & 0x7F80) + 0x80u) << 16));
             const float by = __builtin_amdgcn_exp2f(m - to);
             l *= by;
             const float both = by * (was / above);
@@ -129,14 +125,15 @@ struct Softmax {
             below = (f32_bits(above) >> 16) * 0x00010001u - 0x00010001u;
         }
     }
+    // 2^ROOM / unit
+    __device__ __forceinline__ float inverse() const { return bits_f32((uint32_t)(254 + ROOM) * (1u << 23) - unit()); }
 
-    // scores 2 i and 2 i + 1 to weights
-    __device__ __forceinline__ void weigh(const f32x16& z, const uint32_t (&s)[8], u32x4 (&w)[2], float c, int i) {
-        const float inv = bits_f32((uint32_t)(254 + ROOM) * (1u << 23) - unit());  // 2^ROOM / unit
+    // scores 2 i and 2 i + 1 to weights, r and t their scales over the unit
+    __device__ __forceinline__ void weigh(const f32x16& z, float r, float t, u32x4 (&w)[2], float c, int i) {
         const float a = __builtin_amdgcn_exp2f(fmaf(z[2 * i], c, -m)), b = __builtin_amdgcn_exp2f(fmaf(z[2 * i + 1], c, -m));
         l += a;
         l += b;
-        const float x = a * (bf16lo_f32(s[i]) * inv), y = b * (bf16hi_f32(s[i]) * inv);
+        const float x = a * r, y = b * t;
         // (two to an instruction: left to itself the compiler folds each product into a conversion of its own, at half the rate)
         uint32_t both;
         asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(both) : "v"(x), "v"(y));
@@ -178,28 +175,97 @@ struct TileWords {
     __device__ __forceinline__ f16x8 wide_v(int d, int u) const { return codes_f16(dword(v[d / 2], 2 * (d % 2) + u)); }
 };
 
-// the scales of a lane's half of a tile
+// The scales of a lane's half of a tile, over the unit as f32, and the step that comes before: the maximum and the unit moved, tokens that the
+// pair does not see hidden. Those are the ones from `left` on of a tile that is `hidden` in part: no score, and no scale (what lies there may be
+// anything).
+template <int NG>
 struct TileScales {
+    typedef __attribute__((ext_vector_type(2))) short i16x2;
     uint4 s[2];
+    uint32_t x[8];
+
     __device__ __forceinline__ void load(const uint8_t* scales, int lane) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) s[i] = reinterpret_cast<const uint4*>(scales + 32 * (lane >> 5))[i];
     }
-    __device__ __forceinline__ void get(uint32_t (&x)[8]) const {
+    template <int D>
+    __device__ __forceinline__ void move(Softmax<D>& to, f32x16& z, float c, bool hidden, int left, int lane, float*) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = dword(s[i / 4], i % 4);
+        if (hidden)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (kv4_token(lane >> 5, i) >= left) {
+                    z[i] = -__builtin_inff();
+                    x[i / 2] &= i % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+                }
+        i16x2 big = __builtin_bit_cast(i16x2, to.below);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) big = __builtin_elementwise_max(big, __builtin_bit_cast(i16x2, x[i]));
+        to.move(z, __builtin_bit_cast(uint32_t, big) != to.below, c, [&] {
+            const int most = max((int)big[0], (int)big[1]);
+            return max(most, __builtin_bit_cast(int, xor32(__builtin_bit_cast(float, most))));
+        });
+    }
+    template <int D>
+    __device__ __forceinline__ void weigh(Softmax<D>& to, const f32x16& z, u32x4 (&w)[2], float c, int i) const {
+        const float inv = to.inverse();
+        to.weigh(z, bf16lo_f32(x[i]) * inv, bf16hi_f32(x[i]) * inv, w, c, i);
     }
 };
+// One tile at a time, every pair needs the same 32: each lane makes one of them, and all read them out of LDS, where sixteen of them would be two
+// more instructions each: 500 rows of 32 heads over 16384 tokens 161.6 -> 156.4 us.
+template <>
+struct TileScales<1> {
+    int s;
+    float x[16];
 
-// tokens of a tile from `left` on, which the lane's pair does not see: no score, and no scale (what lies there may be anything)
-__device__ __forceinline__ void hide(f32x16& z, uint32_t (&s)[8], int left, int lane) {
+    __device__ __forceinline__ void load(const uint8_t* scales, int lane) { s = reinterpret_cast<const int16_t*>(scales)[lane & 31]; }
+    __device__ __forceinline__ void share(float mine, int lane, float* room) {
+        room[lane & 31] = mine;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if (kv4_token(lane >> 5, i) >= left) {
-            z[i] = -__builtin_inff();
-            s[i / 2] &= i % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+        for (int i = 0; i < 4; ++i) {
+            const float4 y = reinterpret_cast<const float4*>(room)[4 * (lane >> 5) + i];
+            x[4 * i] = y.x, x[4 * i + 1] = y.y, x[4 * i + 2] = y.z, x[4 * i + 3] = y.w;
         }
-}
+        __builtin_amdgcn_wave_barrier();
+    }
+    template <int D>
+    __device__ __forceinline__ void move(Softmax<D>& to, f32x16& z, float c, bool hidden, int left, int lane, float* room) {
+        const float mine = bits_f32((uint32_t)s << 16);
+        int big = s;
+        if (hidden) {  // (from here on the pairs' units may differ)
+            share(mine, lane, room);
+            big = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (kv4_token(lane >> 5, i) >= left) z[i] = -__builtin_inff(), x[i] = 0.f;
+                big = max(big, (int)f32_bits(x[i]) >> 16);
+            }
+        }
+        to.move(z, big > (int)(to.below & 0xFFFFu), c, [&] {
+            int most = max(big, __builtin_bit_cast(int, xor32(__builtin_bit_cast(float, big))));
+            if (!hidden)
+#pragma unroll
+                for (int d = 1; d < 32; d *= 2) most = max(most, __shfl_xor(most, d, WAVE));
+            return most;
+        });
+        const float inv = to.inverse();
+        if (hidden) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] *= inv;
+        } else {
+            share(mine * inv, lane, room);
+        }
+    }
+    template <int D>
+    __device__ __forceinline__ void weigh(Softmax<D>& to, const f32x16& z, u32x4 (&w)[2], float c, int i) const {
+        to.weigh(z, x[2 * i], x[2 * i + 1], w, c, i);
+    }
+};
 
 __device__ __forceinline__ f32x16 zeros() {
     f32x16 z;
@@ -220,7 +286,7 @@ struct Walk {
     Softmax<D> to;
     QueryFragment<D> q;
     TileWords<D> t[NG];
-    TileScales s;
+    TileScales<NG> s;
     f32x16 z;
 
     __device__ __forceinline__ static int group(int lane) { return NG == 1 ? 0 : (lane & 31) / COLUMNS; }
@@ -249,20 +315,17 @@ struct Walk {
         return all;
     }
 
-    // a batch whose K has been multiplied: `hidden` and left as for `hide`; next_k() asks for the K behind the next batch's, next_v() for the
+    // a batch whose K has been multiplied: `hidden` and left as for its scales; next_k() asks for the K behind the next batch's, next_v() for the
     // next batch's V
     template <class NextK, class NextV>
-    __device__ __forceinline__ void batch(bool hidden, int left, float c, int lane, NextK next_k, NextV next_v) {
-        uint32_t sc[8];
-        s.get(sc);
-        if (hidden) hide(z, sc, left, lane);
-        to.move(z, sc, c);
+    __device__ __forceinline__ void batch(bool hidden, int left, float c, int lane, float* room, NextK next_k, NextV next_v) {
+        s.move(to, z, c, hidden, left, lane, room);
         u32x4 w[2];
         // ahead of the CU's other workgroup meanwhile: two waves in step would multiply together and then wait for the vector unit together
         __builtin_amdgcn_s_setprio(1);
         const f32x16 ahead = scores(lane, [&](int n) {
 #pragma unroll
-            for (int i = 8 * n / PRODUCTS; i < 8 * (n + 1) / PRODUCTS; ++i) to.weigh(z, sc, w, c, i);
+            for (int i = 8 * n / PRODUCTS; i < 8 * (n + 1) / PRODUCTS; ++i) s.weigh(to, z, w, c, i);
         });
         __builtin_amdgcn_s_setprio(0);
         next_k();
@@ -296,6 +359,7 @@ template <int D>
 struct Meet {  // the columns of the four waves
     float o[WAVES * PAIRS][D + 4];
     float m[WAVES * PAIRS], l[WAVES * PAIRS];
+    float scales[WAVES][KV4_TOKENS];  // of a wave's tile
 };
 
 // a tile of pairs' columns, of which `here` are pairs, added up; behind a barrier
@@ -397,7 +461,7 @@ __device__ __forceinline__ void kv4_span(const AttnKv4& p, const KvSpan& a, Meet
             const int next_i = i;
             place = give(next, next_i);
             w.batch(
-                hidden, left, p.c, lane,
+                hidden, left, p.c, lane, meet.scales[wave],
                 [&] {
                     on();
                     request_k(at, i);

@@ -423,6 +423,22 @@ def test_values_of_unlike_size(card, D):
     _attend(card, _rows(g, 40, G, D) * 3.0, pool, tables, [n], [40], G, page)
 
 
+@pytest.mark.parametrize("byte", [0xFF, 0x7F, 0x00])
+@pytest.mark.parametrize("G,rows", [(4, 40), (8, 3), (1, 90)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_large_value_that_not_every_row_sees(card, D, G, rows, byte):
+    """rows before it keep their own precision; so do all where what lies behind the last token has the largest scale there is"""
+    g = gen(9950 + D + G)
+    page, n, at = 32, 300, 300 - rows // 2
+    tables, pages = _tables(g, [n], page)
+    pool = _filled(card, pages, 1, D, page, byte)
+    k, v = _rows(g, n, 1, D), _rows(g, n, 1, D) * 2.0**-9
+    v[at] *= 2.0**60
+    v[at + 1:] *= 2.0**20
+    card.kv4_write(k, v, pool, tables, _i32([n]))
+    _attend(card, _rows(g, rows, G, D), pool, tables, [n], [rows], G, page)
+
+
 def test_far_pages(card):
     """pages whose bytes start past 2^32, in a pool with a row of layers a page"""
     g = gen(9950)
