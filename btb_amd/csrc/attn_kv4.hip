@@ -526,9 +526,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attn_kv4_kernel(AttnKv4 p) {
     const int any = a.len - a.n + last / p.G + 1;
     a.from = a.span * length;
     a.to = min(min(a.from + length, tiles), any < 1 ? 0 : (any - 1) / KV4_TOKENS + 1);
-    // Few pairs: several tiles at a time. At head_dim 128 four of them do not fit the registers: 131072 tokens of one row 36 us by two,
-    // 38 by one, 62 by four; 64 sequences of up to 8192 80, 96 and 137. Tiles that this workgroup alone reads are not kept in the caches: 36 -> 33 and
-    // 80 -> 76, but 61 -> 65 for prompts beside single tokens where others read them too.
+    // Few pairs: several tiles at a time. At head_dim 128 four of them do not fit the registers: 131072 tokens of one row 32.5 us by two,
+    // 33.5 by one, 61 by four; 64 sequences of up to 8192 71, 83 and 135. Tiles that this workgroup alone reads are not kept in the caches: 35 -> 32 and
+    // 78 -> 71, but 54 -> 55 for prompts beside single tokens where others read them too.
     constexpr int NG = D == 64 ? 4 : 2;
     if (a.pairs <= PAIRS / NG)
         kv4_span<D, NG, true>(p, a, meet);
@@ -681,8 +681,8 @@ static Kv4Plan kv4_plan(size_t T, size_t B, size_t Hk, size_t G, size_t keys_cap
     Kv4Plan plan;
     plan.groups = (long long)(ragged ? T * G / PAIRS + B : B * ((T / B * G + PAIRS - 1) / PAIRS));
     const size_t tiles = (keys_cap + KV4_TOKENS - 1) / KV4_TOKENS;
-    // two workgroups a CU, as many as fit (131072 tokens of one row: 32 us, 37 with three, 44 with six; without a second round 500 rows over
-    // 16384 are 175 instead of 183). One of eight waves a CU instead: 64 sequences 74 -> 82, prompts beside single tokens 57 -> 64.
+    // two workgroups a CU, as many as fit (131072 tokens of one row: 32 us, 43 with three, 47 with six; without a second round 500 rows over
+    // 16384 are 160 instead of 173). One of eight waves a CU instead: 64 sequences 71 -> 77, prompts beside single tokens 54 -> 61.
     const size_t want = (size_t)(8 / WAVES) * device_info().cus / (plan.groups * Hk);
     size_t S = want < 1 ? 1 : want;
     // (a second launch, for the join, pays from 32 tiles on: 700 tokens of one row take 12.6 us in two spans, 10.0 in one)
