@@ -31,6 +31,7 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float NONE = -3.0e38f;   // a maximum of nothing: what is subtracted from it underflows to weight 0
 constexpr int ROOM = 11;           // a weight of 1 times the largest scale, in units of the power of two above that, as f16
 constexpr float LAG = 4.f;         // how far, in powers of two, scores may pass the maximum in use: f16 ends at 2^16
+constexpr float FAR = 0x1p20f;     // a maximum from which on its own rounding, half of 2^-3, would tell in the weights' range
 constexpr int PAIRS = 32;          // (row, query head) pairs a workgroup
 
 struct AttnKv4 {
@@ -103,9 +104,10 @@ struct Softmax {
 
     // The maximum and the unit moved to where a tile's scores z and its scales need them. Whether they do each lane asks of its own scores and
     // scales (`past`), and without working out by how much: 500 rows of 32 heads over 16384 tokens take 161 us instead of 166, at head_dim 64 111
-    // instead of 125. most(): the largest of the pair's scales, as bits; NaN is below all.
+    // instead of 125. Where a maximum is so large that its own rounding would tell in the weights, scores are rounded as it was before it is taken from
+    // them: z is then times c, and c 1. most(): the largest of the pair's scales, as bits; NaN is below all.
     template <class Most>
-    __device__ __forceinline__ void move(const f32x16& z, bool past, float c, Most most) {
+    __device__ __forceinline__ void move(f32x16& z, bool past, float& c, Most most) {
         float top = z[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = fmaxf(top, z[i]);
@@ -121,7 +123,14 @@ struct Softmax {
             for (int d = 0; d < DT; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= both;
-            m = to, over = (m + LAG) / c;
+            const bool large = fabsf(to) > FAR && to != NONE;
+            // (a pair with such a maximum comes here with every tile it sees anything of)
+            m = to, over = large ? -__builtin_inff() : (m + LAG) / c;
+            if (__any(large)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) z[i] *= c;
+                c = 1.f;
+            }
             below = (f32_bits(above) >> 16) * 0x00010001u - 0x00010001u;
         }
     }
@@ -189,7 +198,7 @@ struct TileScales {
         for (int i = 0; i < 2; ++i) s[i] = reinterpret_cast<const uint4*>(scales + 32 * (lane >> 5))[i];
     }
     template <int D>
-    __device__ __forceinline__ void move(Softmax<D>& to, f32x16& z, float c, bool hidden, int left, int lane, float*) {
+    __device__ __forceinline__ void move(Softmax<D>& to, f32x16& z, float& c, bool hidden, int left, int lane, float*) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = dword(s[i / 4], i % 4);
         if (hidden)
@@ -234,7 +243,7 @@ struct TileScales<1> {
         __builtin_amdgcn_wave_barrier();
     }
     template <int D>
-    __device__ __forceinline__ void move(Softmax<D>& to, f32x16& z, float c, bool hidden, int left, int lane, float* room) {
+    __device__ __forceinline__ void move(Softmax<D>& to, f32x16& z, float& c, bool hidden, int left, int lane, float* room) {
         const float mine = bits_f32((uint32_t)s << 16);
         int big = s;
         if (hidden) {  // (from here on the pairs' units may differ)

@@ -349,6 +349,37 @@ def test_in_the_place_of_its_rows(card, lens, rows, Hk, G, D):
     assert torch.equal(att, q) and bool(att.any())
 
 
+@pytest.mark.parametrize("size", [2.0**4, 2.0**9, 2.0**12, 2.0**30])
+@pytest.mark.parametrize("G,rows,n", [(4, 40, 240), (4, 1, 240), (2, 3, 9000), (8, 200, 240)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_scores_of_any_size(card, D, G, rows, n, size):
+    """one key is far above the others a row sees: its value is the output, whatever the scores' own rounding"""
+    g = gen(9560 + D + G)
+    page, scale = 64, 0.1
+    held = torch.full((n,), 0.5)
+    held[37], held[n - 30], held[n - 10] = 4.0, 6.0, -6.0
+    tables, pages = _tables(g, [n], page)
+    pool = _filled(card, pages, 1, D, page)
+    k = (held * size).cuda()[:, None, None].expand(n, 1, D).to(torch.bfloat16).contiguous()
+    v = _rows(g, n, 1, D)
+    card.kv4_write(k, v, pool, tables, _i32([n]))
+    q = torch.full((rows, G * D), size, dtype=torch.bfloat16, device="cuda")
+    att, lse = torch.zeros_like(q), torch.zeros(rows, G, device="cuda")
+    scratch = card.attn_kv4_scratch(rows, 1, G, 1, D, n)
+    card.attn_kv4(q, pool, tables, _i32([n]), att, G, 1, D, scale, scratch, first=_first([rows]), lse=lse)
+    torch.cuda.synchronize()
+    V = torch.from_numpy(kv4.held_v(v.double().cpu().numpy())[0][:, 0])
+    scale = float(np.float32(scale))
+    for i in range(rows):
+        sees = n - rows + i + 1
+        best = n - 30 if sees > n - 30 else 37
+        if sees > 37:
+            off = (att[i].view(G, D).double().cpu() - V[best]).abs()
+            assert bool((off <= (W + H) * V[best].abs()).all()), i
+            s = scale * D * size * size * float(held[best])
+            assert np.allclose(lse[i].cpu().numpy(), s, rtol=4 * 2.0**-23, atol=0), i
+
+
 def test_attention_without_anything_to_see(card):
     """lengths of zero and below, rows before the first token, sequences without rows, rows behind the last sequence"""
     g = gen(9600)
