@@ -380,6 +380,32 @@ def test_scores_of_any_size(card, D, G, rows, n, size):
             assert np.allclose(lse[i].cpu().numpy(), s, rtol=4 * 2.0**-23, atol=0), i
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_ragged_sequences(card, D):
+    """more sequences than are looked through at a time, some without rows where the looking goes on; long ones in spans"""
+    g = gen(9580 + D)
+    B, Hk, G, page = 150, 1, 4, 64
+    rows = [(3 * b) % 5 for b in range(B)]
+    rows[62:67], rows[127:129], rows[149], rows[100], rows[140] = [0] * 5, [0, 9], 0, 40, 33
+    lens = [r + (7 * b) % 50 for b, r in enumerate(rows)]
+    lens[3], lens[70], lens[128], lens[140], lens[148] = 1500, 900, 1200, 700, 600
+    tables, pages = _tables(g, lens, page)
+    T, n = sum(rows), sum(lens)
+    pool = _filled(card, pages, Hk, D, page)
+    k, v = _rows(g, n, Hk, D), _rows(g, n, Hk, D)
+    card.kv4_write(k, v, pool, tables, _i32(lens), first=_first(lens))
+    at = torch.cat([torch.arange(e - r, e) for e, r in zip(np.cumsum(lens).tolist(), rows)]).cuda()
+    new_k, new_v = _rows(g, T, Hk, D), _rows(g, T, Hk, D)
+    card.kv4_write(new_k, new_v, pool, tables, _i32(lens), first=_first(rows))  # the last rows once more, others
+    k[at], v[at] = new_k, new_v
+    for what, want, count in (("the pass's", (new_k, new_v), rows), ("all", (k, v), lens)):
+        a, b = (torch.zeros(sum(count), Hk, D, device="cuda") for _ in range(2))
+        card.kv4_read(pool, tables, _i32(lens), a, b, first=_first(count))
+        assert _same(a, kv4.held_k(want[0].double().cpu().numpy())[0]), what
+        assert _same(b, kv4.held_v(want[1].double().cpu().numpy())[0]), what
+    _attend(card, _rows(g, T, Hk * G, D), pool, tables, lens, rows, G, page, cap=1500)
+
+
 def test_attention_without_anything_to_see(card):
     """lengths of zero and below, rows before the first token, sequences without rows, rows behind the last sequence"""
     g = gen(9600)
