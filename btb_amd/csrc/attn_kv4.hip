@@ -723,8 +723,8 @@ static int32_t launch_attn_kv4(const AttnKv4& p, const Kv4Plan& plan, hipStream_
 using namespace btb;
 
 extern "C" size_t btb_hip_attn_kv4_floats(size_t T, size_t B, size_t Hq, size_t Hk, size_t D, size_t keys_cap) {
-    if (T == 0 || T > (1u << 24) || B == 0 || B > 65536 || Hk == 0 || Hq % Hk != 0 || Hq == 0 || Hq / Hk > 64 || (D != 64 && D != 128) ||
-        keys_cap == 0 || keys_cap > (1u << 30))
+    if (T == 0 || T > (1u << 24) || B == 0 || B > 65536 || Hk == 0 || Hk > 1024 || Hq % Hk != 0 || Hq == 0 || Hq / Hk > 64 ||
+        T * Hq > (1u << 24) || (D != 64 && D != 128) || keys_cap == 0 || keys_cap > (1u << 30))
         return 0;
     // a call may come with `first` or without
     const Kv4Plan a = kv4_plan(T, B, Hk, Hq / Hk, keys_cap, true);
@@ -743,7 +743,7 @@ extern "C" int32_t btb_hip_attn_kv4(const void* q, const void* cache, const int3
     auto loose = [](const void* a) { return ((uintptr_t)a & 15u) != 0; };
     AttnKv4 p{};
     if (!kv4_seqs(p.seqs, tables, lens, first, B, W, pages, page, stride, T, Hk, D) ||
-        btb_hip_attn_kv4_floats(T, B, Hq, Hk, D, keys_cap) == 0 || T * Hq > (1u << 24) || !(scale > 0.f) || scale > 3.4e38f || loose(q) || loose(cache) || loose(att) ||
+        btb_hip_attn_kv4_floats(T, B, Hq, Hk, D, keys_cap) == 0 || !(scale > 0.f) || scale > 3.4e38f || loose(q) || loose(cache) || loose(att) ||
         loose(workspace)) {
         set_error("attn_kv4: " KV4_DOMAIN ", up to 64 query heads a kv head, 2^24 rows times query heads, scale > 0, keys_cap 1 .. 2^30; "
                   "q, cache, att and workspace 16-byte aligned");

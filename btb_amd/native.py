@@ -1300,7 +1300,8 @@ class HipCard(CardLaunch):
         """the f32 scratch `attn_kv4` leaves its states in, at these sizes"""
         n = int(self.lib.btb_hip_attn_kv4_floats(T, B, Hq, Hk, D, keys_cap))
         if n == 0:
-            raise ValueError("[hip] attn_kv4 takes head_dim 64 or 128, 1 .. 64 query heads a kv head and keys_cap 1 .. 2^30")
+            raise ValueError("[hip] attn_kv4 takes head_dim 64 or 128, up to 1024 kv heads, 1 .. 64 query heads each, rows times query "
+                             "heads up to 2^24 and keys_cap 1 .. 2^30")
         return torch.empty(n, dtype=torch.float32, device=device)
 
     def attn_kv4(self, q: torch.Tensor, cache: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, att: torch.Tensor, Hq: int, Hk: int,

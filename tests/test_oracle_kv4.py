@@ -184,3 +184,14 @@ def test_outputs_over_each_other_or_the_input():
     assert _read(lib, v=P) == native.ERR_DOMAIN and b"share memory" in lib.btb_hip_last_error()
     for at in (0x1010, 0x1000 + 6 * 32 * 128 * 2 - 16, 0x1000 - 16):  # all but the first 16 bytes, the last, all but the last
         assert _attn(lib, q=P, att=ctypes.c_void_p(at)) == native.ERR_DOMAIN and b"across q" in lib.btb_hip_last_error()
+
+
+@pytest.mark.parametrize("other", [dict(Hk=1025, Hq=1025), dict(Hq=1 << 62, Hk=1 << 62), dict(B=2, Hq=1 << 63, Hk=1 << 63), dict(T=1 << 20, Hq=32),
+                                   dict(B=8, Hq=1 << 63, Hk=1 << 61), dict(T=(1 << 24) + 1), dict(B=65537), dict(keys=1 << 63)])
+def test_a_workspace_is_refused_where_the_call_is(other):
+    """sizes whose product wraps to zero would end the process in a division by it"""
+    a = dict(T=1, B=1, Hq=32, Hk=8, D=128, keys=100)
+    a.update(other)
+    lib = native.load_library()
+    assert lib.btb_hip_attn_kv4_floats(*a.values()) == 0
+    assert lib.btb_hip_attn_kv4_floats(1, 1, 1024, 1024, 128, 100) > 0 and lib.btb_hip_attn_kv4_floats(1 << 18, 1, 64, 1, 64, 1 << 30) > 0
