@@ -253,7 +253,7 @@ static int32_t kv4_rows(Kv4Rows& p, const void* cache, const int32_t* tables, co
                         size_t W, size_t pages, size_t page, int64_t stride, size_t T, size_t Hk, size_t D, int64_t kt, int64_t kh,
                         int64_t vt, int64_t vh, const void* k, const void* v, const char* what) {
     auto loose = [](const void* a) { return ((uintptr_t)a & 15u) != 0; };
-    auto odd = [](size_t n, int64_t s) { return n > 1 && (s < 0 || s % 8 != 0); };  // (one alone has no next)
+    auto odd = [](size_t n, int64_t s) { return n > 1 && (s < 0 || s % 8 != 0 || s > ((int64_t)1 << 46) / (int64_t)n); };  // (one alone has no next)
     if (!kv4_seqs(p.seqs, tables, lens, first, B, W, pages, page, stride, T, Hk, D) || odd(T, kt) || odd(Hk, kh) || odd(T, vt) || odd(Hk, vh) ||
         loose(cache) || loose(k) || loose(v)) {
         set_error(what);

@@ -536,7 +536,7 @@ int32_t btb_hip_kv_evict(const float* mass, int64_t ms, const int32_t* pos, int6
 size_t btb_hip_kv4_tile_bytes(size_t D);
 
 /* The pass's rows into the cache: k and v bf16, row t of head g at t * k_row + g * k_head (v_row, v_head) values, 16-byte aligned,
- * strides multiples of 8. A row in a page outside the pool is not written. No two sequences may write to one page. */
+ * strides multiples of 8, from 0 to 2^46 over the rows, or heads. A row in a page outside the pool is not written. No two sequences may write to one page. */
 int32_t btb_hip_kv4_write(const void* k, const void* v, void* cache, const int32_t* tables, const int32_t* lens,
                           const int32_t* first, size_t B, size_t W, size_t pages, size_t page, int64_t stride, size_t T,
                           size_t Hk, size_t D, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, void* stream);

@@ -195,3 +195,9 @@ def test_a_workspace_is_refused_where_the_call_is(other):
     lib = native.load_library()
     assert lib.btb_hip_attn_kv4_floats(*a.values()) == 0
     assert lib.btb_hip_attn_kv4_floats(1, 1, 1024, 1024, 128, 100) > 0 and lib.btb_hip_attn_kv4_floats(1 << 18, 1, 64, 1, 64, 1 << 30) > 0
+
+
+@pytest.mark.parametrize("other", [dict(kr=1 << 60), dict(kh=1 << 60), dict(vr=(1 << 63) - 8), dict(vh=1 << 44)])
+def test_strides_past_any_memory(other):
+    lib = native.load_library()
+    assert _write(lib, **other) == native.ERR_DOMAIN and _read(lib, **other) == native.ERR_DOMAIN
