@@ -274,6 +274,26 @@ static int32_t kv4_rows(Kv4Rows& p, const void* cache, const int32_t* tables, co
     return OK;
 }
 
+// Whether two outputs of such rows, the second `apart` values behind the first, have a value in common. The differences between their places are
+// apart + i head + j row, |i| < heads and |j| < rows, and each of them holds D values; at other strides the outputs are apart where their ranges are. Rows
+// of one output are D values apart or more.
+static bool kv4_outputs_meet(const Kv4Rows& p, int64_t apart, int64_t D) {
+    const int64_t T = p.seqs.T, Hk = p.Hk;
+    const int64_t kt = T > 1 ? p.kt : 0, vt = T > 1 ? p.vt : 0, kh = Hk > 1 ? p.kh : 0, vh = Hk > 1 ? p.vh : 0;
+    if (apart >= (T - 1) * kt + (Hk - 1) * kh + D || -apart >= (T - 1) * vt + (Hk - 1) * vh + D) return false;
+    if (kt != vt || kh != vh) return true;
+    for (int64_t i = 1 - Hk; i < Hk; ++i) {
+        const int64_t x = apart + i * kh;
+        if (T == 1) {
+            if (x > -D && x < D) return true;
+            continue;
+        }
+        const int64_t rest = (x % kt + kt) % kt, rows = (x - rest) / kt;  // x = rows kt + rest: the rows next to it
+        if ((rest < D && rows > -T && rows < T) || (kt - rest < D && rows + 1 > -T && rows + 1 < T)) return true;
+    }
+    return false;
+}
+
 }  // namespace btb
 
 using namespace btb;
@@ -313,7 +333,8 @@ extern "C" int32_t btb_hip_kv4_read(const void* cache, const int32_t* tables, co
         return (T > 1 && row < (int64_t)D) || (Hk > 1 && head < (int64_t)D) ||
                (T > 1 && Hk > 1 && row < (int64_t)Hk * head && head < (int64_t)T * row);
     };
-    if (shared(k_row, k_head) || shared(v_row, v_head) || k == v) {
+    const int64_t apart = ((int64_t)(uintptr_t)v - (int64_t)(uintptr_t)k) / (out_f32 ? 4 : 2);
+    if (shared(k_row, k_head) || shared(v_row, v_head) || kv4_outputs_meet(p, apart, (int64_t)D)) {
         set_error("kv4_read: rows or heads of an output, or both outputs, share memory");
         return ERR_DOMAIN;
     }

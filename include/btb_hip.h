@@ -542,7 +542,8 @@ int32_t btb_hip_kv4_write(const void* k, const void* v, void* cache, const int32
                           size_t Hk, size_t D, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, void* stream);
 
 /* The pass's rows as the cache holds them: into k and v, laid out as above, f32 (out_f32 != 0) or, rounded, bf16. A row in a page
- * outside the pool reads as zeros. Rows and heads of an output, and the outputs, must not share memory. */
+ * outside the pool reads as zeros. Rows and heads of an output, and the outputs, must not share memory: refused (outputs of equal strides may lie
+ * between each other's rows and heads, others not within each other's range). */
 int32_t btb_hip_kv4_read(const void* cache, const int32_t* tables, const int32_t* lens, const int32_t* first, size_t B,
                          size_t W, size_t pages, size_t page, int64_t stride, size_t T, size_t Hk, size_t D, void* k, void* v,
                          int32_t out_f32, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, void* stream);

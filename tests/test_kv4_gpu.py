@@ -211,6 +211,26 @@ def test_one_row_or_head_of_any_stride(card):
         assert _same(b, torch.from_numpy(want).bfloat16().double().numpy())
 
 
+@pytest.mark.parametrize("T,Hk", [(45, 2), (1, 3), (7, 1), (1, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_read_into_one_fused_tensor(card, T, Hk, dtype):
+    """outputs between each other's rows and heads: a row's keys before its values, a head's, a sequence's, a layer's"""
+    g = gen(9370 + T)
+    D, page = 64, 32
+    tables, pages = _tables(g, [T], page)
+    pool, k, v = _filled(card, pages, Hk, D, page), _rows(g, T, Hk, D), _rows(g, T, Hk, D)
+    card.kv4_write(k, v, pool, tables, _i32([T]))
+    want = [torch.from_numpy(x).to(dtype) for x in (kv4.held_k(k.double().cpu().numpy())[0], kv4.held_v(v.double().cpu().numpy())[0])]
+    for shape, split in (((T, 2 * Hk, D), lambda t: (t[:, :Hk], t[:, Hk:])), ((T, Hk, 2, D), lambda t: (t[:, :, 0], t[:, :, 1])),
+                         ((2, T, Hk, D), lambda t: (t[0], t[1])), ((Hk, 2, T, D), lambda t: (t[:, 0].transpose(0, 1), t[:, 1].transpose(0, 1))),
+                         ((Hk, T, 2, D), lambda t: (t[:, :, 1].transpose(0, 1), t[:, :, 0].transpose(0, 1))),
+                         ((2, Hk, T + 1, D), lambda t: (t[1, :, 1:].transpose(0, 1), t[0, :, :T].transpose(0, 1)))):
+        t = torch.full(shape, 9.0, dtype=dtype, device="cuda")
+        a, b = split(t)
+        card.kv4_read(pool, tables, _i32([T]), a, b)
+        assert torch.equal(a.cpu(), want[0]) and torch.equal(b.cpu(), want[1]), shape
+
+
 def test_rows_that_are_nobodys_and_pages_that_are_not_there(card):
     g = gen(9400)
     Hk, D, page, T = 1, 64, 32, 40

@@ -197,6 +197,36 @@ def test_a_workspace_is_refused_where_the_call_is(other):
     assert lib.btb_hip_attn_kv4_floats(1, 1, 1024, 1024, 128, 100) > 0 and lib.btb_hip_attn_kv4_floats(1 << 18, 1, 64, 1, 64, 1 << 30) > 0
 
 
+@pytest.mark.parametrize("f32", [0, 1])
+def test_read_refuses_outputs_that_lie_across_each_other(f32):
+    lib, size, at = native.load_library(), 4 if f32 else 2, 0x10000000
+
+    def read(apart, **other):
+        """the second output so many values behind the first; strides as given, for both"""
+        a = {**ROWS, **other}
+        return lib.btb_hip_kv4_read(a["cache"], a["tables"], a["lens"], a["first"], a["B"], a["W"], a["pages"], a["page"], a["stride"], a["T"],
+                                    a["Hk"], a["D"], ctypes.c_void_p(at), ctypes.c_void_p(at + apart * size), f32, a["kr"], a["kh"], a["vr"],
+                                    a["vh"], None)
+
+    whole = 6 * 1024  # rows one after another: any place inside the other's
+    for apart in (8, 128, 1024, 1024 + 8, whole - 8, -8, -128, -1024, 8 - whole):
+        assert read(apart) == native.ERR_DOMAIN and b"share memory" in lib.btb_hip_last_error(), apart
+    fused = dict(kr=2048, vr=2048)  # room for the other between the rows: 1024 values in, and only there
+    for apart in (1024 - 8, 1024 + 8, 2048, 4096 - 8, -8, 8 - 1024, 2048 * 5 + 8):
+        assert read(apart, **fused) == native.ERR_DOMAIN, apart
+    heads = dict(kr=128, vr=128, kh=6 * 256, vh=6 * 256)  # head after head, with room between them
+    for apart in (6 * 128 - 8, 8, -8, 6 * 256, 7 * 6 * 256 + 8):
+        assert read(apart, **heads) == native.ERR_DOMAIN, apart
+    one = dict(B=1, T=1, kr=0, vr=0, kh=256, vh=256)  # a row alone, and a head alone
+    for apart in (8, -8, 120, 256, 256 * 7 + 120):
+        assert read(apart, **one) == native.ERR_DOMAIN, apart
+    alone = dict(Hk=1, kr=256, vr=256, kh=0, vh=0, stride=2 * 4288)
+    for apart in (8, -8, 120, 256, 256 * 5 + 120):
+        assert read(apart, **alone) == native.ERR_DOMAIN, apart
+    for other in (dict(kr=2048, vr=1024), dict(vr=2048), dict(kr=128, kh=1024)):  # unlike strides, inside each other's range
+        assert read(1024, **other) == native.ERR_DOMAIN, other
+
+
 @pytest.mark.parametrize("other", [dict(kr=1 << 60), dict(kh=1 << 60), dict(vr=(1 << 63) - 8), dict(vh=1 << 44)])
 def test_strides_past_any_memory(other):
     lib = native.load_library()
