@@ -40,11 +40,14 @@ struct AttnKv4 {
     const uint8_t* cache;
     uint16_t* att;
     float* lse;
-    float* part;     // a pair's spans: maximum and sum [T Hq, S, 2], then outputs [T Hq, S, D]
+    float* part;     // a pair's spans: maximum and sum [T Hq, S, 2], then, from the next 16 bytes on, outputs [T Hq, S, D]
     float c;         // scale log2(e)
     int Hq, Hk, G;
     int S;           // spans a sequence at most
 };
+
+// floats of `states` spans' maxima and sums: the outputs behind them are written and read 16 bytes at a time
+__host__ __device__ __forceinline__ size_t kv4_states(size_t states) { return (2 * states + 3) / 4 * 4; }
 
 // tiles a span of a sequence of `tiles`, each span but the last: what S spans come to, two a wave at least
 constexpr int LEAST = 2 * WAVES;
@@ -401,7 +404,7 @@ __device__ __forceinline__ void kv4_meet(const AttnKv4& p, const KvSpan& a, cons
         } else {
             const size_t slot = at_pair * p.S + a.span;
             if (dim == 0) reinterpret_cast<float2*>(p.part)[slot] = make_float2(to, sum);
-            *reinterpret_cast<float4*>(p.part + 2 * (size_t)p.seqs.T * p.Hq * p.S + slot * D + dim) = x;
+            *reinterpret_cast<float4*>(p.part + kv4_states((size_t)p.seqs.T * p.Hq * p.S) + slot * D + dim) = x;
         }
     }
 }
@@ -574,7 +577,7 @@ __device__ __forceinline__ bool kv4_parts(const AttnKv4& p, unsigned pair, int D
     const int tiles = (p.seqs.held(p.seqs.len(b)) + KV4_TOKENS - 1) / KV4_TOKENS, length = kv4_span_tiles(p, tiles);
     parts.spans = (tiles + length - 1) / length;
     parts.ml = reinterpret_cast<const float2*>(p.part) + (size_t)pair * p.S;
-    parts.o = p.part + 2 * (size_t)p.seqs.T * p.Hq * p.S + (size_t)pair * p.S * D;
+    parts.o = p.part + kv4_states((size_t)p.seqs.T * p.Hq * p.S) + (size_t)pair * p.S * D;
     return parts.spans > 1;
 }
 __device__ __forceinline__ void kv4_lse(const AttnKv4& p, unsigned pair, float m, float l) {
@@ -733,7 +736,7 @@ extern "C" size_t btb_hip_attn_kv4_floats(size_t T, size_t B, size_t Hq, size_t 
         const Kv4Plan e = kv4_plan(T, B, Hk, Hq / Hk, keys_cap, false);
         if ((size_t)e.S > S) S = (size_t)e.S;
     }
-    return S == 1 ? 4 : T * Hq * S * (D + 2);
+    return S == 1 ? 4 : kv4_states(T * Hq * S) + T * Hq * S * D;
 }
 
 extern "C" int32_t btb_hip_attn_kv4(const void* q, const void* cache, const int32_t* tables, const int32_t* lens, const int32_t* first,

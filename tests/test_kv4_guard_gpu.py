@@ -9,6 +9,7 @@ import torch
 
 from .helpers import gen
 from .test_guard_gpu import Fenced
+from .test_kv4_gpu import _check, _put
 
 pytestmark = pytest.mark.gpu
 
@@ -58,6 +59,25 @@ def test_rows_and_attention(card, lens, rows, Hk, G, D, page, cap):
     card.attn_kv4(q, pool, tables, _i32(lens), att.t, Hk * G, Hk, D, 0.1, ws.t, first=first(rows), lse=lse.t, keys_cap=cap)
     for o, what in ((att, "att"), (lse, "lse"), (ws, "the workspace")):
         o.check(f"attn_kv4: {what}")
+
+
+@pytest.mark.parametrize("lens,rows,G,D", [([9000], 1, 3, 128), ([9000], 1, 3, 64), ([1400], 1, 1, 64), ([1400], 1, 3, 128),
+                                           ([3001, 2000, 33, 900, 1, 1500, 2999], 1, 5, 128), ([2500, 40, 2100], 1, 3, 64)])
+def test_an_odd_number_of_spans(card, lens, rows, G, D):
+    """rows x heads x spans odd, few of them and many: the workspace of exactly its size, and the rows are the oracle's"""
+    g = gen(11050 + sum(lens) + G)
+    pool, tables, _, _ = _put(card, g, lens, 1, D, 64)
+    T, cap = rows * len(lens), max(lens)
+    q = torch.randn(T, G, D, generator=g).to(torch.bfloat16).cuda()
+    att, lse = Fenced((T, G * D), torch.bfloat16), Fenced((T, G), torch.float32)
+    floats = card.attn_kv4_scratch(T, len(lens), G, 1, D, cap).numel()
+    ws = Fenced((floats,), torch.float32)
+    assert floats > 4 and ws.t.data_ptr() % 16 == 0
+    scale = D**-0.5
+    card.attn_kv4(q.view(T, -1), pool, tables, _i32(lens), att.t, G, 1, D, scale, ws.t, lse=lse.t, keys_cap=cap)
+    for o, what in ((att, "att"), (lse, "lse"), (ws, "the workspace")):
+        o.check(f"attn_kv4: {what}")
+    _check(q, pool, tables, lens, [rows] * len(lens), att.t, lse.t, scale, G, 64)
 
 
 @pytest.mark.parametrize("L,pages,nb,B,W,page", [(1, 7, 16, 3, 3, 32), (3, 50, 4288, 6, 9, 64), (2, 33, 16400, 2, 20, 96)])

@@ -231,3 +231,10 @@ def test_read_refuses_outputs_that_lie_across_each_other(f32):
 def test_strides_past_any_memory(other):
     lib = native.load_library()
     assert _write(lib, **other) == native.ERR_DOMAIN and _read(lib, **other) == native.ERR_DOMAIN
+
+
+@pytest.mark.parametrize("T,B,Hq,D,keys", [(1, 1, 3, 128, 9000), (1, 1, 1, 64, 1400), (7, 7, 5, 128, 3001), (3, 3, 3, 64, 2500)])
+def test_spans_outputs_lie_in_whole_pieces(T, B, Hq, D, keys):
+    """an odd number of maxima and sums is filled up to 16 bytes: the outputs behind them are written 16 bytes at a time"""
+    n = native.load_library().btb_hip_attn_kv4_floats(T, B, Hq, 1, D, keys)
+    assert n > 4 and n % 4 == 0  # (outputs are a multiple of four floats themselves)
