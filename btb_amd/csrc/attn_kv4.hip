@@ -14,6 +14,8 @@
 // bf16 weight would be off by 2^-8, two of them cost twice the products. The unit in the maximum instead of in the scales would save a product
 // a weight (1 % of the time), but not the last bits of lse.
 
+#include <cfloat>
+
 #include "btb_kv4.hpp"
 #include "btb_tuning.hpp"
 
@@ -746,9 +748,9 @@ extern "C" int32_t btb_hip_attn_kv4(const void* q, const void* cache, const int3
     auto loose = [](const void* a) { return ((uintptr_t)a & 15u) != 0; };
     AttnKv4 p{};
     if (!kv4_seqs(p.seqs, tables, lens, first, B, W, pages, page, stride, T, Hk, D) ||
-        btb_hip_attn_kv4_floats(T, B, Hq, Hk, D, keys_cap) == 0 || !(scale > 0.f) || scale > 3.4e38f || loose(q) || loose(cache) || loose(att) ||
+        btb_hip_attn_kv4_floats(T, B, Hq, Hk, D, keys_cap) == 0 || !(scale > 0.f) || scale > FLT_MAX / LOG2E || loose(q) || loose(cache) || loose(att) ||
         loose(workspace)) {
-        set_error("attn_kv4: " KV4_DOMAIN ", up to 64 query heads a kv head, 2^24 rows times query heads, scale > 0, keys_cap 1 .. 2^30; "
+        set_error("attn_kv4: " KV4_DOMAIN ", up to 64 query heads a kv head, 2^24 rows times query heads, scale from above 0 to 2^128 / log2(e), keys_cap 1 .. 2^30; "
                   "q, cache, att and workspace 16-byte aligned");
         return ERR_DOMAIN;
     }

@@ -400,6 +400,39 @@ def test_scores_of_any_size(card, D, G, rows, n, size):
             assert np.allclose(lse[i].cpu().numpy(), s, rtol=4 * 2.0**-23, atol=0), i
 
 
+@pytest.mark.parametrize("size,scale", [(2.0**58, 1.0), (1.0, 2.0**115), (2.0**58, 2.0**-116), (2.0**-40, 2.0**83), (2.0**-60, 2.0**127)])
+@pytest.mark.parametrize("G,rows,n", [(4, 40, 240), (4, 1, 240), (2, 3, 9000)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_products_and_scales_at_their_ends(card, D, G, rows, n, size, scale):
+    """products of q and k, and scales, near f32's largest and smallest: the key far above the others gives its value. D 6 size^2 is up to
+    2^125.6, and that times scale log2(e) up to 2^126.2; the best of them is 128 or more above the next
+    (D 2 size^2 scale)"""
+    g = gen(9570 + D + G)
+    page = 64
+    held = torch.full((n,), 0.5)
+    held[37], held[n - 30], held[n - 10] = 4.0, 6.0, -6.0
+    tables, pages = _tables(g, [n], page)
+    pool = _filled(card, pages, 1, D, page)
+    k = (held * size).cuda()[:, None, None].expand(n, 1, D).to(torch.bfloat16).contiguous()
+    v = _rows(g, n, 1, D)
+    card.kv4_write(k, v, pool, tables, _i32([n]))
+    q = torch.full((rows, G * D), size, dtype=torch.bfloat16, device="cuda")
+    att, lse = torch.zeros_like(q), torch.zeros(rows, G, device="cuda")
+    scratch = card.attn_kv4_scratch(rows, 1, G, 1, D, n)
+    card.attn_kv4(q, pool, tables, _i32([n]), att, G, 1, D, scale, scratch, first=_first([rows]), lse=lse)
+    torch.cuda.synchronize()
+    V = torch.from_numpy(kv4.held_v(v.double().cpu().numpy())[0][:, 0])
+    least = D * 2.0 * size * size * scale
+    for i in range(rows):
+        sees = n - rows + i + 1
+        best = n - 30 if sees > n - 30 else 37
+        assert sees > 37 and least >= 128
+        off = (att[i].view(G, D).double().cpu() - V[best]).abs()
+        assert bool((off <= (W + H) * V[best].abs()).all()), i
+        s = scale * D * size * size * float(held[best])
+        assert np.allclose(lse[i].cpu().numpy(), s, rtol=4 * 2.0**-23, atol=0), i
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_many_ragged_sequences(card, D):
     """more sequences than are looked through at a time, some without rows where the looking goes on; long ones in spans"""

@@ -238,3 +238,10 @@ def test_spans_outputs_lie_in_whole_pieces(T, B, Hq, D, keys):
     """an odd number of maxima and sums is filled up to 16 bytes: the outputs behind them are written 16 bytes at a time"""
     n = native.load_library().btb_hip_attn_kv4_floats(T, B, Hq, 1, D, keys)
     assert n > 4 and n % 4 == 0  # (outputs are a multiple of four floats themselves)
+
+
+@pytest.mark.parametrize("scale", [2.359e38, 2.4e38, 3.4e38])
+def test_a_scale_whose_exponent_overflows(scale):
+    """scores go through exp2: scale log2(e) is an f32 number too"""
+    lib = native.load_library()
+    assert _attn(lib, scale=scale) == native.ERR_DOMAIN and b"scale" in lib.btb_hip_last_error()
