@@ -37,6 +37,7 @@ class Paged:
         self.held: list[list[int]] = [[] for _ in range(seqs)]  # each sequence's pages
         self.length = [0] * seqs
         self.named = [0] * pages                                # how many sequences hold each page
+        self._sent = True                                       # whether tables and lens are the books'
         self._narrow, self._wide = _Pass(self, seqs), _Pass(self, rows)
 
     @property
@@ -67,15 +68,15 @@ class Paged:
                 raise ValueError(f"[paged] sequence {b} has {self.length[b]} of {self.longest} tokens, {len(part)} more were given")
         grown = {b: -(-(self.length[b] + len(part)) // self.page) - len(self.held[b]) for b, part in left.items()}
         fresh = self._take(sum(grown.values()), "a pass")
-        for b, n in grown.items():
-            for p in fresh[:n]:
-                self.named[p] = 1
-            self.held[b] += fresh[:n]
-            fresh = fresh[n:]
-        if any(grown.values()):
-            self._books()
         out: dict[int, torch.Tensor] = {}
         try:
+            for b, n in grown.items():
+                for p in fresh[:n]:
+                    self.named[p] = 1
+                self.held[b] += fresh[:n]
+                fresh = fresh[n:]
+            if any(grown.values()) or not self._sent:
+                self._books()
             while left:
                 p = self._narrow if sum(len(part) for part in left.values()) <= self.seqs else self._wide
                 room, now = p.T, {}
@@ -87,10 +88,11 @@ class Paged:
                 out.update({b: logits[i].clone() for i, b in enumerate(now) if b not in left})  # (the next pass writes over them)
         except BaseException:
             for b in grown:  # pages that it has not come to need
-                whole = -(-self.length[b] // self.page)
-                for p in self.held[b][whole:]:
-                    self.named[p] -= 1
-                del self.held[b][whole:]
+                del self.held[b][-(-self.length[b] // self.page):]
+            self.named = [0] * len(self.named)
+            for row in self.held:
+                for p in row:
+                    self.named[p] += 1
             self._books()
             raise
         return out
@@ -105,6 +107,8 @@ class Paged:
         parts = {dst: src for dst, src in branches.items() if self.length[src] % self.page}
         fresh = dict(zip(parts, self._take(len(parts), "a fork")))
         none = next(iter(fresh.values()), 0)
+        if not self._sent:
+            self._books()
         i32 = dict(dtype=torch.int32, device=self.lens.device)
         self.card.pages_fork(self.pool, self.tables, self.lens, torch.tensor(list(branches.values()), **i32),
                              torch.tensor(list(branches), **i32), torch.tensor([fresh.get(d, none) for d in branches], **i32), self.page)
@@ -123,6 +127,8 @@ class Paged:
 
     def compact(self) -> int:
         """the pages in use moved to the front of the pool; how many they are"""
+        if not self._sent:
+            self._books()
         self.card.pages_compact(self.pool, self.tables, self.lens, self.page)
         used = [p for p, k in enumerate(self.named) if k]
         n = len(used)
@@ -138,10 +144,12 @@ class Paged:
         self._narrow.capture()
 
     def _books(self) -> None:
-        """tables and lengths as the books have them, on the GPU"""
+        """tables and lengths as the books have them, on the GPU; where that fails, the next call sends them"""
+        self._sent = False
         width = self.tables.shape[1]
         self.tables.copy_(torch.tensor([row + [-1] * (width - len(row)) for row in self.held], dtype=torch.int32))
         self.lens.copy_(torch.tensor(self.length, dtype=torch.int32))
+        self._sent = True
 
 
 class _Pass:

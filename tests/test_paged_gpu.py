@@ -229,3 +229,47 @@ def test_a_pass_that_raises(card, stack):
     assert one.advance({}) == {}
     one.fork({})
     _books(one)
+
+
+class _Broken:
+    """a tensor that takes nothing"""
+
+    def __init__(self, t):
+        self.shape = t.shape
+
+    def copy_(self, *_):
+        raise RuntimeError("no")
+
+
+def test_books_that_cannot_be_sent(card, stack):
+    """a call whose tables do not reach the GPU leaves the books as they were, and the next one sends them"""
+    cfg, w = stack
+    one, two = (Paged(card, cfg, w, 3, 12, page=32, rows=40, longest=160) for _ in range(2))
+    for f in (one, two):
+        f.advance({0: _long(50, 7), 1: _long(20, 3)})
+    real, free = one.tables, one.free
+
+    def broken(call, *args):
+        one.tables = _Broken(real)
+        with pytest.raises(RuntimeError, match="no"):
+            call(*args)
+        one.tables = real
+
+    broken(one.advance, {0: _long(30, 5), 2: _long(70, 9)})  # two prompts that need pages
+    assert one.length == [50, 20, 0] and one.free == free and [len(h) for h in one.held] == [2, 1, 0]
+    a, b = (f.advance({0: [9], 1: [8]}) for f in (one, two))  # needs none
+    _books(one)
+    assert all(torch.equal(a[s], b[s]) for s in a)
+    for call in (lambda f: f.compact(), lambda f: f.fork({0: 1}), lambda f: f.advance({1: [4]})):
+        broken(one.end, 0)
+        two.end(0)
+        call(one)
+        call(two)
+        _books(one)
+        assert one.held == two.held and one.length == two.length
+        for f in (one, two):
+            if f.length[0]:
+                f.end(0)
+            f.advance({0: _long(40, 3)})
+    a, b = (f.advance({0: [3], 1: [2]}) for f in (one, two))
+    assert all(torch.equal(a[s], b[s]) for s in a)
