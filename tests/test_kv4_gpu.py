@@ -354,6 +354,23 @@ def test_attention(card, lens, rows, Hk, G, D, page, cap):
     assert torch.equal(a[0], again[0]) and torch.equal(a[1], again[1])
 
 
+@pytest.mark.parametrize("lens,rows,G,D,cap", [
+    # one span of more than 256 tiles, and of more than 512: a wave looks its next 64 places up on the way
+    ([17000], [1], 4, 64, 64), ([17000], [1], 4, 128, 64),                    # four and two tiles at a time, past the caches
+    ([9000, 8300], [9, 1], 8, 64, 64), ([9000, 8300], [9, 1], 8, 128, 64),    # a tile at a time, and what is left of it by four and two
+    ([16500], [40], 2, 64, 64), ([8192 + 33], [33], 1, 128, 64),
+    # more spans than a join asks for at once: 64 at head_dim 128, 128 at 64
+    ([34000], [1], 3, 128, 34000), ([36000], [1], 1, 64, 36000), ([66000], [1], 4, 64, 66000),
+])
+def test_long_walks_and_joins(card, lens, rows, G, D, cap):
+    g = gen(9540 + sum(lens) + D)
+    pool, tables, _, _ = _put(card, g, lens, 1, D, 64)
+    floats, q = card.attn_kv4_scratch(sum(rows), len(lens), G, 1, D, cap).numel(), _rows(g, sum(rows), G, D)
+    spans = floats // (sum(rows) * G * (D + 2)) if floats > 4 else 1
+    assert spans == 1 if cap == 64 else spans > (64 if D == 128 else 128), spans
+    _attend(card, q, pool, tables, lens, rows, G, 64, cap=cap)
+
+
 @pytest.mark.parametrize("lens,rows,Hk,G,D", [([9000], [1], 1, 2, 64), ([1500, 40], [1, 1], 2, 4, 128), ([129, 64, 0, 2000], [100, 64, 2, 1], 2, 5, 128)])
 def test_in_the_place_of_its_rows(card, lens, rows, Hk, G, D):
     """att is q: many spans, few, none"""

@@ -273,3 +273,31 @@ def test_books_that_cannot_be_sent(card, stack):
             f.advance({0: _long(40, 3)})
     a, b = (f.advance({0: [3], 1: [2]}) for f in (one, two))
     assert all(torch.equal(a[s], b[s]) for s in a)
+
+
+def test_a_fork_without_a_free_page(card, stack):
+    """a branch of a sequence that ends inside a page needs one of its own: with none free nothing changes; of whole pages it needs none"""
+    cfg, w = stack
+    f = Paged(card, cfg, w, 4, 4, page=32, rows=8, longest=80)
+    f.advance({0: _long(40, 7), 1: _long(64, 5)})
+    assert f.free == 0
+    torch.cuda.synchronize()
+    was = f.tables.clone(), f.lens.clone(), f.pool.clone(), [list(h) for h in f.held], list(f.length), list(f.named)
+    for branches in ({2: 0}, {2: 1, 3: 0}):
+        with pytest.raises(RuntimeError, match="a fork needs 1 pages, 0 are free"):
+            f.fork(branches)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(was, (f.tables, f.lens, f.pool))) and was[3:] == (f.held, f.length, f.named)
+        _books(f)
+    f.fork({2: 1})
+    _books(f)
+    assert f.held[2] == f.held[1] and f.free == 0
+    f.end(1)
+    with pytest.raises(RuntimeError):
+        f.fork({3: 0})  # (its pages are the branch's still)
+    f.end(2)
+    f.fork({3: 0})
+    _books(f)
+    assert f.held[3][0] == f.held[0][0] and f.held[3][1] != f.held[0][1] and f.free == 1
+    a = f.advance({0: [5], 3: [5]})
+    assert torch.equal(a[0], a[3])
