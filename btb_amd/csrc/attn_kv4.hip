@@ -13,6 +13,10 @@
 // largest one so far: at most 2^15 (the maximum may lag by 2^4), in full precision down to 2^-25 of the largest, and 2^-36 of it is lost at most. A
 // bf16 weight would be off by 2^-8, two of them cost twice the products. The unit in the maximum instead of in the scales would save a product
 // a weight (1 % of the time), but not the last bits of lse.
+//
+// Times beside a choice are those of its two sides on the code as it was then. As it is now, 32 query heads over 8 x 128: one row of 700 tokens
+// 8.4 us, of 131072 32; 64 sequences of up to 8192 70 .. 75; prompts beside single tokens 54; 500 rows over 16384 150 .. 157 (at head_dim 64 over 4
+// heads 109).
 
 #include <cfloat>
 
@@ -163,7 +167,7 @@ struct TileWords {
     uint4 k[STEPS], v[STEPS];
     uint32_t e;
 
-    // ONCE: no other workgroup reads the tile
+    // ONCE: past the caches (another workgroup may read the tile all the same)
     template <bool ONCE>
     __device__ __forceinline__ static uint4 piece(const uint8_t* at, int i) {
         const uint4* from = reinterpret_cast<const uint4*>(at) + i;
@@ -228,7 +232,7 @@ struct TileScales {
     }
 };
 // One tile at a time, every pair needs the same 32: each lane makes one of them, and all read them out of LDS, where sixteen of them would be two
-// more instructions each: 500 rows of 32 heads over 16384 tokens 161.6 -> 156.4 us.
+// more instructions each: 500 rows of 32 heads over 16384 tokens 162 -> 150 us, at head_dim 64 over 4 heads 125 -> 109.
 template <>
 struct TileScales<1> {
     int s;
@@ -337,7 +341,7 @@ struct Walk {
         u32x4 w[2];
         // Behind the CU's other workgroup where the vector unit is the bound, ahead of it with V's products and what is asked of memory: two
         // waves in step would multiply together and then wait for the vector unit together. The other way round 500 rows over 16384 tokens take
-        // 155.7 us instead of 150.7 and 64 sequences of up to 8192 75 instead of 70; with no difference 160 and 76.
+        // 155.6 us instead of 150.3 and 64 sequences of up to 8192 73 instead of 71; with no difference 158.5 and 75.
         __builtin_amdgcn_s_setprio(0);
         const f32x16 ahead = scores(lane, [&](int n) {
 #pragma unroll
@@ -540,9 +544,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attn_kv4_kernel(AttnKv4 p) {
     const int any = a.len - a.n + last / p.G + 1;
     a.from = a.span * length;
     a.to = min(min(a.from + length, tiles), any < 1 ? 0 : (any - 1) / KV4_TOKENS + 1);
-    // Few pairs: several tiles at a time. At head_dim 128 four of them do not fit the registers: 131072 tokens of one row 32.5 us by two,
-    // 33.5 by one, 61 by four; 64 sequences of up to 8192 71, 83 and 135. Tiles that this workgroup alone reads are not kept in the caches: 35 -> 32 and
-    // 78 -> 71, but 54 -> 55 for prompts beside single tokens where others read them too.
+    // Few pairs: several tiles at a time. At head_dim 128 four of them do not fit the registers: 131072 tokens of one row 32.2 us by two,
+    // 33.4 by one, 61 by four; 64 sequences of up to 8192 71, 85 and 135. The tiles of a sequence that has but these pairs go past the caches: 35 -> 32 and
+    // 78 -> 71 (55 -> 56 for prompts beside single tokens, 14 -> 15.4 for seven passes of eight rows, if what is left of longer ones does too: the whole tiles of
+    // pairs read the same). Branches read their common pages each for itself that way: 16 sequences of 1500 tokens with three branches each take 20.0 instead
+    // of 18.7, 64 of 1500 with nothing in common 24 instead of 26; of 6000 52 for 52, and 69 for 77.
     constexpr int NG = D == 64 ? 4 : 2;
     if (a.pairs <= PAIRS / NG)
         kv4_span<D, NG, true>(p, a, meet);
@@ -695,11 +701,14 @@ static Kv4Plan kv4_plan(size_t T, size_t B, size_t Hk, size_t G, size_t keys_cap
     Kv4Plan plan;
     plan.groups = (long long)(ragged ? T * G / PAIRS + B : B * ((T / B * G + PAIRS - 1) / PAIRS));
     const size_t tiles = (keys_cap + KV4_TOKENS - 1) / KV4_TOKENS;
-    // two workgroups a CU, as many as fit (131072 tokens of one row: 32 us, 43 with three, 47 with six; without a second round 500 rows over
-    // 16384 are 160 instead of 173). One of eight waves a CU instead: 64 sequences 71 -> 77, prompts beside single tokens 54 -> 61.
+    // two workgroups a CU, as many as fit (131072 tokens of one row: 32 us, 42 with three, 46 with six; with a span more, and so a second round,
+    // 500 rows over 16384 are 165 instead of 150, 64 sequences 77 instead of 71). One of eight waves a CU instead: 64 sequences 71 -> 77, prompts beside single
+    // tokens 54 -> 61. Groups are those that B sequences with T rows between them may have, whichever of them have any: with `first` 32 sequences of 8192
+    // have one span (60 us, 51 without), and 131072 tokens of one among 64 take 753.
     const size_t want = (size_t)(8 / WAVES) * device_info().cus / (plan.groups * Hk);
     size_t S = want < 1 ? 1 : want;
-    // (a second launch, for the join, pays from 32 tiles on: 700 tokens of one row take 12.6 us in two spans, 10.0 in one)
+    // (a second launch, for the join, pays from 32 tiles on: 700 tokens of one row take 10.5 us in two spans, 8.4 in one; the rule goes
+    // by keys_cap: under one of 32768 they take 1.1 more)
     const size_t most = tiles < 32 ? 1 : tiles / LEAST;
     if (S > most) S = most;
     if (S > (size_t)MOST_SPANS) S = MOST_SPANS;

@@ -1288,7 +1288,7 @@ class HipCard(CardLaunch):
     def kv4_read(self, cache: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                  first: torch.Tensor | None = None) -> None:
         """the pass's rows as the cache holds them, into k and v [T, Hk, D] (views; float32, exact, or bfloat16): `kv4_write`'s
-        other way round. Zeros where the page is not the pool's."""
+        other way round. Zeros where the page is not the pool's. k and v may lie between each other's rows or heads, with equal strides."""
         dev = torch._C._cuda_getDevice()
         (T, Hk, D), ks, vs = self._kv4_rows("kv4_read", dev, k, v, True)
         B, W, pages, page, stride = self._kv4_seqs("kv4_read", dev, cache, tables, lens, first, T, Hk, D)
@@ -1310,7 +1310,8 @@ class HipCard(CardLaunch):
         """att [T, Hq D] = attention of the pass's rows q [T, Hq D], which are their sequences' last ones as in `kv4_write`, each over
         its sequence's tokens up to itself, out of a layer's pool in 4 bits; lse (float32 [T, Hq]): the rows' log-sum-exp.
         keys_cap: about how long the longest sequence is (0: as long as the tables allow); it goes into the launch's
-        shape and the scratch's size only."""
+        shape and the scratch's size only. The launch is shaped for sequences that all have rows: a few that have, of many, are
+        faster by a call of their own."""
         dev, mine, bf, f32 = torch._C._cuda_getDevice(), self._mine, torch.bfloat16, torch.float32
         if not (mine(q, bf, dev) and mine(att, bf, dev) and mine(scratch, f32, dev) and (lse is None or mine(lse, f32, dev))):
             raise ValueError("[hip] attn_kv4: q and att are bfloat16, scratch and lse float32, all contiguous on the current GPU")

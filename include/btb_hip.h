@@ -551,10 +551,12 @@ int32_t btb_hip_kv4_read(const void* cache, const int32_t* tables, const int32_t
 /* Attention of the pass's rows, q [T, Hq D] bf16, each over its sequence's tokens up to its own place: att [T, Hq D] bf16 and, where lse is
  * not NULL, the rows' log-sum-exp [T, Hq] f32 (natural units, of scale q . k). A row with no token to see gets zeros and -inf. keys_cap: about how
  * many tokens the longest sequence has; it sizes the launch and the workspace (btb_hip_attn_kv4_floats of them, this call's own; 0: the sizes are
- * refused), a longer sequence takes longer. Sums are f32; a weight goes to the product with V as f16, to 2^-11 of itself (or 2^-36 of the largest,
- * both times their values' scales), so values times 16 times a sequence's tokens have to be f32 numbers yet (a scale below 2^-100 counts as that in what
- * is lost); q . k, before the scale and summed in any order, and scores times log2(e) may have any size below 2^127. Hq / Hk up to 64, T Hq up to 2^24, scale
- * above 0 and times log2(e) an f32 number; q, cache, att and workspace 16-byte aligned, att q itself or apart from it. */
+ * refused), a longer sequence takes longer. A sequence is cut into as many spans as fit the card if all B have rows: a few that have, of many,
+ * are faster by a call with their tables, lengths and rows alone (131072 tokens of one 33 us, among 64 753). Sums are f32; a weight goes to the
+ * product with V as f16, to 2^-11 of itself (or 2^-36 of the largest, both times their values' scales; a scale below 2^-100 counts as that in
+ * what is lost), so values times 16 times a sequence's tokens have to be f32 numbers yet; q . k, before the scale and summed in any order, and
+ * scores times log2(e) may have any size below 2^127. Hq / Hk up to 64, T Hq up to 2^24, scale above 0 and times log2(e) an f32 number; q, cache,
+ * att and workspace 16-byte aligned, att q itself or apart from it. */
 size_t btb_hip_attn_kv4_floats(size_t T, size_t B, size_t Hq, size_t Hk, size_t D, size_t keys_cap);
 int32_t btb_hip_attn_kv4(const void* q, const void* cache, const int32_t* tables, const int32_t* lens, const int32_t* first,
                          void* att, float* lse, size_t B, size_t W, size_t pages, size_t page, int64_t stride, size_t T, size_t Hq,
